@@ -619,9 +619,8 @@ int fmarl_create(const FmarlConfig *cfg, void **handle) {
     h->side = nullptr; h->ev_commit = h->ev_staged = nullptr;
     h->cap_id = h->cap_stage_id = 0;
     if (h->async) {
-        int prio_lo = 0, prio_hi = 0;   // lowest priority: staging only fills what the step kernels leave idle
-        (void)hipDeviceGetStreamPriorityRange(&prio_lo, &prio_hi);
-        if (hipStreamCreateWithPriority(&h->side, hipStreamNonBlocking, prio_lo) != hipSuccess ||
+        // the default priority, like every stream here: work on streams of different priorities has hung on this machine
+        if (hipStreamCreateWithFlags(&h->side, hipStreamNonBlocking) != hipSuccess ||
             hipEventCreateWithFlags(&h->ev_commit, hipEventDisableTiming) != hipSuccess ||
             hipEventCreateWithFlags(&h->ev_staged, hipEventDisableTiming) != hipSuccess) {
             delete h;

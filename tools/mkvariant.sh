@@ -12,6 +12,6 @@ if [ -n "$REV" ]; then
   (cd $R && git archive $REV fair_marl_amd/csrc include | tar -x -C $SRC)
 fi
 mkdir -p $R/fair_marl_amd/csrc/variants
-(cd $SRC/fair_marl_amd/csrc && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -mllvm -disable-machine-licm \
+(cd $SRC/fair_marl_amd/csrc && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -mllvm -disable-machine-licm -Xclang -target-feature -Xclang -packed-fp32-ops \
    -shared -fPIC "$@" -o $R/fair_marl_amd/csrc/variants/libfmarl_$NAME.so libfmarl.hip)
 echo "built fair_marl_amd/csrc/variants/libfmarl_$NAME.so from ${REV:-the working tree} $*"
