@@ -72,6 +72,20 @@ class FmarlBatchDst(C.Structure):
                                           'old_action_log_probs', 'adv_targ', 'available_actions', 'env_slot')]
 
 
+T_F32, T_BF16, T_F16 = 0, 1, 2
+
+
+class FmarlRows(C.Structure):
+    _fields_ = [('data', C.c_void_p), ('stride_l', C.c_int64), ('stride_b', C.c_int64), ('stride_h', C.c_int64)]
+
+
+class FmarlMemory(C.Structure):
+    _fields_ = [('L', C.c_int64), ('B', C.c_int64), ('H', C.c_int32), ('dk', C.c_int32), ('dv', C.c_int32), ('dtype', C.c_int32),
+                ('scale', C.c_float), ('shared_decay', C.c_int32), ('q', FmarlRows), ('k', FmarlRows), ('v', FmarlRows),
+                ('log_decay', C.c_void_p), ('decay_stride_l', C.c_int64), ('decay_stride_b', C.c_int64), ('decay_stride_h', C.c_int64),
+                ('masks', C.c_void_p), ('mask_stride_l', C.c_int64), ('mask_stride_b', C.c_int64), ('state', C.c_void_p)]
+
+
 _SIGS = {
     'fmarl_create': (C.c_int, [C.POINTER(FmarlConfig), C.POINTER(C.c_void_p)]),
     'fmarl_destroy': (C.c_int, [C.c_void_p]),
@@ -124,6 +138,11 @@ _SIGS = {
     'fmarl_advantages_sums': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_float, C.c_void_p, C.c_void_p]),
     'fmarl_advantages_apply': (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     'fmarl_minibatch_gather': (C.c_int, [C.POINTER(FmarlBatchSrc), C.POINTER(FmarlBatchDst), C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p]),
+    'fmarl_memory_step': (C.c_int, [C.POINTER(FmarlMemory), C.POINTER(FmarlRows), C.c_void_p, C.c_void_p]),
+    'fmarl_memory_workspace': (C.c_size_t, [C.POINTER(FmarlMemory), C.c_int]),
+    'fmarl_memory_chunk': (C.c_int, [C.POINTER(FmarlMemory), C.POINTER(FmarlRows), C.c_void_p, C.c_void_p, C.c_void_p]),
+    'fmarl_memory_chunk_backward': (C.c_int, [C.POINTER(FmarlMemory), C.POINTER(FmarlRows), C.c_void_p, C.POINTER(FmarlRows), C.POINTER(FmarlRows),
+                                              C.POINTER(FmarlRows), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 EXPORTS = tuple(_SIGS)
 _lib = None

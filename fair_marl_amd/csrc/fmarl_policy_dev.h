@@ -1,0 +1,63 @@
+// What the policy operators' kernels share (gfx950): element types, four-element loads and stores, MFMA vector types.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/fmarl.h"
+
+namespace fmarl {
+namespace policy {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Vec4;
+template <> struct Vec4<float> { typedef f32x4 type; };
+template <> struct Vec4<__bf16> { typedef bf16x4 type; };
+template <> struct Vec4<_Float16> { typedef f16x4 type; };
+
+// four consecutive elements at p: one load where `vec` (p is a multiple of four elements of the type), else element by element, zero beyond `left`
+template <typename T>
+__device__ __forceinline__ typename Vec4<T>::type load4(const T *p, int left, bool vec) {
+    typedef typename Vec4<T>::type V;
+    V v = {(T)0.f, (T)0.f, (T)0.f, (T)0.f};
+    if (vec) {
+        if (left > 0) v = *(const V *)p;   // (left is a multiple of four here)
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) if (r < left) v[r] = p[r];
+    }
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T *p, f32x4 a, int left, bool vec) {
+    typedef typename Vec4<T>::type V;
+    const V v = {(T)a[0], (T)a[1], (T)a[2], (T)a[3]};   // round to nearest even, once, at the end
+    if (vec) {
+        if (left > 0) *(V *)p = v;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) if (r < left) p[r] = v[r];
+    }
+}
+
+template <typename V> __device__ __forceinline__ f32x4 widen(V v) { return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]}; }
+
+// LDS of one wave: its writes before this are seen by its reads behind it (the LDS answers a wave in order; this holds the compiler)
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32: 1 ulp, 0 below 2^-126
+
+}  // namespace policy
+
+int policy_fail(int code, const char *fmt, const char *a = "");   // libfmarl.hip: the text of fmarl_last_error()
+
+}  // namespace fmarl

@@ -1,4 +1,4 @@
-// libfmarl.so -- C-ABI (include/fmarl.h) over the gfx950 kernels.  Single translation unit.
+// libfmarl.so -- C-ABI (include/fmarl.h) over the gfx950 kernels.  One translation unit; the policy operators are another (fmarl_policy.hip).
 #include <cstdio>
 #include <cstdlib>
 #include <cmath>
@@ -17,6 +17,7 @@
 #include "fmarl_graph.hip"
 #include "fmarl_rebuild.hip"
 #include "fmarl_learner.hip"
+#include "fmarl_policy_dev.h"
 
 using namespace fmarl;
 
@@ -28,6 +29,11 @@ int fail(int code, const char *fmt, const char *a = "") {
     snprintf(g_err, sizeof g_err, fmt, a);
     return code;
 }
+}  // namespace
+
+int fmarl::policy_fail(int code, const char *fmt, const char *a) { return fail(code, fmt, a); }   // (fmarl_policy.hip: the same text)
+
+namespace {
 #define HIP_OK(call)                                                        \
     do {                                                                    \
         hipError_t e_ = (call);                                             \

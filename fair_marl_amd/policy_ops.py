@@ -1,0 +1,179 @@
+"""The policy's operators on the device: what a recurrent policy computes on the fields of the rollout buffer.
+
+* ``memory_chunk`` / ``memory_step``: linear attention with a decay per head -- the policy's memory.  Where the reference runs a GRU over
+  ``rnn_states`` and ``masks`` (onpolicy/algorithms/utils/rnn.py:26-84: one step in the rollout, chunks of ``data_chunk_length`` with the
+  episodes' ends inside in the update), these carry a matrix per head through the same slots.
+
+All run on the current stream of their tensors' device, take any strides as long as the last axis is contiguous (a tensor whose last axis is
+not is copied), read nothing back and are capturable in a graph.  Gradients come through torch.autograd; ``memory_chunk_backward`` is the
+same gradient as a plain call, for a step that is captured without an autograd graph.  There is no CPU form: tensors off the GPU are refused.
+"""
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.T_F32, torch.bfloat16: _lib.T_BF16, torch.float16: _lib.T_F16}
+
+
+def _need(ok, text, *args):
+    if not ok:
+        raise ValueError(text % args if args else text)
+
+
+def _same_device(op, first, *rest):
+    _need(first.is_cuda, '%s: tensors must be on a GPU, got one on %s', op, first.device)
+    for t in rest:
+        _need(t is None or t.device == first.device, '%s: all tensors must be on %s', op, first.device)
+
+
+def _last(t):
+    """t with a contiguous last axis."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _rows(t):
+    """FmarlRows of a (L, B, H, d) or (B, H, d) tensor."""
+    s = t.stride()
+    return _lib.FmarlRows(t.data_ptr(), s[0] if len(s) == 4 else 0, s[-3], s[-2])
+
+
+# ---- memory ---------------------------------------------------------------------------------------------------------------------
+def _memory_args(op, q, k, v, log_decay, state, masks, scale, lead):
+    """The checked, laid out arguments: (FmarlMemory, tensors to keep)."""
+    _same_device(op, q, k, v, log_decay, state, masks)
+    _need(q.dtype in _DTYPES and k.dtype == q.dtype and v.dtype == q.dtype, '%s: q, k and v must be of one type out of float32, bfloat16, float16', op)
+    _need(q.dim() == lead + 2 and k.shape == q.shape and v.shape[:-1] == q.shape[:-1] and v.dim() == q.dim(),
+          '%s: q and k (%sB, H, dk), v (%sB, H, dv), got %s, %s, %s', op, 'L, ' * (lead - 1), 'L, ' * (lead - 1), tuple(q.shape), tuple(k.shape), tuple(v.shape))
+    L = q.shape[0] if lead == 2 else 1
+    B, H, dk, dv = q.shape[-3], q.shape[-2], q.shape[-1], v.shape[-1]
+    _need(log_decay.dtype == torch.float32, '%s: log_decay must be float32', op)
+    token = log_decay.dim() != 1
+    _need(tuple(log_decay.shape) == (tuple(q.shape[:-1]) if token else (H,)), '%s: log_decay must be (H,) or %s, got %s', op, tuple(q.shape[:-1]),
+          tuple(log_decay.shape))
+    if masks is not None:
+        _need(masks.numel() == L * B, '%s: masks must hold %d entries, got %s', op, L * B, tuple(masks.shape))
+        masks = masks.to(torch.float32).reshape(L, B)
+    if state is not None:
+        _need(state.dtype == torch.float32 and state.numel() == B * H * dk * dv, '%s: state must be float32 with B H dk dv = %d entries, got %s %s', op,
+              B * H * dk * dv, state.dtype, tuple(state.shape))
+        state = state.contiguous()
+    q, k, v = _last(q), _last(k), _last(v)
+    gs = log_decay.stride()
+    m = _lib.FmarlMemory(L, B, H, dk, dv, _DTYPES[q.dtype], dk ** -0.5 if scale is None else float(scale), 0 if token else 1, _rows(q), _rows(k), _rows(v),
+                         log_decay.data_ptr(), gs[0] if len(gs) == 3 else 0, gs[-2] if token else 0, gs[-1], _ptr(masks),
+                         masks.stride(0) if masks is not None else 0, masks.stride(1) if masks is not None else 0, _ptr(state))
+    return m, (q, k, v, log_decay, state, masks)
+
+
+def _launch_chunk(m, keep):
+    q, v = keep[0], keep[2]
+    dev = q.device
+    out = torch.empty(v.shape, dtype=v.dtype, device=dev)
+    state = torch.empty(m.B, m.H, m.dk, m.dv, dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        ws = torch.empty(lib.fmarl_memory_workspace(m, 0), dtype=torch.uint8, device=dev)
+        _lib.check(lib.fmarl_memory_chunk(m, _rows(out), state.data_ptr(), ws.data_ptr(), _stream(dev)), 'fmarl_memory_chunk')
+    return out, state
+
+
+def _launch_chunk_backward(m, keep, d_out, d_state, want_decay=True):
+    q, k, v, g, state = keep[:5]
+    dev = q.device
+    d_out = _last(d_out)
+    if d_state is not None:
+        d_state = d_state.contiguous()
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+    dg = torch.empty(g.shape, dtype=torch.float32, device=dev) if want_decay else None
+    ds = torch.empty(m.B, m.H, m.dk, m.dv, dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        ws = torch.empty(lib.fmarl_memory_workspace(m, 1), dtype=torch.uint8, device=dev)
+        _lib.check(lib.fmarl_memory_chunk_backward(m, _rows(d_out), _ptr(d_state), _rows(dq), _rows(dk), _rows(dv), _ptr(dg), ds.data_ptr(), ws.data_ptr(),
+                                                   _stream(dev)), 'fmarl_memory_chunk_backward')
+    return dq, dk, dv, dg, ds
+
+
+class _MemoryChunk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, masks, scale):
+        m, keep = _memory_args('memory_chunk', q, k, v, log_decay, state, masks, scale, 2)
+        ctx.save_for_backward(*keep)
+        ctx.scale, ctx.state_shape = m.scale, None if state is None else state.shape
+        ctx.set_materialize_grads(False)
+        return _launch_chunk(m, keep)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, d_state):
+        q, k, v, g, state, masks = ctx.saved_tensors
+        m, keep = _memory_args('memory_chunk', q, k, v, g, state, masks, ctx.scale, 2)
+        if d_out is None:
+            d_out = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
+        dq, dk, dv, dg, ds = _launch_chunk_backward(m, keep, d_out, d_state, ctx.needs_input_grad[3])
+        return dq, dk, dv, dg, None if state is None else ds.view(ctx.state_shape), None, None
+
+
+def memory_chunk(q, k, v, log_decay, state=None, masks=None, scale=None):
+    """Linear attention with a decay per head over L tokens of B sequences: ``(out, last_state)``.
+
+        S_t = r_t exp(log_decay_t) S_{t-1} + k_t^T v_t,    out_t = scale q_t S_t,    r_t = 0 where masks_t == 0, else 1
+
+    q, k (L, B, H, dk), v (L, B, H, dv) of one type (float32, bfloat16, float16), 1 <= dk, dv <= 128; out has v's type.  log_decay float32: (H,)
+    or one per token, (L, B, H); -inf forgets everything.  state: what the sequences bring, float32 with B H dk dv entries in any shape
+    (the generator's ``rnn_states`` rows), None for zeros; the last state comes back as (B, H, dk, dv).  masks: L B entries as the
+    generator's ``masks`` (0: an episode starts at the token).  scale: dk ** -0.5 if None.  Rows ordered (L, chunk) as ``recurrent_generator``
+    yields them are this layout: ``q.view(L, chunks, H, dk)``.  States, decays and all sums are float32 (the decays' prefix sums float64).
+    Differentiable in q, k, v, log_decay and state, once."""
+    _need(q.dim() == 4 and v.dim() == 4, 'memory_chunk: q, k (L, B, H, dk) and v (L, B, H, dv), got %s, %s', tuple(q.shape), tuple(v.shape))
+    if q.shape[0] == 0 or q.shape[1] == 0:
+        _memory_args('memory_chunk', q, k, v, log_decay, state, masks, scale, 2)
+        shape = (q.shape[1], q.shape[2], q.shape[3], v.shape[3])
+        return v.clone(), torch.zeros(shape, dtype=torch.float32, device=q.device) if state is None else state.reshape(shape).clone()
+    return _MemoryChunk.apply(q, k, v, log_decay, state, masks, scale)
+
+
+def memory_chunk_backward(q, k, v, log_decay, d_out, d_state=None, state=None, masks=None, scale=None):
+    """The gradients of ``memory_chunk`` as a plain call: (dq, dk, dv, d_log_decay, d_state0) from d_out (L, B, H, dv) and the gradient of the last
+    state (None: zeros)."""
+    m, keep = _memory_args('memory_chunk_backward', q, k, v, log_decay, state, masks, scale, 2)
+    _need(m.L > 0 and m.B > 0, 'memory_chunk_backward: no tokens')
+    _same_device('memory_chunk_backward', q, d_out, d_state)
+    _need(d_out.shape == v.shape and d_out.dtype == v.dtype, 'memory_chunk_backward: d_out must be %s %s', tuple(v.shape), v.dtype)
+    if d_state is not None:
+        _need(d_state.dtype == torch.float32 and d_state.numel() == m.B * m.H * m.dk * m.dv, 'memory_chunk_backward: d_state must be float32 (B, H, dk, dv)')
+    return _launch_chunk_backward(m, keep, d_out, d_state)
+
+
+def memory_step(q, k, v, log_decay, state, masks=None, scale=None, out_state=None):
+    """``memory_chunk`` for one token per sequence, as an env step of the rollout takes it: ``(out, out_state)``.  q, k (B, H, dk), v (B, H, dv), log_decay
+    (H,) or (B, H), masks B entries, state None or float32 with B H dk dv entries.  out_state: where the new state goes (float32, contiguous; the buffer's next slot, or ``state``
+    itself), a new (B, H, dk, dv) tensor if None.  No gradient: refused where one would be recorded."""
+    _need(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, state))),
+          'memory_step records no gradient: call it under torch.no_grad(), or use memory_chunk')
+    m, keep = _memory_args('memory_step', q, k, v, log_decay, state, masks, scale, 1)
+    dev, n = q.device, m.B * m.H * m.dk * m.dv
+    if out_state is None:
+        out_state = torch.empty(m.B, m.H, m.dk, m.dv, dtype=torch.float32, device=dev)
+    else:
+        _need(out_state.device == dev and out_state.dtype == torch.float32 and out_state.numel() == n and out_state.is_contiguous(),
+              'memory_step: out_state must be contiguous float32 with %d entries on %s', n, dev)
+        if keep[4] is not None:
+            gap = abs(out_state.data_ptr() - keep[4].data_ptr())
+            _need(gap == 0 or gap >= 4 * n, 'memory_step: out_state overlaps state without being it')
+    out = torch.empty(v.shape, dtype=v.dtype, device=dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.check(lib.fmarl_memory_step(m, _rows(out), out_state.data_ptr(), _stream(dev)), 'fmarl_memory_step')
+    return out, out_state

@@ -503,6 +503,46 @@ typedef struct FmarlBatchDst {
 int fmarl_minibatch_gather(const FmarlBatchSrc *src, const FmarlBatchDst *dst, const int64_t *index, int64_t rows, int mode,
                            int chunk, void *stream);
 
+/* ---- the policy's operators ------------------------------------------------------------------------------------------------
+ * What a recurrent policy computes on the fields of the rollout buffer, beside the env step and before the gradient step.  Stateless;
+ * they run on the current device, on `stream`; nothing is read back, nothing synchronises, all are capturable.  Arrays of `dtype`
+ * FMARL_T_*; states, decays, masks and statistics are float32, products and sums are formed in float32 or wider. */
+#define FMARL_T_F32 0
+#define FMARL_T_BF16 1
+#define FMARL_T_F16 2
+
+/* A (L, B, H, d) array whose last axis is contiguous; strides in elements (0 repeats a row; not for outputs). */
+typedef struct FmarlRows {
+    void *data;
+    int64_t stride_l, stride_b, stride_h;
+} FmarlRows;
+
+/* Linear attention with a decay per head: the memory of a recurrent policy (what the reference keeps in the GRU behind rnn_states and masks,
+ * onpolicy/algorithms/utils/rnn.py:26-84, here as a matrix per head).  Token t of sequence b, head h:
+ *     S_t = r_t exp(g_t) S_{t-1} + k_t^T v_t,    out_t = scale q_t S_t,    r_t = 0 where masks_t == 0 (an episode starts), else 1.
+ * q, k (L, B, H, dk), v (L, B, H, dv), 1 <= dk, dv <= 128; masks (L, B) or NULL; log_decay g (L, B, H) by its strides; -inf
+ * forgets everything.  state (B, H, dk, dv) contiguous, NULL: zeros.  A state that is not carried on is not read
+ * into the next one, whatever it holds. */
+typedef struct FmarlMemory {
+    int64_t L, B;
+    int32_t H, dk, dv, dtype;
+    float scale;
+    int32_t shared_decay;          /* 1: one decay per head (its gradient is (H)); 0: one per token (its gradient is (L, B, H)) */
+    FmarlRows q, k, v;
+    const float *log_decay; int64_t decay_stride_l, decay_stride_b, decay_stride_h;
+    const float *masks; int64_t mask_stride_l, mask_stride_b;
+    const float *state;
+} FmarlMemory;
+/* one token (L == 1): a rollout's env step; state_out may be `state` itself */
+int fmarl_memory_step(const FmarlMemory *m, const FmarlRows *out, float *state_out, void *stream);
+/* L >= 1 tokens; workspace: fmarl_memory_workspace(m, backward) bytes, 16-byte aligned, contents free after the stream's work */
+size_t fmarl_memory_workspace(const FmarlMemory *m, int backward);
+int fmarl_memory_chunk(const FmarlMemory *m, const FmarlRows *out, float *state_out, void *workspace, void *stream);
+/* gradients: d_out and d_state (B, H, dk, dv; NULL: zeros) in; d_q, d_k, d_v, d_log_decay (contiguous; NULL:
+ * not wanted) and d_state0 (NULL: not wanted) out */
+int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, const float *d_state, const FmarlRows *d_q, const FmarlRows *d_k,
+                                const FmarlRows *d_v, float *d_log_decay, float *d_state0, void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

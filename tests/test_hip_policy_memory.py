@@ -1,0 +1,256 @@
+"""-m gpu: the policy's memory (linear attention with a decay per head) against its recurrence in float64, token by token, and its gradients
+against their formulas and against differences.
+
+Tolerances: every output is a sum of products; each term passes at most 2 L + dk + dv additions and products and one power of two whose argument
+(at most 126 before it underflows) is rounded to float32, so the error is at most gamma = (2 L + dk + dv + 200) 2^-24 times the same sum over
+the terms' magnitudes (the recurrence run on absolute values), and half a step of the output's type on top.  The decay's gradient is a running
+difference: its bound is the running sum of the bounds of what is added up."""
+import math
+
+import pytest
+import torch
+
+import fair_marl_amd as fm
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def recurrence(q, k, v, g, S, fresh, scale, d_out=None, d_state=None):
+    """float64: (out, last state) or, with d_out, (out, last state, dq, dk, dv, dg, dS0); g (L, B, H), fresh (L, B)."""
+    L = q.shape[0]
+    states, outs = [], []
+    fresh = fresh[..., None] | (g == -math.inf)
+    a = torch.where(fresh, torch.zeros_like(g), torch.exp(g))[..., None, None]
+    keep = lambda t, S: torch.where(fresh[t][..., None, None], torch.zeros_like(S), a[t] * S)  # noqa: E731
+    for t in range(L):
+        states.append(S)
+        S = keep(t, S) + k[t][..., None] * v[t][..., None, :]
+        outs.append((q[t][..., None] * S).sum(-2) * scale)
+    if d_out is None:
+        return torch.stack(outs), S
+    G, last = d_state, S
+    dq, dk, dv, dg = [], [], [], []
+    for t in reversed(range(L)):
+        now = keep(t, states[t]) + k[t][..., None] * v[t][..., None, :]
+        dq.append((now * d_out[t][..., None, :]).sum(-1) * scale)
+        G = G + scale * q[t][..., None] * d_out[t][..., None, :]
+        dk.append((G * v[t][..., None, :]).sum(-1))
+        dv.append((G * k[t][..., None]).sum(-2))
+        G = keep(t, G)
+        dg.append(torch.where(fresh[t], torch.zeros_like(g[t]), (G * states[t]).sum((-1, -2))))
+    r = lambda x: torch.stack(x[::-1])  # noqa: E731
+    return torch.stack(outs), last, r(dq), r(dk), r(dv), r(dg), G
+
+
+def make(L, B, H, dk, dv, dtype, decay, seed, reset=0.1):
+    gen = torch.Generator().manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    q, k, v, do = (rn(L, B, H, d).to(dtype) for d in (dk, dk, dv, dv))
+    g = torch.nn.functional.logsigmoid(3 * rn(*((L, B, H) if decay == 'token' else (H,))) + 2)
+    masks = (torch.rand(L, B, generator=gen) > reset).float()
+    return [t.to(DEV) for t in (q, k, v, g, rn(B, H, dk, dv), masks, do, rn(B, H, dk, dv))]
+
+
+def close(got, want, bound, name=''):
+    got = got.double()
+    half = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}
+    err = (got - want).abs() - bound
+    assert got.shape == want.shape and bool((err <= 0).all()), '%s: %.3g over its bound at %s' % (name, float(err.max()), int(err.argmax()))
+    return half
+
+
+def step_of(t, want):
+    return want.abs() * (torch.finfo(t.dtype).eps / 2) + (2.0 ** -25 if t.dtype == F16 else 0.0)
+
+
+def compare(got, q, k, v, g, S, masks, scale, do, dS):
+    """got: (out, last, dq, dk, dv, dg, dS0) of the framework, dg (L, B, H) or (H,)"""
+    L, B, H, dk = q.shape
+    gamma = (2 * L + dk + v.shape[-1] + 200) * 2.0 ** -24
+    gd = g.double().expand(L, B, H)
+    args = [x.double() for x in (q, k, v)], gd, S.double(), masks == 0
+    want = recurrence(*args[0], *args[1:], scale, do.double(), dS.double())
+    mag = recurrence(*[x.abs() for x in args[0]], gd, S.double().abs(), masks == 0, scale, do.double().abs(), dS.double().abs())
+    for i, name in ((0, 'out'), (1, 'state'), (2, 'dq'), (3, 'dk'), (4, 'dv'), (6, 'dS0')):
+        close(got[i], want[i], gamma * mag[i] + step_of(got[i], want[i]), name)
+    add = (q.double().abs() * mag[2]).sum(-1) + (k.double().abs() * mag[3]).sum(-1)
+    run = (S.double().abs() * mag[6]).sum((-1, -2)) + torch.cumsum(add, 0)
+    if g.dim() == 3:
+        close(got[5], want[5], gamma * run + step_of(got[5], want[5]), 'dg')
+    else:
+        close(got[5], want[5].sum((0, 1)), gamma * run.sum((0, 1)) + step_of(got[5], want[5].sum((0, 1))), 'dg')
+
+
+SHAPES = [(1, 3, 2, 16, 16), (10, 37, 4, 16, 16), (16, 5, 1, 5, 7), (17, 2, 3, 33, 20), (31, 300, 4, 16, 16), (100, 3, 2, 64, 64), (130, 2, 2, 128, 128),
+          (300, 1, 1, 40, 72), (257, 2, 1, 1, 1), (64, 2, 2, 64, 32), (513, 2, 3, 8, 128), (65, 1, 3, 128, 8), (1000, 3, 1, 24, 24)]
+
+
+@pytest.mark.parametrize('decay', ['token', 'head'])
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+def test_chunk_and_gradients(shape, dtype, decay):
+    q, k, v, g, S, masks, do, dS = make(*shape, dtype, decay, seed=sum(shape))
+    leaves = [t.requires_grad_() for t in (q, k, v, g, S)]
+    out, last = fm.memory_chunk(q, k, v, g, S, masks)
+    grads = torch.autograd.grad((out, last), leaves, (do, dS))
+    assert out.dtype == dtype and last.dtype == F32 and all(a.dtype == b.dtype and a.shape == b.shape for a, b in zip(grads, leaves))
+    with torch.no_grad():
+        compare((out, last) + grads, q, k, v, g, S, masks, shape[3] ** -0.5, do, dS)
+
+
+@pytest.mark.parametrize('shape', [(10, 9, 4, 16, 16), (200, 2, 2, 40, 24)], ids=str)
+def test_views_of_one_projection_in_any_order(shape):
+    L, B, H, dk, dv = shape
+    gen = torch.Generator().manual_seed(5)
+    # batch-major storage, heads inside, odd offsets: no row starts on a multiple of four elements
+    big = torch.randn(B, L, H * (2 * dk + dv) + 3, generator=gen).to(DEV)
+    q, k, v = (t.transpose(0, 1).unflatten(-1, (H, -1)) for t in big[..., 1:-2].split([H * dk, H * dk, H * dv], -1))
+    _, _, _, g, S, masks, do, dS = make(*shape, F32, 'token', seed=6)
+    g = g.permute(2, 1, 0).contiguous().permute(2, 1, 0)
+    masks = masks.t().contiguous().t()
+    want = fm.memory_chunk(q.contiguous(), k.contiguous(), v.contiguous(), g.contiguous(), S, masks.contiguous())
+    got = fm.memory_chunk(q, k, v, g, S, masks)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    do2 = do.permute(3, 0, 1, 2).contiguous().permute(1, 2, 3, 0)    # last axis not contiguous: copied
+    a = fm.memory_chunk_backward(q, k, v, g, do2, dS, S, masks)
+    b = fm.memory_chunk_backward(q.contiguous(), k.contiguous(), v.contiguous(), g.contiguous(), do, dS, S, masks)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize('shape', [(12, 2, 2, 16, 16), (150, 1, 1, 20, 36)], ids=str)
+def test_gradient_against_differences(shape):
+    """central differences of the float64 recurrence along one direction: the truncation is O(h^2) = 1e-8 relative, the framework's gradient float32"""
+    q, k, v, g, S, masks, do, dS = make(*shape, F32, 'token', seed=11)
+    grads = fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks)
+    gen = torch.Generator().manual_seed(12)
+    dirs = [torch.randn(t.shape, generator=gen).to(DEV).double() for t in (q, k, v, g, S)]
+
+    def f(h):
+        args = [t.double() + h * d for t, d in zip((q, k, v, g, S), dirs)]
+        o, last = recurrence(*args, masks == 0, shape[3] ** -0.5)
+        return float((o * do.double()).sum() + (last * dS.double()).sum())
+    h = 1e-4
+    want = (f(h) - f(-h)) / (2 * h)
+    parts = [(a.double() * d).sum() for a, d in zip(grads, dirs)]
+    assert abs(float(sum(parts)) - want) < 1e-5 * max(1.0, sum(float((a.double() * d).abs().sum()) for a, d in zip(grads, dirs)))
+
+
+@pytest.mark.parametrize('shape', [(7, 2, 16, 16), (3, 1, 5, 7), (700, 4, 16, 16), (2, 3, 64, 128), (5, 2, 33, 100), (2, 1, 1, 1), (9, 1, 128, 4)], ids=str)
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+def test_step_is_one_token(shape, dtype):
+    B, H, dk, dv = shape
+    q, k, v, g, S, masks, _, _ = make(1, *shape, dtype, 'token', seed=3, reset=0.4)
+    for gg in (g[0], g[0, 0].contiguous()):
+        want, last = recurrence(q.double(), k.double(), v.double(), gg.double().expand(1, B, H), S.double(), masks == 0, 0.3)
+        mag, mlast = recurrence(q.double().abs(), k.double().abs(), v.double().abs(), gg.double().expand(1, B, H), S.double().abs(), masks == 0, 0.3)
+        gamma = (dk + 140) * 2.0 ** -24
+        out, new = fm.memory_step(q[0], k[0], v[0], gg, S, masks[0], 0.3)
+        close(out, want[0], gamma * mag[0] + step_of(out, want[0]), 'out')
+        close(new, last, gamma * mlast + step_of(new, last), 'state')
+        mine = S.clone()
+        out2, same = fm.memory_step(q[0], k[0], v[0], gg, mine, masks[0], 0.3, out_state=mine)     # in place
+        assert same is mine and torch.equal(mine, new) and torch.equal(out2, out)
+
+
+def test_rows_that_start_afresh_see_nothing_of_before():
+    """what an episode left behind -- infinities and NaN too -- stays behind, in the state and inside a chunk; later tokens never reach earlier ones"""
+    q, k, v, g, S, masks, do, dS = make(40, 4, 2, 16, 16, F32, 'token', seed=8)
+    masks.fill_(1)
+    masks[0, 0] = 0
+    masks[21, 1] = 0
+    masks[:, 3] = 0                       # every token alone
+    g[13, 2, 1] = -math.inf               # the same by the decay, one head
+    S[0] = math.nan
+    v[20, 1, :, 3], k[18, 1] = math.inf, math.nan
+    S[2, 1] = math.inf
+    k[39, 3], v[39, 0, 0, 0] = math.nan, math.inf
+    out, last = fm.memory_chunk(q, k, v, g, S, masks)
+    want, wlast = recurrence(q.double(), k.double(), v.double(), g.double(), S.double(), masks == 0, 0.25)
+    assert torch.equal(torch.isfinite(out), torch.isfinite(want)) and torch.equal(torch.isfinite(last), torch.isfinite(wlast))
+    assert bool(torch.isfinite(out[:39, 0]).all()) and bool(torch.isfinite(out[21:, 1]).all()) and bool(torch.isfinite(out[:39, 3]).all())
+    fin = torch.isfinite(want)
+    assert float((out.double() - want)[fin].abs().max()) < 1e-4
+    one = fm.memory_step(q[0], k[0], v[0], g[0], S, masks[0])
+    assert bool(torch.isfinite(one[0][0]).all()) and bool(torch.isfinite(one[1][0]).all())
+    # a column of the batch whose steps all start afresh: out_t = scale (q.k) v
+    assert float((out[:39, 3].double() - 0.25 * ((q * k).double().sum(-1, keepdim=True) * v.double())[:39, 3]).abs().max()) < 1e-5
+    # backwards: nothing of the later episode reaches the tokens before its start
+    do[30, 1] = math.nan
+    v[20, 1, :, 3], k[18, 1], S[0], S[2, 1], k[39, 3], v[39, 0, 0, 0] = 0.0, 0.0, 0.0, 0.0, 0.0, 0.0
+    dq, dk, dv, dg, ds = fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks)
+    for t in (dq, dk, dv):
+        assert bool(torch.isfinite(t[:21, 1]).all()) and bool(torch.isfinite(t[:, (0, 2, 3)]).all())
+    assert bool(torch.isfinite(ds).all()) and bool((dg[:, 3] == 0).all()) and float(dg[21, 1].abs().max()) == 0 and float(dg[13, 2, 1]) == 0
+
+
+def test_decays_of_every_size():
+    """decays that forget all within a token beside such that forget nothing, and growth: the prefix sums do not lose the small ones behind the large"""
+    shape = (90, 3, 2, 16, 16)
+    q, k, v, g, S, masks, do, dS = make(*shape, F32, 'token', seed=2)
+    masks.fill_(1)
+    g[:, 0] = torch.where(torch.rand(90, 2, device=DEV) < 0.2, -5000.0, -1e-3)
+    g[:, 1] = 0.0
+    g[:, 2] = 0.05
+    out, last = fm.memory_chunk(q, k, v, g, S, masks)
+    compare((out, last) + fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks), q, k, v, g, S, masks, 0.25, do, dS)
+
+
+def test_lengths_of_zero():
+    z = lambda *s: torch.randn(*s, device=DEV)  # noqa: E731
+    S = z(2, 3, 4, 5).requires_grad_()
+    out, last = fm.memory_chunk(z(0, 2, 3, 4), z(0, 2, 3, 4), z(0, 2, 3, 5), z(3), S)
+    assert out.shape == (0, 2, 3, 5) and torch.equal(last, S) and torch.equal(torch.autograd.grad(last.sum(), S)[0], torch.ones_like(S))
+    out, last = fm.memory_chunk(z(6, 0, 3, 4), z(6, 0, 3, 4), z(6, 0, 3, 5), z(3))
+    assert out.shape == (6, 0, 3, 5) and last.shape == (0, 3, 4, 5)
+    out, last = fm.memory_step(z(0, 3, 4), z(0, 3, 4), z(0, 3, 5), z(3), None)
+    assert out.shape == (0, 3, 5) and last.shape == (0, 3, 4, 5)
+
+
+def test_only_one_output_is_used():
+    q, k, v, g, S, masks, do, dS = make(20, 2, 2, 16, 16, F32, 'head', seed=4)
+    leaves = [t.requires_grad_() for t in (q, k, v, g, S)]
+    zero, none = torch.zeros_like(do), None
+    for use, d in ((0, do), (1, dS)):
+        got = torch.autograd.grad(fm.memory_chunk(q, k, v, g, S, masks)[use], leaves, d)
+        want = fm.memory_chunk_backward(q, k, v, g, do if use == 0 else zero, dS if use == 1 else none, S, masks)
+        assert all(torch.equal(a, b.view_as(a)) for a, b in zip(got, want))
+
+
+def test_streams_and_graphs():
+    """two streams at once, a captured pass that is replayed on other inputs between eager work: every result equals the eager one"""
+    shape = (200, 3, 2, 32, 32)
+    q, k, v, g, S, masks, do, dS = make(*shape, F32, 'token', seed=9)
+    run = lambda: fm.memory_chunk(q, k, v, g, S, masks) + fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks)  # noqa: E731
+    want = [t.clone() for t in run()]
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for st in side:
+        with torch.cuda.stream(st):
+            got.append(run())
+    torch.cuda.synchronize()
+    for r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = run()
+        graphs.append((graph, res))
+    for seed in (20, 21, 22):
+        for dst, src in zip((q, k, v, g, S, masks, do, dS), make(*shape, F32, 'token', seed=seed)):
+            dst.copy_(src)
+        want = [t.clone() for t in run()]
+        for graph, res in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(res, want))
+
+
+def test_same_bits_again():
+    q, k, v, g, S, masks, do, dS = make(700, 2, 2, 64, 64, BF16, 'head', seed=10)
+    a = fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks)
+    b = fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
