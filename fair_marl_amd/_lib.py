@@ -86,6 +86,12 @@ class FmarlMemory(C.Structure):
                 ('masks', C.c_void_p), ('mask_stride_l', C.c_int64), ('mask_stride_b', C.c_int64), ('state', C.c_void_p)]
 
 
+class FmarlBlock(C.Structure):
+    _fields_ = [('rows', C.c_int64)] + [(k, C.c_int32) for k in ('dim', 'groups', 'dtype', 'x_dtype', 'kind', 'gate_act', 'post_norm', 'pre_norm')] + \
+               [('eps', C.c_float), ('reserved', C.c_int32), ('x', C.c_void_p), ('x_stride', C.c_int64), ('branch', C.c_void_p), ('branch_stride', C.c_int64),
+                ('gate', C.c_void_p), ('gate_stride', C.c_int64)] + [(k, C.c_void_p) for k in ('scale', 'post_weight', 'post_bias', 'pre_weight', 'pre_bias')]
+
+
 _SIGS = {
     'fmarl_create': (C.c_int, [C.POINTER(FmarlConfig), C.POINTER(C.c_void_p)]),
     'fmarl_destroy': (C.c_int, [C.c_void_p]),
@@ -143,6 +149,10 @@ _SIGS = {
     'fmarl_memory_chunk': (C.c_int, [C.POINTER(FmarlMemory), C.POINTER(FmarlRows), C.c_void_p, C.c_void_p, C.c_void_p]),
     'fmarl_memory_chunk_backward': (C.c_int, [C.POINTER(FmarlMemory), C.POINTER(FmarlRows), C.c_void_p, C.POINTER(FmarlRows), C.POINTER(FmarlRows),
                                               C.POINTER(FmarlRows), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    'fmarl_block_norm': (C.c_int, [C.POINTER(FmarlBlock), C.c_void_p, C.c_void_p, C.c_void_p]),
+    'fmarl_block_norm_workspace': (C.c_size_t, [C.POINTER(FmarlBlock)]),
+    'fmarl_block_norm_backward': (C.c_int, [C.POINTER(FmarlBlock), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+                                            C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 EXPORTS = tuple(_SIGS)
 _lib = None

@@ -61,3 +61,14 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 int policy_fail(int code, const char *fmt, const char *a = "");   // libfmarl.hip: the text of fmarl_last_error()
 
 }  // namespace fmarl
+
+#define HIP_OK(call)                                                                                        \
+    do {                                                                                                    \
+        hipError_t e_ = (call);                                                                             \
+        if (e_ != hipSuccess) return fmarl::policy_fail(FMARL_EHIP, #call ": %s", hipGetErrorString(e_));   \
+    } while (0)
+
+namespace {
+inline int elem_bytes(int dtype) { return dtype == FMARL_T_F32 ? 4 : 2; }
+inline size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+}  // namespace

@@ -1,4 +1,4 @@
-// libfmarl.so -- C-ABI (include/fmarl.h) over the gfx950 kernels.  One translation unit; the policy operators are another (fmarl_policy.hip).
+// libfmarl.so -- C-ABI (include/fmarl.h) over the gfx950 kernels.  One translation unit; the policy operators (fmarl_memory.hip, fmarl_block.hip, fmarl_actions.hip) are others.
 #include <cstdio>
 #include <cstdlib>
 #include <cmath>
@@ -17,7 +17,6 @@
 #include "fmarl_graph.hip"
 #include "fmarl_rebuild.hip"
 #include "fmarl_learner.hip"
-#include "fmarl_policy_dev.h"
 
 using namespace fmarl;
 
@@ -31,7 +30,8 @@ int fail(int code, const char *fmt, const char *a = "") {
 }
 }  // namespace
 
-int fmarl::policy_fail(int code, const char *fmt, const char *a) { return fail(code, fmt, a); }   // (fmarl_policy.hip: the same text)
+// the same text for the other translation units' entry points (fmarl_policy_dev.h)
+namespace fmarl { int policy_fail(int code, const char *fmt, const char *a) { return fail(code, fmt, a); } }
 
 namespace {
 #define HIP_OK(call)                                                        \

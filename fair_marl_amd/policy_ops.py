@@ -3,6 +3,7 @@
 * ``memory_chunk`` / ``memory_step``: linear attention with a decay per head -- the policy's memory.  Where the reference runs a GRU over
   ``rnn_states`` and ``masks`` (onpolicy/algorithms/utils/rnn.py:26-84: one step in the rollout, chunks of ``data_chunk_length`` with the
   episodes' ends inside in the update), these carry a matrix per head through the same slots.
+* ``block_norm``: the end of a residual block and the start of the next in one pass -- norm of the branch, gate, residual scale, residual, norm.
 
 All run on the current stream of their tensors' device, take any strides as long as the last axis is contiguous (a tensor whose last axis is
 not is copied), read nothing back and are capturable in a graph.  Gradients come through torch.autograd; ``memory_chunk_backward`` is the
@@ -177,3 +178,92 @@ def memory_step(q, k, v, log_decay, state, masks=None, scale=None, out_state=Non
     with torch.cuda.device(dev):
         _lib.check(lib.fmarl_memory_step(m, _rows(out), out_state.data_ptr(), _stream(dev)), 'fmarl_memory_step')
     return out, out_state
+
+
+# ---- block_norm -----------------------------------------------------------------------------------------------------------------
+_WEIGHTS = ('scale', 'post_weight', 'post_bias', 'pre_weight', 'pre_bias')
+
+
+def _block_args(x, branch, gate, weights, groups, kind, gate_act, post_norm, pre_norm, eps):
+    """(FmarlBlock, 2-d views of x, branch and gate, the float32 weights); what has to live until the launch is in there."""
+    _same_device('block_norm', x, branch, gate, *weights)
+    D = x.shape[-1] if x.dim() else 0
+    dtype = x.dtype if branch is None else branch.dtype
+    _need(dtype in _DTYPES and x.dtype in (dtype, torch.float32), 'block_norm: float32, bfloat16 or float16; x of the branch\'s type or float32, got %s, %s',
+          x.dtype, dtype)
+    for name, t in (('branch', branch), ('gate', gate)):
+        _need(t is None or (t.shape == x.shape and t.dtype == dtype), 'block_norm: %s must be %s %s', name, tuple(x.shape), dtype)
+    for name, w in zip(_WEIGHTS, weights):
+        _need(w is None or (tuple(w.shape) == (D,) and w.dtype == torch.float32), 'block_norm: %s must be float32 (%d,)', name, D)
+    _need(kind in ('rms', 'layer'), 'block_norm: kind must be rms or layer, got %r', kind)
+    _need(gate_act in ('sigmoid', 'silu'), 'block_norm: gate_act must be sigmoid or silu, got %r', gate_act)
+    rows = [None if t is None else _last(t.reshape(-1, D)) for t in (x, branch, gate)]
+    weights = [None if w is None else w.contiguous() for w in weights]
+    st = lambda t: 0 if t is None else t.stride(0)  # noqa: E731
+    b = _lib.FmarlBlock(rows[0].shape[0], D, int(groups), _DTYPES[dtype], _DTYPES[x.dtype], int(kind == 'layer'), int(gate_act == 'silu'), int(bool(post_norm)),
+                        int(bool(pre_norm)), float(eps), 0, _ptr(rows[0]), st(rows[0]), _ptr(rows[1]), st(rows[1]), _ptr(rows[2]), st(rows[2]),
+                        *[_ptr(w) for w in weights])
+    return b, rows, weights
+
+
+class _BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias, options):
+        weights = (scale, post_weight, post_bias, pre_weight, pre_bias)
+        b, rows, weights = _block_args(x, branch, gate, weights, *options)
+        dev = x.device
+        y = None if branch is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        h = torch.empty(x.shape, dtype=x.dtype if branch is None else branch.dtype, device=dev) if options[4] else None
+        lib = _lib.load()
+        with torch.cuda.device(dev):
+            _lib.check(lib.fmarl_block_norm(b, _ptr(y), _ptr(h), _stream(dev)), 'fmarl_block_norm')
+        ctx.save_for_backward(x, branch, gate, *weights)
+        ctx.options = options
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        x, branch, gate, *weights = ctx.saved_tensors
+        if dy is None and dh is None:
+            return (None,) * 9
+        need = ctx.needs_input_grad
+        b, rows, weights = _block_args(x, branch, gate, weights, *ctx.options)
+        dev, D = x.device, x.shape[-1]
+        dy, dh = (None if t is None else _last(t.reshape(-1, D)) for t in (dy, dh))
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dbranch, dgate = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (branch, gate))
+        dw = [torch.empty(D, dtype=torch.float32, device=dev) if w is not None and n else None for w, n in zip(weights, need[3:8])]
+        lib = _lib.load()
+        with torch.cuda.device(dev):
+            ws = torch.empty(lib.fmarl_block_norm_workspace(b), dtype=torch.uint8, device=dev)
+            _lib.check(lib.fmarl_block_norm_backward(b, _ptr(dy), 0 if dy is None else dy.stride(0), _ptr(dh), 0 if dh is None else dh.stride(0), dx.data_ptr(),
+                                                     _ptr(dbranch), _ptr(dgate), (C.c_void_p * 5)(*[_ptr(t) for t in dw]), ws.data_ptr(), _stream(dev)),
+                       'fmarl_block_norm_backward')
+        return (dx, dbranch, dgate, *dw, None)
+
+
+def block_norm(x, branch=None, gate=None, scale=None, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, groups=1, kind='rms',
+               gate_act='sigmoid', post_norm=True, pre_norm=True, eps=1e-5):
+    """The end of a residual block and the start of the next one in one pass: ``(y, h)``.
+
+        u = n_groups(branch) post_weight + post_bias,   y = x + scale u act(gate),   h = n(y) pre_weight + pre_bias
+
+    over the last axis of x (..., D), D <= 8192; n is ``'rms'`` (a / sqrt(mean a^2 + eps)) or ``'layer'`` (LayerNorm, what the reference's MLPs use:
+    onpolicy/algorithms/utils/mlp.py:25-40); ``groups`` equal runs of the branch's columns (its heads) are normed by themselves.  branch and gate: x's
+    shape, of one type; x has that type or is float32 (a residual stream kept wide); y has x's type, h the branch's.  scale, weights and
+    biases: float32 (D,).  Whatever is None is left out (factor 1, bias 0).  Without a branch y is x and h = n(x) pre_weight + pre_bias: the first
+    block's start; ``post_norm=False`` takes the branch as it is, ``pre_norm=False`` returns h = None: the last block's end.  h is formed from y before its
+    rounding.  Differentiable in all tensors, once; nothing but the inputs is kept for the backward pass."""
+    _need(x.dim() >= 1 and 1 <= x.shape[-1] <= 8192, 'block_norm: the last axis must hold 1..8192 elements, got %s', tuple(x.shape))
+    D = x.shape[-1]
+    _need(isinstance(groups, int) and 1 <= groups <= 256 and D % groups == 0, 'block_norm: groups must lie in 1..256 and divide %d, got %r', D, groups)
+    _need(branch is not None or (gate is None and scale is None and post_weight is None and post_bias is None),
+          'block_norm: gate, scale and post weights need a branch')
+    _need(post_norm or (post_weight is None and post_bias is None), 'block_norm: post weights need post_norm')
+    _need(pre_norm or (pre_weight is None and pre_bias is None), 'block_norm: pre weights need pre_norm')
+    _need(branch is not None or pre_norm, 'block_norm: without a branch and without pre_norm there is nothing to do')
+    _need(eps >= 0, 'block_norm: eps must not be negative')
+    y, h = _BlockNorm.apply(x, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias, (groups, kind, gate_act, bool(post_norm), bool(pre_norm), eps))
+    return (x if branch is None else y), h

@@ -543,6 +543,30 @@ int fmarl_memory_chunk(const FmarlMemory *m, const FmarlRows *out, float *state_
 int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, const float *d_state, const FmarlRows *d_q, const FmarlRows *d_k,
                                 const FmarlRows *d_v, float *d_log_decay, float *d_state0, void *workspace, void *stream);
 
+/* The end of a residual block and the start of the next one, a row of `dim` at a time, with n(a) = a / sqrt(mean a^2 + eps) (kind 0, rms) or
+ * (a - mean a) / sqrt(var a + eps) (kind 1, layer: the LayerNorm of onpolicy/algorithms/utils/mlp.py:25-40):
+ *     u = n_groups(branch) post_weight + post_bias (branch itself without post_norm);  r = u act(gate);  y = x + scale r;  h = n(y) pre_weight + pre_bias.
+ * n_groups norms each of `groups` equal runs of columns (the heads) by itself; act: 0 sigmoid, 1 silu.  1 <= dim <= 8 192, groups <= 256 divide it.  branch NULL: only h =
+ * n(x) .. is formed; gate, scale, weights and biases NULL: 1, 1, 1, 0.  x and y of x_dtype, the others of dtype; x_dtype is dtype or float32.
+ * Scale, weights and biases are float32 (dim).  Row strides in elements; outputs contiguous (rows, dim). */
+typedef struct FmarlBlock {
+    int64_t rows;
+    int32_t dim, groups, dtype, x_dtype, kind, gate_act, post_norm, pre_norm;
+    float eps;
+    int32_t reserved;
+    const void *x; int64_t x_stride;
+    const void *branch; int64_t branch_stride;
+    const void *gate; int64_t gate_stride;
+    const float *scale, *post_weight, *post_bias, *pre_weight, *pre_bias;
+} FmarlBlock;
+/* y: NULL allowed without branch; h: NULL allowed without pre_norm */
+int fmarl_block_norm(const FmarlBlock *b, void *y, void *h, void *stream);
+/* gradients: d_y, d_h (NULL: zeros) in; d_x, d_branch, d_gate and d_weights[5] = scale, post_weight, post_bias, pre_weight, pre_bias (float32 (dim), each NULL: not wanted) out;
+ * workspace: fmarl_block_norm_workspace(b) bytes */
+size_t fmarl_block_norm_workspace(const FmarlBlock *b);
+int fmarl_block_norm_backward(const FmarlBlock *b, const void *d_y, int64_t d_y_stride, const void *d_h, int64_t d_h_stride, void *d_x, void *d_branch,
+                              void *d_gate, float *const *d_weights, void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
