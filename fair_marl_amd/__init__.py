@@ -12,7 +12,7 @@ from .env_wrappers import (DummyVecEnv, GraphDummyVecEnv, GraphSubprocVecEnv,  #
                            ShareVecEnv, SubprocVecEnv)
 from .MPE_env import GraphMPEEnv, MPEEnv  # noqa: F401
 from .pipeline import PipelinedRollout  # noqa: F401
-from .policy_ops import block_norm, memory_chunk, memory_chunk_backward, memory_step  # noqa: F401
+from .policy_ops import action_log_probs, block_norm, memory_chunk, memory_chunk_backward, memory_step  # noqa: F401
 from .rollout_buffer import DeviceRolloutBuffer  # noqa: F401
 from .sharding import SpanGather, SpanRecord, StepRecord, TrajectoryGather, shard_range  # noqa: F401
 from .spaces import Box, Discrete  # noqa: F401

@@ -92,6 +92,12 @@ class FmarlBlock(C.Structure):
                 ('gate', C.c_void_p), ('gate_stride', C.c_int64)] + [(k, C.c_void_p) for k in ('scale', 'post_weight', 'post_bias', 'pre_weight', 'pre_bias')]
 
 
+class FmarlActions(C.Structure):
+    _fields_ = [('rows', C.c_int64)] + [(k, C.c_int32) for k in ('features', 'actions', 'dtype', 'action_type', 'available_type', 'reserved')] + \
+               [('x', C.c_void_p), ('x_stride', C.c_int64), ('weight', C.c_void_p), ('weight_stride', C.c_int64), ('bias', C.c_void_p), ('action', C.c_void_p),
+                ('available', C.c_void_p), ('available_stride', C.c_int64)]
+
+
 _SIGS = {
     'fmarl_create': (C.c_int, [C.POINTER(FmarlConfig), C.POINTER(C.c_void_p)]),
     'fmarl_destroy': (C.c_int, [C.c_void_p]),
@@ -153,6 +159,9 @@ _SIGS = {
     'fmarl_block_norm_workspace': (C.c_size_t, [C.POINTER(FmarlBlock)]),
     'fmarl_block_norm_backward': (C.c_int, [C.POINTER(FmarlBlock), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
                                             C.c_void_p, C.c_void_p, C.c_void_p]),
+    'fmarl_action_log_probs': (C.c_int, [C.POINTER(FmarlActions), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    'fmarl_action_log_probs_workspace': (C.c_size_t, [C.POINTER(FmarlActions), C.c_int]),
+    'fmarl_action_log_probs_backward': (C.c_int, [C.POINTER(FmarlActions)] + [C.c_void_p] * 9),
 }
 EXPORTS = tuple(_SIGS)
 _lib = None

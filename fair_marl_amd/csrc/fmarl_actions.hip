@@ -1,0 +1,759 @@
+// Log-probability and entropy of discrete actions from the policy's features on gfx950, without keeping the logits:
+//     z = x W^T + bias, -inf where an action is not available;   log_prob = z_a - lse,  entropy = lse - sum_v p_v z_v,  p = e^{z - lse}
+//     dz_v = dlog_prob (1[v = a] - p_v) - dentropy p_v (log p_v + entropy);   dx = dz W,  dW = dz^T x,  dbias = sum dz.
+// Rows that take no part (a negative action: padding; nothing available) give 0, 0 and no gradient.  The logits are formed again for the
+// gradient.  Two ways to do it:
+//   * few actions (five per agent: the env's own): one pass over x per direction, W in LDS, bound by HBM -- actions_few_kernel;
+//   * many (the joint actions of several agents): matrix products of 128 x 128 tiles on the matrix units whose epilogues hold the softmax's running
+//     maximum and sums per tile (forwards) or write dz for a piece of the actions at a time (backwards) -- actions_gemm_kernel.
+#include "fmarl_policy_dev.h"
+
+namespace fmarl {
+namespace policy {
+
+constexpr float kLog2e = 1.44269504f;
+
+struct Actions {
+    int64_t rows;
+    int K, V, act_type, avail_u8, xvec, dxvec;
+    const char *x; int64_t xs;
+    const char *w; int64_t ws;
+    const float *bias;
+    const void *act;
+    const void *avail; int64_t as;
+    float *logp, *ent, *lse;                          // forward outputs; backward: ent and lse are read
+    const float *dlogp, *dent;                        // NULL: zeros
+    char *dx;
+    float *partial;                                   // (workgroups, V * K + V)
+};
+
+// negative: the row takes no part; V and beyond (a NaN too): no such action
+__device__ __forceinline__ int action_of(const Actions &a, int64_t row) {
+    if (a.act_type == 0) {
+        const int64_t v = ((const int64_t *)a.act)[row];
+        return v < 0 ? -1 : v > 0x7fffffff ? 0x7fffffff : (int)v;
+    }
+    if (a.act_type == 1) return ((const int32_t *)a.act)[row];
+    const float f = ((const float *)a.act)[row];
+    return f < 0.f ? -1 : f < 2147483000.f ? (int)f : 0x7fffffff;
+}
+
+// which of the actions v .. v + 3 exist and are available to a row, as bits.  Loads at clamped places and selects, no branch per action: the four loads leave
+// together.  (A branch per action around `z = -inf` was dropped by the compiler, ROCm 7.2: the condition was formed and the assignment left out.)
+__device__ __forceinline__ uint32_t available4(const Actions &a, int64_t row, int v) {
+    const bool real = row < a.rows;
+    uint32_t bits = 0;
+    if (a.avail) {
+        const int64_t at = (real ? row : a.rows - 1) * a.as;
+        if (a.avail_u8) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bits |= ((const uint8_t *)a.avail)[at + min(v + r, a.V - 1)] != 0 ? 1u << r : 0u;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bits |= ((const float *)a.avail)[at + min(v + r, a.V - 1)] != 0.f ? 1u << r : 0u;
+        }
+    } else bits = 15u;
+    const int left = real ? a.V - v : 0;
+    return bits & (left >= 4 ? 15u : left > 0 ? (1u << left) - 1 : 0u);
+}
+
+__device__ __forceinline__ float exp_of(float x) { return exp2_fast(x * kLog2e); }
+
+// what the tiles' (max, sum e^{z - max}, sum (z - max) e^{z - max}) say of a row; top == -inf and !some: nothing available
+__device__ __forceinline__ void row_result(const Actions &a, int64_t row, int act, float top, float s, float t, bool some, float za) {
+    float lp = 0.f, en = 0.f, ls = __builtin_inff();
+    if (act >= 0 && some) {
+        const float l = logf(s);
+        lp = (za - top) - l; en = l - t / s; ls = top + l;
+        if (act >= a.V) { lp = en = __builtin_nanf(""); ls = __builtin_inff(); }   // no such action: seen in the result, without a gradient
+    }
+    a.logp[row] = lp; a.ent[row] = en; a.lse[row] = ls;
+}
+
+// dz of one logit; `in`: the row takes part
+__device__ __forceinline__ float dlogit(float z, bool hot, bool in, float lse, float ent, float dl, float de) {
+    const float lp = z - lse, p = exp_of(lp), d = dl * ((hot ? 1.f : 0.f) - p) - de * (p * (lp + ent));
+    return in && z != -__builtin_inff() ? d : 0.f;
+}
+
+// ---- few actions ------------------------------------------------------------------------------------------------------------
+// 16 rows a wave at a time, logits as z^T = W x^T in the accumulator layout of mfma_f32_16x16x4f32 (row 4 * (lane / 16) + r: action, column lane % 16: row of
+// x), so a row's softmax is over a lane's registers and two lane exchanges, and dx^T = W^T dz^T takes dz^T as it lies.  VT * 16 >= V, KT * 16 >= K.  x is loaded
+// once, in float4s; float32 products for every type.  The gradient of W is summed over a wave's tiles in registers, over the workgroup in LDS and
+// over the workgroups by actions_sums_kernel, always in the same order.
+template <typename T, int VT, int KT, bool BACK>
+__global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
+    constexpr int PK = 16 * KT + 4;
+    __shared__ __align__(16) float lw[16 * VT * PK], lb[16 * VT];
+    __shared__ __align__(16) float lx[BACK ? 4 * 16 * PK : 4], lt[BACK ? 4 * 16 * 20 : 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g4 = (lane >> 4) * 4;
+    for (int i = threadIdx.x; i < 16 * VT * PK; i += 256) {
+        const int v = i / PK, k = i % PK;
+        lw[i] = v < a.V && k < a.K ? (float)((const T *)a.w)[v * a.ws + k] : 0.f;
+    }
+    for (int v = threadIdx.x; v < 16 * VT; v += 256) lb[v] = a.bias && v < a.V ? a.bias[v] : 0.f;
+    __syncthreads();
+    float *wx = lx + (BACK ? wave * 16 * PK : 0), *wt = lt + (BACK ? wave * 16 * 20 : 0);
+    f32x4 accw[BACK ? VT : 1][BACK ? KT : 1], accb[BACK ? VT : 1];
+    if (BACK)
+#pragma unroll
+        for (int j = 0; j < VT; ++j) {
+            accb[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KT; ++k) accw[j][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    const int64_t tiles = (a.rows + 15) / 16, step = (int64_t)gridDim.x * 4;
+    typedef typename Vec4<T>::type V4;
+    V4 next[KT];
+    auto fetch = [&](int64_t tile) {
+        const int64_t row = tile * 16 + c;
+#pragma unroll
+        for (int k = 0; k < KT; ++k) next[k] = load4<T>((const T *)a.x + row * a.xs + 16 * k + g4, row < a.rows ? a.K - 16 * k - g4 : 0, a.xvec);
+    };
+    int64_t tile = (int64_t)blockIdx.x * 4 + wave;
+    if (tile < tiles) fetch(tile);
+    for (; tile < tiles; tile += step) {
+        const int64_t row = tile * 16 + c;
+        const bool real = row < a.rows;
+        f32x4 x[KT], z[VT];
+#pragma unroll
+        for (int k = 0; k < KT; ++k) x[k] = widen(next[k]);
+        const int act = real ? action_of(a, row) : -1;
+        float lse = 0.f, ent = 0.f, dl = 0.f, de = 0.f;
+        if (BACK && real) { lse = a.lse[row]; ent = a.ent[row]; dl = a.dlogp ? a.dlogp[row] : 0.f; de = a.dent ? a.dent[row] : 0.f; }
+        if (tile + step < tiles) fetch(tile + step);
+#pragma unroll
+        for (int j = 0; j < VT; ++j) {
+            z[j] = *(const f32x4 *)(lb + 16 * j + g4);
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                const f32x4 w = *(const f32x4 *)(lw + (16 * j + c) * PK + 16 * k + g4);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[r], x[k][r], z[j], 0, 0, 0);
+            }
+            const uint32_t ok = available4(a, row, 16 * j + g4);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[j][r] = (ok >> r) & 1 ? z[j][r] : -__builtin_inff();
+        }
+        if (!BACK) {
+            float top = -__builtin_inff(), s = 0.f, t = 0.f, za = 0.f;
+            bool some = false;
+#pragma unroll
+            for (int j = 0; j < VT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) { top = fmaxf(top, z[j][r]); some |= !(z[j][r] == -__builtin_inff()); }
+            top = fmaxf(top, __shfl_xor(top, 16)); top = fmaxf(top, __shfl_xor(top, 32));
+#pragma unroll
+            for (int j = 0; j < VT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool none = z[j][r] == -__builtin_inff();
+                    const float d = none ? 0.f : z[j][r] - top, e = none ? 0.f : exp_of(d);
+                    s += e; t += d * e;
+                    za = 16 * j + g4 + r == act ? z[j][r] : za;
+                }
+            int any = some;
+#pragma unroll
+            for (int off = 16; off < 64; off <<= 1) { s += __shfl_xor(s, off); t += __shfl_xor(t, off); za += __shfl_xor(za, off); any |= __shfl_xor(any, off); }
+            if (lane < 16 && real) row_result(a, row, act, top, s, t, any != 0, za);
+        } else {
+            const bool in = real && lse != __builtin_inff();
+#pragma unroll
+            for (int j = 0; j < VT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[j][r] = dlogit(z[j][r], 16 * j + g4 + r == act, in, lse, ent, dl, de);
+            wave_sync();
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                *(f32x4 *)(wx + c * PK + 16 * k + g4) = in ? x[k] : f32x4{0.f, 0.f, 0.f, 0.f};   // what a padded row holds (NaN too) does not reach dW
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < VT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o = __builtin_amdgcn_mfma_f32_16x16x4f32(lw[(16 * j + g4 + r) * PK + 16 * k + c], z[j][r], o, 0, 0, 0);
+                if (real) store4<T>((T *)a.dx + row * a.K + 16 * k + g4, o, a.K - 16 * k - g4, a.dxvec);
+            }
+#pragma unroll
+            for (int j = 0; j < VT; ++j) {
+                accb[j] += z[j];
+                *(f32x4 *)(wt + c * 20 + g4) = z[j];
+                wave_sync();
+                float d[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) d[r] = wt[(g4 + r) * 20 + c];
+#pragma unroll
+                for (int k = 0; k < KT; ++k)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) accw[j][k] = __builtin_amdgcn_mfma_f32_16x16x4f32(d[r], wx[(g4 + r) * PK + 16 * k + c], accw[j][k], 0, 0, 0);
+                wave_sync();
+            }
+        }
+    }
+    if (BACK) {
+        // the four waves' sums one after the other, through W's place in LDS
+        float *mine = a.partial + (int64_t)blockIdx.x * ((int64_t)a.V * a.K + a.V);
+        __syncthreads();
+        for (int w = 0; w < 4; ++w) {
+            if (wave == w) {
+#pragma unroll
+                for (int j = 0; j < VT; ++j) {
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float *p = lw + (16 * j + g4 + r) * PK + 16 * k + c;
+                            *p = w ? *p + accw[j][k][r] : accw[j][k][r];
+                        }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float s = accb[j][r];
+#pragma unroll
+                        for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off);
+                        if (c == 0) lb[16 * j + g4 + r] = w ? lb[16 * j + g4 + r] + s : s;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < a.V * a.K; i += 256) mine[i] = lw[(i / a.K) * PK + i % a.K];
+        for (int v = threadIdx.x; v < a.V; v += 256) mine[(int64_t)a.V * a.K + v] = lb[v];
+    }
+}
+
+// sums over the workgroups: 16 entries a workgroup, 16 threads an entry, float64, a fixed order
+template <typename T>
+__global__ __launch_bounds__(256) void actions_sums_kernel(const float *partial, int parts, int64_t n, int64_t nw, T *dw, float *db) {
+    __shared__ double red[16][17];
+    const int c = threadIdx.x & 15, s = threadIdx.x >> 4;
+    const int64_t i = (int64_t)blockIdx.x * 16 + c;
+    double sum = 0.0;
+    if (i < n) for (int p = s; p < parts; p += 16) sum += (double)partial[p * n + i];
+    red[s][c] = sum;
+    __syncthreads();
+    if (s == 0 && i < n) {
+        for (int k = 1; k < 16; ++k) sum += red[k][c];
+        if (i < nw) dw[i] = (T)(float)sum;
+        else if (db) db[i - nw] = (float)sum;
+    }
+}
+
+// ---- many actions -----------------------------------------------------------------------------------------------------------
+// dst (rows_pad, cols_pad) <- src (rows, cols; row stride), zeros around; or its transpose (cols_pad, rows_pad), with `lse` without the rows that take no
+// part (what they hold, NaN too, does not reach dW).  64 x 64 tiles.
+template <typename T, bool TRANS>
+__global__ __launch_bounds__(256) void actions_pack_kernel(const T *src, int64_t stride, int64_t rows, int cols, T *dst, int64_t rows_pad, int cols_pad, const float *lse) {
+    __shared__ T tile[64][66];
+    const int64_t r0 = (int64_t)blockIdx.x * 64;
+    const int c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int64_t r = r0 + ty + 4 * i;
+        T v = r < rows && c0 + tx < cols ? src[r * stride + c0 + tx] : (T)0.f;
+        if (TRANS && lse && r < rows && lse[r] == __builtin_inff()) v = (T)0.f;
+        if (TRANS) tile[ty + 4 * i][tx] = v;
+        else dst[r * cols_pad + c0 + tx] = v;
+    }
+    if (TRANS) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dst[(int64_t)(c0 + ty + 4 * i) * rows_pad + r0 + tx] = tile[tx][ty + 4 * i];
+    }
+}
+
+enum { kStore = 0, kStats = 1, kDlogits = 2 };
+
+struct Gemm {
+    const char *A, *B;             // rows of lda / ldb elements, 128-byte steps of the contraction contiguous; both padded to whole tiles
+    int64_t lda, ldb;
+    int ta, tb, splits, steps;     // 128-row tiles of A and B, parts of the contraction, 128-byte steps in all
+    float *out; int64_t ldo, split_out;     // kStore: out[split][row of B][row of A]
+    Actions act;                   // kStats, kDlogits: A = W (actions), B = x (rows); row0 / v0: where the tiles begin in them
+    int64_t row0; int v0;
+    float *stats; int64_t stat_stride;      // kStats: (slots of 64 actions, 3, stat_stride)
+    float *za;                     // kStats: the taken action's logit, by row of the chunk
+    char *dz, *dzt; int64_t ldz, ldzt;      // kDlogits: dz (rows, ldz) and its transpose
+    float *db; int64_t ldb_part;   // kDlogits: (tiles of 64 rows, ldb_part) sums over the rows
+    const float *dz_scale;         // kDlogits: NULL or the power of two that dz is stored times
+};
+
+template <typename T> struct Frag;
+template <> struct Frag<__bf16> {
+    typedef bf16x8 type;
+    static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag<_Float16> {
+    typedef f16x8 type;
+    static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag<float> {   // four steps of four: the order of the contraction is free as long as both sides share it
+    typedef f32x4 type;
+    static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// Tiles of 128 x 128, four waves of 64 x 64, steps of 128 bytes along the contraction.  A step's rows go from memory straight to LDS (16 bytes a
+// lane, 64 lanes side by side), the next step's while this one is multiplied.  The LDS image is linear -- the hardware writes lane after lane --
+// so the 16-byte pieces of a row are permuted on the way in by the addresses the lanes load from (piece p of row r lies in place p ^ (r & 7)): the 16 rows that
+// a fragment read touches then spread over the banks.
+template <typename T, int EPI>
+__global__ __launch_bounds__(256) void actions_gemm_kernel(Gemm q) {
+    constexpr int kTile = 128 * 128;                                           // bytes of one operand's step
+    constexpr int PZ = 128 + 16 / (int)sizeof(T);                              // kDlogits: row of the transposing buffer, elements
+    constexpr int kLds = EPI == kDlogits && 128 * PZ * (int)sizeof(T) > 4 * kTile ? 128 * PZ * (int)sizeof(T) : 4 * kTile;
+    __shared__ __align__(128) char lds[kLds];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, g4 = g * 4;
+    // workgroups go round the eight XCDs in turn: each XCD takes a run of neighbouring tiles, whose operands its L2 then holds
+    const int n = q.ta * q.tb * q.splits, per = n / 8, extra = n % 8, xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
+    int id = xcd * per + min(xcd, extra) + nth;
+    const int ia = id % q.ta; id /= q.ta;
+    const int ib = id % q.tb, split = id / q.tb;
+    const int s0 = (int)((int64_t)q.steps * split / q.splits), s1 = (int)((int64_t)q.steps * (split + 1) / q.splits);
+    const char *pa = q.A + (int64_t)ia * 128 * q.lda * sizeof(T), *pb = q.B + (int64_t)ib * 128 * q.ldb * sizeof(T);
+    const int lr = lane >> 3, lp = (lane & 7) ^ lr;                            // row and piece this lane loads of each eight rows
+    auto load = [&](int s, int buf) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = (wave * 4 + i) * 8;
+            const char *ga = pa + ((int64_t)(r + lr) * q.lda) * sizeof(T) + (int64_t)s * 128 + lp * 16;
+            const char *gb = pb + ((int64_t)(r + lr) * q.ldb) * sizeof(T) + (int64_t)s * 128 + lp * 16;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)ga, (__attribute__((address_space(3))) void *)(lds + buf * 2 * kTile + r * 128), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)gb, (__attribute__((address_space(3))) void *)(lds + buf * 2 * kTile + kTile + r * 128), 16, 0, 0);
+        }
+    };
+    const int ra = (wave & 1) * 64, rb = (wave >> 1) * 64;
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (s0 < s1) load(s0, 0);
+    for (int s = s0; s < s1; ++s) {
+        const int buf = (s - s0) & 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's share of the step is in LDS
+        __syncthreads();                                   // everybody's is, and nobody reads the other buffer any more
+        if (s + 1 < s1) load(s + 1, buf ^ 1);
+        const char *la = lds + buf * 2 * kTile, *lb = la + kTile;
+        typedef typename Frag<T>::type F;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            F fa[4], fb[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                fa[i] = *(const F *)(la + (ra + 16 * i + c) * 128 + (((kk * 4 + g) ^ (c & 7)) * 16));
+                fb[i] = *(const F *)(lb + (rb + 16 * i + c) * 128 + (((kk * 4 + g) ^ (c & 7)) * 16));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = Frag<T>::mma(fa[i], fb[j], acc[i][j]);
+        }
+    }
+    if (EPI == kStore) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float *o = q.out + split * q.split_out + ((int64_t)ib * 128 + rb + 16 * j + c) * q.ldo + (int64_t)ia * 128 + ra + g4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(f32x4 *)(o + 16 * i) = acc[i][j];
+        }
+        return;
+    }
+    const Actions &a = q.act;
+    const int vbase = q.v0 + ia * 128 + ra + g4;
+    float bias[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) { const int v = vbase + 16 * i + r; bias[i][r] = a.bias && v < a.V ? a.bias[v] : 0.f; }
+    if (EPI == kDlogits) __syncthreads();   // the operands' LDS is dead from here on
+    const float scale = EPI == kDlogits && q.dz_scale ? *q.dz_scale : 1.f;
+    float dbs[4][4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t m = (int64_t)ib * 128 + rb + 16 * j + c, row = q.row0 + m;   // row of the chunk, row of x
+        const bool real = row < a.rows;
+        const int act = real ? action_of(a, row) : -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t ok = available4(a, row, vbase + 16 * i);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = (ok >> r) & 1 ? acc[i][j][r] + bias[i][r] : -__builtin_inff();
+        }
+        if (EPI == kStats) {
+            float top = -__builtin_inff(), s = 0.f, t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float z = acc[i][j][r];
+                    top = fmaxf(top, z != z ? __builtin_inff() : z);      // a NaN is not passed over: it makes the sums NaN
+                    if (vbase + 16 * i + r == act) q.za[m] = z;
+                }
+            top = fmaxf(top, __shfl_xor(top, 16)); top = fmaxf(top, __shfl_xor(top, 32));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool none = acc[i][j][r] == -__builtin_inff();
+                    const float d = none ? 0.f : acc[i][j][r] - top, e = none ? 0.f : exp_of(d);
+                    s += e; t += d * e;
+                }
+            s += __shfl_xor(s, 16); s += __shfl_xor(s, 32);
+            t += __shfl_xor(t, 16); t += __shfl_xor(t, 32);
+            if (g == 0 && real) {
+                float *o = q.stats + (int64_t)(ia * 2 + (wave & 1)) * 3 * q.stat_stride + m;
+                o[0] = top; o[q.stat_stride] = s; o[2 * q.stat_stride] = t;
+            }
+        } else {
+            float lse = 0.f, ent = 0.f, dl = 0.f, de = 0.f;
+            if (real) { lse = a.lse[row]; ent = a.ent[row]; dl = a.dlogp ? a.dlogp[row] : 0.f; de = a.dent ? a.dent[row] : 0.f; }
+            const bool in = real && lse != __builtin_inff();
+            T *zrow = (T *)lds + (rb + 16 * j + c) * PZ + ra + g4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f32x4 d;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    d[r] = dlogit(acc[i][j][r], vbase + 16 * i + r == act, in, lse, ent, dl, de);
+                    dbs[i][r] += d[r];
+                }
+                store4<T>(zrow + 16 * i, d * scale, 4, true);   // rounded to the operands' type: what the two products below read
+            }
+        }
+    }
+    if (EPI == kDlogits) {
+        // sums over this wave's 64 rows, from the unrounded values
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float s = dbs[i][r];
+#pragma unroll
+                for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off);
+                if (c == 0) q.db[(int64_t)(ib * 2 + (wave >> 1)) * q.ldb_part + ia * 128 + ra + 16 * i + g4 + r] = s;
+            }
+        __syncthreads();
+        constexpr int W = 16 / sizeof(T), kPer = 128 / W;   // elements per 16-byte piece, pieces per row
+        typedef typename Frag<T>::type P;
+        const T *zl = (const T *)lds;
+        for (int i = threadIdx.x; i < 128 * kPer; i += 256) {
+            const int r = i / kPer, p = i % kPer;
+            *(P *)((T *)q.dz + ((int64_t)ib * 128 + r) * q.ldz + ia * 128 + p * W) = *(const P *)(zl + r * PZ + p * W);
+        }
+        for (int i = threadIdx.x; i < 128 * kPer; i += 256) {
+            const int v = i % 128, p = i / 128;   // neighbouring lanes: neighbouring columns of the buffer
+            P o;
+#pragma unroll
+            for (int e = 0; e < W; ++e) o[e] = zl[(p * W + e) * PZ + v];
+            *(P *)((T *)q.dzt + ((int64_t)ia * 128 + v) * q.ldzt + (int64_t)ib * 128 + p * W) = o;
+        }
+    }
+}
+
+// the row's result from its slots of 64 actions
+__global__ __launch_bounds__(256) void actions_join_kernel(Actions a, const float *stats, int64_t stride, int slots, const float *za, int64_t row0, int64_t count) {
+    const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (m >= count) return;
+    float top = -__builtin_inff(), s = 0.f, t = 0.f;
+    bool some = false;
+    for (int i = 0; i < slots; ++i) {
+        const float *p = stats + (int64_t)i * 3 * stride + m;
+        const float t1 = p[0], s1 = p[stride], d1 = p[2 * stride];
+        if (t1 == -__builtin_inff()) continue;
+        some = true;
+        if (t1 > top) {
+            const float f = top == -__builtin_inff() ? 0.f : exp_of(top - t1);
+            t = f == 0.f ? 0.f : f * (t + (top - t1) * s);
+            s *= f; top = t1;
+            s += s1; t += d1;
+        } else {
+            const float f = exp_of(t1 - top);
+            s += f * s1; t += f == 0.f ? 0.f : f * (d1 + (t1 - top) * s1);
+        }
+    }
+    const int act = action_of(a, row0 + m);
+    row_result(a, row0 + m, act, top, s, t, some, act >= 0 && act < a.V ? za[m] : 0.f);
+}
+
+// out[row][col] = scale * sum of the parts (+ what `sum` holds); `sum` takes it while more is to come
+template <typename T>
+__global__ __launch_bounds__(256) void actions_reduce_kernel(const float *part, int64_t split_stride, int splits, int64_t ld, float *sum, int first, int last, T *out,
+                                                             int64_t rows, int cols, const float *inv_scale) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * cols) return;
+    const int64_t r = i / cols, at = r * ld + (i - r * cols);
+    float s = first ? 0.f : sum[at];
+    for (int k = 0; k < splits; ++k) s += part[k * split_stride + at];
+    if (last) out[i] = (T)(inv_scale ? s / *inv_scale : s);
+    else sum[at] = s;
+}
+
+__global__ __launch_bounds__(256) void actions_bias_kernel(const float *part, int64_t ld, int parts, float *db, int n, int add) {
+    __shared__ double red[16][17];
+    const int c = threadIdx.x & 15, s = threadIdx.x >> 4, v = blockIdx.x * 16 + c;
+    double sum = 0.0;
+    if (v < n) for (int p = s; p < parts; p += 16) sum += (double)part[p * ld + v];
+    red[s][c] = sum;
+    __syncthreads();
+    if (s == 0 && v < n) {
+        for (int k = 1; k < 16; ++k) sum += red[k][c];
+        db[v] = (float)(add ? (double)db[v] + sum : sum);
+    }
+}
+
+// float16 operands: dz is stored times the power of two that brings the largest |dlog_prob| + |dentropy| (1 + log V) to 2^12, so that small upstream gradients
+// (a mean over a million rows) do not fall below float16's smallest numbers; the products are divided by it again.  One workgroup.
+__global__ __launch_bounds__(1024) void actions_scale_kernel(Actions a, float *scale) {
+    __shared__ float red[16];
+    const float lv = 1.f + logf((float)a.V);
+    float m = 0.f;
+    for (int64_t r = threadIdx.x; r < a.rows; r += 1024) {
+        if (a.lse[r] == __builtin_inff()) continue;
+        const float v = (a.dlogp ? fabsf(a.dlogp[r]) : 0.f) + (a.dent ? fabsf(a.dent[r]) : 0.f) * lv;
+        if (v < __builtin_inff()) m = fmaxf(m, v);
+    }
+    for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) m = fmaxf(m, red[w]);
+        int e = 0;
+        if (m > 0.f) (void)frexpf(m, &e);
+        *scale = ldexpf(1.f, min(120, max(-120, 12 - e)));
+    }
+}
+
+}  // namespace policy
+}  // namespace fmarl
+
+using namespace fmarl;
+using namespace fmarl::policy;
+
+namespace {
+
+int actions_check(const FmarlActions *a, const char *who) {
+    if (!a) return policy_fail(FMARL_EINVAL, "%s: null argument", who);
+    if (a->rows < 0 || a->rows > (1ll << 36)) return policy_fail(FMARL_EINVAL, "%s: bad number of rows", who);
+    if (a->features < 1 || a->features > 16384) return policy_fail(FMARL_EINVAL, "%s: features must lie in 1..16384", who);
+    if (a->actions < 1 || a->actions > (1 << 20)) return policy_fail(FMARL_EINVAL, "%s: actions must lie in 1..1048576", who);
+    if (a->dtype < FMARL_T_F32 || a->dtype > FMARL_T_F16) return policy_fail(FMARL_EINVAL, "%s: unknown dtype", who);
+    if (a->action_type < 0 || a->action_type > 2 || a->available_type < 0 || a->available_type > 1) return policy_fail(FMARL_EINVAL, "%s: unknown action_type or available_type", who);
+    if (a->rows > 0 && (!a->x || !a->weight || !a->action)) return policy_fail(FMARL_EINVAL, "%s: null argument", who);
+    return FMARL_OK;
+}
+
+Actions actions_args(const FmarlActions *a) {
+    Actions s = {};
+    const int e = elem_bytes(a->dtype);
+    s.rows = a->rows; s.K = a->features; s.V = a->actions; s.act_type = a->action_type; s.avail_u8 = a->available_type;
+    s.x = (const char *)a->x; s.xs = a->x_stride; s.w = (const char *)a->weight; s.ws = a->weight_stride; s.bias = a->bias;
+    s.act = a->action; s.avail = a->available; s.as = a->available_stride;
+    s.xvec = (a->features & 3) == 0 && (a->x_stride & 3) == 0 && ((uintptr_t)a->x & (4 * e - 1)) == 0;
+    return s;
+}
+
+// Few actions: the tiles of W's gradient (16 x 16, four registers a lane each) have to stay in registers beside the operands, and padding V to 16 must not cost
+// more than the products of the other way
+bool actions_few(const FmarlActions *a) {
+    const int vt = (a->actions + 15) / 16, kt = (a->features + 15) / 16;
+    return vt <= 4 && kt <= 16 && (vt <= 1 ? 1 : vt <= 2 ? 2 : 4) * (kt <= 2 ? 2 : kt <= 4 ? 4 : kt <= 8 ? 8 : 16) <= 16;
+}
+
+int few_workgroups(const FmarlActions *a) {   // four waves of 16 rows each; 1 024 of them fill the chip, and their partial sums stay small
+    const int64_t n = (a->rows + 63) / 64;
+    return (int)(n < 1 ? 1 : n < 1024 ? n : 1024);
+}
+
+template <typename T, bool BACK>
+int launch_few(const Actions &s, int blocks, hipStream_t st) {
+    const int vt = (s.V + 15) / 16, kt = (s.K + 15) / 16;
+#define FMARL_FEW(VT, KT) hipLaunchKernelGGL((actions_few_kernel<T, VT, KT, BACK>), dim3(blocks), dim3(256), 0, st, s)
+    if (vt <= 1) { if (kt <= 2) FMARL_FEW(1, 2); else if (kt <= 4) FMARL_FEW(1, 4); else if (kt <= 8) FMARL_FEW(1, 8); else FMARL_FEW(1, 16); }
+    else if (vt <= 2) { if (kt <= 2) FMARL_FEW(2, 2); else if (kt <= 4) FMARL_FEW(2, 4); else FMARL_FEW(2, 8); }
+    else { if (kt <= 2) FMARL_FEW(4, 2); else FMARL_FEW(4, 4); }
+#undef FMARL_FEW
+    HIP_OK(hipGetLastError());
+    return FMARL_OK;
+}
+
+template <bool BACK>
+int launch_few_t(int dtype, const Actions &s, int blocks, hipStream_t st) {
+    return dtype == FMARL_T_F32 ? launch_few<float, BACK>(s, blocks, st) : dtype == FMARL_T_BF16 ? launch_few<__bf16, BACK>(s, blocks, st) : launch_few<_Float16, BACK>(s, blocks, st);
+}
+
+int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+// The sizes of the way for many actions.  Rows go in chunks and (backwards) actions in pieces, so that what is kept of a chunk -- three floats per row and 64 actions,
+// or dz and its transpose -- stays within 256 MB, the size of the last-level cache.
+struct Plan {
+    int64_t Kp, Vp, Mc, P;        // padded features and actions, rows of a chunk, actions of a piece
+    int split_x, split_w;         // parts of the contraction of dx and dW
+    size_t xp, wp, stats, za, xt, wt, dz, dzt, out, sumx, sumw, db, scale, total;
+};
+
+Plan actions_plan(const FmarlActions *a, bool backward) {
+    Plan p = {};
+    const int64_t e = elem_bytes(a->dtype), M = up(a->rows, 128), budget = 256ll << 20;
+    p.Kp = up(a->features, 128); p.Vp = up(a->actions, 128);
+    const int64_t keep = backward ? 2 * e * 128 : 12 * (p.Vp / 64);   // bytes per row that a chunk cannot do without
+    int64_t mc = budget / keep / 128 * 128;
+    if (mc > 65536) mc = 65536;
+    if (mc < 1024) mc = 1024;
+    p.Mc = M < mc ? M : mc;
+    p.P = budget / (2 * e * p.Mc) / 128 * 128;
+    if (p.P < 128) p.P = 128;
+    if (p.P > p.Vp) p.P = p.Vp;
+    const int64_t tx = (p.Mc / 128) * (p.Kp / 128), tw = (p.P / 128) * (p.Kp / 128), per = 128 / e;
+    auto parts = [&](int64_t tiles, int64_t steps) {   // two workgroups per CU, none with fewer than eight steps
+        int64_t n = (512 + tiles - 1) / tiles;
+        if (n > steps / 8) n = steps / 8;
+        return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+    };
+    p.split_x = parts(tx, p.P / per); p.split_w = parts(tw, p.Mc / per);
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t at = off; off += up256(bytes); return at; };
+    p.xp = take(e * p.Mc * p.Kp); p.wp = take(e * p.Vp * p.Kp);
+    if (!backward) { p.stats = take(12 * (p.Vp / 64) * p.Mc); p.za = take(4 * p.Mc); }
+    else {
+        p.xt = take(e * p.Mc * p.Kp); p.wt = take(e * p.Vp * p.Kp);
+        p.dz = take(e * p.Mc * p.P); p.dzt = take(e * p.Mc * p.P);
+        const int64_t ox = p.split_x * p.Mc * p.Kp, ow = p.split_w * p.P * p.Kp;
+        p.out = take(4 * (ox > ow ? ox : ow));
+        p.sumx = take(p.P < p.Vp ? 4 * p.Mc * p.Kp : 0);
+        p.sumw = take(p.Mc < M ? 4 * p.Vp * p.Kp : 0);
+        p.db = take(4 * (p.Mc / 64) * p.P);
+        p.scale = take(4);
+    }
+    p.total = off;
+    return p;
+}
+
+template <typename T, bool TRANS>
+void pack(const T *src, int64_t stride, int64_t rows, int cols, T *dst, int64_t rows_pad, int64_t cols_pad, const float *lse, hipStream_t st) {
+    hipLaunchKernelGGL((actions_pack_kernel<T, TRANS>), dim3((unsigned)(rows_pad / 64), (unsigned)(cols_pad / 64)), dim3(256), 0, st, src, stride, rows, cols, dst,
+                       rows_pad, (int)cols_pad, lse);
+}
+
+template <typename T, int EPI>
+void gemm(const Gemm &q, hipStream_t st) {
+    hipLaunchKernelGGL((actions_gemm_kernel<T, EPI>), dim3((unsigned)(q.ta * q.tb * q.splits)), dim3(256), 0, st, q);
+}
+
+template <typename T>
+int many_forward(const Actions &s, const Plan &p, char *base, hipStream_t st) {
+    const int64_t per = 128 / (int64_t)sizeof(T);
+    T *xp = (T *)(base + p.xp), *wp = (T *)(base + p.wp);
+    pack<T, false>((const T *)s.w, s.ws, s.V, s.K, wp, p.Vp, p.Kp, nullptr, st);
+    for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
+        const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 128);
+        pack<T, false>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xp, mp, p.Kp, nullptr, st);
+        Gemm q = {};
+        q.A = (const char *)wp; q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(p.Vp / 128); q.tb = (int)(mp / 128); q.splits = 1; q.steps = (int)(p.Kp / per);
+        q.act = s; q.row0 = r0; q.stats = (float *)(base + p.stats); q.stat_stride = p.Mc; q.za = (float *)(base + p.za);
+        gemm<T, kStats>(q, st);
+        hipLaunchKernelGGL(actions_join_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, st, s, (const float *)q.stats, p.Mc, (int)(p.Vp / 64), (const float *)q.za, r0, m);
+        HIP_OK(hipGetLastError());
+    }
+    return FMARL_OK;
+}
+
+template <typename T>
+void reduce(const float *part, int64_t split_stride, int splits, int64_t ld, float *sum, bool first, bool last, T *out, int64_t rows, int cols, const float *scale, hipStream_t st) {
+    hipLaunchKernelGGL((actions_reduce_kernel<T>), dim3((unsigned)((rows * cols + 255) / 256)), dim3(256), 0, st, part, split_stride, splits, ld, sum, (int)first, (int)last, out, rows,
+                       cols, scale);
+}
+
+template <typename T>
+int many_backward(const Actions &s, const Plan &p, T *dx, T *dw, float *db, char *base, hipStream_t st) {
+    const int64_t per = 128 / (int64_t)sizeof(T);
+    T *xp = (T *)(base + p.xp), *wp = (T *)(base + p.wp), *xt = (T *)(base + p.xt), *wt = (T *)(base + p.wt), *dz = (T *)(base + p.dz), *dzt = (T *)(base + p.dzt);
+    float *out = (float *)(base + p.out), *sumx = (float *)(base + p.sumx), *sumw = (float *)(base + p.sumw), *dbp = (float *)(base + p.db);
+    const float *scale = nullptr;
+    if (sizeof(T) == 2 && (float)(T)1e-30f == 0.f) {   // float16
+        scale = (const float *)(base + p.scale);
+        hipLaunchKernelGGL(actions_scale_kernel, dim3(1), dim3(1024), 0, st, s, (float *)(base + p.scale));
+    }
+    pack<T, false>((const T *)s.w, s.ws, s.V, s.K, wp, p.Vp, p.Kp, nullptr, st);
+    pack<T, true>((const T *)s.w, s.ws, s.V, s.K, wt, p.Vp, p.Kp, nullptr, st);
+    for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
+        const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 128);
+        pack<T, false>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xp, mp, p.Kp, nullptr, st);
+        pack<T, true>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xt, mp, p.Kp, s.lse + r0, st);
+        for (int64_t v0 = 0; v0 < p.Vp; v0 += p.P) {
+            const int64_t n = p.Vp - v0 < p.P ? p.Vp - v0 : p.P, nv = s.V - v0 < n ? s.V - v0 : n;   // of this piece: padded and real actions
+            Gemm q = {};
+            q.A = (const char *)(wp + v0 * p.Kp); q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(n / 128); q.tb = (int)(mp / 128); q.splits = 1; q.steps = (int)(p.Kp / per);
+            q.act = s; q.row0 = r0; q.v0 = (int)v0; q.dz = (char *)dz; q.dzt = (char *)dzt; q.ldz = p.P; q.ldzt = p.Mc; q.db = dbp; q.ldb_part = p.P; q.dz_scale = scale;
+            gemm<T, kDlogits>(q, st);
+            if (db) hipLaunchKernelGGL(actions_bias_kernel, dim3((unsigned)((nv + 15) / 16)), dim3(256), 0, st, (const float *)dbp, p.P, (int)(mp / 64), db + v0, (int)nv, (int)(r0 > 0));
+            q = Gemm{};   // dx += dz W: rows of W^T (features) against rows of dz
+            q.A = (const char *)(wt + v0); q.lda = p.Vp; q.B = (const char *)dz; q.ldb = p.P; q.ta = (int)(p.Kp / 128); q.tb = (int)(mp / 128); q.steps = (int)(n / per);
+            q.splits = p.split_x < q.steps ? p.split_x : q.steps; q.out = out; q.ldo = p.Kp; q.split_out = p.Mc * p.Kp;
+            gemm<T, kStore>(q, st);
+            reduce<T>(out, q.split_out, q.splits, p.Kp, sumx, v0 == 0, v0 + n >= p.Vp, dx + r0 * s.K, m, s.K, scale, st);
+            q.A = (const char *)xt; q.lda = mp; q.B = (const char *)dzt; q.ldb = p.Mc; q.tb = (int)(n / 128); q.steps = (int)(mp / per);   // dW: rows of x^T against rows of dz^T
+            q.splits = p.split_w < q.steps ? p.split_w : q.steps; q.split_out = p.P * p.Kp;
+            gemm<T, kStore>(q, st);
+            reduce<T>(out, q.split_out, q.splits, p.Kp, sumw + v0 * p.Kp, r0 == 0, r0 + m >= s.rows, dw + v0 * s.K, nv, s.K, scale, st);
+            HIP_OK(hipGetLastError());
+        }
+    }
+    return FMARL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fmarl_action_log_probs_workspace(const FmarlActions *a, int backward) {
+    if (actions_check(a, "fmarl_action_log_probs_workspace")) return 0;
+    if (actions_few(a)) return backward ? up256((size_t)few_workgroups(a) * ((size_t)a->actions * a->features + a->actions) * 4) : 256;
+    return actions_plan(a, backward != 0).total;
+}
+
+int fmarl_action_log_probs(const FmarlActions *a, float *log_probs, float *entropy, float *lse, void *workspace, void *stream) {
+    if (int rc = actions_check(a, "fmarl_action_log_probs")) return rc;
+    if (a->rows == 0) return FMARL_OK;
+    if (!log_probs || !entropy || !lse || !workspace) return policy_fail(FMARL_EINVAL, "fmarl_action_log_probs: null argument");
+    hipStream_t st = (hipStream_t)stream;
+    Actions s = actions_args(a);
+    s.logp = log_probs; s.ent = entropy; s.lse = lse;
+    if (actions_few(a)) {
+        const int64_t n = (a->rows + 63) / 64;
+        return launch_few_t<false>(a->dtype, s, (int)(n < 2048 ? n : 2048), st);
+    }
+    const Plan p = actions_plan(a, false);
+    return a->dtype == FMARL_T_F32 ? many_forward<float>(s, p, (char *)workspace, st)
+         : a->dtype == FMARL_T_BF16 ? many_forward<__bf16>(s, p, (char *)workspace, st) : many_forward<_Float16>(s, p, (char *)workspace, st);
+}
+
+int fmarl_action_log_probs_backward(const FmarlActions *a, const float *entropy, const float *lse, const float *d_log_probs, const float *d_entropy,
+                                    void *d_x, void *d_weight, float *d_bias, void *workspace, void *stream) {
+    if (int rc = actions_check(a, "fmarl_action_log_probs_backward")) return rc;
+    if (a->rows < 1) return policy_fail(FMARL_EINVAL, "fmarl_action_log_probs_backward: rows must be positive");
+    if (!entropy || !lse || !d_x || !d_weight || !workspace) return policy_fail(FMARL_EINVAL, "fmarl_action_log_probs_backward: null argument");
+    hipStream_t st = (hipStream_t)stream;
+    Actions s = actions_args(a);
+    s.ent = (float *)entropy; s.lse = (float *)lse; s.dlogp = d_log_probs; s.dent = d_entropy; s.dx = (char *)d_x; s.partial = (float *)workspace;
+    s.dxvec = (a->features & 3) == 0 && ((uintptr_t)d_x & (4 * elem_bytes(a->dtype) - 1)) == 0;
+    if (actions_few(a)) {
+        const int parts = few_workgroups(a);
+        if (int rc = launch_few_t<true>(a->dtype, s, parts, st)) return rc;
+        const int64_t nw = (int64_t)a->actions * a->features, n = nw + a->actions;
+        const dim3 grid((unsigned)((n + 15) / 16));
+        if (a->dtype == FMARL_T_F32) hipLaunchKernelGGL((actions_sums_kernel<float>), grid, dim3(256), 0, st, (const float *)workspace, parts, n, nw, (float *)d_weight, d_bias);
+        else if (a->dtype == FMARL_T_BF16) hipLaunchKernelGGL((actions_sums_kernel<__bf16>), grid, dim3(256), 0, st, (const float *)workspace, parts, n, nw, (__bf16 *)d_weight, d_bias);
+        else hipLaunchKernelGGL((actions_sums_kernel<_Float16>), grid, dim3(256), 0, st, (const float *)workspace, parts, n, nw, (_Float16 *)d_weight, d_bias);
+        HIP_OK(hipGetLastError());
+        return FMARL_OK;
+    }
+    const Plan p = actions_plan(a, true);
+    char *ws = (char *)workspace;
+    return a->dtype == FMARL_T_F32 ? many_backward<float>(s, p, (float *)d_x, (float *)d_weight, d_bias, ws, st)
+         : a->dtype == FMARL_T_BF16 ? many_backward<__bf16>(s, p, (__bf16 *)d_x, (__bf16 *)d_weight, d_bias, ws, st)
+                                    : many_backward<_Float16>(s, p, (_Float16 *)d_x, (_Float16 *)d_weight, d_bias, ws, st);
+}
+
+}  // extern "C"

@@ -4,6 +4,8 @@
   ``rnn_states`` and ``masks`` (onpolicy/algorithms/utils/rnn.py:26-84: one step in the rollout, chunks of ``data_chunk_length`` with the
   episodes' ends inside in the update), these carry a matrix per head through the same slots.
 * ``block_norm``: the end of a residual block and the start of the next in one pass -- norm of the branch, gate, residual scale, residual, norm.
+* ``action_log_probs``: log-probability and entropy of the taken actions straight from the features (the reference's ``ACTLayer.evaluate_actions``,
+  onpolicy/algorithms/utils/act.py:120-177), for the env's five actions as for the joint actions of several agents; no logits are kept.
 
 All run on the current stream of their tensors' device, take any strides as long as the last axis is contiguous (a tensor whose last axis is
 not is copied), read nothing back and are capturable in a graph.  Gradients come through torch.autograd; ``memory_chunk_backward`` is the
@@ -267,3 +269,83 @@ def block_norm(x, branch=None, gate=None, scale=None, post_weight=None, post_bia
     _need(eps >= 0, 'block_norm: eps must not be negative')
     y, h = _BlockNorm.apply(x, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias, (groups, kind, gate_act, bool(post_norm), bool(pre_norm), eps))
     return (x if branch is None else y), h
+
+
+# ---- action_log_probs -----------------------------------------------------------------------------------------------------------
+_ACTION_TYPES = {torch.int64: 0, torch.int32: 1, torch.float32: 2}
+
+
+def _action_args(features, weight, bias, actions, available):
+    """(FmarlActions, the laid out tensors, which have to live until the launch)."""
+    _same_device('action_log_probs', features, weight, bias, actions, available)
+    K, V = weight.shape[1], weight.shape[0]
+    _need(features.dtype in _DTYPES and weight.dtype == features.dtype, 'action_log_probs: features and weight must be of one type out of float32, bfloat16, float16')
+    _need(bias is None or (tuple(bias.shape) == (V,) and bias.dtype == torch.float32), 'action_log_probs: bias must be (%d,)', V)
+    x, w = _last(features.reshape(-1, K)), _last(weight)
+    M = x.shape[0]
+    _need(actions.dtype in _ACTION_TYPES and actions.numel() == M, 'action_log_probs: actions must be int64, int32 or float32 with %d entries, got %s %s', M,
+          actions.dtype, tuple(actions.shape))
+    actions = actions.reshape(M).contiguous()
+    if available is not None:
+        _need(available.dtype in (torch.float32, torch.bool, torch.uint8) and available.numel() == M * V and available.shape[-1] == V,
+              'action_log_probs: available_actions must be float32, bool or uint8 (..., %d) with %d entries, got %s %s', V, M * V, available.dtype, tuple(available.shape))
+        available = _last(available.reshape(M, V))
+    if bias is not None:
+        bias = bias.contiguous()
+    a = _lib.FmarlActions(M, K, V, _DTYPES[x.dtype], _ACTION_TYPES[actions.dtype], int(available is not None and available.dtype != torch.float32), 0, x.data_ptr(),
+                          x.stride(0), w.data_ptr(), w.stride(0), _ptr(bias), actions.data_ptr(), _ptr(available), 0 if available is None else available.stride(0))
+    return a, (x, w, bias, actions, available)
+
+
+class _ActionLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, features, weight, bias, actions, available):
+        a, keep = _action_args(features, weight, bias, actions, available)
+        dev, shape = features.device, features.shape[:-1]
+        log_probs, entropy, lse = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3))
+        lib = _lib.load()
+        with torch.cuda.device(dev):
+            ws = torch.empty(lib.fmarl_action_log_probs_workspace(a, 0), dtype=torch.uint8, device=dev)
+            _lib.check(lib.fmarl_action_log_probs(a, log_probs.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ws.data_ptr(), _stream(dev)), 'fmarl_action_log_probs')
+        ctx.save_for_backward(features, weight, bias, actions, available, entropy, lse)
+        ctx.set_materialize_grads(False)
+        return log_probs, entropy
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_log_probs, d_entropy):
+        features, weight, bias, actions, available, entropy, lse = ctx.saved_tensors
+        if d_log_probs is None and d_entropy is None:
+            return (None,) * 5
+        a, keep = _action_args(features, weight, bias, actions, available)
+        dev = features.device
+        dx, dw = torch.empty(features.shape, dtype=features.dtype, device=dev), torch.empty(weight.shape, dtype=weight.dtype, device=dev)
+        db = torch.empty(bias.shape, dtype=torch.float32, device=dev) if bias is not None and ctx.needs_input_grad[2] else None
+        if a.rows == 0:
+            return dx, dw.zero_(), None if db is None else db.zero_(), None, None
+        dl, de = (None if t is None else t.contiguous() for t in (d_log_probs, d_entropy))
+        lib = _lib.load()
+        with torch.cuda.device(dev):
+            ws = torch.empty(lib.fmarl_action_log_probs_workspace(a, 1), dtype=torch.uint8, device=dev)
+            _lib.check(lib.fmarl_action_log_probs_backward(a, entropy.data_ptr(), lse.data_ptr(), _ptr(dl), _ptr(de), dx.data_ptr(), dw.data_ptr(), _ptr(db), ws.data_ptr(),
+                                                           _stream(dev)), 'fmarl_action_log_probs_backward')
+        return dx, dw, db, None, None
+
+
+def action_log_probs(features, weight, bias, actions, available_actions=None):
+    """Log-probability and entropy of discrete actions: ``(log_probs, entropy)``, float32, of the features' leading shape.
+
+        z = features weight^T + bias, -inf where available_actions == 0;   log_probs = z_action - lse(z),   entropy = -sum_v p_v log p_v
+
+    features (..., K), weight (V, K) of one type (float32, bfloat16, float16), K <= 16 384, V <= 1 048 576; bias (V,) float32 or the weight's type, or None; actions:
+    one per row, int64, int32 or float32 (the buffer's ``actions``; a trailing 1 is fine); available_actions: (..., V) float32, bool or uint8, or None.  A row with a
+    negative action (padding) or nothing available takes no part: 0, 0 and no gradient.  An unavailable action has log-probability
+    -inf, one that does not exist (>= V) NaN (and no gradient).  The logits are never stored: for many actions the softmax runs over pieces of them, and they
+    are formed again for the gradient.  Differentiable in features, weight and bias, once.  Half precision operands: products are exact, sums float32; the
+    gradient's dz is rounded to the operands' type before its two products."""
+    _need(weight.dim() == 2 and features.dim() >= 1 and features.shape[-1] == weight.shape[1] and 1 <= weight.shape[1] <= 16384 and 1 <= weight.shape[0] <= 1 << 20,
+          'action_log_probs: features (..., K) and weight (V, K) with K in 1..16384, V in 1..1048576, got %s, %s', tuple(features.shape), tuple(weight.shape))
+    if bias is not None and bias.dtype != torch.float32:
+        _need(bias.dtype == weight.dtype, 'action_log_probs: bias must be float32 or of the weight\'s type')
+        bias = bias.float()
+    return _ActionLogProbs.apply(features, weight, bias, actions, available_actions)

@@ -567,6 +567,28 @@ size_t fmarl_block_norm_workspace(const FmarlBlock *b);
 int fmarl_block_norm_backward(const FmarlBlock *b, const void *d_y, int64_t d_y_stride, const void *d_h, int64_t d_h_stride, void *d_x, void *d_branch,
                               void *d_gate, float *const *d_weights, void *workspace, void *stream);
 
+/* Log-probability and entropy of discrete actions from the policy's features, without keeping the logits (what ACTLayer.evaluate_actions forms with a Linear and a
+ * masked Categorical, onpolicy/algorithms/utils/act.py:120-177, distributions.py:15-37):
+ *     z = x W^T + bias, -inf where available == 0;  log_prob = z_action - lse(z);  entropy = -sum_v p_v log p_v.
+ * x (rows, features) by its row stride, weight (actions, features) by its row stride, of dtype; bias float32 (actions) or NULL; action (rows) of action_type 0 int64, 1 int32, 2 float32 (the
+ * buffer's); available (rows, actions) by its row stride, 0 float32, 1 bytes, or NULL.  A row with a negative action or nothing available takes no part: 0, 0, no gradient.  An action that
+ * does not exist (>= actions) gives NaN, without a gradient; one that is not available -inf.  log_prob, entropy, lse: float32 (rows); lse, +inf where
+ * a row takes no part, is what the backward call wants back beside entropy. */
+typedef struct FmarlActions {
+    int64_t rows;
+    int32_t features, actions, dtype, action_type, available_type, reserved;
+    const void *x; int64_t x_stride;
+    const void *weight; int64_t weight_stride;
+    const float *bias;
+    const void *action;
+    const void *available; int64_t available_stride;
+} FmarlActions;
+size_t fmarl_action_log_probs_workspace(const FmarlActions *a, int backward);
+int fmarl_action_log_probs(const FmarlActions *a, float *log_probs, float *entropy, float *lse, void *workspace, void *stream);
+/* d_log_probs, d_entropy (rows; NULL: zeros) in; d_x (rows, features), d_weight (actions, features) contiguous of dtype, d_bias float32 (NULL: not wanted) out; rows >= 1 */
+int fmarl_action_log_probs_backward(const FmarlActions *a, const float *entropy, const float *lse, const float *d_log_probs, const float *d_entropy,
+                                    void *d_x, void *d_weight, float *d_bias, void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
