@@ -462,7 +462,8 @@ int memory_check(const FmarlMemory *m, const char *who) {
     if (m->dtype < FMARL_T_F32 || m->dtype > FMARL_T_F16) return policy_fail(FMARL_EINVAL, "%s: unknown dtype", who);
     if (m->shared_decay < 0 || m->shared_decay > 1 || (m->shared_decay && (m->decay_stride_l || m->decay_stride_b)))
         return policy_fail(FMARL_EINVAL, "%s: shared_decay must be 0, or 1 with strides of 0 over tokens and sequences", who);
-    if (m->B > (1ll << 31) / m->H || m->L > (1ll << 40)) return policy_fail(FMARL_EINVAL, "%s: too many sequences or tokens", who);
+    // a wave per head and slice: a launch holds fewer than 2^32 threads
+    if (m->B >= (1ll << 26) / m->H || m->L > (1ll << 40)) return policy_fail(FMARL_EINVAL, "%s: too many sequences (B H must stay below 2^26) or tokens", who);
     if (m->L > 0 && m->B > 0 && (!m->q.data || !m->k.data || !m->v.data || !m->log_decay)) return policy_fail(FMARL_EINVAL, "%s: null argument", who);
     return FMARL_OK;
 }
@@ -531,7 +532,7 @@ void launch_walk_t(const Walk &w, unsigned blocks, hipStream_t st) {
 int launch_walk(Walk w, int dtype, hipStream_t st) {
     w.slices = slices_of(w.dy, w.dz);
     const int64_t blocks = (w.B * w.H * w.nseg * w.slices + 3) / 4;
-    if (blocks > 0x7fffffff) return policy_fail(FMARL_EINVAL, "memory: too many sequences");
+    if (blocks > 0xffffff) return policy_fail(FMARL_EINVAL, "memory: too many sequences");
     if (dtype == FMARL_T_F32) launch_walk_t<float>(w, (unsigned)blocks, st);
     else if (dtype == FMARL_T_BF16) launch_walk_t<__bf16>(w, (unsigned)blocks, st);
     else launch_walk_t<_Float16>(w, (unsigned)blocks, st);
@@ -560,7 +561,6 @@ int segment_states(const FmarlMemory *m, const FmarlRows &y, const FmarlRows &z,
     w.state_out = seg_states; w.o_y = m->dv; w.o_z = 1; w.seg_state_out = heads * elems; w.seg_decay = seg_decay;
     if (int rc = launch_walk(w, m->dtype, st)) return rc;
     const int64_t blocks = (heads * elems + 255) / 256;
-    if (blocks > 0x7fffffff) return policy_fail(FMARL_EINVAL, "memory: too many sequences");
     hipLaunchKernelGGL(memory_join_kernel, dim3((unsigned)blocks), dim3(256), 0, st, seg_states, (const float *)seg_decay, init, last, heads, (int)elems, w.nseg, (int)reverse);
     HIP_OK(hipGetLastError());
     return FMARL_OK;
@@ -582,7 +582,6 @@ int fmarl_memory_step(const FmarlMemory *m, const FmarlRows *out, float *state_o
     s.state = m->state; s.state_out = state_out; s.B = m->B; s.H = m->H; s.dk = m->dk; s.dv = m->dv; s.scale = m->scale;
     const bool vec = (m->dv & 3) == 0 && (((uintptr_t)m->state | (uintptr_t)state_out) & 15) == 0;
     const int64_t blocks = (m->B * m->H + 3) / 4;
-    if (blocks > 0x7fffffff) return policy_fail(FMARL_EINVAL, "fmarl_memory_step: too many sequences");
     hipStream_t st = (hipStream_t)stream;
 #define FMARL_STEP(T) do { if (vec) hipLaunchKernelGGL((memory_step_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, s); \
                            else hipLaunchKernelGGL((memory_step_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, st, s); } while (0)

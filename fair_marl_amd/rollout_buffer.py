@@ -27,7 +27,7 @@ import ctypes as C
 
 import torch
 
-from . import _lib
+from . import _lib, policy_ops
 
 
 class DeviceRolloutBuffer(object):
@@ -182,6 +182,38 @@ class DeviceRolloutBuffer(object):
                          (self.available_actions, available_actions)):
             if src is not None:
                 dst[t + 1].copy_(src.reshape(dst[t + 1].shape))
+
+    def memory_step(self, t, q, k, v, log_decay, scale=None, critic=False):
+        """The policy's memory at buffer step t (``policy_ops.memory_step``): one token per (env, agent) from the recurrent states and masks of slot t,
+        the new states straight into slot t + 1 (no copy: ``insert_policy`` then gets no states).  q, k (n, N, H, dk), v (n, N, H, dv) with
+        H dk dv = recurrent_N hidden_size; log_decay (H,) or (n, N, H).  Returns out (n, N, H, dv).  ``critic``: the critic's states."""
+        self._need_policy()
+        if not 0 <= t < self.T:
+            raise ValueError('memory_step: buffer step %d of %d' % (t, self.T))
+        states = self.rnn_states_critic if critic else self.rnn_states
+        n, N = self.engine.n_envs, self.engine.cfg.N
+        if q.dim() != 4 or v.dim() != 4 or q.shape[:2] != (n, N) or q.shape[2] * q.shape[3] * v.shape[3] != states[t, 0, 0].numel():
+            raise ValueError('memory_step: q, k (%d, %d, H, dk), v (.., dv) with H dk dv = %d (recurrent_N * hidden_size of attach_policy), got %s, %s'
+                             % (n, N, states[t, 0, 0].numel(), tuple(q.shape), tuple(v.shape)))
+        flat = lambda x: x.reshape((n * N,) + x.shape[2:])  # noqa: E731
+        out, _ = policy_ops.memory_step(flat(q), flat(k), flat(v), log_decay if log_decay.dim() == 1 else flat(log_decay), states[t], self.masks[t], scale,
+                                        out_state=states[t + 1])
+        return out.view((n, N) + out.shape[1:])
+
+    def insert_actions(self, t, features, weight, bias, actions):
+        """The taken actions and their log-probabilities under softmax(features weight^T + bias) over the available actions of slot t
+        (``policy_ops.action_log_probs``) into the slots of buffer step t: what the runner's collect stores
+        (onpolicy/runner/shared/graph_mpe_runner.py:360-436).  features (n, N, K), actions (n, N) or (n, N, 1).  Returns (log_probs, entropy), (n, N, 1)."""
+        self._need_policy()
+        if not 0 <= t < self.T:
+            raise ValueError('insert_actions: buffer step %d of %d' % (t, self.T))
+        if self.actions.shape[-1] != 1:
+            raise ValueError('insert_actions: act_dim must be 1, the buffer has %d' % self.actions.shape[-1])
+        with torch.no_grad():
+            log_probs, entropy = policy_ops.action_log_probs(features, weight, bias, actions, None if self.available_actions is None else self.available_actions[t])
+        self.actions[t].copy_(actions.reshape(self.actions[t].shape))
+        self.action_log_probs[t].copy_(log_probs.reshape(self.action_log_probs[t].shape))
+        return log_probs.unsqueeze(-1), entropy.unsqueeze(-1)
 
     def _need_policy(self):
         if self.value_preds is None:
