@@ -8,6 +8,8 @@
 //     out_t = sum_{s before or at t} w(t, s) (x_t . y_s) z_s + (what the walk carries):
 //     o: x, y, z = q, k, v forwards;  dq: do, v, k forwards (state S^T);  dk: v, do, q backwards (state G^T);  dv: k, q, do backwards.
 // memory_walk_kernel is that walk.
+#include <type_traits>
+
 #include "fmarl_policy_dev.h"
 
 namespace fmarl {
@@ -246,6 +248,293 @@ __global__ __launch_bounds__(256) void memory_walk_kernel(Walk a) {
     if (a.seg_decay && slice == 0 && lane == 0) a.seg_decay[seg * heads + bh] = whole;
 }
 
+// ---- small heads ------------------------------------------------------------------------------------------------------------
+// dy <= 32: the recurrence itself, token by token, on the vector units.  16 lanes (a DPP row) hold one head: lane c column c of its slice of the state, 16 NY
+// values of y each; y and x are broadcast from the lane that holds them by the multiply's own operand (row_newbcast), so a token costs three
+// instructions per 64 state entries and no LDS.  Four neighbouring heads share a wave: 256 bytes of a token's row side by side.  Against the matrix walk at
+// heads of 16 x 16, where half of every 16-token tile is above the diagonal and chunks of ten tokens waste the rest: 239 -> 156 us for 30 720 x 4 heads of ten
+// tokens (float32, 566 MB: 111 us at the copy rate of 5.1 TB/s).
+template <int M> __device__ __forceinline__ float row_lane(float v) {   // lane M of each row of 16, in every lane of the row
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + M, 0xf, 0xf, true));
+}
+
+template <int M, int N, typename F> __device__ __forceinline__ void unroll(F f) {
+    if constexpr (M < N) { f(std::integral_constant<int, M>()); unroll<M + 1, N>(f); }
+}
+
+template <int CTRL> __device__ __forceinline__ float row_turn(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
+__device__ __forceinline__ float row_sum(float v) {   // over the 16 lanes of a row, in every lane: rotations by 8, 4, 2, 1
+    v += row_turn<0x128>(v); v += row_turn<0x124>(v); v += row_turn<0x122>(v); v += row_turn<0x121>(v);
+    return v;
+}
+
+// sum_m x_m S[m], x_m in lane m of the row; four partial sums, so that no add waits for the one before.  In assembly because the compiler does not put the lane
+// selection into a multiply-add (it emits a move for each: twice the instructions); s_nop 1: the two wait states between a vector write of x and its
+// use by another lane.
+__device__ __forceinline__ float row_dot16(float x, const float *S) {
+    float a, b, c, d;
+    asm("s_nop 1\n\t"
+        "v_mul_f32_dpp %0, %4, %5 row_newbcast:0 row_mask:0xf bank_mask:0xf\n\t"
+        "v_mul_f32_dpp %1, %4, %6 row_newbcast:1 row_mask:0xf bank_mask:0xf\n\t"
+        "v_mul_f32_dpp %2, %4, %7 row_newbcast:2 row_mask:0xf bank_mask:0xf\n\t"
+        "v_mul_f32_dpp %3, %4, %8 row_newbcast:3 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %4, %9 row_newbcast:4 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %1, %4, %10 row_newbcast:5 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %2, %4, %11 row_newbcast:6 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %3, %4, %12 row_newbcast:7 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %4, %13 row_newbcast:8 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %1, %4, %14 row_newbcast:9 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %2, %4, %15 row_newbcast:10 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %3, %4, %16 row_newbcast:11 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %4, %17 row_newbcast:12 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %1, %4, %18 row_newbcast:13 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %2, %4, %19 row_newbcast:14 row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %3, %4, %20 row_newbcast:15 row_mask:0xf bank_mask:0xf"
+        : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
+        : "v"(x), "v"(S[0]), "v"(S[1]), "v"(S[2]), "v"(S[3]), "v"(S[4]), "v"(S[5]), "v"(S[6]), "v"(S[7]), "v"(S[8]), "v"(S[9]), "v"(S[10]), "v"(S[11]), "v"(S[12]),
+          "v"(S[13]), "v"(S[14]), "v"(S[15]));
+    return (a + b) + (c + d);
+}
+
+template <int NY> __device__ __forceinline__ float row_dot(const float (&x)[NY], const float (&S)[16 * NY]) {
+    float o = row_dot16(x[0], S);
+    if constexpr (NY == 2) o += row_dot16(x[1], S + 16);
+    return o;
+}
+
+// S <- keep ? a S + y z : y z, y_m in lane m of the row: one multiply that selects the lane, one multiply-add.  Selected, not multiplied by zero, where the state
+// is not kept: whatever it held is gone.
+template <int NY> __device__ __forceinline__ void row_update(float (&S)[16 * NY], float a, bool fresh, const float (&y)[NY], float z) {
+    if (__ballot(fresh))
+#pragma unroll
+        for (int m = 0; m < 16 * NY; ++m) S[m] = fresh ? 0.f : S[m];
+    unroll<0, 16 * NY>([&](auto m) { S[m] = __builtin_fmaf(S[m], a, row_lane<m % 16>(y[m / 16]) * z); });
+}
+
+// S[m] <- element (m, z) of a state; `run`: its y axis is contiguous and float4s line up
+template <int N> __device__ __forceinline__ void row_state(float (&S)[N], const float *p, int64_t s_y, int dy, bool real, bool run) {
+    if (run) {
+#pragma unroll
+        for (int m = 0; m < N; m += 4) {
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            if (real && m < dy) v = *(const f32x4 *)(p + m);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[m + r] = v[r];
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < N; ++m) S[m] = real && m < dy ? p[m * s_y] : 0.f;
+    }
+}
+
+template <typename T, int NY, bool DOT>
+__global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
+    constexpr int TB = NY == 1 ? 8 : 4;   // tokens whose rows are in flight while as many are computed
+    const int lane = threadIdx.x & 63, c = lane & 15;
+    const int64_t heads = a.B * a.H, groups = (heads + 3) / 4;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= groups * a.nseg * a.slices) return;
+    const int64_t mine = unit % groups * 4 + (lane >> 4), rest = unit / groups;
+    const bool have = mine < heads;
+    const int64_t bh = have ? mine : heads - 1;
+    const int slice = (int)(rest % a.slices), seg = (int)(rest / a.slices);
+    const int64_t b = bh / a.H;
+    const int h = (int)(bh - b * a.H);
+    const int z = slice * 16 + c, dy = a.dy;
+    const bool zin = z < a.dz;
+    const int64_t t_begin = (int64_t)seg * a.seg_len, t_end = min(a.L, t_begin + a.seg_len), count = t_end - t_begin;
+    const T *px = a.state_only ? nullptr : (const T *)a.x.p + b * a.x.sb + h * a.x.sh + c, *py = (const T *)a.y.p + b * a.y.sb + h * a.y.sh + c;
+    const T *pz = (const T *)a.z.p + b * a.z.sb + h * a.z.sh + z, *pw = DOT ? (const T *)a.w.p + b * a.w.sb + h * a.w.sh + z : nullptr;
+    T *po = a.state_only ? nullptr : (T *)a.out.p + b * a.out.sb + h * a.out.sh + z;
+    const float *pg = a.g + b * a.gb + h * a.gh, *pm = a.masks ? a.masks + b * a.mb : nullptr;
+
+    float S[16 * NY];
+    if (a.state) {
+        const float *ps = a.state + seg * a.seg_state_in + bh * (int64_t)a.dy * a.dz + (int64_t)z * a.s_z;
+        row_state(S, ps, a.s_y, dy, zin, a.s_y == 1 && (dy & 3) == 0 && ((uintptr_t)a.state & 15) == 0);
+    } else {
+#pragma unroll
+        for (int m = 0; m < 16 * NY; ++m) S[m] = 0.f;
+    }
+    float whole = 1.f;
+    float nx[TB][NY], ny[TB][NY], nz[TB], nw[TB], ng = 0.f, nm = 1.f;
+    // step i of the walk is token i of the segment, or token i from its end
+    auto token = [&](int64_t i) { return a.reverse ? t_end - 1 - i : t_begin + i; };
+    auto fetch = [&](int64_t i0) {
+#pragma unroll
+        for (int i = 0; i < TB; ++i) {
+            const bool in = i0 + i < count;
+            const int64_t t = in ? token(i0 + i) : t_begin;
+#pragma unroll
+            for (int n = 0; n < NY; ++n) {
+                const bool yin = in && 16 * n + c < dy;
+                nx[i][n] = px && yin ? (float)px[t * a.x.sl + 16 * n] : 0.f;
+                ny[i][n] = yin ? (float)py[t * a.y.sl + 16 * n] : 0.f;
+            }
+            nz[i] = in && zin ? (float)pz[t * a.z.sl] : 0.f;
+            if (DOT) nw[i] = in && zin ? (float)pw[t * a.w.sl] : 0.f;
+        }
+        const bool in = c < TB && i0 + c < count;   // lane c: the decay of step i0 + c
+        const int64_t t = in ? token(i0 + c) : t_begin;
+        ng = in ? pg[t * a.gl] : 0.f;
+        nm = in && pm ? pm[t * a.ml] : 1.f;
+    };
+    fetch(0);
+    for (int64_t i0 = 0; i0 < count; i0 += TB) {
+        float x[TB][NY], y[TB][NY], zz[TB], ww[TB];
+#pragma unroll
+        for (int i = 0; i < TB; ++i) {
+#pragma unroll
+            for (int n = 0; n < NY; ++n) { x[i][n] = nx[i][n]; y[i][n] = ny[i][n] * a.y_scale; }
+            zz[i] = nz[i]; ww[i] = DOT ? nw[i] : 0.f;
+        }
+        const float fresh_l = nm == 0.f || ng == -__builtin_inff() ? 1.f : 0.f;
+        const float decay_l = fresh_l != 0.f ? 0.f : exp2_fast((float)((double)ng * 1.4426950408889634074));
+        if (i0 + TB < count) fetch(i0 + TB);
+        unroll<0, TB>([&](auto ii) {
+            constexpr int i = ii;
+            if (i0 + i < count) {
+                const float d = row_lane<i>(decay_l);
+                const bool fresh = row_lane<i>(fresh_l) != 0.f;
+                if (a.state_only) whole *= fresh ? 0.f : d;
+                else {
+                    float nd = row_dot<NY>(x[i], S);       // from the tokens before (backwards: behind); forwards the token's decay lies between
+                    if (!a.reverse) nd = fresh ? 0.f : nd * d;
+                    float xy = 0.f;
+#pragma unroll
+                    for (int n = 0; n < NY; ++n) xy += x[i][n] * y[i][n];
+                    xy = row_sum(xy);
+                    const int64_t t = token(i0 + i);
+                    if (have && zin) po[t * a.out.sl] = (T)((nd + xy * zz[i]) * a.out_scale);
+                    if (DOT) {
+                        const float dot = row_sum(nd * a.out_scale * ww[i]);
+                        if (have && c == 0) a.dot[((slice * a.L + t) * a.B + b) * a.H + h] = dot;
+                    }
+                }
+                if (!a.reverse) row_update<NY>(S, d, fresh, y[i], zz[i]);
+                else {
+                    row_update<NY>(S, d, false, y[i], zz[i] * d);
+                    if (__ballot(fresh))
+#pragma unroll
+                        for (int m = 0; m < 16 * NY; ++m) S[m] = fresh ? 0.f : S[m];
+                }
+            }
+        });
+    }
+    if (a.state_out && have && zin) {
+        float *ps = a.state_out + seg * a.seg_state_out + bh * (int64_t)a.dy * a.dz + (int64_t)z * a.o_z;
+#pragma unroll
+        for (int m = 0; m < 16 * NY; ++m) if (m < dy) ps[m * a.o_y] = S[m];
+    }
+    if (a.seg_decay && slice == 0 && c == 0 && have) a.seg_decay[seg * heads + bh] = whole;
+}
+
+// All gradients of up to 16 tokens of heads up to 16 x 16 in one pass (the update's chunks): q, k, v and dout stay in registers -- 16 lanes a head, as above --, the state is walked
+// forwards for dq, its gradient backwards for dk (lane = row) and dv (lane = column).  dg_t = <S_L, dS_L> + sum_{i >= t} (q_i . dq_i - k_i . dk_i), each
+// without the token's own term, 0 where an episode starts.  Reads and writes everything once: 928 MB for 30 720 x 4 heads of ten tokens, 182 us at the copy
+// rate; it takes 221 us, three walks and the decay's kernel took 872 us.
+struct ShortGrad {
+    WalkRows q, k, v, o, dq, dk, dv;
+    const float *g; int64_t gl, gb, gh;
+    const float *masks; int64_t ml, mb;
+    const float *state, *d_state;
+    float *d_state0, *dg;            // NULL: not wanted
+    double *partial;                 // (B, H) sums of dg, or NULL
+    int64_t B;
+    int L, H, dk_dim, dv_dim, wide;  // wide: states are read and written in float4s
+    float scale;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void memory_short_backward_kernel(ShortGrad a) {
+    const int lane = threadIdx.x & 63, c = lane & 15;
+    const int64_t heads = a.B * a.H;
+    const int64_t mine = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 + (lane >> 4);
+    if ((mine & ~(int64_t)3) >= heads) return;
+    const bool have = mine < heads;
+    const int64_t bh = have ? mine : heads - 1;
+    const int64_t b = bh / a.H;
+    const int h = (int)(bh - b * a.H), K = a.dk_dim, V = a.dv_dim, L = a.L;
+    const bool kin = c < K, vin = c < V;
+    float q[16], k[16], v[16], o[16], xs[16];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+        const bool in = t < L;
+        q[t] = in && kin ? (float)((const T *)a.q.p)[t * a.q.sl + b * a.q.sb + h * a.q.sh + c] : 0.f;
+        k[t] = in && kin ? (float)((const T *)a.k.p)[t * a.k.sl + b * a.k.sb + h * a.k.sh + c] : 0.f;
+        v[t] = in && vin ? (float)((const T *)a.v.p)[t * a.v.sl + b * a.v.sb + h * a.v.sh + c] : 0.f;
+        o[t] = in && vin ? (float)((const T *)a.o.p)[t * a.o.sl + b * a.o.sb + h * a.o.sh + c] : 0.f;
+    }
+    const float gl = c < L ? a.g[c * a.gl + b * a.gb + h * a.gh] : 0.f, ml = c < L && a.masks ? a.masks[c * a.ml + b * a.mb] : 1.f;
+    const int64_t at = bh * (int64_t)K * V;
+    float S[16], G[16], C[16];        // S, G: row c of the state and of its gradient; C: column c of the gradient
+    if (a.state) row_state(S, a.state + at + c * V, 1, V, kin, a.wide);
+    else {
+#pragma unroll
+        for (int m = 0; m < 16; ++m) S[m] = 0.f;
+    }
+    const float fresh_l = ml == 0.f || gl == -__builtin_inff() ? 1.f : 0.f;
+    const float decay_l = fresh_l != 0.f ? 0.f : exp2_fast((float)((double)gl * 1.4426950408889634074));
+    unroll<0, 16>([&](auto tt) {
+        constexpr int t = tt;
+        if (t < L) {
+            const bool fresh = row_lane<t>(fresh_l) != 0.f;
+            const float d = row_lane<t>(decay_l), x1[1] = {o[t]}, nd = fresh ? 0.f : row_dot<1>(x1, S) * d, vo = row_sum(v[t] * o[t]);
+            if (have && kin) ((T *)a.dq.p)[t * a.dq.sl + b * a.dq.sb + h * a.dq.sh + c] = (T)((nd + k[t] * vo) * a.scale);
+            xs[t] = row_sum(q[t] * nd) * a.scale;
+            const float y1[1] = {v[t]};
+            row_update<1>(S, d, fresh, y1, k[t]);
+            q[t] *= a.scale;           // from here on only in G's and dk's, dv's own terms
+        }
+    });
+    float run = 0.f;
+    if (a.d_state) {
+        row_state(G, a.d_state + at + c * V, 1, V, kin, a.wide);
+        row_state(C, a.d_state + at + c, V, K, vin, false);
+#pragma unroll
+        for (int m = 0; m < 16; ++m) run += S[m] * G[m];
+        run = row_sum(run);
+    } else {
+#pragma unroll
+        for (int m = 0; m < 16; ++m) G[m] = C[m] = 0.f;
+    }
+    double sum = 0.0;
+    unroll<0, 16>([&](auto tt) {
+        constexpr int t = 15 - tt;
+        if (t < L) {
+            const float v1[1] = {v[t]}, k1[1] = {k[t]}, q1[1] = {q[t]}, o1[1] = {o[t]};
+            const float nk = row_dot<1>(v1, G), nv = row_dot<1>(k1, C), vo = row_sum(v[t] * o[t]), qk = row_sum(q[t] * k[t]);
+            if (have && kin) ((T *)a.dk.p)[t * a.dk.sl + b * a.dk.sb + h * a.dk.sh + c] = (T)(nk + q[t] * vo);
+            if (have && vin) ((T *)a.dv.p)[t * a.dv.sl + b * a.dv.sb + h * a.dv.sh + c] = (T)(nv + o[t] * qk);
+            run += xs[t] - row_sum(k[t] * nk);
+            const bool fresh = row_lane<t>(fresh_l) != 0.f;
+            const float dg = fresh ? 0.f : run, d = row_lane<t>(decay_l);
+            if (fresh) run = 0.f;
+            sum += dg;
+            if (a.dg && have && c == 0) a.dg[t * heads + bh] = dg;
+            row_update<1>(G, d, false, o1, q[t] * d);
+            row_update<1>(C, d, false, q1, o[t] * d);
+            if (__ballot(fresh))
+#pragma unroll
+                for (int m = 0; m < 16; ++m) { G[m] = fresh ? 0.f : G[m]; C[m] = fresh ? 0.f : C[m]; }
+        }
+    });
+    if (a.d_state0 && have && kin) {
+        float *p = a.d_state0 + at + c * V;
+        if (a.wide) {
+#pragma unroll
+            for (int m = 0; m < 16; m += 4) if (m < V) *(f32x4 *)(p + m) = f32x4{G[m], G[m + 1], G[m + 2], G[m + 3]};
+        } else {
+#pragma unroll
+            for (int m = 0; m < 16; ++m) if (m < V) p[m] = G[m];
+        }
+    }
+    if (a.partial && have && c == 0) a.partial[bh] = sum;
+}
+
 // The states at the segments' starts (backwards: behind their ends) from what each segment adds to an empty state: in place, one thread per element.
 __global__ __launch_bounds__(256) void memory_join_kernel(float *seg_states, const float *seg_decay, const float *init, float *last,
                                                           int64_t heads, int elems, int nseg, int reverse) {
@@ -480,10 +769,17 @@ Segments memory_segments(const FmarlMemory *m) {
     return {(int)((m->L + len - 1) / len), (int)len};
 }
 
+// The recurrence on the vector units for y up to 32 wide, the matrix walk beyond: at 16 x 16 the former takes half the latter's time, at 64 x 64
+// its three instructions per 64 state entries would cost twice the matrix units' time
+bool small_heads(int dy) { return dy <= 32; }
+
 int tiles(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : 8; }
 // columns of z that one wave takes, in tiles of 16: the state's dy x dz accumulators have to fit its registers beside the operands
 int slice_tiles(int dy, int dz) { const int t = tiles(dz), most = tiles(dy) == 8 ? 2 : 4; return t > most ? most : t; }
-int slices_of(int dy, int dz) { const int w = 16 * slice_tiles(dy, dz); return (dz + w - 1) / w; }
+int slices_of(int dy, int dz) { const int w = small_heads(dy) ? 16 : 16 * slice_tiles(dy, dz); return (dz + w - 1) / w; }
+
+// up to 16 tokens of heads up to 16 x 16: every gradient in one kernel, whose registers hold all of it
+bool short_backward(const FmarlMemory *m) { return m->L <= 16 && m->dk <= 16 && m->dv <= 16; }
 
 struct Workspace {
     size_t seg_s, seg_g, decay, dot_q, dot_k, partial, d_state, total;
@@ -499,7 +795,8 @@ Workspace memory_layout(const FmarlMemory *m, int backward) {
         if (backward) w.seg_g = take(4 * s.nseg * heads * elems);
         w.decay = take(4 * s.nseg * heads);
     }
-    if (backward) {
+    if (backward && short_backward(m)) w.partial = take(8 * heads);
+    else if (backward) {
         w.dot_q = take(4 * (size_t)slices_of(m->dv, m->dk) * m->L * heads);
         w.dot_k = take(4 * (size_t)slices_of(m->dv, m->dk) * m->L * heads);
         w.partial = take(8 * heads);
@@ -521,17 +818,18 @@ void launch_walk_nz(const Walk &w, unsigned blocks, hipStream_t st) {
 
 template <typename T>
 void launch_walk_t(const Walk &w, unsigned blocks, hipStream_t st) {
-    switch (tiles(w.dy)) {
-    case 1: launch_walk_nz<T, 1>(w, blocks, st); break;
-    case 2: launch_walk_nz<T, 2>(w, blocks, st); break;
-    case 4: launch_walk_nz<T, 4>(w, blocks, st); break;
-    default: launch_walk_nz<T, 8>(w, blocks, st); break;
-    }
+    if (w.dy <= 16 && w.w.p) hipLaunchKernelGGL((memory_rows_kernel<T, 1, true>), dim3(blocks), dim3(256), 0, st, w);
+    else if (w.dy <= 16) hipLaunchKernelGGL((memory_rows_kernel<T, 1, false>), dim3(blocks), dim3(256), 0, st, w);
+    else if (w.dy <= 32 && w.w.p) hipLaunchKernelGGL((memory_rows_kernel<T, 2, true>), dim3(blocks), dim3(256), 0, st, w);
+    else if (w.dy <= 32) hipLaunchKernelGGL((memory_rows_kernel<T, 2, false>), dim3(blocks), dim3(256), 0, st, w);
+    else if (w.dy <= 64) launch_walk_nz<T, 4>(w, blocks, st);
+    else launch_walk_nz<T, 8>(w, blocks, st);
 }
 
 int launch_walk(Walk w, int dtype, hipStream_t st) {
     w.slices = slices_of(w.dy, w.dz);
-    const int64_t blocks = (w.B * w.H * w.nseg * w.slices + 3) / 4;
+    const int64_t heads = w.B * w.H, units = small_heads(w.dy) ? (heads + 3) / 4 : heads;   // waves per segment and slice
+    const int64_t blocks = (units * w.nseg * w.slices + 3) / 4;
     if (blocks > 0xffffff) return policy_fail(FMARL_EINVAL, "memory: too many sequences");
     if (dtype == FMARL_T_F32) launch_walk_t<float>(w, (unsigned)blocks, st);
     else if (dtype == FMARL_T_BF16) launch_walk_t<__bf16>(w, (unsigned)blocks, st);
@@ -632,6 +930,24 @@ int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, co
     char *base = (char *)workspace;
     const Walk w0 = walk_base(m);
     const int64_t heads = m->B * m->H;
+    if (short_backward(m)) {
+        ShortGrad g = {};
+        const int dt = m->dtype;
+        g.q = walk_rows(m->q, m->dk, dt); g.k = walk_rows(m->k, m->dk, dt); g.v = walk_rows(m->v, m->dv, dt); g.o = walk_rows(*d_out, m->dv, dt);
+        g.dq = walk_rows(*d_q, m->dk, dt); g.dk = walk_rows(*d_k, m->dk, dt); g.dv = walk_rows(*d_v, m->dv, dt);
+        g.g = w0.g; g.gl = w0.gl; g.gb = w0.gb; g.gh = w0.gh; g.masks = w0.masks; g.ml = w0.ml; g.mb = w0.mb;
+        g.state = m->state; g.d_state = d_state; g.d_state0 = d_state0; g.dg = m->shared_decay ? nullptr : d_log_decay;
+        g.partial = m->shared_decay && d_log_decay ? (double *)(base + ws.partial) : nullptr;
+        g.B = m->B; g.L = (int)m->L; g.H = m->H; g.dk_dim = m->dk; g.dv_dim = m->dv; g.scale = m->scale;
+        g.wide = (m->dv & 3) == 0 && (((uintptr_t)m->state | (uintptr_t)d_state | (uintptr_t)d_state0) & 15) == 0;
+        const dim3 grid((unsigned)((heads + 15) / 16));
+        if (dt == FMARL_T_F32) hipLaunchKernelGGL(memory_short_backward_kernel<float>, grid, dim3(256), 0, st, g);
+        else if (dt == FMARL_T_BF16) hipLaunchKernelGGL(memory_short_backward_kernel<__bf16>, grid, dim3(256), 0, st, g);
+        else hipLaunchKernelGGL(memory_short_backward_kernel<_Float16>, grid, dim3(256), 0, st, g);
+        if (g.partial) hipLaunchKernelGGL(decay_sum_kernel, dim3((unsigned)m->H), dim3(256), 0, st, (const double *)g.partial, d_log_decay, m->B, m->H);
+        HIP_OK(hipGetLastError());
+        return FMARL_OK;
+    }
     const int elems = m->dk * m->dv;
     float *seg_s = (float *)(base + ws.seg_s), *seg_g = (float *)(base + ws.seg_g), *decay = (float *)(base + ws.decay);
     float *ds0 = d_state0 ? d_state0 : (float *)(base + ws.d_state);
