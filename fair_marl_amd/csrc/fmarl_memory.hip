@@ -7,7 +7,7 @@
 // o, dq, dk and dv are the same walk over the tokens, forwards or backwards, with the operands in other roles:
 //     out_t = sum_{s before or at t} w(t, s) (x_t . y_s) z_s + (what the walk carries):
 //     o: x, y, z = q, k, v forwards;  dq: do, v, k forwards (state S^T);  dk: v, do, q backwards (state G^T);  dv: k, q, do backwards.
-// memory_walk_kernel is that walk.
+// memory_tiles_kernel (large heads, the matrix units) and memory_rows_kernel (small ones) are that walk.
 #include <type_traits>
 
 #include "fmarl_policy_dev.h"
@@ -37,222 +37,375 @@ struct Walk {
     float y_scale, out_scale;
 };
 
-// One wave walks one (batch, head, segment of the tokens, slice of at most 16 NZ columns of z) in chunks of 16 tokens; the state (16 NY x 16 NZ)
-// stays in registers in the accumulator layout of mfma_f32_16x16x4f32 (row 4 * (lane / 16) + r, column lane % 16).  That layout is also a valid
-// B operand that contracts over the rows in the order k = 4 * (lane / 16) + r, and the A operand of its transpose, so neither the weights
-// (kept as P^T: rows s, columns t) nor the state ever moves between lanes:
-//     P^T = y x^T;  out^T = z^T P^T + S^T x^T;  S = e^C S + (u y)^T z.
-// Float32 products and sums throughout (the inputs' bf16 / f16 values are exact in it); the decays' prefix sums are float64, so a weight
-// e^{C_t - C_s} is right to float32 however fast the tokens before forgot.  A weight is selected, not multiplied to zero: what an episode left
-// behind (infinities too) does not reach the next one; a chunk that holds a value that is not finite is walked token by token, so that
-// it reaches later tokens only.
-template <typename T, int NY, int NZ>
-__global__ __launch_bounds__(256) void memory_walk_kernel(Walk a) {
-    constexpr int PY = 16 * NY + 4, PZ = 16 * NZ + 4;   // 4 rows apart = 16 banks apart: column reads of four row groups do not meet
-    constexpr int kWave = 16 * (2 * PY + 2 * PZ) + 32 + 16;
-    __shared__ __align__(16) float lds[4 * kWave];
+// ---- large heads ------------------------------------------------------------------------------------------------------------
+// A workgroup walks one (batch, head, segment) in chunks of 32 tokens; wave w holds columns 16 w .. 16 w + 15 of the state (float32, in the accumulator layout of
+// mfma_f32_16x16x32_bf16: row 4 * (lane / 16) + r, column lane % 16), so a chunk is read once for all of it:
+//     P^T = y x^T, weighted (three 16 x 16 tiles, shared out over the waves);  out^T = z^T P^T + S^T x^T;  S = e^C S + y^T (u z).
+// All products are bfloat16 ones of exact pieces: a bfloat16 value is one piece, a float16 value two, a float32 value three (8 + 8 + 8 bits), and what is
+// formed in float32 (P, S, u z) is cut into two or three; products whose place is below 2^-24 of the result (2^-16 where the output has 8 or 11 bits) are left out.  Per
+// product of 16 x 16 x 32 that is 1 to 6 instructions of 16 cycles against eight of 32 cycles of mfma_f32_16x16x4f32.
+// The accumulator layout serves as either operand's layout if the contraction runs in the order 8 * (lane / 16) + 4 * tile + r for the index 16 * tile + 4 * (lane / 16) + r
+// (two tiles to a contraction of 32): rows in LDS are stored in that order, so every operand is one 16-byte read.
+// The decays' prefix sums are float64, so a weight e^{C_t - C_s} is right to float32 however fast the tokens before forgot.  A weight is selected, not multiplied to
+// zero: what an episode left behind (infinities too) does not reach the next one; a chunk that holds a value that is not finite is walked token by token, so
+// that it reaches later tokens only.
+// pieces of an input (in), of P and the state as operands (p), highest order (sum of the pieces' numbers) kept in x y (in_order) and in out (out_order); u z has three pieces, kept to
+// order 2.  DOT: out is dotted with w before its rounding, for the decay's gradient, a difference of such sums: out to float32 there too.
+template <typename T, bool DOT> struct Pieces;
+template <bool DOT> struct Pieces<__bf16, DOT> { static constexpr int in = 1, p = DOT ? 3 : 2, in_order = 0, out_order = DOT ? 2 : 1; };
+template <bool DOT> struct Pieces<_Float16, DOT> { static constexpr int in = 2, p = DOT ? 3 : 2, in_order = 2, out_order = DOT ? 2 : 1; };
+template <bool DOT> struct Pieces<float, DOT> { static constexpr int in = 3, p = 3, in_order = 2, out_order = 2; };
+
+template <int N> __device__ __forceinline__ void cut(float v, __bf16 (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) { p[i] = (__bf16)v; v -= (float)p[i]; }
+}
+
+// the pieces of four inputs, piece by piece; a bfloat16 value is its own
+template <typename T, int N> __device__ __forceinline__ void cut4(typename Vec4<T>::type v, bf16x4 (&p)[N]) {
+    f32x4 f = widen(v);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) { p[i][r] = (__bf16)f[r]; f[r] -= (float)p[i][r]; }
+}
+template <> __device__ __forceinline__ void cut4<__bf16, 1>(bf16x4 v, bf16x4 (&p)[1]) { p[0] = v; }
+
+// whether one of the four is not finite: its exponent's bits are all set
+__device__ __forceinline__ bool not_finite(f32x4 v) { return !(v[0] - v[0] == 0.f && v[1] - v[1] == 0.f && v[2] - v[2] == 0.f && v[3] - v[3] == 0.f); }
+__device__ __forceinline__ bool not_finite(bf16x4 v) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 u = __builtin_bit_cast(u32x2, v);
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) bad |= (u[i] & 0x7f80u) == 0x7f80u || (u[i] & 0x7f800000u) == 0x7f800000u;
+    return bad;
+}
+__device__ __forceinline__ bool not_finite(f16x4 v) { return not_finite(widen(v)); }
+
+template <int NA, int NB, int ORDER>
+__device__ __forceinline__ f32x4 mma_pieces(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 c) {
+#pragma unroll
+    for (int i = NA - 1; i >= 0; --i)
+#pragma unroll
+        for (int j = NB - 1; j >= 0; --j)
+            if (i + j <= ORDER) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], c, 0, 0, 0);
+    return c;
+}
+
+// prefix sum over lanes 0 .. 31 (lanes 32 .. 63 repeat it): rows of 16 by lane shifts, the second row plus the first one's total
+template <int CTRL> __device__ __forceinline__ double row_shift(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+
+__device__ __forceinline__ double scan32(double v, int lane) {
+    v += row_shift<0x111>(v); v += row_shift<0x112>(v); v += row_shift<0x114>(v); v += row_shift<0x118>(v);   // (lanes without a source add 0)
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t l0 = __builtin_amdgcn_readlane((int)(uint32_t)u, 15), h0 = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 15);
+    return lane & 16 ? v + __builtin_bit_cast(double, ((uint64_t)h0 << 32) | l0) : v;
+}
+
+// LDS of a workgroup, in bytes: x, y (32 tokens), y^T, z^T (rows of 32 tokens), P^T, per-token floats
+template <typename T, bool DOT> __host__ __device__ constexpr int tiles_lds(int nk, int nz) {
+    return Pieces<T, DOT>::in * 2 * (2 * 32 * (32 * nk + 8) + (32 * nk + 16 * nz) * 40) + Pieces<T, DOT>::p * 2 * 32 * 40 + 32 * 8 + 4 * 32 * 4 + 8 * 32 * 4;
+}
+
+template <typename T, int NK, bool DOT, bool VEC>
+__global__ __launch_bounds__(512) void memory_tiles_kernel(Walk a) {
+    typedef Pieces<T, DOT> PC;
+    constexpr int NP = PC::in, PP = PC::p, XS = 32 * NK + 8;
     typedef typename Vec4<T>::type V;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g4 = (lane >> 4) * 4;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
-    const int64_t heads = a.B * a.H;
-    if (unit >= heads * a.nseg * a.slices) return;
-    // neighbouring waves take neighbouring heads of one batch entry: their rows share cache lines
-    const int64_t bh = unit % heads;
-    const int64_t rest = unit / heads;
-    const int slice = (int)(rest % a.slices), seg = (int)(rest / a.slices);
+    extern __shared__ __align__(16) char smem[];
+    const int nz = (a.dz + 15) / 16, threads = blockDim.x;
+    __bf16 *lx = (__bf16 *)smem, *ly = lx + NP * 32 * XS, *lyt = ly + NP * 32 * XS, *lzt = lyt + NP * 32 * NK * 40, *lp = lzt + NP * 16 * nz * 40;
+    double *lc = (double *)(lp + PP * 32 * 40);
+    float *lwin = (float *)(lc + 32), *lwout = lwin + 32, *lown = lwout + 32, *ldot = lown + 64, *lall = lown + 32;   // ldot: (waves, 32)
+    uint32_t *lfr = (uint32_t *)(lown + 40);   // [0] tokens that start afresh; [1], [2]: a value is not finite, by the chunk's parity (cleared in the chunk between)
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6, c = lane & 15, g = lane >> 4, g4 = g * 4;
+    const int64_t heads = a.B * a.H, bh = blockIdx.x % heads;
+    const int seg = (int)(blockIdx.x / heads);
     const int64_t b = bh / a.H;
-    const int h = (int)(bh - b * a.H);
-    const int z0 = slice * 16 * NZ, dz = min(a.dz - z0, 16 * NZ), dy = a.dy;
-    const int64_t t_begin = (int64_t)seg * a.seg_len, t_end = min(a.L, t_begin + a.seg_len);
+    const int h = (int)(bh - b * a.H), dy = a.dy, dz = a.dz;
+    const int64_t t_begin = (int64_t)seg * a.seg_len, t_end = min(a.L, t_begin + a.seg_len), chunks = (t_end - t_begin + 31) / 32;
+    const T *px = a.state_only ? nullptr : (const T *)a.x.p + b * a.x.sb + h * a.x.sh, *py = (const T *)a.y.p + b * a.y.sb + h * a.y.sh;
+    const T *pz = (const T *)a.z.p + b * a.z.sb + h * a.z.sh, *pw = DOT ? (const T *)a.w.p + b * a.w.sb + h * a.w.sh : nullptr;
+    T *po = a.state_only ? nullptr : (T *)a.out.p + b * a.out.sb + h * a.out.sh;
+    const int zc = 16 * wave;                  // this wave's columns of z; waves beyond nz only load and help with P
+    const bool holds = wave < nz;
 
-    float *lx = lds + wave * kWave, *ly = lx + 16 * PY, *lz = ly + 16 * PY, *lw = lz + 16 * PZ;
-    double *lc = (double *)(lw + 16 * PZ);      // prefix sums of the chunk's log decays
-    const T *px = (const T *)a.x.p + b * a.x.sb + h * a.x.sh, *py = (const T *)a.y.p + b * a.y.sb + h * a.y.sh;
-    const T *pz = (const T *)a.z.p + b * a.z.sb + h * a.z.sh + z0, *pw = a.w.p ? (const T *)a.w.p + b * a.w.sb + h * a.w.sh + z0 : nullptr;
-    T *po = a.state_only ? nullptr : (T *)a.out.p + b * a.out.sb + h * a.out.sh + z0;
+    f32x4 S[2 * NK];
+#pragma unroll
+    for (int i = 0; i < 2 * NK; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int y = 16 * i + g4 + r, z = zc + c;
+            S[i][r] = holds && a.state && y < dy && z < dz ? a.state[seg * a.seg_state_in + bh * (int64_t)dy * dz + y * a.s_y + z * a.s_z] : 0.f;
+        }
+    if (tid < 3) lfr[tid] = 0;
+    for (int i = tid; i < PP * 32 * 40; i += threads) lp[i] = (__bf16)0.f;   // the tile beyond the diagonal stays zero
+    float whole = 1.f;
 
-    f32x4 S[NY][NZ];
+    // a thread's share of a chunk: NK pieces of four of x and of y each, two at most of z.  Where they lie is worked out once; from chunk to chunk the
+    // pointers move on by 32 tokens
+    const int64_t t_first = a.reverse ? t_begin + 32 * (chunks - 1) : t_begin, dir = a.reverse ? -32 : 32;
+    V rx[NK], ry[NK], rz[2];
+    const T *qx[NK], *qy[NK], *qz[2];
+    int xtok[NK], xleft[NK], ztok[2], zleft[2];
 #pragma unroll
-    for (int i = 0; i < NY; ++i)
+    for (int n = 0; n < NK; ++n) {
+        const int idx = tid + threads * n, col = (idx % (8 * NK)) * 4;
+        xtok[n] = idx / (8 * NK); xleft[n] = xtok[n] < 32 ? dy - col : 0;
+        qx[n] = px + (t_first + xtok[n]) * a.x.sl + col; qy[n] = py + (t_first + xtok[n]) * a.y.sl + col;
+    }
 #pragma unroll
-        for (int j = 0; j < NZ; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int y = 16 * i + g4 + r, z = 16 * j + c;
-                S[i][j][r] = a.state && y < dy && z < dz
-                    ? a.state[seg * a.seg_state_in + bh * (int64_t)a.dy * a.dz + y * a.s_y + (z0 + z) * a.s_z] : 0.f;
-            }
-    float whole = 1.f;   // state_only: the decay over the whole segment
-
-    const int64_t chunks = (t_end - t_begin + 15) / 16;
-    V rx[NY], ry[NY], rz[NZ], rw[NZ];
+    for (int n = 0; n < 2; ++n) {
+        const int idx = tid + threads * n;
+        ztok[n] = idx / (4 * nz);
+        const int col = (idx - ztok[n] * 4 * nz) * 4;
+        zleft[n] = ztok[n] < 32 ? dz - col : 0;
+        qz[n] = pz + (t_first + ztok[n]) * a.z.sl + col;
+    }
     float rg = 0.f, rm = 1.f;
+    const float *qg = a.g + (t_first + (lane & 31)) * a.gl + b * a.gb + h * a.gh, *qm = a.masks ? a.masks + (t_first + (lane & 31)) * a.ml + b * a.mb : nullptr;
     auto fetch = [&](int64_t t0) {
+        const int count = (int)min((int64_t)32, t_end - t0);
 #pragma unroll
-        for (int n = 0; n < NY; ++n) {
-            const int idx = lane + 64 * n, tok = idx / (4 * NY), col = (idx % (4 * NY)) * 4;
-            const int64_t t = t0 + tok;
-            const int left = t < t_end ? dy - col : 0;
-            if (!a.state_only) rx[n] = load4<T>(px + t * a.x.sl + col, left, a.x.vec);
-            ry[n] = load4<T>(py + t * a.y.sl + col, left, a.y.vec);
+        for (int n = 0; n < NK; ++n) {
+            const int left = xtok[n] < count ? xleft[n] : 0;
+            if (!a.state_only) rx[n] = load4<T>(qx[n], left, VEC);
+            ry[n] = load4<T>(qy[n], left, VEC);
+            qx[n] += dir * a.x.sl; qy[n] += dir * a.y.sl;
         }
 #pragma unroll
-        for (int n = 0; n < NZ; ++n) {
-            const int idx = lane + 64 * n, tok = idx / (4 * NZ), col = (idx % (4 * NZ)) * 4;
-            const int64_t t = t0 + tok;
-            const int left = t < t_end ? dz - col : 0;
-            rz[n] = load4<T>(pz + t * a.z.sl + col, left, a.z.vec);
-            if (pw) rw[n] = load4<T>(pw + t * a.w.sl + col, left, a.w.vec);
+        for (int n = 0; n < 2; ++n) {
+            rz[n] = load4<T>(qz[n], ztok[n] < count ? zleft[n] : 0, VEC);
+            qz[n] += dir * a.z.sl;
         }
-        const int64_t t = t0 + c;
-        rg = t < t_end ? a.g[t * a.gl + b * a.gb + h * a.gh] : 0.f;
-        rm = t < t_end && a.masks ? a.masks[t * a.ml + b * a.mb] : 1.f;
+        if (wave == 0) {
+            rg = (lane & 31) < count ? *qg : 0.f;
+            rm = qm && (lane & 31) < count ? *qm : 1.f;
+            qg += dir * a.gl;
+            if (qm) qm += dir * a.ml;
+        }
     };
-    auto chunk_at = [&](int64_t n) { return t_begin + 16 * (a.reverse ? chunks - 1 - n : n); };
+    auto slot = [](int s) { return 8 * ((s >> 2) & 3) + 4 * (s >> 4) + (s & 3); };   // place of index s of 32 in a stored row
+    auto chunk_at = [&](int64_t n) { return t_begin + 32 * (a.reverse ? chunks - 1 - n : n); };
     fetch(chunk_at(0));
     for (int64_t n = 0; n < chunks; ++n) {
         const int64_t t0 = chunk_at(n);
-        float bad = 0.f;   // not zero (NaN) where a value of y or z is not finite
-        float ndt = 0.f;   // this lane's token's own weight (x . y), for the diagonal
-        const float gt = rg, mt = rm;
-        V sy[NY], sz[NZ];
-#pragma unroll
-        for (int k = 0; k < NY; ++k) { sy[k] = ry[k]; const f32x4 f = widen(ry[k]); bad += f[0] * 0.f + f[1] * 0.f + f[2] * 0.f + f[3] * 0.f; }
-#pragma unroll
-        for (int k = 0; k < NZ; ++k) { sz[k] = rz[k]; const f32x4 f = widen(rz[k]); bad += f[0] * 0.f + f[1] * 0.f + f[2] * 0.f + f[3] * 0.f; }
-        const bool careful = __ballot(!(bad == 0.f)) != 0;
-        wave_sync();
-        if (!a.state_only)
-#pragma unroll
-            for (int k = 0; k < NY; ++k) { const int idx = lane + 64 * k; *(f32x4 *)(lx + (idx / (4 * NY)) * PY + (idx % (4 * NY)) * 4) = widen(rx[k]); }
-        if (pw)
-#pragma unroll
-            for (int k = 0; k < NZ; ++k) { const int idx = lane + 64 * k; *(f32x4 *)(lw + (idx / (4 * NZ)) * PZ + (idx % (4 * NZ)) * 4) = widen(rw[k]); }
-        if (n + 1 < chunks) fetch(chunk_at(n + 1));   // in flight while this chunk is computed
-
-        const int subs = careful ? 16 : 1;
+        const int flag = 1 + (int)(n & 1);
+        int subs = 1;
         for (int sub = 0; sub < subs; ++sub) {
-            const int only = a.reverse ? 15 - sub : sub;
-            const bool live = !careful || c == only;      // this lane's token takes part in this pass
-            wave_sync();
+            const int only = subs == 1 ? -1 : a.reverse ? 31 - sub : sub;   // token by token: the others are zeros
+            __syncthreads();                                                // the chunk before is done with the LDS
+            bool bad = false;
+            const V zero = {(T)0.f, (T)0.f, (T)0.f, (T)0.f};
 #pragma unroll
-            for (int k = 0; k < NY; ++k) {
-                const int idx = lane + 64 * k, tok = idx / (4 * NY);
-                *(f32x4 *)(ly + tok * PY + (idx % (4 * NY)) * 4) = !careful || tok == only ? widen(sy[k]) : f32x4{0.f, 0.f, 0.f, 0.f};
-            }
+            for (int k = 0; k < NK; ++k) {
+                const int tok = xtok[k], col = ((tid + threads * k) % (8 * NK)) * 4, at = tok * XS + (col & ~31) + slot(col & 31);
+                if (tok < 32) {
+                    bf16x4 cx[NP], cy[NP];
+                    cut4<T, NP>(only < 0 || tok == only ? ry[k] : zero, cy);
+                    bad |= not_finite(ry[k]);
+                    if (!a.state_only) {
+                        cut4<T, NP>(rx[k], cx);
 #pragma unroll
-            for (int k = 0; k < NZ; ++k) {
-                const int idx = lane + 64 * k, tok = idx / (4 * NZ);
-                *(f32x4 *)(lz + tok * PZ + (idx % (4 * NZ)) * 4) = !careful || tok == only ? widen(sz[k]) : f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-            // prefix sums of the log decays (base 2), tokens that start afresh as bits
-            const bool fresh = live && (mt == 0.f || gt == -__builtin_inff());
-            const uint32_t fr = (uint32_t)(__ballot(fresh) & 0xffff);
-            double C = live && !fresh ? (double)gt * 1.4426950408889634074 : 0.0;
-#pragma unroll
-            for (int off = 1; off < 16; off <<= 1) { const double o = __shfl_up(C, off, 16); if (c >= off) C += o; }
-            if (lane < 16) lc[lane] = C;
-            wave_sync();
-            const double C15 = lc[15];
-            // `head`: decay from before the chunk up to and with token c; `tail`: from behind token c to the chunk's end
-            const bool head_ok = (fr & ((2u << c) - 1)) == 0, tail_ok = (fr >> (c + 1)) == 0;
-            const float head = head_ok ? exp2_fast((float)C) : 0.f, tail = tail_ok ? exp2_fast((float)(C15 - C)) : 0.f;
-            const bool all_ok = fr == 0;
-            const float all = all_ok ? exp2_fast((float)C15) : 0.f;
-            const bool in_ok = a.reverse ? tail_ok : head_ok;      // the carried state reaches this lane's token
-            const float win = a.reverse ? tail : head, wout = (a.reverse ? head : tail) * a.y_scale;
-
-            if (!a.state_only) {
-                f32x4 P = {0.f, 0.f, 0.f, 0.f};
-                f32x4 xr[NY];
-#pragma unroll
-                for (int i = 0; i < NY; ++i) {
-                    xr[i] = *(const f32x4 *)(lx + c * PY + 16 * i + g4);
-                    const f32x4 yr = *(const f32x4 *)(ly + c * PY + 16 * i + g4);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) P = __builtin_amdgcn_mfma_f32_16x16x4f32(yr[r], xr[i][r], P, 0, 0, 0);
-                }
-                float own = 0.f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int s = g4 + r;
-                    const double Cs = lc[s];
-                    const int lo = min(s, c), hi = max(s, c);
-                    const bool order = a.reverse ? s >= c : s <= c;
-                    const bool ok = order && ((fr >> (lo + 1)) & ((1u << (hi - lo)) - 1)) == 0;
-                    const float wt = exp2_fast((float)(a.reverse ? Cs - C : C - Cs)) * a.y_scale;
-                    P[r] = ok ? P[r] * wt : 0.f;
-                    if (s == c) { own = P[r]; if (pw) P[r] = 0.f; }
-                }
-                if (pw) { own += __shfl_xor(own, 16); own += __shfl_xor(own, 32); ndt = own; }
-                float dot = 0.f;
-#pragma unroll
-                for (int j = 0; j < NZ; ++j) {
-                    f32x4 o = {0.f, 0.f, 0.f, 0.f}, in = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o = __builtin_amdgcn_mfma_f32_16x16x4f32(lz[(g4 + r) * PZ + 16 * j + c], P[r], o, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < NY; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) in = __builtin_amdgcn_mfma_f32_16x16x4f32(S[i][j][r], xr[i][r], in, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[r] = (in_ok ? o[r] + win * in[r] : o[r]) * a.out_scale;
-                    const int z = 16 * j + g4;
-                    if (pw) {
-                        const f32x4 wv = *(const f32x4 *)(lw + c * PZ + z), zv = *(const f32x4 *)(lz + c * PZ + z);
-                        dot += o[0] * wv[0] + o[1] * wv[1] + o[2] * wv[2] + o[3] * wv[3];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[r] += ndt * a.out_scale * zv[r];
+                        for (int i = 0; i < NP; ++i) { *(bf16x4 *)(lx + i * 32 * XS + at) = cx[i]; *(bf16x4 *)(ly + i * 32 * XS + at) = cy[i]; }
                     }
-                    const int64_t t = t0 + c;
-                    if (t < t_end && live) store4<T>(po + t * a.out.sl + z, o, dz - z, a.out.vec);
-                }
-                if (pw) {
-                    dot += __shfl_xor(dot, 16); dot += __shfl_xor(dot, 32);
-                    const int64_t t = t0 + c;
-                    if (lane < 16 && t < t_end && live) a.dot[((slice * a.L + t) * a.B + b) * a.H + h] = dot;
+#pragma unroll
+                    for (int i = 0; i < NP; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) lyt[(i * 32 * NK + col + r) * 40 + slot(tok)] = cy[i][r];
                 }
             }
-            // S = all * S + sum_s wout_s y_s z_s
-            float u[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) u[r] = __shfl(wout, g4 + r);
+            for (int k = 0; k < 2; ++k) {
+                const int tok = ztok[k], col = (tid + threads * k - tok * 4 * nz) * 4;
+                if (tok < 32) {
+                    bf16x4 cz[NP];
+                    cut4<T, NP>(only < 0 || tok == only ? rz[k] : zero, cz);
+                    bad |= not_finite(rz[k]);
 #pragma unroll
-            for (int i = 0; i < NY; ++i) {
-                float yv[4];
+                    for (int i = 0; i < NP; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) yv[r] = ly[(g4 + r) * PY + 16 * i + c] * u[r];
-#pragma unroll
-                for (int j = 0; j < NZ; ++j) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) S[i][j][r] = all_ok ? S[i][j][r] * all : 0.f;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) S[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(yv[r], lz[(g4 + r) * PZ + 16 * j + c], S[i][j], 0, 0, 0);
+                        for (int r = 0; r < 4; ++r) lzt[(i * 16 * nz + col + r) * 40 + slot(tok)] = cz[i][r];
                 }
             }
-            whole *= all;
+            if (subs == 1 && __ballot(bad) && lane == 0) lfr[flag] = 1;
+            if (tid == 0) lfr[3 - flag] = 0;
+            if (wave == 0) {
+                // prefix sums of the log decays (base 2), tokens that start afresh as bits; `head`: decay from before the chunk up to and with the token, `tail`: from behind it on
+                const bool live = only < 0 || (lane & 31) == only;
+                const bool fresh = live && (rm == 0.f || rg == -__builtin_inff());
+                const uint32_t fr = (uint32_t)__ballot(fresh);
+                const int s = lane & 31;
+                const double C = scan32(live && !fresh ? (double)rg * 1.4426950408889634074 : 0.0, lane);
+                const uint64_t u = __builtin_bit_cast(uint64_t, C);
+                const double last = __builtin_bit_cast(double, ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 31) << 32) |
+                                                                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 31));
+                const bool head_ok = (fr & (0xffffffffu >> (31 - s))) == 0, tail_ok = s == 31 || (fr >> (s + 1)) == 0;
+                const float head = head_ok ? exp2_fast((float)C) : 0.f, tail = tail_ok ? exp2_fast((float)(last - C)) : 0.f;
+                if (lane < 32) {
+                    lc[s] = C;
+                    lwin[s] = (a.reverse ? tail_ok : head_ok) ? (a.reverse ? tail : head) : -1.f;   // -1: nothing carried reaches the token
+                    lwout[s] = (a.reverse ? head : tail) * a.y_scale;
+                }
+                if (lane == 0) lfr[0] = fr;
+                if (lane == 31) lall[0] = fr == 0 ? exp2_fast((float)C) : -1.f;
+            }
+            __syncthreads();
+            if (subs == 1 && lfr[flag]) {   // a value that is not finite: again, token by token
+                subs = 32;
+                sub = -1;
+                continue;
+            }
+            if (subs == 1 && n + 1 < chunks) fetch(chunk_at(n + 1));   // in flight while this chunk is computed
+            const uint32_t fr = lfr[0];
+            const float all = lall[0];
+            if (!a.state_only) {
+                // P^T: (s tile, t tile) = (0, 0), (1, 1) and the one between
+                for (int tile = wave; tile < 3; tile += waves) {
+                    const int ts = tile == 2 ? (a.reverse ? 1 : 0) : tile, tt = tile == 2 ? 1 - ts : tile;
+                    f32x4 P = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kk = 0; kk < NK; ++kk) {
+                        bf16x8 fy[NP], fx[NP];
+#pragma unroll
+                        for (int i = 0; i < NP; ++i) {
+                            fy[i] = *(const bf16x8 *)(ly + (i * 32 + 16 * ts + c) * XS + 32 * kk + 8 * g);
+                            fx[i] = *(const bf16x8 *)(lx + (i * 32 + 16 * tt + c) * XS + 32 * kk + 8 * g);
+                        }
+                        P = mma_pieces<NP, NP, PC::in_order>(fy, fx, P);
+                    }
+                    const int t = 16 * tt + c;
+                    const double Ct = lc[t];
+                    __bf16 cp[4][PP];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int s = 16 * ts + g4 + r;
+                        const double Cs = lc[s];
+                        const int lo = min(s, t), hi = max(s, t);
+                        const bool ok = (a.reverse ? s >= t : s <= t) && ((fr >> lo >> 1) & ((1u << (hi - lo)) - 1)) == 0;
+                        const float wt = exp2_fast((float)(a.reverse ? Cs - Ct : Ct - Cs)) * a.y_scale;
+                        float p = ok ? P[r] * wt : 0.f;
+                        if (DOT && s == t) { lown[t] = p; p = 0.f; }   // the token's own term: apart
+                        cut(p, cp[r]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < PP; ++i) *(bf16x4 *)(lp + (i * 32 + t) * 40 + 8 * g + 4 * ts) = bf16x4{cp[0][i], cp[1][i], cp[2][i], cp[3][i]};
+                }
+                __syncthreads();
+            }
+            if (holds) {
+                bf16x8 zt[NP];
+#pragma unroll
+                for (int i = 0; i < NP; ++i) zt[i] = *(const bf16x8 *)(lzt + (i * 16 * nz + zc + c) * 40 + 8 * g);
+                if (!a.state_only) {
+                    f32x4 in[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                    for (int kk = 0; kk < NK; ++kk) {
+                        bf16x8 st[PP];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            __bf16 c0[PP], c1[PP];
+                            cut(S[2 * kk][r], c0); cut(S[2 * kk + 1][r], c1);
+#pragma unroll
+                            for (int i = 0; i < PP; ++i) { st[i][r] = c0[i]; st[i][4 + r] = c1[i]; }
+                        }
+#pragma unroll
+                        for (int tt = 0; tt < 2; ++tt) {
+                            bf16x8 fx[NP];
+#pragma unroll
+                            for (int i = 0; i < NP; ++i) fx[i] = *(const bf16x8 *)(lx + (i * 32 + 16 * tt + c) * XS + 32 * kk + 8 * g);
+                            in[tt] = mma_pieces<PP, NP, PC::out_order>(st, fx, in[tt]);
+                        }
+                    }
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt) {
+                        const int tl = 16 * tt + c;
+                        const int64_t t = t0 + tl;
+                        const bool store = t < t_end && (only < 0 || tl == only);
+                        const int z = zc + g4;
+                        V wv, zv;
+                        if (DOT) {
+                            wv = load4<T>(pw + t * a.w.sl + z, store ? dz - z : 0, VEC);
+                            zv = load4<T>(pz + t * a.z.sl + z, store ? dz - z : 0, VEC);
+                        }
+                        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+                        bf16x8 fp[PP];
+#pragma unroll
+                        for (int i = 0; i < PP; ++i) fp[i] = *(const bf16x8 *)(lp + (i * 32 + tl) * 40 + 8 * g);
+                        o = mma_pieces<NP, PP, PC::out_order>(zt, fp, o);
+                        const float win = lwin[tl];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[r] = (win != -1.f ? o[r] + win * in[tt][r] : o[r]) * a.out_scale;
+                        if (DOT) {
+                            const f32x4 wf = widen(wv), zf = widen(zv);
+                            float dot = o[0] * wf[0] + o[1] * wf[1] + o[2] * wf[2] + o[3] * wf[3];
+                            dot += __shfl_xor(dot, 16); dot += __shfl_xor(dot, 32);
+                            if (g == 0) ldot[wave * 32 + tl] = dot;
+                            const float own = lown[tl] * a.out_scale;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) o[r] += own * zf[r];
+                        }
+                        if (store) store4<T>(po + t * a.out.sl + z, o, dz - z, VEC);
+                    }
+                }
+                // S = all * S + y^T (u z): u z in the place of z's column, exact to float32
+                bf16x8 uz[3];
+                const f32x4 u0 = *(const f32x4 *)(lwout + g4), u1 = *(const f32x4 *)(lwout + 16 + g4);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    float zf = (float)zt[0][r];
+#pragma unroll
+                    for (int i = 1; i < NP; ++i) zf += (float)zt[i][r];
+                    __bf16 cu[3];
+                    cut(zf * (r < 4 ? u0[r & 3] : u1[r & 3]), cu);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) uz[i][r] = cu[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 2 * NK; ++i) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[i][r] = all != -1.f ? S[i][r] * all : 0.f;
+                    bf16x8 yt[NP];
+#pragma unroll
+                    for (int k = 0; k < NP; ++k) yt[k] = *(const bf16x8 *)(lyt + (k * 32 * NK + 16 * i + c) * 40 + 8 * g);
+                    S[i] = mma_pieces<NP, 3, 2>(yt, uz, S[i]);
+                }
+            }
+            whole *= all != -1.f ? all : 0.f;
+            if (DOT) {
+                __syncthreads();
+                const int64_t t = t0 + lane;
+                if (wave == 0 && lane < 32 && t < t_end && (only < 0 || lane == only)) {
+                    float d = 0.f;
+                    for (int w = 0; w < nz; ++w) d += ldot[w * 32 + lane];
+                    a.dot[(t * a.B + b) * a.H + h] = d;
+                }
+            }
         }
+        if (subs > 1 && n + 1 < chunks) fetch(chunk_at(n + 1));
     }
-    if (a.state_out) {
+    if (a.state_out && holds) {
 #pragma unroll
-        for (int i = 0; i < NY; ++i)
+        for (int i = 0; i < 2 * NK; ++i)
 #pragma unroll
-            for (int j = 0; j < NZ; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int y = 16 * i + g4 + r, z = 16 * j + c;
-                    if (y < dy && z < dz)
-                        a.state_out[seg * a.seg_state_out + bh * (int64_t)a.dy * a.dz + y * a.o_y + (z0 + z) * a.o_z] = S[i][j][r];
-                }
+            for (int r = 0; r < 4; ++r) {
+                const int y = 16 * i + g4 + r, z = zc + c;
+                if (y < dy && z < dz) a.state_out[seg * a.seg_state_out + bh * (int64_t)dy * dz + y * a.o_y + z * a.o_z] = S[i][r];
+            }
     }
-    if (a.seg_decay && slice == 0 && lane == 0) a.seg_decay[seg * heads + bh] = whole;
+    if (a.seg_decay && tid == 0) a.seg_decay[seg * heads + bh] = whole;
 }
 
 // ---- small heads ------------------------------------------------------------------------------------------------------------
 // dy <= 32: the recurrence itself, token by token, on the vector units.  16 lanes (a DPP row) hold one head: lane c column c of its slice of the state, 16 NY
 // values of y each; y and x are broadcast from the lane that holds them by the multiply's own operand (row_newbcast), so a token costs three
-// instructions per 64 state entries and no LDS.  Four neighbouring heads share a wave: 256 bytes of a token's row side by side.  Against the matrix walk at
-// heads of 16 x 16, where half of every 16-token tile is above the diagonal and chunks of ten tokens waste the rest: 239 -> 156 us for 30 720 x 4 heads of ten
+// instructions per 64 state entries and no LDS.  Four neighbouring heads share a wave: 256 bytes of a token's row side by side.  Against a walk on the
+// matrix units, where half of every 16-token tile is above the diagonal and chunks of ten tokens waste the rest: 239 -> 156 us for 30 720 x 4 heads of ten
 // tokens (float32, 566 MB: 111 us at the copy rate of 5.1 TB/s).
 template <int M> __device__ __forceinline__ float row_lane(float v) {   // lane M of each row of 16, in every lane of the row
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + M, 0xf, 0xf, true));
@@ -757,26 +910,25 @@ int memory_check(const FmarlMemory *m, const char *who) {
     return FMARL_OK;
 }
 
-// Waves that walk at once: a batch with fewer heads than 2 048 (8 waves per CU) has its tokens cut into segments that are walked side by side, at least 64 tokens
-// each (a segment costs a second read of k and v and a state in the workspace, which shorter ones would not repay).
+// The recurrence on the vector units for y up to 32 wide, the matrix units beyond: at 16 x 16 the former takes two thirds of the latter's time, at 64 x 64
+// its three instructions per 64 state entries and token would cost twice the matrix units' time
+bool small_heads(int dy) { return dy <= 32; }
+
+// A batch with few heads has its tokens cut into segments that are walked side by side: so many that 2 048 waves of four small heads or 1 024 workgroups of a large one
+// are at work (8 waves, 4 workgroups per CU), at least 64 tokens each (a segment costs a second read of k and v and a state in the workspace, which shorter
+// ones would not repay).
 struct Segments { int nseg, len; };
 Segments memory_segments(const FmarlMemory *m) {
-    const int64_t heads = m->B * m->H;
-    int64_t n = (2048 + heads - 1) / heads, most = m->L / 64;
+    const int64_t heads = m->B * m->H, units = small_heads(m->dk) ? (heads + 3) / 4 : heads, want = small_heads(m->dk) ? 2048 : 1024;
+    int64_t n = (want + units - 1) / units, most = m->L / 64;
     if (n > most) n = most;
     if (n < 2) return {1, (int)(m->L > 0x40000000 ? 0x40000000 : m->L)};
-    const int64_t len = ((m->L + n - 1) / n + 15) / 16 * 16;
+    const int64_t len = ((m->L + n - 1) / n + 31) / 32 * 32;
     return {(int)((m->L + len - 1) / len), (int)len};
 }
 
-// The recurrence on the vector units for y up to 32 wide, the matrix walk beyond: at 16 x 16 the former takes half the latter's time, at 64 x 64
-// its three instructions per 64 state entries would cost twice the matrix units' time
-bool small_heads(int dy) { return dy <= 32; }
-
-int tiles(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : 8; }
-// columns of z that one wave takes, in tiles of 16: the state's dy x dz accumulators have to fit its registers beside the operands
-int slice_tiles(int dy, int dz) { const int t = tiles(dz), most = tiles(dy) == 8 ? 2 : 4; return t > most ? most : t; }
-int slices_of(int dy, int dz) { const int w = small_heads(dy) ? 16 : 16 * slice_tiles(dy, dz); return (dz + w - 1) / w; }
+// columns of z that a wave of the small heads' kernel takes: 16; the large heads' workgroup takes them all
+int slices_of(int dy, int dz) { return small_heads(dy) ? (dz + 15) / 16 : 1; }
 
 // up to 16 tokens of heads up to 16 x 16: every gradient in one kernel, whose registers hold all of it
 bool short_backward(const FmarlMemory *m) { return m->L <= 16 && m->dk <= 16 && m->dv <= 16; }
@@ -806,34 +958,43 @@ Workspace memory_layout(const FmarlMemory *m, int backward) {
     return w;
 }
 
-template <typename T, int NY>
-void launch_walk_nz(const Walk &w, unsigned blocks, hipStream_t st) {
-    switch (slice_tiles(w.dy, w.dz)) {
-    case 1: hipLaunchKernelGGL((memory_walk_kernel<T, NY, 1>), dim3(blocks), dim3(256), 0, st, w); break;
-    case 2: hipLaunchKernelGGL((memory_walk_kernel<T, NY, 2>), dim3(blocks), dim3(256), 0, st, w); break;
-    default:
-        if constexpr (NY < 8) hipLaunchKernelGGL((memory_walk_kernel<T, NY, 4>), dim3(blocks), dim3(256), 0, st, w);
-    }
+template <typename T, int NK, bool DOT, bool VEC>
+int launch_tiles(const Walk &w, int64_t blocks, hipStream_t st) {
+    const int nz = (w.dz + 15) / 16, lds = tiles_lds<T, DOT>(NK, nz);
+    if (lds > 64 * 1024) HIP_OK(hipFuncSetAttribute((const void *)memory_tiles_kernel<T, NK, DOT, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL((memory_tiles_kernel<T, NK, DOT, VEC>), dim3((unsigned)blocks), dim3(64 * (nz < 4 ? 4 : nz)), lds, st, w);
+    return FMARL_OK;
+}
+
+template <typename T, int NK>
+int launch_tiles_as(const Walk &w, int64_t blocks, hipStream_t st) {
+    const bool vec = (w.state_only || (w.x.vec && w.out.vec)) && w.y.vec && w.z.vec && (!w.w.p || w.w.vec);
+    if (w.w.p) return vec ? launch_tiles<T, NK, true, true>(w, blocks, st) : launch_tiles<T, NK, true, false>(w, blocks, st);
+    return vec ? launch_tiles<T, NK, false, true>(w, blocks, st) : launch_tiles<T, NK, false, false>(w, blocks, st);
 }
 
 template <typename T>
-void launch_walk_t(const Walk &w, unsigned blocks, hipStream_t st) {
-    if (w.dy <= 16 && w.w.p) hipLaunchKernelGGL((memory_rows_kernel<T, 1, true>), dim3(blocks), dim3(256), 0, st, w);
-    else if (w.dy <= 16) hipLaunchKernelGGL((memory_rows_kernel<T, 1, false>), dim3(blocks), dim3(256), 0, st, w);
-    else if (w.dy <= 32 && w.w.p) hipLaunchKernelGGL((memory_rows_kernel<T, 2, true>), dim3(blocks), dim3(256), 0, st, w);
-    else if (w.dy <= 32) hipLaunchKernelGGL((memory_rows_kernel<T, 2, false>), dim3(blocks), dim3(256), 0, st, w);
-    else if (w.dy <= 64) launch_walk_nz<T, 4>(w, blocks, st);
-    else launch_walk_nz<T, 8>(w, blocks, st);
+int launch_walk_t(const Walk &w, hipStream_t st) {
+    const int64_t heads = w.B * w.H;
+    if (small_heads(w.dy)) {
+        const int64_t blocks = ((heads + 3) / 4 * w.nseg * w.slices + 3) / 4;
+        if (blocks > 0xffffff) return policy_fail(FMARL_EINVAL, "memory: too many sequences");
+        const dim3 grid((unsigned)blocks);
+        if (w.dy <= 16 && w.w.p) hipLaunchKernelGGL((memory_rows_kernel<T, 1, true>), grid, dim3(256), 0, st, w);
+        else if (w.dy <= 16) hipLaunchKernelGGL((memory_rows_kernel<T, 1, false>), grid, dim3(256), 0, st, w);
+        else if (w.w.p) hipLaunchKernelGGL((memory_rows_kernel<T, 2, true>), grid, dim3(256), 0, st, w);
+        else hipLaunchKernelGGL((memory_rows_kernel<T, 2, false>), grid, dim3(256), 0, st, w);
+        return FMARL_OK;
+    }
+    const int64_t blocks = heads * w.nseg;
+    if (blocks > 0x7fffff) return policy_fail(FMARL_EINVAL, "memory: too many sequences for heads of this size");
+    return w.dy <= 64 ? launch_tiles_as<T, 2>(w, blocks, st) : launch_tiles_as<T, 4>(w, blocks, st);
 }
 
 int launch_walk(Walk w, int dtype, hipStream_t st) {
     w.slices = slices_of(w.dy, w.dz);
-    const int64_t heads = w.B * w.H, units = small_heads(w.dy) ? (heads + 3) / 4 : heads;   // waves per segment and slice
-    const int64_t blocks = (units * w.nseg * w.slices + 3) / 4;
-    if (blocks > 0xffffff) return policy_fail(FMARL_EINVAL, "memory: too many sequences");
-    if (dtype == FMARL_T_F32) launch_walk_t<float>(w, (unsigned)blocks, st);
-    else if (dtype == FMARL_T_BF16) launch_walk_t<__bf16>(w, (unsigned)blocks, st);
-    else launch_walk_t<_Float16>(w, (unsigned)blocks, st);
+    const int rc = dtype == FMARL_T_F32 ? launch_walk_t<float>(w, st) : dtype == FMARL_T_BF16 ? launch_walk_t<__bf16>(w, st) : launch_walk_t<_Float16>(w, st);
+    if (rc) return rc;
     HIP_OK(hipGetLastError());
     return FMARL_OK;
 }
