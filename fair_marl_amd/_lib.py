@@ -154,7 +154,7 @@ _SIGS = {
     'fmarl_memory_workspace': (C.c_size_t, [C.POINTER(FmarlMemory), C.c_int]),
     'fmarl_memory_chunk': (C.c_int, [C.POINTER(FmarlMemory), C.POINTER(FmarlRows), C.c_void_p, C.c_void_p, C.c_void_p]),
     'fmarl_memory_chunk_backward': (C.c_int, [C.POINTER(FmarlMemory), C.POINTER(FmarlRows), C.c_void_p, C.POINTER(FmarlRows), C.POINTER(FmarlRows),
-                                              C.POINTER(FmarlRows), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+                                              C.POINTER(FmarlRows), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     'fmarl_block_norm': (C.c_int, [C.POINTER(FmarlBlock), C.c_void_p, C.c_void_p, C.c_void_p]),
     'fmarl_block_norm_workspace': (C.c_size_t, [C.POINTER(FmarlBlock)]),
     'fmarl_block_norm_backward': (C.c_int, [C.POINTER(FmarlBlock), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,

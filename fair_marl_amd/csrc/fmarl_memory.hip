@@ -21,19 +21,21 @@ struct WalkRows {            // a (L, B, H, d) tensor whose last axis is contigu
     int vec;                 // rows start on multiples of four elements and hold a multiple of four
 };
 
+// A walk goes through its tokens in memory order; the host turns the arrays round for a backwards one (the last token first, negative strides).  Forwards a token's decay lies
+// before it, backwards behind it: with `shift` the state is decayed by the token before's, and by the last one's at the end.
 struct Walk {
-    WalkRows x, y, z, w, out;          // w: NULL, or what out is dotted with for the decay's gradient
+    WalkRows x, y, z, w, out;          // w: what out is dotted with for the decay's gradient, or NULL
     const float *g; int64_t gl, gb, gh;
     const float *masks; int64_t ml, mb;
-    const float *state;                // initial state, NULL: zeros; element (y, z) of (b, h) at (b * H + h) * state_elems + y * s_y + z * s_z
+    const float *state;                // initial state, NULL: zeros; element (y, z) of (b, h) at (b * H + h) * dy * dz + y * s_y + z * s_z
     float *state_out;                  // NULL: not wanted
     int64_t s_y, s_z, o_y, o_z;        // the strides of the two
     int64_t seg_state_in, seg_state_out;   // elements from one segment's states to the next one's (0: the same for all)
     float *seg_decay;                  // state_only: the segment's whole decay, (nseg, B * H)
-    float *dot;                        // (slices, L, B, H) sums of out * w without the token's own term
+    float *dot; int64_t dot_sl, dot_sh, dot_slice;   // sums of out * w without the token's own term: strides of token, (b, h) and slice
     int64_t L, B;
     int H, dy, dz, nseg, seg_len, slices;
-    int reverse, state_only;
+    int shift, state_only;
     float y_scale, out_scale;
 };
 
@@ -55,11 +57,6 @@ template <typename T, bool DOT> struct Pieces;
 template <bool DOT> struct Pieces<__bf16, DOT> { static constexpr int in = 1, p = DOT ? 3 : 2, in_order = 0, out_order = DOT ? 2 : 1; };
 template <bool DOT> struct Pieces<_Float16, DOT> { static constexpr int in = 2, p = DOT ? 3 : 2, in_order = 2, out_order = DOT ? 2 : 1; };
 template <bool DOT> struct Pieces<float, DOT> { static constexpr int in = 3, p = 3, in_order = 2, out_order = 2; };
-
-template <int N> __device__ __forceinline__ void cut(float v, __bf16 (&p)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) { p[i] = (__bf16)v; v -= (float)p[i]; }
-}
 
 // the pieces of four inputs, piece by piece; a bfloat16 value is its own
 template <typename T, int N> __device__ __forceinline__ void cut4(typename Vec4<T>::type v, bf16x4 (&p)[N]) {
@@ -112,145 +109,158 @@ template <typename T, bool DOT> __host__ __device__ constexpr int tiles_lds(int 
     return Pieces<T, DOT>::in * 2 * (2 * 32 * (32 * nk + 8) + (32 * nk + 16 * nz) * 40) + Pieces<T, DOT>::p * 2 * 32 * 40 + 32 * 8 + 4 * 32 * 4 + 8 * 32 * 4;
 }
 
-template <typename T, int NK, bool DOT, bool VEC>
-__global__ __launch_bounds__(512) void memory_tiles_kernel(Walk a) {
+enum { kOut = 0, kOutDot = 1, kState = 2 };   // what a walk leaves: out; out and its dots with w; the state alone
+
+template <typename T, int NK, int MODE, bool VEC>
+__global__ __launch_bounds__(512) void memory_tiles_kernel(Walk arg) {
+    constexpr bool DOT = MODE == kOutDot, OUT = MODE != kState;
     typedef Pieces<T, DOT> PC;
     constexpr int NP = PC::in, PP = PC::p, XS = 32 * NK + 8;
     typedef typename Vec4<T>::type V;
     extern __shared__ __align__(16) char smem[];
-    const int nz = (a.dz + 15) / 16, threads = blockDim.x;
+    // the arguments are read where they are used, through a pointer the compiler cannot see through: all at once they do not fit the scalar registers (a hundred
+    // were spilled into vector lanes, 400 v_readlane in the loop: 55 us instead of 33 us at 8 x 8 heads of 4 096 tokens)
+    typedef const Walk __attribute__((address_space(4))) *WalkArg;
+    uint64_t at_args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at_args));
+    const Walk &a = *(const Walk *)(WalkArg)at_args;
+    (void)arg;
+    const int dy = a.dy, dz = a.dz, nz = (dz + 15) / 16, threads = blockDim.x;
     __bf16 *lx = (__bf16 *)smem, *ly = lx + NP * 32 * XS, *lyt = ly + NP * 32 * XS, *lzt = lyt + NP * 32 * NK * 40, *lp = lzt + NP * 16 * nz * 40;
     double *lc = (double *)(lp + PP * 32 * 40);
     float *lwin = (float *)(lc + 32), *lwout = lwin + 32, *lown = lwout + 32, *ldot = lown + 64, *lall = lown + 32;   // ldot: (waves, 32)
     uint32_t *lfr = (uint32_t *)(lown + 40);   // [0] tokens that start afresh; [1], [2]: a value is not finite, by the chunk's parity (cleared in the chunk between)
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6, c = lane & 15, g = lane >> 4, g4 = g * 4;
-    const int64_t heads = a.B * a.H, bh = blockIdx.x % heads;
-    const int seg = (int)(blockIdx.x / heads);
-    const int64_t b = bh / a.H;
-    const int h = (int)(bh - b * a.H), dy = a.dy, dz = a.dz;
-    const int64_t t_begin = (int64_t)seg * a.seg_len, t_end = min(a.L, t_begin + a.seg_len), chunks = (t_end - t_begin + 31) / 32;
-    const T *px = a.state_only ? nullptr : (const T *)a.x.p + b * a.x.sb + h * a.x.sh, *py = (const T *)a.y.p + b * a.y.sb + h * a.y.sh;
-    const T *pz = (const T *)a.z.p + b * a.z.sb + h * a.z.sh, *pw = DOT ? (const T *)a.w.p + b * a.w.sb + h * a.w.sh : nullptr;
-    T *po = a.state_only ? nullptr : (T *)a.out.p + b * a.out.sb + h * a.out.sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4, g4 = g * 4;
+    const int heads = (int)(a.B * a.H), bh = blockIdx.x % heads, seg = blockIdx.x / heads;
+    const int64_t b = bh / a.H, h = bh - b * a.H;
+    const int64_t t_begin = (int64_t)seg * a.seg_len;
+    const int length = (int)min(a.L - t_begin, (int64_t)a.seg_len), chunks = (length + 31) / 32;
     const int zc = 16 * wave;                  // this wave's columns of z; waves beyond nz only load and help with P
     const bool holds = wave < nz;
 
     f32x4 S[2 * NK];
+    if (a.state) {
+        const float *ps = a.state + seg * a.seg_state_in + bh * (int64_t)(dy * dz) + (zc + c) * a.s_z;
+        const int64_t s_y = a.s_y;
 #pragma unroll
-    for (int i = 0; i < 2 * NK; ++i)
+        for (int i = 0; i < 2 * NK; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int y = 16 * i + g4 + r, z = zc + c;
-            S[i][r] = holds && a.state && y < dy && z < dz ? a.state[seg * a.seg_state_in + bh * (int64_t)dy * dz + y * a.s_y + z * a.s_z] : 0.f;
-        }
+            for (int r = 0; r < 4; ++r) { const int y = 16 * i + g4 + r; S[i][r] = y < dy && zc + c < dz ? ps[y * s_y] : 0.f; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2 * NK; ++i) S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     if (tid < 3) lfr[tid] = 0;
-    for (int i = tid; i < PP * 32 * 40; i += threads) lp[i] = (__bf16)0.f;   // the tile beyond the diagonal stays zero
+    if (OUT) for (int i = tid; i < PP * 32 * 40; i += threads) lp[i] = (__bf16)0.f;   // the tile beyond the diagonal stays zero
     float whole = 1.f;
 
     // a thread's share of a chunk: NK pieces of four of x and of y each, two at most of z.  Where they lie is worked out once; from chunk to chunk the
     // pointers move on by 32 tokens
-    const int64_t t_first = a.reverse ? t_begin + 32 * (chunks - 1) : t_begin, dir = a.reverse ? -32 : 32;
-    V rx[NK], ry[NK], rz[2];
-    const T *qx[NK], *qy[NK], *qz[2];
-    int xtok[NK], xleft[NK], ztok[2], zleft[2];
+    auto slot = [](int s) { return 8 * ((s >> 2) & 3) + 4 * (s >> 4) + (s & 3); };   // place of index s of 32 in a stored row
+    V rx[OUT ? NK : 1], ry[NK], rz[2];
+    const T *qx[OUT ? NK : 1], *qy[NK], *qz[2];
+    int xtok[NK], ztok[2];   // the piece's token; beyond every chunk if it lies outside the row
+    int xat[NK], yat[NK], zat[2];
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
-        const int idx = tid + threads * n, col = (idx % (8 * NK)) * 4;
-        xtok[n] = idx / (8 * NK); xleft[n] = xtok[n] < 32 ? dy - col : 0;
-        qx[n] = px + (t_first + xtok[n]) * a.x.sl + col; qy[n] = py + (t_first + xtok[n]) * a.y.sl + col;
+        const int idx = tid + threads * n, col = (idx % (8 * NK)) * 4, tok = idx / (8 * NK);
+        xtok[n] = tok < 32 ? tok : 1 << 20;
+        xat[n] = tok * XS + (col & ~31) + slot(col & 31);
+        yat[n] = col * 40 + slot(tok & 31);
+        if (OUT) qx[n] = (const T *)a.x.p + b * a.x.sb + h * a.x.sh + (t_begin + tok) * a.x.sl + col;
+        qy[n] = (const T *)a.y.p + b * a.y.sb + h * a.y.sh + (t_begin + tok) * a.y.sl + col;
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-        const int idx = tid + threads * n;
-        ztok[n] = idx / (4 * nz);
-        const int col = (idx - ztok[n] * 4 * nz) * 4;
-        zleft[n] = ztok[n] < 32 ? dz - col : 0;
-        qz[n] = pz + (t_first + ztok[n]) * a.z.sl + col;
+        const int idx = tid + threads * n, tok = idx / (4 * nz), col = (idx - tok * 4 * nz) * 4;
+        ztok[n] = tok < 32 ? tok : 1 << 20;
+        zat[n] = col * 40 + slot(tok & 31);
+        qz[n] = (const T *)a.z.p + b * a.z.sb + h * a.z.sh + (t_begin + tok) * a.z.sl + col;
     }
+    const int shift = a.shift, tl = lane & 31;
+    const float *qg = a.g + b * a.gb + h * a.gh + (t_begin + tl - shift) * a.gl, *qm = a.masks ? a.masks + b * a.mb + (t_begin + tl - shift) * a.ml : nullptr;
+    const int64_t sx = 32 * a.x.sl, sy = 32 * a.y.sl, sz = 32 * a.z.sl, sg = 32 * a.gl, sm = 32 * a.ml;
     float rg = 0.f, rm = 1.f;
-    const float *qg = a.g + (t_first + (lane & 31)) * a.gl + b * a.gb + h * a.gh, *qm = a.masks ? a.masks + (t_first + (lane & 31)) * a.ml + b * a.mb : nullptr;
-    auto fetch = [&](int64_t t0) {
-        const int count = (int)min((int64_t)32, t_end - t0);
+    auto fetch = [&](int t0) {   // the chunk from token t0 of the segment on
+        const int count = length - t0;
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
-            const int left = xtok[n] < count ? xleft[n] : 0;
-            if (!a.state_only) rx[n] = load4<T>(qx[n], left, VEC);
-            ry[n] = load4<T>(qy[n], left, VEC);
-            qx[n] += dir * a.x.sl; qy[n] += dir * a.y.sl;
+            const int left = xtok[n] < count ? dy - ((tid + threads * n) % (8 * NK)) * 4 : 0;
+            if (OUT) { rx[n] = load4<T>(qx[n], left, VEC); qx[n] += sx; }
+            ry[n] = load4<T>(qy[n], left, VEC); qy[n] += sy;
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            rz[n] = load4<T>(qz[n], ztok[n] < count ? zleft[n] : 0, VEC);
-            qz[n] += dir * a.z.sl;
+            rz[n] = load4<T>(qz[n], ztok[n] < count ? dz - (zat[n] / 160) * 4 : 0, VEC);   // (zat / 40 is the column)
+            qz[n] += sz;
         }
         if (wave == 0) {
-            rg = (lane & 31) < count ? *qg : 0.f;
-            rm = qm && (lane & 31) < count ? *qm : 1.f;
-            qg += dir * a.gl;
-            if (qm) qm += dir * a.ml;
+            const bool in = tl < count && (!shift || t0 + tl > 0);
+            rg = in ? *qg : 0.f;
+            rm = in && qm ? *qm : 1.f;
+            qg += sg;
+            if (qm) qm += sm;
         }
     };
-    auto slot = [](int s) { return 8 * ((s >> 2) & 3) + 4 * (s >> 4) + (s & 3); };   // place of index s of 32 in a stored row
-    auto chunk_at = [&](int64_t n) { return t_begin + 32 * (a.reverse ? chunks - 1 - n : n); };
-    fetch(chunk_at(0));
-    for (int64_t n = 0; n < chunks; ++n) {
-        const int64_t t0 = chunk_at(n);
-        const int flag = 1 + (int)(n & 1);
+    // where this lane's part of out goes, of w and z (its own token's) comes from: token c of the chunk's first half
+    T *qo = OUT ? (T *)a.out.p + b * a.out.sb + h * a.out.sh + (t_begin + c) * a.out.sl + zc + g4 : nullptr;
+    const T *qw = DOT ? (const T *)a.w.p + b * a.w.sb + h * a.w.sh + (t_begin + c) * a.w.sl + zc + g4 : nullptr;
+    const T *qv = DOT ? (const T *)a.z.p + b * a.z.sb + h * a.z.sh + (t_begin + c) * a.z.sl + zc + g4 : nullptr;
+    const int64_t so = OUT ? 16 * a.out.sl : 0, sw = DOT ? 16 * a.w.sl : 0;
+    const float y_scale = a.y_scale, out_scale = a.out_scale;
+    const int zleft = dz - zc - g4;
+    fetch(0);
+    for (int n = 0; n < chunks; ++n) {
+        const int flag = 1 + (n & 1), count = length - 32 * n;
         int subs = 1;
         for (int sub = 0; sub < subs; ++sub) {
-            const int only = subs == 1 ? -1 : a.reverse ? 31 - sub : sub;   // token by token: the others are zeros
-            __syncthreads();                                                // the chunk before is done with the LDS
+            const int only = subs == 1 ? -1 : sub;   // token by token: the others are zeros
+            __syncthreads();                         // the chunk before is done with the LDS
             bool bad = false;
             const V zero = {(T)0.f, (T)0.f, (T)0.f, (T)0.f};
 #pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                const int tok = xtok[k], col = ((tid + threads * k) % (8 * NK)) * 4, at = tok * XS + (col & ~31) + slot(col & 31);
-                if (tok < 32) {
+            for (int k = 0; k < NK; ++k)
+                if (xtok[k] < 32) {
                     bf16x4 cx[NP], cy[NP];
-                    cut4<T, NP>(only < 0 || tok == only ? ry[k] : zero, cy);
+                    cut4<T, NP>(only < 0 || xtok[k] == only ? ry[k] : zero, cy);
                     bad |= not_finite(ry[k]);
-                    if (!a.state_only) {
+                    if (OUT) {
                         cut4<T, NP>(rx[k], cx);
 #pragma unroll
-                        for (int i = 0; i < NP; ++i) { *(bf16x4 *)(lx + i * 32 * XS + at) = cx[i]; *(bf16x4 *)(ly + i * 32 * XS + at) = cy[i]; }
+                        for (int i = 0; i < NP; ++i) { *(bf16x4 *)(lx + i * 32 * XS + xat[k]) = cx[i]; *(bf16x4 *)(ly + i * 32 * XS + xat[k]) = cy[i]; }
                     }
 #pragma unroll
                     for (int i = 0; i < NP; ++i)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) lyt[(i * 32 * NK + col + r) * 40 + slot(tok)] = cy[i][r];
+                        for (int r = 0; r < 4; ++r) lyt[(i * 32 * NK + r) * 40 + yat[k]] = cy[i][r];
                 }
-            }
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int tok = ztok[k], col = (tid + threads * k - tok * 4 * nz) * 4;
-                if (tok < 32) {
+            for (int k = 0; k < 2; ++k)
+                if (ztok[k] < 32) {
                     bf16x4 cz[NP];
-                    cut4<T, NP>(only < 0 || tok == only ? rz[k] : zero, cz);
+                    cut4<T, NP>(only < 0 || ztok[k] == only ? rz[k] : zero, cz);
                     bad |= not_finite(rz[k]);
 #pragma unroll
                     for (int i = 0; i < NP; ++i)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) lzt[(i * 16 * nz + col + r) * 40 + slot(tok)] = cz[i][r];
+                        for (int r = 0; r < 4; ++r) lzt[(i * 16 * nz + r) * 40 + zat[k]] = cz[i][r];
                 }
-            }
             if (subs == 1 && __ballot(bad) && lane == 0) lfr[flag] = 1;
             if (tid == 0) lfr[3 - flag] = 0;
             if (wave == 0) {
                 // prefix sums of the log decays (base 2), tokens that start afresh as bits; `head`: decay from before the chunk up to and with the token, `tail`: from behind it on
-                const bool live = only < 0 || (lane & 31) == only;
+                const bool live = only < 0 || tl == only;
                 const bool fresh = live && (rm == 0.f || rg == -__builtin_inff());
                 const uint32_t fr = (uint32_t)__ballot(fresh);
-                const int s = lane & 31;
                 const double C = scan32(live && !fresh ? (double)rg * 1.4426950408889634074 : 0.0, lane);
                 const uint64_t u = __builtin_bit_cast(uint64_t, C);
                 const double last = __builtin_bit_cast(double, ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 31) << 32) |
                                                                    (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 31));
-                const bool head_ok = (fr & (0xffffffffu >> (31 - s))) == 0, tail_ok = s == 31 || (fr >> (s + 1)) == 0;
-                const float head = head_ok ? exp2_fast((float)C) : 0.f, tail = tail_ok ? exp2_fast((float)(last - C)) : 0.f;
+                const bool head_ok = (fr & (0xffffffffu >> (31 - tl))) == 0, tail_ok = tl == 31 || (fr >> (tl + 1)) == 0;
                 if (lane < 32) {
-                    lc[s] = C;
-                    lwin[s] = (a.reverse ? tail_ok : head_ok) ? (a.reverse ? tail : head) : -1.f;   // -1: nothing carried reaches the token
-                    lwout[s] = (a.reverse ? head : tail) * a.y_scale;
+                    lc[tl] = C;
+                    lwin[tl] = head_ok ? exp2_fast((float)C) : -1.f;   // -1: nothing carried reaches the token
+                    lwout[tl] = tail_ok ? exp2_fast((float)(last - C)) * y_scale : 0.f;
                 }
                 if (lane == 0) lfr[0] = fr;
                 if (lane == 31) lall[0] = fr == 0 ? exp2_fast((float)C) : -1.f;
@@ -261,13 +271,13 @@ __global__ __launch_bounds__(512) void memory_tiles_kernel(Walk a) {
                 sub = -1;
                 continue;
             }
-            if (subs == 1 && n + 1 < chunks) fetch(chunk_at(n + 1));   // in flight while this chunk is computed
-            const uint32_t fr = lfr[0];
+            if (subs == 1 && n + 1 < chunks) fetch(32 * (n + 1));   // in flight while this chunk is computed
             const float all = lall[0];
-            if (!a.state_only) {
-                // P^T: (s tile, t tile) = (0, 0), (1, 1) and the one between
-                for (int tile = wave; tile < 3; tile += waves) {
-                    const int ts = tile == 2 ? (a.reverse ? 1 : 0) : tile, tt = tile == 2 ? 1 - ts : tile;
+            if (OUT) {
+                // P^T: (s tile, t tile) = (0, 0), (1, 1), (0, 1): one wave each
+                if (wave < 3) {
+                    const uint32_t fr = lfr[0];
+                    const int ts = wave == 1, tt = wave != 0;
                     f32x4 P = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int kk = 0; kk < NK; ++kk) {
@@ -281,20 +291,20 @@ __global__ __launch_bounds__(512) void memory_tiles_kernel(Walk a) {
                     }
                     const int t = 16 * tt + c;
                     const double Ct = lc[t];
-                    __bf16 cp[4][PP];
+                    bf16x4 cp[PP];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int s = 16 * ts + g4 + r;
-                        const double Cs = lc[s];
-                        const int lo = min(s, t), hi = max(s, t);
-                        const bool ok = (a.reverse ? s >= t : s <= t) && ((fr >> lo >> 1) & ((1u << (hi - lo)) - 1)) == 0;
-                        const float wt = exp2_fast((float)(a.reverse ? Cs - Ct : Ct - Cs)) * a.y_scale;
-                        float p = ok ? P[r] * wt : 0.f;
+                        // no token afresh in (s, t]: bits s + 1 .. t
+                        const uint32_t between = (0xfffffffeu << s) & (0xffffffffu >> (31 - t));
+                        const float wt = exp2_fast((float)(Ct - lc[s])) * y_scale;
+                        float p = s <= t && (fr & between) == 0 ? P[r] * wt : 0.f;
                         if (DOT && s == t) { lown[t] = p; p = 0.f; }   // the token's own term: apart
-                        cut(p, cp[r]);
+#pragma unroll
+                        for (int i = 0; i < PP; ++i) { cp[i][r] = (__bf16)p; p -= (float)cp[i][r]; }
                     }
 #pragma unroll
-                    for (int i = 0; i < PP; ++i) *(bf16x4 *)(lp + (i * 32 + t) * 40 + 8 * g + 4 * ts) = bf16x4{cp[0][i], cp[1][i], cp[2][i], cp[3][i]};
+                    for (int i = 0; i < PP; ++i) *(bf16x4 *)(lp + (i * 32 + t) * 40 + 8 * g + 4 * ts) = cp[i];
                 }
                 __syncthreads();
             }
@@ -302,17 +312,16 @@ __global__ __launch_bounds__(512) void memory_tiles_kernel(Walk a) {
                 bf16x8 zt[NP];
 #pragma unroll
                 for (int i = 0; i < NP; ++i) zt[i] = *(const bf16x8 *)(lzt + (i * 16 * nz + zc + c) * 40 + 8 * g);
-                if (!a.state_only) {
+                if (OUT) {
                     f32x4 in[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
                     for (int kk = 0; kk < NK; ++kk) {
                         bf16x8 st[PP];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            __bf16 c0[PP], c1[PP];
-                            cut(S[2 * kk][r], c0); cut(S[2 * kk + 1][r], c1);
+                        for (int r = 0; r < 8; ++r) {
+                            float v = S[2 * kk + r / 4][r % 4];
 #pragma unroll
-                            for (int i = 0; i < PP; ++i) { st[i][r] = c0[i]; st[i][4 + r] = c1[i]; }
+                            for (int i = 0; i < PP; ++i) { st[i][r] = (__bf16)v; v -= (float)st[i][r]; }
                         }
 #pragma unroll
                         for (int tt = 0; tt < 2; ++tt) {
@@ -324,33 +333,31 @@ __global__ __launch_bounds__(512) void memory_tiles_kernel(Walk a) {
                     }
 #pragma unroll
                     for (int tt = 0; tt < 2; ++tt) {
-                        const int tl = 16 * tt + c;
-                        const int64_t t = t0 + tl;
-                        const bool store = t < t_end && (only < 0 || tl == only);
-                        const int z = zc + g4;
+                        const int t = 16 * tt + c;
+                        const bool store = t < count && (only < 0 || t == only);
                         V wv, zv;
                         if (DOT) {
-                            wv = load4<T>(pw + t * a.w.sl + z, store ? dz - z : 0, VEC);
-                            zv = load4<T>(pz + t * a.z.sl + z, store ? dz - z : 0, VEC);
+                            wv = load4<T>(qw + tt * sw, store ? zleft : 0, VEC);
+                            zv = load4<T>(qv + tt * (sz >> 1), store ? zleft : 0, VEC);
                         }
                         f32x4 o = {0.f, 0.f, 0.f, 0.f};
                         bf16x8 fp[PP];
 #pragma unroll
-                        for (int i = 0; i < PP; ++i) fp[i] = *(const bf16x8 *)(lp + (i * 32 + tl) * 40 + 8 * g);
+                        for (int i = 0; i < PP; ++i) fp[i] = *(const bf16x8 *)(lp + (i * 32 + t) * 40 + 8 * g);
                         o = mma_pieces<NP, PP, PC::out_order>(zt, fp, o);
-                        const float win = lwin[tl];
+                        const float win = lwin[t];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) o[r] = (win != -1.f ? o[r] + win * in[tt][r] : o[r]) * a.out_scale;
+                        for (int r = 0; r < 4; ++r) o[r] = (win != -1.f ? o[r] + win * in[tt][r] : o[r]) * out_scale;
                         if (DOT) {
                             const f32x4 wf = widen(wv), zf = widen(zv);
                             float dot = o[0] * wf[0] + o[1] * wf[1] + o[2] * wf[2] + o[3] * wf[3];
                             dot += __shfl_xor(dot, 16); dot += __shfl_xor(dot, 32);
-                            if (g == 0) ldot[wave * 32 + tl] = dot;
-                            const float own = lown[tl] * a.out_scale;
+                            if (g == 0) ldot[wave * 32 + t] = dot;
+                            const float own = lown[t] * out_scale;
 #pragma unroll
                             for (int r = 0; r < 4; ++r) o[r] += own * zf[r];
                         }
-                        if (store) store4<T>(po + t * a.out.sl + z, o, dz - z, VEC);
+                        if (store) store4<T>(qo + tt * so, o, zleft, VEC);
                     }
                 }
                 // S = all * S + y^T (u z): u z in the place of z's column, exact to float32
@@ -358,18 +365,20 @@ __global__ __launch_bounds__(512) void memory_tiles_kernel(Walk a) {
                 const f32x4 u0 = *(const f32x4 *)(lwout + g4), u1 = *(const f32x4 *)(lwout + 16 + g4);
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
-                    float zf = (float)zt[0][r];
+                    float v = (float)zt[0][r];
 #pragma unroll
-                    for (int i = 1; i < NP; ++i) zf += (float)zt[i][r];
-                    __bf16 cu[3];
-                    cut(zf * (r < 4 ? u0[r & 3] : u1[r & 3]), cu);
+                    for (int i = 1; i < NP; ++i) v += (float)zt[i][r];
+                    v *= r < 4 ? u0[r & 3] : u1[r & 3];
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) uz[i][r] = cu[i];
+                    for (int i = 0; i < 3; ++i) { uz[i][r] = (__bf16)v; v -= (float)uz[i][r]; }
+                }
+                if (all == -1.f) {
+#pragma unroll
+                    for (int i = 0; i < 2 * NK; ++i) S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
                 }
 #pragma unroll
                 for (int i = 0; i < 2 * NK; ++i) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) S[i][r] = all != -1.f ? S[i][r] * all : 0.f;
+                    S[i] *= all;
                     bf16x8 yt[NP];
 #pragma unroll
                     for (int k = 0; k < NP; ++k) yt[k] = *(const bf16x8 *)(lyt + (k * 32 * NK + 16 * i + c) * 40 + 8 * g);
@@ -379,26 +388,37 @@ __global__ __launch_bounds__(512) void memory_tiles_kernel(Walk a) {
             whole *= all != -1.f ? all : 0.f;
             if (DOT) {
                 __syncthreads();
-                const int64_t t = t0 + lane;
-                if (wave == 0 && lane < 32 && t < t_end && (only < 0 || lane == only)) {
+                if (wave == 0 && lane < 32 && lane < count && (only < 0 || lane == only)) {
                     float d = 0.f;
                     for (int w = 0; w < nz; ++w) d += ldot[w * 32 + lane];
-                    a.dot[(t * a.B + b) * a.H + h] = d;
+                    a.dot[(t_begin + 32 * n + lane) * a.dot_sl + bh * a.dot_sh] = d;
                 }
             }
         }
-        if (subs > 1 && n + 1 < chunks) fetch(chunk_at(n + 1));
+        if (subs > 1 && n + 1 < chunks) fetch(32 * (n + 1));
+        if (OUT) qo += 2 * so;
+        if (DOT) { qw += 2 * sw; qv += sz; }
     }
-    if (a.state_out && holds) {
+    asm volatile("" : "+s"(at_args));
+    const Walk &e = *(const Walk *)(WalkArg)at_args;
+    float behind = 1.f;   // the last token's own decay, where it lies behind it; -1: nothing is carried on
+    if (shift) {
+        const int64_t t = t_begin + length - 1;
+        const float gt = e.g[t * e.gl + b * e.gb + h * e.gh], mt = e.masks ? e.masks[t * e.ml + b * e.mb] : 1.f;
+        behind = mt == 0.f || gt == -__builtin_inff() ? -1.f : exp2_fast((float)((double)gt * 1.4426950408889634074));
+    }
+    if (e.state_out && holds) {
+        float *ps = e.state_out + seg * e.seg_state_out + bh * (int64_t)(dy * dz) + (zc + c) * e.o_z;
+        const int64_t o_y = e.o_y;
 #pragma unroll
         for (int i = 0; i < 2 * NK; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int y = 16 * i + g4 + r, z = zc + c;
-                if (y < dy && z < dz) a.state_out[seg * a.seg_state_out + bh * (int64_t)dy * dz + y * a.o_y + z * a.o_z] = S[i][r];
+                const int y = 16 * i + g4 + r;
+                if (y < dy && zc + c < dz) ps[y * o_y] = behind != -1.f ? S[i][r] * behind : 0.f;
             }
     }
-    if (a.seg_decay && tid == 0) a.seg_decay[seg * heads + bh] = whole;
+    if (MODE == kState && e.seg_decay && tid == 0) e.seg_decay[(int64_t)seg * heads + bh] = behind != -1.f ? whole * behind : 0.f;
 }
 
 // ---- small heads ------------------------------------------------------------------------------------------------------------
@@ -514,13 +534,11 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
     }
     float whole = 1.f;
     float nx[TB][NY], ny[TB][NY], nz[TB], nw[TB], ng = 0.f, nm = 1.f;
-    // step i of the walk is token i of the segment, or token i from its end
-    auto token = [&](int64_t i) { return a.reverse ? t_end - 1 - i : t_begin + i; };
     auto fetch = [&](int64_t i0) {
 #pragma unroll
         for (int i = 0; i < TB; ++i) {
             const bool in = i0 + i < count;
-            const int64_t t = in ? token(i0 + i) : t_begin;
+            const int64_t t = in ? t_begin + i0 + i : t_begin;
 #pragma unroll
             for (int n = 0; n < NY; ++n) {
                 const bool yin = in && 16 * n + c < dy;
@@ -530,8 +548,8 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
             nz[i] = in && zin ? (float)pz[t * a.z.sl] : 0.f;
             if (DOT) nw[i] = in && zin ? (float)pw[t * a.w.sl] : 0.f;
         }
-        const bool in = c < TB && i0 + c < count;   // lane c: the decay of step i0 + c
-        const int64_t t = in ? token(i0 + c) : t_begin;
+        const bool in = c < TB && i0 + c < count && (!a.shift || i0 + c > 0);   // lane c: the decay before token i0 + c
+        const int64_t t = in ? t_begin + i0 + c - a.shift : t_begin;
         ng = in ? pg[t * a.gl] : 0.f;
         nm = in && pm ? pm[t * a.ml] : 1.f;
     };
@@ -554,28 +572,30 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
                 const bool fresh = row_lane<i>(fresh_l) != 0.f;
                 if (a.state_only) whole *= fresh ? 0.f : d;
                 else {
-                    float nd = row_dot<NY>(x[i], S);       // from the tokens before (backwards: behind); forwards the token's decay lies between
-                    if (!a.reverse) nd = fresh ? 0.f : nd * d;
+                    float nd = row_dot<NY>(x[i], S);       // from the tokens before
+                    nd = fresh ? 0.f : nd * d;
                     float xy = 0.f;
 #pragma unroll
                     for (int n = 0; n < NY; ++n) xy += x[i][n] * y[i][n];
                     xy = row_sum(xy);
-                    const int64_t t = token(i0 + i);
+                    const int64_t t = t_begin + i0 + i;
                     if (have && zin) po[t * a.out.sl] = (T)((nd + xy * zz[i]) * a.out_scale);
                     if (DOT) {
                         const float dot = row_sum(nd * a.out_scale * ww[i]);
-                        if (have && c == 0) a.dot[((slice * a.L + t) * a.B + b) * a.H + h] = dot;
+                        if (have && c == 0) a.dot[slice * a.dot_slice + t * a.dot_sl + bh * a.dot_sh] = dot;
                     }
                 }
-                if (!a.reverse) row_update<NY>(S, d, fresh, y[i], zz[i]);
-                else {
-                    row_update<NY>(S, d, false, y[i], zz[i] * d);
-                    if (__ballot(fresh))
-#pragma unroll
-                        for (int m = 0; m < 16 * NY; ++m) S[m] = fresh ? 0.f : S[m];
-                }
+                row_update<NY>(S, d, fresh, y[i], zz[i]);
             }
         });
+    }
+    if (a.shift) {   // the last token's own decay lies behind it
+        const float gt = pg[(t_end - 1) * a.gl], mt = pm ? pm[(t_end - 1) * a.ml] : 1.f;
+        const bool fresh = mt == 0.f || gt == -__builtin_inff();
+        const float d = exp2_fast((float)((double)gt * 1.4426950408889634074));
+#pragma unroll
+        for (int m = 0; m < 16 * NY; ++m) S[m] = fresh ? 0.f : S[m] * d;
+        whole *= fresh ? 0.f : d;
     }
     if (a.state_out && have && zin) {
         float *ps = a.state_out + seg * a.seg_state_out + bh * (int64_t)a.dy * a.dz + (int64_t)z * a.o_z;
@@ -688,15 +708,14 @@ __global__ __launch_bounds__(256) void memory_short_backward_kernel(ShortGrad a)
     if (a.partial && have && c == 0) a.partial[bh] = sum;
 }
 
-// The states at the segments' starts (backwards: behind their ends) from what each segment adds to an empty state: in place, one thread per element.
+// The states at the segments' starts from what each segment adds to an empty state: in place, one thread per element.
 __global__ __launch_bounds__(256) void memory_join_kernel(float *seg_states, const float *seg_decay, const float *init, float *last,
-                                                          int64_t heads, int elems, int nseg, int reverse) {
+                                                          int64_t heads, int elems, int nseg) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = heads * elems;
     if (i >= total) return;
     const int64_t bh = i / elems;
     float S = init ? init[i] : 0.f;
-    for (int n = 0; n < nseg; ++n) {
-        const int seg = reverse ? nseg - 1 - n : n;
+    for (int seg = 0; seg < nseg; ++seg) {
         const float d = seg_decay[seg * heads + bh], u = seg_states[seg * total + i];
         seg_states[seg * total + i] = S;
         S = (d == 0.f ? 0.f : d * S) + u;
@@ -709,7 +728,8 @@ __global__ __launch_bounds__(256) void memory_join_kernel(float *seg_states, con
 // One workgroup of `blockDim` threads per (batch, head); every thread takes a run of tokens, the runs are joined by a scan.
 // THREADS = 1 workgroup of 256 serves 256 (batch, head) pairs, one per thread: short sequences.
 struct DecayGrad {
-    const float *dot_q, *dot_k;      // (slices_q | slices_k, L, B, H)
+    const float *dot_q, *dot_k;      // (slices_q | slices_k), L and (B, H) by these strides
+    int64_t dot_sl, dot_sh;
     const float *state, *d_state;    // (B, H, elems); state may be NULL
     const float *g; int64_t gl, gb, gh;
     const float *masks; int64_t ml, mb;
@@ -720,7 +740,7 @@ struct DecayGrad {
 };
 
 __device__ __forceinline__ double decay_step(const DecayGrad &a, int64_t t, int64_t bh) {
-    const int64_t n = a.L * a.B * a.H, i = t * a.B * a.H + bh;
+    const int64_t n = a.L * a.B * a.H, i = t * a.dot_sl + bh * a.dot_sh;
     double d = 0.0;
     for (int s = 0; s < a.slices_q; ++s) d += a.dot_q[s * n + i];
     for (int s = 0; s < a.slices_k; ++s) d -= a.dot_k[s * n + i];
@@ -914,13 +934,13 @@ int memory_check(const FmarlMemory *m, const char *who) {
 // its three instructions per 64 state entries and token would cost twice the matrix units' time
 bool small_heads(int dy) { return dy <= 32; }
 
-// A batch with few heads has its tokens cut into segments that are walked side by side: so many that 2 048 waves of four small heads or 1 024 workgroups of a large one
-// are at work (8 waves, 4 workgroups per CU), at least 64 tokens each (a segment costs a second read of k and v and a state in the workspace, which shorter
-// ones would not repay).
+// A batch with few heads has its tokens cut into segments that are walked side by side: up to 2 048 waves of four small heads or 768 workgroups of a large one (what
+// is resident at a time: 8 waves, 3 workgroups per CU -- one more would be a second round), at least 64 tokens each (a segment costs a second
+// read of k and v and a state in the workspace, which shorter ones would not repay).
 struct Segments { int nseg, len; };
 Segments memory_segments(const FmarlMemory *m) {
-    const int64_t heads = m->B * m->H, units = small_heads(m->dk) ? (heads + 3) / 4 : heads, want = small_heads(m->dk) ? 2048 : 1024;
-    int64_t n = (want + units - 1) / units, most = m->L / 64;
+    const int64_t heads = m->B * m->H, units = small_heads(m->dk) ? (heads + 3) / 4 : heads, want = small_heads(m->dk) ? 2048 : 768;
+    int64_t n = want / units, most = m->L / 64;
     if (n > most) n = most;
     if (n < 2) return {1, (int)(m->L > 0x40000000 ? 0x40000000 : m->L)};
     const int64_t len = ((m->L + n - 1) / n + 31) / 32 * 32;
@@ -958,19 +978,20 @@ Workspace memory_layout(const FmarlMemory *m, int backward) {
     return w;
 }
 
-template <typename T, int NK, bool DOT, bool VEC>
+template <typename T, int NK, int MODE, bool VEC>
 int launch_tiles(const Walk &w, int64_t blocks, hipStream_t st) {
-    const int nz = (w.dz + 15) / 16, lds = tiles_lds<T, DOT>(NK, nz);
-    if (lds > 64 * 1024) HIP_OK(hipFuncSetAttribute((const void *)memory_tiles_kernel<T, NK, DOT, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    hipLaunchKernelGGL((memory_tiles_kernel<T, NK, DOT, VEC>), dim3((unsigned)blocks), dim3(64 * (nz < 4 ? 4 : nz)), lds, st, w);
+    const int nz = (w.dz + 15) / 16, lds = tiles_lds<T, MODE == kOutDot>(NK, nz);
+    if (lds > 64 * 1024) HIP_OK(hipFuncSetAttribute((const void *)memory_tiles_kernel<T, NK, MODE, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL((memory_tiles_kernel<T, NK, MODE, VEC>), dim3((unsigned)blocks), dim3(64 * (nz < 4 ? 4 : nz)), lds, st, w);
     return FMARL_OK;
 }
 
 template <typename T, int NK>
 int launch_tiles_as(const Walk &w, int64_t blocks, hipStream_t st) {
     const bool vec = (w.state_only || (w.x.vec && w.out.vec)) && w.y.vec && w.z.vec && (!w.w.p || w.w.vec);
-    if (w.w.p) return vec ? launch_tiles<T, NK, true, true>(w, blocks, st) : launch_tiles<T, NK, true, false>(w, blocks, st);
-    return vec ? launch_tiles<T, NK, false, true>(w, blocks, st) : launch_tiles<T, NK, false, false>(w, blocks, st);
+    if (w.state_only) return vec ? launch_tiles<T, NK, kState, true>(w, blocks, st) : launch_tiles<T, NK, kState, false>(w, blocks, st);
+    if (w.w.p) return vec ? launch_tiles<T, NK, kOutDot, true>(w, blocks, st) : launch_tiles<T, NK, kOutDot, false>(w, blocks, st);
+    return vec ? launch_tiles<T, NK, kOut, true>(w, blocks, st) : launch_tiles<T, NK, kOut, false>(w, blocks, st);
 }
 
 template <typename T>
@@ -999,6 +1020,9 @@ int launch_walk(Walk w, int dtype, hipStream_t st) {
     return FMARL_OK;
 }
 
+// the decay's gradient by a thread per (batch, head) while its tokens are few; otherwise by a workgroup per (batch, head), whose threads share the tokens
+bool few_tokens(int64_t L) { return L <= 64; }
+
 Walk walk_base(const FmarlMemory *m) {
     Walk w = {};
     const Segments s = memory_segments(m);
@@ -1006,21 +1030,39 @@ Walk walk_base(const FmarlMemory *m) {
     w.masks = m->masks; w.ml = m->mask_stride_l; w.mb = m->mask_stride_b;
     w.L = m->L; w.B = m->B; w.H = m->H; w.nseg = s.nseg; w.seg_len = s.len;
     w.y_scale = w.out_scale = 1.f;
+    // as the decay's kernel reads them: a thread per head (heads side by side), or a workgroup per head (tokens side by side)
+    const bool few = few_tokens(m->L);
+    w.dot_sl = few ? m->B * m->H : 1; w.dot_sh = few ? 1 : m->L; w.dot_slice = m->L * m->B * m->H;
     return w;
 }
 
-// the states at the segments' starts (reverse: the gradients of the states behind their ends) into seg_states; the last one of the walk into `last`
+void turn(WalkRows &r, int64_t L, int dtype) {   // the last token first
+    if (!r.p) return;
+    r.p += (L - 1) * r.sl * elem_bytes(dtype);
+    r.sl = -r.sl;
+}
+
+// a backwards walk: every array the last token first, decays behind their tokens
+void turn_round(Walk &w, int dtype) {
+    turn(w.x, w.L, dtype); turn(w.y, w.L, dtype); turn(w.z, w.L, dtype); turn(w.w, w.L, dtype); turn(w.out, w.L, dtype);
+    w.g += (w.L - 1) * w.gl; w.gl = -w.gl;
+    if (w.masks) { w.masks += (w.L - 1) * w.ml; w.ml = -w.ml; }
+    if (w.dot) { w.dot += (w.L - 1) * w.dot_sl; w.dot_sl = -w.dot_sl; }
+    w.shift = 1;
+}
+
+// the states at the segments' starts (of the backwards walk: the gradients of the states behind the tokens) into seg_states; the walk's last one into `last`
 int segment_states(const FmarlMemory *m, const FmarlRows &y, const FmarlRows &z, bool reverse, const float *init, float *last, float *seg_states,
                    float *seg_decay, hipStream_t st) {
     Walk w = walk_base(m);
     const int64_t heads = m->B * m->H, elems = (int64_t)m->dk * m->dv;
     w.y = walk_rows(y, m->dk, m->dtype); w.z = walk_rows(z, m->dv, m->dtype);
-    w.dy = m->dk; w.dz = m->dv; w.state_only = 1; w.reverse = reverse;
-    if (reverse) w.y_scale = m->scale;
+    w.dy = m->dk; w.dz = m->dv; w.state_only = 1;
+    if (reverse) { w.y_scale = m->scale; turn_round(w, m->dtype); }
     w.state_out = seg_states; w.o_y = m->dv; w.o_z = 1; w.seg_state_out = heads * elems; w.seg_decay = seg_decay;
     if (int rc = launch_walk(w, m->dtype, st)) return rc;
     const int64_t blocks = (heads * elems + 255) / 256;
-    hipLaunchKernelGGL(memory_join_kernel, dim3((unsigned)blocks), dim3(256), 0, st, seg_states, (const float *)seg_decay, init, last, heads, (int)elems, w.nseg, (int)reverse);
+    hipLaunchKernelGGL(memory_join_kernel, dim3((unsigned)blocks), dim3(256), 0, st, seg_states, (const float *)seg_decay, init, last, heads, (int)elems, w.nseg);
     HIP_OK(hipGetLastError());
     return FMARL_OK;
 }
@@ -1080,7 +1122,8 @@ int fmarl_memory_chunk(const FmarlMemory *m, const FmarlRows *out, float *state_
 }
 
 int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, const float *d_state, const FmarlRows *d_q, const FmarlRows *d_k,
-                                const FmarlRows *d_v, float *d_log_decay, float *d_state0, void *workspace, void *stream) {
+                                const FmarlRows *d_v, float *d_log_decay, float *d_state0, const void *forward_workspace, void *workspace,
+                                void *stream) {
     if (int rc = memory_check(m, "fmarl_memory_chunk_backward")) return rc;
     if (m->B == 0) return FMARL_OK;
     if (m->L < 1) return policy_fail(FMARL_EINVAL, "fmarl_memory_chunk_backward: L must be positive");
@@ -1113,7 +1156,8 @@ int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, co
     float *seg_s = (float *)(base + ws.seg_s), *seg_g = (float *)(base + ws.seg_g), *decay = (float *)(base + ws.decay);
     float *ds0 = d_state0 ? d_state0 : (float *)(base + ws.d_state);
     if (w0.nseg > 1) {
-        if (int rc = segment_states(m, m->k, m->v, false, m->state, nullptr, seg_s, decay, st)) return rc;
+        if (forward_workspace) seg_s = (float *)((char *)forward_workspace + memory_layout(m, 0).seg_s);   // (only read)
+        else if (int rc = segment_states(m, m->k, m->v, false, m->state, nullptr, seg_s, decay, st)) return rc;
         if (int rc = segment_states(m, m->q, *d_out, true, d_state, ds0, seg_g, decay, st)) return rc;
     }
     const int64_t seg_elems = w0.nseg > 1 ? heads * elems : 0;
@@ -1126,12 +1170,14 @@ int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, co
     if (int rc = launch_walk(w, dt, st)) return rc;
     w = w0;        // dk: backwards
     w.x = v; w.y = o; w.z = q; w.w = k; w.out = walk_rows(*d_k, m->dk, dt); w.dot = (float *)(base + ws.dot_k);
-    w.dy = m->dv; w.dz = m->dk; w.y_scale = m->scale; w.s_y = 1; w.s_z = m->dv; w.reverse = 1;
+    w.dy = m->dv; w.dz = m->dk; w.y_scale = m->scale; w.s_y = 1; w.s_z = m->dv;
+    turn_round(w, dt);
     w.state = w0.nseg > 1 ? seg_g : d_state; w.seg_state_in = seg_elems;
     if (int rc = launch_walk(w, dt, st)) return rc;
     w = w0;        // dv, and the gradient of the initial state
     w.x = k; w.y = q; w.z = o; w.out = walk_rows(*d_v, m->dv, dt);
-    w.dy = m->dk; w.dz = m->dv; w.y_scale = m->scale; w.s_y = w.o_y = m->dv; w.s_z = w.o_z = 1; w.reverse = 1;
+    w.dy = m->dk; w.dz = m->dv; w.y_scale = m->scale; w.s_y = w.o_y = m->dv; w.s_z = w.o_z = 1;
+    turn_round(w, dt);
     w.state = w0.nseg > 1 ? seg_g : d_state; w.seg_state_in = seg_elems;
     if (w0.nseg == 1) w.state_out = ds0;
     if (int rc = launch_walk(w, dt, st)) return rc;
@@ -1142,8 +1188,8 @@ int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, co
         g.state = m->state; g.d_state = ds0; g.g = w0.g; g.gl = w0.gl; g.gb = w0.gb; g.gh = w0.gh; g.masks = w0.masks; g.ml = w0.ml; g.mb = w0.mb;
         g.dg = shared ? nullptr : d_log_decay; g.partial = shared ? (double *)(base + ws.partial) : nullptr;
         g.L = m->L; g.B = m->B; g.H = m->H; g.elems = elems; g.slices_q = g.slices_k = slices_of(m->dv, m->dk);
-        // a thread per (batch, head) while its tokens are few; otherwise a workgroup per (batch, head), whose threads share the tokens
-        if (m->L <= 64) hipLaunchKernelGGL(decay_grad_short_kernel, dim3((unsigned)((heads + 255) / 256)), dim3(256), 0, st, g);
+        g.dot_sl = w0.dot_sl; g.dot_sh = w0.dot_sh;
+        if (few_tokens(m->L)) hipLaunchKernelGGL(decay_grad_short_kernel, dim3((unsigned)((heads + 255) / 256)), dim3(256), 0, st, g);
         else hipLaunchKernelGGL(decay_grad_long_kernel, dim3((unsigned)heads), dim3(1024), 0, st, g);
         if (shared) hipLaunchKernelGGL(decay_sum_kernel, dim3((unsigned)m->H), dim3(256), 0, st, (const double *)(base + ws.partial), d_log_decay, m->B, m->H);
         HIP_OK(hipGetLastError());

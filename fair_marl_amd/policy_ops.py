@@ -88,10 +88,10 @@ def _launch_chunk(m, keep):
     with torch.cuda.device(dev):
         ws = torch.empty(lib.fmarl_memory_workspace(m, 0), dtype=torch.uint8, device=dev)
         _lib.check(lib.fmarl_memory_chunk(m, _rows(out), state.data_ptr(), ws.data_ptr(), _stream(dev)), 'fmarl_memory_chunk')
-    return out, state
+    return out, state, ws
 
 
-def _launch_chunk_backward(m, keep, d_out, d_state, want_decay=True):
+def _launch_chunk_backward(m, keep, d_out, d_state, want_decay=True, forward_ws=None):
     q, k, v, g, state = keep[:5]
     dev = q.device
     d_out = _last(d_out)
@@ -103,7 +103,8 @@ def _launch_chunk_backward(m, keep, d_out, d_state, want_decay=True):
     lib = _lib.load()
     with torch.cuda.device(dev):
         ws = torch.empty(lib.fmarl_memory_workspace(m, 1), dtype=torch.uint8, device=dev)
-        _lib.check(lib.fmarl_memory_chunk_backward(m, _rows(d_out), _ptr(d_state), _rows(dq), _rows(dk), _rows(dv), _ptr(dg), ds.data_ptr(), ws.data_ptr(),
+        _lib.check(lib.fmarl_memory_chunk_backward(m, _rows(d_out), _ptr(d_state), _rows(dq), _rows(dk), _rows(dv), _ptr(dg), ds.data_ptr(), _ptr(forward_ws),
+                                                   ws.data_ptr(),
                                                    _stream(dev)), 'fmarl_memory_chunk_backward')
     return dq, dk, dv, dg, ds
 
@@ -112,10 +113,12 @@ class _MemoryChunk(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, masks, scale):
         m, keep = _memory_args('memory_chunk', q, k, v, log_decay, state, masks, scale, 2)
+        out, last, ws = _launch_chunk(m, keep)
         ctx.save_for_backward(*keep)
+        ctx.forward_ws = ws if any(ctx.needs_input_grad) else None   # long sequences: the states at their segments' starts
         ctx.scale, ctx.state_shape = m.scale, None if state is None else state.shape
         ctx.set_materialize_grads(False)
-        return _launch_chunk(m, keep)
+        return out, last
 
     @staticmethod
     @once_differentiable
@@ -124,7 +127,7 @@ class _MemoryChunk(torch.autograd.Function):
         m, keep = _memory_args('memory_chunk', q, k, v, g, state, masks, ctx.scale, 2)
         if d_out is None:
             d_out = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
-        dq, dk, dv, dg, ds = _launch_chunk_backward(m, keep, d_out, d_state, ctx.needs_input_grad[3])
+        dq, dk, dv, dg, ds = _launch_chunk_backward(m, keep, d_out, d_state, ctx.needs_input_grad[3], ctx.forward_ws)
         return dq, dk, dv, dg, None if state is None else ds.view(ctx.state_shape), None, None
 
 

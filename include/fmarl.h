@@ -539,9 +539,11 @@ int fmarl_memory_step(const FmarlMemory *m, const FmarlRows *out, float *state_o
 size_t fmarl_memory_workspace(const FmarlMemory *m, int backward);
 int fmarl_memory_chunk(const FmarlMemory *m, const FmarlRows *out, float *state_out, void *workspace, void *stream);
 /* gradients: d_out and d_state (B, H, dk, dv; NULL: zeros) in; d_q, d_k, d_v, d_log_decay (contiguous; NULL:
- * not wanted) and d_state0 (NULL: not wanted) out */
+ * not wanted) and d_state0 (NULL: not wanted) out.  forward_workspace: what fmarl_memory_chunk left in its workspace for the same m (long sequences: the
+ * states at the segments' starts), or NULL: formed again */
 int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, const float *d_state, const FmarlRows *d_q, const FmarlRows *d_k,
-                                const FmarlRows *d_v, float *d_log_decay, float *d_state0, void *workspace, void *stream);
+                                const FmarlRows *d_v, float *d_log_decay, float *d_state0, const void *forward_workspace, void *workspace,
+                                void *stream);
 
 /* The end of a residual block and the start of the next one, a row of `dim` at a time, with n(a) = a / sqrt(mean a^2 + eps) (kind 0, rms) or
  * (a - mean a) / sqrt(var a + eps) (kind 1, layer: the LayerNorm of onpolicy/algorithms/utils/mlp.py:25-40):

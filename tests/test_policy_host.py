@@ -62,15 +62,15 @@ def test_memory_entry_points_refuse(lib):
                      (dict(shared_decay=1), b'shared_decay'), (dict(B=1 << 31), b'too many'), (dict(log_decay=None), b'null'), (dict(q=_lib.FmarlRows()), b'null')):
         assert lib.fmarl_memory_chunk(memory(**kw), rows, p, p, None) == 1 and text in err(), kw
         assert lib.fmarl_memory_workspace(memory(**kw), 1) == 0 and text in err()
-        assert lib.fmarl_memory_chunk_backward(memory(**kw), rows, None, rows, rows, rows, None, None, p, None) == 1 and text in err()
+        assert lib.fmarl_memory_chunk_backward(memory(**kw), rows, None, rows, rows, rows, None, None, None, p, None) == 1 and text in err()
     assert lib.fmarl_memory_chunk(None, rows, p, p, None) == 1 and b'null' in err()
     assert lib.fmarl_memory_chunk(memory(L=0), rows, p, p, None) == 1 and b'positive' in err()
     assert lib.fmarl_memory_chunk(memory(), None, p, p, None) == 1 and lib.fmarl_memory_chunk(memory(), rows, None, p, None) == 1 and lib.fmarl_memory_chunk(memory(), rows, p, None, None) == 1
     assert lib.fmarl_memory_step(memory(), rows, p, None) == 1 and b'L must be 1' in err()
     assert lib.fmarl_memory_step(memory(L=1), None, p, None) == 1 and lib.fmarl_memory_step(memory(L=1), rows, None, None) == 1
     for args in ((None, None, rows, rows, rows), (rows, None, None, rows, rows), (rows, None, rows, None, rows), (rows, None, rows, rows, None)):
-        assert lib.fmarl_memory_chunk_backward(memory(), *args, None, None, p, None) == 1 and b'null' in err()
-    assert lib.fmarl_memory_chunk_backward(memory(), rows, None, rows, rows, rows, None, None, None, None) == 1
+        assert lib.fmarl_memory_chunk_backward(memory(), *args, None, None, None, p, None) == 1 and b'null' in err()
+    assert lib.fmarl_memory_chunk_backward(memory(), rows, None, rows, rows, rows, None, None, None, None, None) == 1
     assert lib.fmarl_memory_chunk(memory(B=0), rows, p, p, None) == 0 and lib.fmarl_memory_step(memory(L=1, B=0), rows, p, None) == 0     # nothing to do
     # the workspace: nothing to cut for many sequences, segment states for few and long ones, more of it backwards
     assert lib.fmarl_memory_workspace(memory(L=10, B=100000), 0) == 256
