@@ -23,35 +23,45 @@ struct Block {
     float *partial;                                         // (workgroups, 5, dim): the weights' gradients of each workgroup's rows
 };
 
+// floats of a team's row in LDS: the row, then its groups' means
+__host__ __device__ inline int block_row_floats(int dim, int groups) { return ((dim + 3) & ~3) + ((groups + 3) & ~3); }
+
 enum { kGroupRow = 0, kGroupLanes = 1, kGroupLds = 2 };     // how a group's elements lie over the team: all of it, 2^k neighbouring lanes, anyhow
 
 // A row belongs to a team of TL threads, TL * 4 * NV >= dim: thread l holds the four columns from (n TL + l) 4 on, n < NV, so that a team's loads are
-// consecutive.  Teams of 16 (four rows a wave) up to dim 128, of a wave up to 1 024, of a workgroup beyond.
+// consecutive.  Teams of 16 lanes up to dim 64, 32, 64, then of a workgroup of 128 ... 1 024: four columns a thread (eight beyond 2 048), so that the weights and the sums of
+// their gradients fit the registers four waves a SIMD deep.  (A wave per row of 1 024, sixteen columns a lane, held 256 + 96 registers: one wave a SIMD, 226 us for
+// 16 383 bf16 rows backwards.)  The next row's loads are in flight while a row is computed.  What a team of several waves exchanges lies in one of two places in turn: a
+// barrier before the reads is enough, the next but one write comes behind another.
+struct Exchange { float *red, *row; int row_floats, flip; };
+
 template <int TL>
-__device__ __forceinline__ float team_sum(float v, float *red) {
+__device__ __forceinline__ void team_sum2(float &v, float &w, Exchange &x) {
 #pragma unroll
-    for (int off = 1; off < (TL < 64 ? TL : 64); off <<= 1) v += __shfl_xor(v, off);
+    for (int off = 1; off < (TL < 64 ? TL : 64); off <<= 1) { v += __shfl_xor(v, off); w += __shfl_xor(w, off); }
     if (TL > 64) {
+        float *red = x.red + x.flip * 32;
+        x.flip ^= 1;
+        if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = v; red[16 + (threadIdx.x >> 6)] = w; }
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0.f;
+        v = w = 0.f;
 #pragma unroll
-        for (int w = 0; w < TL / 64; ++w) v += red[w];
+        for (int k = 0; k < TL / 64; ++k) { v += red[k]; w += red[16 + k]; }
     }
-    return v;
 }
+
+template <int TL> __device__ __forceinline__ float team_sum(float v, Exchange &x) { float w = 0.f; team_sum2<TL>(v, w, x); return v; }
 
 template <int TL> __device__ __forceinline__ void team_sync() { if (TL > 64) __syncthreads(); else wave_sync(); }
 
 // v <- the mean over the group of each element; columns beyond dim hold 0 before and anything behind
 template <int TL, int NV>
-__device__ __forceinline__ void group_means(const Block &a, float (&v)[NV][4], int l, float *row, float *red) {
+__device__ __forceinline__ void group_means(const Block &a, float (&v)[NV][4], int l, Exchange &x) {
     if (a.group_mode == kGroupRow) {
         float s = 0.f;
 #pragma unroll
         for (int n = 0; n < NV; ++n) s += (v[n][0] + v[n][1]) + (v[n][2] + v[n][3]);
-        s = team_sum<TL>(s, red) * (1.f / a.dim);
+        s = team_sum<TL>(s, x) * (1.f / a.dim);
 #pragma unroll
         for (int n = 0; n < NV; ++n)
 #pragma unroll
@@ -69,8 +79,9 @@ __device__ __forceinline__ void group_means(const Block &a, float (&v)[NV][4], i
     } else {
         const int size = a.dim / a.groups;
         const float inv = 1.f / size;
-        float *sums = row + ((a.dim + 3) & ~3);
-        team_sync<TL>();
+        float *row = x.row + x.flip * x.row_floats, *sums = row + ((a.dim + 3) & ~3);
+        x.flip ^= 1;
+        if (TL <= 64) team_sync<TL>();
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int col = (n * TL + l) * 4;
@@ -98,11 +109,11 @@ __device__ __forceinline__ void group_means(const Block &a, float (&v)[NV][4], i
 }
 
 template <int TL, int NV>
-__device__ __forceinline__ void row_means(const Block &a, float (&v)[NV][4], float &mean, float *red) {
+__device__ __forceinline__ void row_means(const Block &a, float (&v)[NV][4], float &mean, Exchange &x) {
     float s = 0.f;
 #pragma unroll
     for (int n = 0; n < NV; ++n) s += (v[n][0] + v[n][1]) + (v[n][2] + v[n][3]);
-    mean = team_sum<TL>(s, red) * (1.f / a.dim);
+    mean = team_sum<TL>(s, x) * (1.f / a.dim);
 }
 
 #define FMARL_EACH(body)                                                \
@@ -112,38 +123,45 @@ __device__ __forceinline__ void row_means(const Block &a, float (&v)[NV][4], flo
 
 // n (in place) and 1 / sqrt(..) of the groups of o; two passes over the registers where the mean is taken off first
 template <int TL, int NV>
-__device__ __forceinline__ void norm_groups(const Block &a, float (&o)[NV][4], float (&inv)[NV][4], int l, float *row, float *red) {
+__device__ __forceinline__ void norm_groups(const Block &a, float (&o)[NV][4], float (&inv)[NV][4], int l, Exchange &x) {
     if (a.layer) {
         FMARL_EACH(inv[n][r] = o[n][r])
-        group_means<TL, NV>(a, inv, l, row, red);
+        group_means<TL, NV>(a, inv, l, x);
         FMARL_EACH(o[n][r] = in ? o[n][r] - inv[n][r] : 0.f)
     }
     FMARL_EACH(inv[n][r] = o[n][r] * o[n][r])
-    group_means<TL, NV>(a, inv, l, row, red);
+    group_means<TL, NV>(a, inv, l, x);
     FMARL_EACH(inv[n][r] = rsqrtf(inv[n][r] + a.eps); o[n][r] *= inv[n][r])
 }
 
 template <int TL, int NV>
-__device__ __forceinline__ float norm_row(const Block &a, float (&y)[NV][4], int l, float *red) {
+__device__ __forceinline__ float norm_row(const Block &a, float (&y)[NV][4], int l, Exchange &x) {
     float mean;
     if (a.layer) {
-        row_means<TL, NV>(a, y, mean, red);
+        row_means<TL, NV>(a, y, mean, x);
         FMARL_EACH(y[n][r] = in ? y[n][r] - mean : 0.f)
     }
     float s = 0.f;
     FMARL_EACH(s += y[n][r] * y[n][r])
-    const float inv = rsqrtf(team_sum<TL>(s, red) * (1.f / a.dim) + a.eps);
+    const float inv = rsqrtf(team_sum<TL>(s, x) * (1.f / a.dim) + a.eps);
     FMARL_EACH(y[n][r] *= inv)
     return inv;
 }
 
 template <typename T, int TL, int NV>
-__device__ __forceinline__ void load_row(const Block &a, float (&v)[NV][4], const char *base, int64_t stride, int64_t row, int l) {
+__device__ __forceinline__ void fetch_row(const Block &a, typename Vec4<T>::type (&v)[NV], const char *base, int64_t stride, int64_t row, int l) {
+    if (!base) return;   // (what is not given stays zero)
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
         const int col = (n * TL + l) * 4;
-        f32x4 w = {0.f, 0.f, 0.f, 0.f};
-        if (base) w = widen(load4<T>((const T *)base + row * stride + col, row < a.rows ? a.dim - col : 0, a.vec));
+        v[n] = load4<T>((const T *)base + row * stride + col, row < a.rows ? a.dim - col : 0, a.vec);
+    }
+}
+
+template <typename V, int NV> __device__ __forceinline__ void widen_row(float (&v)[NV][4], const V (&raw)[NV]) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        const f32x4 w = widen(raw[n]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[n][r] = w[r];
     }
@@ -171,24 +189,32 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(Block a) {
     extern __shared__ __align__(16) float lds[];
     const int l = threadIdx.x % TL, team = threadIdx.x / TL;
     constexpr int kTeams = THREADS / TL;
-    float *red = lds, *row_lds = lds + 16 + team * (((a.dim + 3) & ~3) + a.groups);
+    Exchange ex = {lds, lds + 64 + team * 2 * block_row_floats(a.dim, a.groups), block_row_floats(a.dim, a.groups), 0};
     float sc[NV][4], pw[NV][4], pb[NV][4], rw[NV][4], rb[NV][4];
     load_weights<TL, NV>(a, sc, a.scale, 1.f, l);
     load_weights<TL, NV>(a, pw, a.post_w, 1.f, l);
     load_weights<TL, NV>(a, pb, a.post_b, 0.f, l);
     load_weights<TL, NV>(a, rw, a.pre_w, 1.f, l);
     load_weights<TL, NV>(a, rb, a.pre_b, 0.f, l);
-    // every thread of the workgroup makes the same trips: rows beyond the last one are loaded as zeros and not stored
-    for (int64_t row0 = (int64_t)blockIdx.x * kTeams; row0 < a.rows; row0 += (int64_t)gridDim.x * kTeams) {
+    typename Vec4<TX>::type nx[NV] = {};
+    typename Vec4<TB>::type no[NV] = {}, ng[NV] = {};
+    const int64_t step = (int64_t)gridDim.x * kTeams;
+    auto fetch = [&](int64_t row) {
+        fetch_row<TX, TL, NV>(a, nx, a.x, a.xs, row, l);
+        fetch_row<TB, TL, NV>(a, no, a.branch, a.bs, row, l);
+        fetch_row<TB, TL, NV>(a, ng, a.gate, a.gs, row, l);
+    };
+    fetch((int64_t)blockIdx.x * kTeams + team);
+    // every thread of the workgroup makes the same trips: rows beyond the last one are zeros and not stored
+    for (int64_t row0 = (int64_t)blockIdx.x * kTeams; row0 < a.rows; row0 += step) {
         const int64_t row = row0 + team;
         float y[NV][4], o[NV][4], g[NV][4];
-        load_row<TX, TL, NV>(a, y, a.x, a.xs, row, l);
+        widen_row(y, nx); widen_row(o, no); widen_row(g, ng);
+        fetch(row + step);
         if (a.branch) {
-            load_row<TB, TL, NV>(a, o, a.branch, a.bs, row, l);
-            if (a.gate) load_row<TB, TL, NV>(a, g, a.gate, a.gs, row, l);
             if (a.post_norm) {
                 float inv[NV][4];
-                norm_groups<TL, NV>(a, o, inv, l, row_lds, red);
+                norm_groups<TL, NV>(a, o, inv, l, ex);
                 FMARL_EACH(o[n][r] = o[n][r] * pw[n][r] + pb[n][r])
             }
             if (a.gate) FMARL_EACH(const float s = sigmoid(g[n][r]); o[n][r] *= a.silu ? g[n][r] * s : s)
@@ -196,7 +222,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(Block a) {
             store_row<TX, TL, NV>(a, y, a.y, row, l);
         }
         if (a.h) {
-            norm_row<TL, NV>(a, y, l, red);
+            norm_row<TL, NV>(a, y, l, ex);
             FMARL_EACH(y[n][r] = y[n][r] * rw[n][r] + rb[n][r])
             store_row<TB, TL, NV>(a, y, a.h, row, l);
         }
@@ -208,7 +234,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_backward_kernel(Block a) {
     extern __shared__ __align__(16) float lds[];
     const int l = threadIdx.x % TL, team = threadIdx.x / TL;
     constexpr int kTeams = THREADS / TL;
-    float *red = lds, *row_lds = lds + 16 + team * (((a.dim + 3) & ~3) + a.groups);
+    Exchange ex = {lds, lds + 64 + team * 2 * block_row_floats(a.dim, a.groups), block_row_floats(a.dim, a.groups), 0};
     float sc[NV][4], pw[NV][4], pb[NV][4], rw[NV][4];
     load_weights<TL, NV>(a, sc, a.scale, 1.f, l);
     load_weights<TL, NV>(a, pw, a.post_w, 1.f, l);
@@ -217,28 +243,37 @@ __global__ __launch_bounds__(THREADS) void block_norm_backward_kernel(Block a) {
     float acc[5][NV][4];
 #pragma unroll
     for (int k = 0; k < 5; ++k) FMARL_EACH(acc[k][n][r] = 0.f)
-    for (int64_t row0 = (int64_t)blockIdx.x * kTeams; row0 < a.rows; row0 += (int64_t)gridDim.x * kTeams) {
+    typename Vec4<TX>::type nx[NV] = {}, nd[NV] = {};
+    typename Vec4<TB>::type no[NV] = {}, ng[NV] = {}, nh[NV] = {};
+    const int64_t step = (int64_t)gridDim.x * kTeams;
+    auto fetch = [&](int64_t row) {
+        fetch_row<TX, TL, NV>(a, nx, a.x, a.xs, row, l);
+        fetch_row<TB, TL, NV>(a, no, a.branch, a.bs, row, l);
+        fetch_row<TB, TL, NV>(a, ng, a.gate, a.gs, row, l);
+        fetch_row<TX, TL, NV>(a, nd, a.dy, a.dys, row, l);
+        fetch_row<TB, TL, NV>(a, nh, a.dh, a.dhs, row, l);
+    };
+    fetch((int64_t)blockIdx.x * kTeams + team);
+    for (int64_t row0 = (int64_t)blockIdx.x * kTeams; row0 < a.rows; row0 += step) {
         const int64_t row = row0 + team;
         float y[NV][4], u[NV][4], g[NV][4], inv[NV][4], d[NV][4], dh[NV][4];
-        load_row<TX, TL, NV>(a, y, a.x, a.xs, row, l);
-        load_row<TB, TL, NV>(a, u, a.branch, a.bs, row, l);
-        load_row<TB, TL, NV>(a, g, a.gate, a.gs, row, l);
-        load_row<TX, TL, NV>(a, d, a.dy, a.dys, row, l);
-        load_row<TB, TL, NV>(a, dh, a.dh, a.dhs, row, l);
+        widen_row(y, nx); widen_row(u, no); widen_row(g, ng); widen_row(d, nd); widen_row(dh, nh);
+        fetch(row + step);
         // forward again: u = n(branch) from here on, y unrounded
         if (a.branch) {
-            if (a.post_norm) norm_groups<TL, NV>(a, u, inv, l, row_lds, red);
+            if (a.post_norm) norm_groups<TL, NV>(a, u, inv, l, ex);
             FMARL_EACH(const float s = a.gate ? sigmoid(g[n][r]) : 1.f;
                        const float f = a.gate && a.silu ? g[n][r] * s : s;
                        y[n][r] = in ? y[n][r] + sc[n][r] * (u[n][r] * pw[n][r] + pb[n][r]) * f : 0.f)
         }
         if (a.pre_norm && a.dh) {
-            const float yi = norm_row<TL, NV>(a, y, l, red);   // y: its norm from here on
+            const float yi = norm_row<TL, NV>(a, y, l, ex);   // y: its norm from here on
             float m1 = 0.f, m2 = 0.f;
             FMARL_EACH(acc[3][n][r] += dh[n][r] * y[n][r]; acc[4][n][r] += dh[n][r]; dh[n][r] *= rw[n][r];
                        m1 += dh[n][r]; m2 += dh[n][r] * y[n][r])
-            m2 = team_sum<TL>(m2, red) * (1.f / a.dim);
-            m1 = a.layer ? team_sum<TL>(m1, red) * (1.f / a.dim) : 0.f;
+            team_sum2<TL>(m1, m2, ex);
+            m2 *= 1.f / a.dim;
+            m1 = a.layer ? m1 * (1.f / a.dim) : 0.f;
             FMARL_EACH(d[n][r] += yi * (dh[n][r] - y[n][r] * m2 - m1))
         }
         store_row<TX, TL, NV>(a, d, a.dx, row, l);
@@ -257,11 +292,11 @@ __global__ __launch_bounds__(THREADS) void block_norm_backward_kernel(Block a) {
             if (a.post_norm) {
                 float m[NV][4];
                 FMARL_EACH(m[n][r] = d[n][r] * u[n][r])
-                group_means<TL, NV>(a, m, l, row_lds, red);
+                group_means<TL, NV>(a, m, l, ex);
                 FMARL_EACH(u[n][r] = d[n][r] - u[n][r] * m[n][r])
                 if (a.layer) {
                     FMARL_EACH(m[n][r] = d[n][r])
-                    group_means<TL, NV>(a, m, l, row_lds, red);
+                    group_means<TL, NV>(a, m, l, ex);
                     FMARL_EACH(u[n][r] -= m[n][r])
                 }
                 FMARL_EACH(d[n][r] = in ? u[n][r] * inv[n][r] : 0.f)
@@ -290,17 +325,19 @@ __global__ __launch_bounds__(THREADS) void block_norm_backward_kernel(Block a) {
 
 struct BlockSums { float *out[5]; const float *partial; int dim, parts; };
 
-// 32 columns a workgroup, eight threads a column: each adds every eighth workgroup's partial in float64, then the eight are added in order
+// 8 columns a workgroup, 32 threads a column: each adds every 32nd workgroup's partial in float64, then the 32 are added in order
 __global__ __launch_bounds__(256) void block_sums_kernel(BlockSums a) {
-    __shared__ double red[8][33];
-    const int c = threadIdx.x & 31, s = threadIdx.x >> 5, n = 5 * a.dim, i = blockIdx.x * 32 + c;
+    __shared__ double red[32][9];
+    const int c = threadIdx.x & 7, s = threadIdx.x >> 3, n = 5 * a.dim, i = blockIdx.x * 8 + c;
     double sum = 0.0;
-    if (i < n && a.out[i / a.dim])
-        for (int p = s; p < a.parts; p += 8) sum += (double)a.partial[(int64_t)p * n + i];
+    if (i < n && a.out[i / a.dim]) {
+#pragma unroll 8
+        for (int p = s; p < a.parts; p += 32) sum += (double)a.partial[(int64_t)p * n + i];
+    }
     red[s][c] = sum;
     __syncthreads();
     if (s == 0 && i < n && a.out[i / a.dim]) {
-        for (int k = 1; k < 8; ++k) sum += red[k][c];
+        for (int k = 1; k < 32; ++k) sum += red[k][c];
         a.out[i / a.dim][i % a.dim] = (float)sum;
     }
 }
@@ -337,31 +374,33 @@ Block block_args(const FmarlBlock *b) {
     a.x = (const char *)b->x; a.branch = (const char *)b->branch; a.gate = (const char *)b->gate; a.xs = b->x_stride; a.bs = b->branch_stride; a.gs = b->gate_stride;
     a.scale = b->scale; a.post_w = b->post_weight; a.post_b = b->post_bias; a.pre_w = b->pre_weight; a.pre_b = b->pre_bias;
     const int lanes = b->dim / b->groups / 4;
-    const int team = b->dim <= 128 ? 16 : 64;
+    const int team = b->dim <= 64 ? 16 : b->dim <= 128 ? 32 : 64;   // lanes that can exchange without LDS
     a.group_mode = b->groups == 1 ? kGroupRow : b->dim / b->groups % 4 == 0 && (lanes & (lanes - 1)) == 0 && lanes <= team ? kGroupLanes : kGroupLds;
     return a;
 }
 
 bool row_aligned(const void *p, int64_t stride, int bytes) { return ((uintptr_t)p & (4 * bytes - 1)) == 0 && (stride & 3) == 0; }
 
-// Workgroups of the backward pass: enough to fill the chip (4 per CU), and few beside the rows, so that their partial sums of the weights' gradients
-// (5 dim floats each) stay below a sixteenth of the bytes of the rows
-int block_workgroups(const FmarlBlock *b) {
-    int64_t n = (b->rows + 15) / 16;
-    if (n > 1024) n = 1024;
-    return (int)(n < 1 ? 1 : n);
+int block_threads(int dim) { return dim <= 256 ? 256 : dim <= 512 ? 128 : dim <= 1024 ? 256 : dim <= 4096 ? 512 : 1024; }
+
+// Workgroups: what is resident at a time -- forwards five waves a SIMD, backwards three --, each looping over its share of the rows; backwards few beside the
+// rows, so that their partial sums of the weights' gradients (5 dim floats each) stay below a sixteenth of the bytes of the rows
+int block_workgroups(const FmarlBlock *b, bool backward) {
+    const int threads = block_threads(b->dim), teams = b->dim <= 64 ? 16 : b->dim <= 128 ? 8 : b->dim <= 256 ? 4 : 1;
+    const int64_t want = backward ? (b->rows + 15) / 16 : (b->rows + teams - 1) / teams, most = (backward ? 3 : 5) * 65536 / threads;
+    return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
 template <typename TX, typename TB, int TL, int NV, int THREADS>
 int launch_block_as(const Block &a, bool backward, int blocks, hipStream_t st) {
-    const size_t teams = THREADS / TL, row = ((a.dim + 3) & ~3) + a.groups;
-    size_t lds = 16 + (a.group_mode == kGroupLds ? teams * row : 0);
+    const size_t teams = THREADS / TL;
+    size_t lds = 64 + (a.group_mode == kGroupLds ? teams * 2 * block_row_floats(a.dim, a.groups) : 0);
     if (backward && teams > 1 && lds < teams * a.dim) lds = teams * a.dim;
-    if (backward) hipLaunchKernelGGL((block_norm_backward_kernel<TX, TB, TL, NV, THREADS>), dim3(blocks), dim3(THREADS), 4 * lds, st, a);
-    else {
-        const int64_t want = (a.rows + teams - 1) / teams;
-        hipLaunchKernelGGL((block_norm_kernel<TX, TB, TL, NV, THREADS>), dim3((unsigned)(want < 4096 ? want : 4096)), dim3(THREADS), 4 * lds, st, a);
-    }
+    lds *= 4;
+    const void *kernel = backward ? (const void *)block_norm_backward_kernel<TX, TB, TL, NV, THREADS> : (const void *)block_norm_kernel<TX, TB, TL, NV, THREADS>;
+    if (lds > 64 * 1024) HIP_OK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    if (backward) hipLaunchKernelGGL((block_norm_backward_kernel<TX, TB, TL, NV, THREADS>), dim3(blocks), dim3(THREADS), lds, st, a);
+    else hipLaunchKernelGGL((block_norm_kernel<TX, TB, TL, NV, THREADS>), dim3(blocks), dim3(THREADS), lds, st, a);
     HIP_OK(hipGetLastError());
     return FMARL_OK;
 }
@@ -369,12 +408,12 @@ int launch_block_as(const Block &a, bool backward, int blocks, hipStream_t st) {
 template <typename TX, typename TB>
 int launch_block_t(const Block &a, bool backward, int blocks, hipStream_t st) {
     if (a.dim <= 64) return launch_block_as<TX, TB, 16, 1, 256>(a, backward, blocks, st);
-    if (a.dim <= 128) return launch_block_as<TX, TB, 16, 2, 256>(a, backward, blocks, st);
+    if (a.dim <= 128) return launch_block_as<TX, TB, 32, 1, 256>(a, backward, blocks, st);
     if (a.dim <= 256) return launch_block_as<TX, TB, 64, 1, 256>(a, backward, blocks, st);
-    if (a.dim <= 512) return launch_block_as<TX, TB, 64, 2, 256>(a, backward, blocks, st);
-    if (a.dim <= 1024) return launch_block_as<TX, TB, 64, 4, 256>(a, backward, blocks, st);
-    if (a.dim <= 2048) return launch_block_as<TX, TB, 256, 2, 256>(a, backward, blocks, st);
-    if (a.dim <= 4096) return launch_block_as<TX, TB, 256, 4, 256>(a, backward, blocks, st);
+    if (a.dim <= 512) return launch_block_as<TX, TB, 128, 1, 128>(a, backward, blocks, st);
+    if (a.dim <= 1024) return launch_block_as<TX, TB, 256, 1, 256>(a, backward, blocks, st);
+    if (a.dim <= 2048) return launch_block_as<TX, TB, 512, 1, 512>(a, backward, blocks, st);
+    if (a.dim <= 4096) return launch_block_as<TX, TB, 512, 2, 512>(a, backward, blocks, st);
     return launch_block_as<TX, TB, 1024, 2, 1024>(a, backward, blocks, st);
 }
 
@@ -397,12 +436,12 @@ int fmarl_block_norm(const FmarlBlock *b, void *y, void *h, void *stream) {
     const int xb = elem_bytes(b->x_dtype), tb = elem_bytes(b->dtype);
     a.y = b->branch ? (char *)y : nullptr; a.h = b->pre_norm ? (char *)h : nullptr;
     a.vec = (b->dim & 3) == 0 && row_aligned(a.x, a.xs, xb) && row_aligned(a.branch, a.bs, tb) && row_aligned(a.gate, a.gs, tb) && row_aligned(a.y, 0, xb) && row_aligned(a.h, 0, tb);
-    return launch_block(b, a, false, 0, (hipStream_t)stream);
+    return launch_block(b, a, false, block_workgroups(b, false), (hipStream_t)stream);
 }
 
 size_t fmarl_block_norm_workspace(const FmarlBlock *b) {
     if (block_check(b, "fmarl_block_norm_workspace")) return 0;
-    return (size_t)block_workgroups(b) * 5 * b->dim * 4;
+    return (size_t)block_workgroups(b, true) * 5 * b->dim * 4;
 }
 
 int fmarl_block_norm_backward(const FmarlBlock *b, const void *d_y, int64_t d_y_stride, const void *d_h, int64_t d_h_stride, void *d_x, void *d_branch,
@@ -417,14 +456,14 @@ int fmarl_block_norm_backward(const FmarlBlock *b, const void *d_y, int64_t d_y_
     a.dx = (char *)d_x; a.dbranch = (char *)d_branch; a.dgate = (char *)d_gate; a.partial = (float *)workspace;
     a.vec = (b->dim & 3) == 0 && row_aligned(a.x, a.xs, xb) && row_aligned(a.branch, a.bs, tb) && row_aligned(a.gate, a.gs, tb) && row_aligned(a.dy, a.dys, xb) &&
             row_aligned(a.dh, a.dhs, tb) && row_aligned(a.dx, 0, xb) && row_aligned(a.dbranch, 0, tb) && row_aligned(a.dgate, 0, tb);
-    const int blocks = block_workgroups(b);
+    const int blocks = block_workgroups(b, true);
     if (int rc = launch_block(b, a, true, blocks, (hipStream_t)stream)) return rc;
     BlockSums s = {};
     bool any = false;
     for (int k = 0; k < 5; ++k) { s.out[k] = d_weights[k]; any = any || d_weights[k]; }
     if (any) {
         s.partial = (const float *)workspace; s.dim = b->dim; s.parts = blocks;
-        hipLaunchKernelGGL(block_sums_kernel, dim3((5 * b->dim + 31) / 32), dim3(256), 0, (hipStream_t)stream, s);
+        hipLaunchKernelGGL(block_sums_kernel, dim3((5 * b->dim + 7) / 8), dim3(256), 0, (hipStream_t)stream, s);
         HIP_OK(hipGetLastError());
     }
     return FMARL_OK;
