@@ -19,17 +19,23 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.T_F32, torch.bfloat16: _lib.T_BF16, torch.float16: _lib.T_F16}
+_F32 = torch.float32
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)   # (2 us less per call than torch.cuda.current_stream(..).cuda_stream)
 
 
-def _need(ok, text, *args):
-    if not ok:
-        raise ValueError(text % args if args else text)
+# A call's host time is most of a small call's: arguments are checked by plain conditions, messages are formed only when one fails.
+def _refuse(text, *args):
+    raise ValueError(text % args if args else text)
 
 
 def _same_device(op, first, *rest):
-    _need(first.is_cuda, '%s: tensors must be on a GPU, got one on %s', op, first.device)
+    if not first.is_cuda:
+        _refuse('%s: tensors must be on a GPU, got one on %s', op, first.device)
+    dev = first.device
     for t in rest:
-        _need(t is None or t.device == first.device, '%s: all tensors must be on %s', op, first.device)
+        if t is not None and t.device != dev:
+            _refuse('%s: all tensors must be on %s, got one on %s', op, dev, t.device)
+    return dev
 
 
 def _last(t):
@@ -41,8 +47,28 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _wants_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _run(entry, dev, *args):
+    """One call of the C-ABI on dev's current stream."""
+    lib = _lib.load()
+    if torch.cuda.current_device() == dev.index:
+        rc = getattr(lib, entry)(*args, _raw_stream(dev.index) if _raw_stream else torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(lib, entry)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _lib.check(rc, entry)
+
+
+def _workspace(like, nbytes):
+    return like.new_empty(nbytes, dtype=torch.uint8)
 
 
 def _rows(t):
@@ -55,57 +81,58 @@ def _rows(t):
 def _memory_args(op, q, k, v, log_decay, state, masks, scale, lead):
     """The checked, laid out arguments: (FmarlMemory, tensors to keep)."""
     _same_device(op, q, k, v, log_decay, state, masks)
-    _need(q.dtype in _DTYPES and k.dtype == q.dtype and v.dtype == q.dtype, '%s: q, k and v must be of one type out of float32, bfloat16, float16', op)
-    _need(q.dim() == lead + 2 and k.shape == q.shape and v.shape[:-1] == q.shape[:-1] and v.dim() == q.dim(),
-          '%s: q and k (%sB, H, dk), v (%sB, H, dv), got %s, %s, %s', op, 'L, ' * (lead - 1), 'L, ' * (lead - 1), tuple(q.shape), tuple(k.shape), tuple(v.shape))
-    L = q.shape[0] if lead == 2 else 1
-    B, H, dk, dv = q.shape[-3], q.shape[-2], q.shape[-1], v.shape[-1]
-    _need(log_decay.dtype == torch.float32, '%s: log_decay must be float32', op)
-    token = log_decay.dim() != 1
-    _need(tuple(log_decay.shape) == (tuple(q.shape[:-1]) if token else (H,)), '%s: log_decay must be (H,) or %s, got %s', op, tuple(q.shape[:-1]),
-          tuple(log_decay.shape))
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        _refuse('%s: q, k and v must be of one type out of float32, bfloat16, float16, got %s, %s, %s', op, q.dtype, k.dtype, v.dtype)
+    shape, vshape = q.shape, v.shape
+    if len(shape) != lead + 2 or k.shape != shape or len(vshape) != lead + 2 or vshape[:-1] != shape[:-1]:
+        _refuse('%s: q and k (%sB, H, dk), v (%sB, H, dv), got %s, %s, %s', op, 'L, ' * (lead - 1), 'L, ' * (lead - 1), tuple(shape), tuple(k.shape), tuple(vshape))
+    B, H, dk = shape[-3:]
+    L, dv = shape[0] if lead == 2 else 1, vshape[-1]
+    gs = log_decay.stride()
+    token = len(gs) != 1
+    if log_decay.dtype != _F32 or log_decay.shape != (shape[:-1] if token else (H,)):
+        _refuse('%s: log_decay must be float32 (H,) or %s, got %s %s', op, tuple(shape[:-1]), log_decay.dtype, tuple(log_decay.shape))
+    ml = mb = 0
     if masks is not None:
-        _need(masks.numel() == L * B, '%s: masks must hold %d entries, got %s', op, L * B, tuple(masks.shape))
-        masks = masks.to(torch.float32).reshape(L, B)
+        if masks.numel() != L * B:
+            _refuse('%s: masks must hold %d entries, got %s', op, L * B, tuple(masks.shape))
+        if masks.dtype != _F32:
+            masks = masks.to(_F32)
+        if lead == 1:
+            masks = masks.reshape(B)
+            mb = masks.stride(0)
+        else:
+            masks = masks.reshape(L, B)
+            ml, mb = masks.stride()
     if state is not None:
-        _need(state.dtype == torch.float32 and state.numel() == B * H * dk * dv, '%s: state must be float32 with B H dk dv = %d entries, got %s %s', op,
-              B * H * dk * dv, state.dtype, tuple(state.shape))
+        if state.dtype != _F32 or state.numel() != B * H * dk * dv:
+            _refuse('%s: state must be float32 with B H dk dv = %d entries, got %s %s', op, B * H * dk * dv, state.dtype, tuple(state.shape))
         state = state.contiguous()
     q, k, v = _last(q), _last(k), _last(v)
-    gs = log_decay.stride()
     m = _lib.FmarlMemory(L, B, H, dk, dv, _DTYPES[q.dtype], dk ** -0.5 if scale is None else float(scale), 0 if token else 1, _rows(q), _rows(k), _rows(v),
-                         log_decay.data_ptr(), gs[0] if len(gs) == 3 else 0, gs[-2] if token else 0, gs[-1], _ptr(masks),
-                         masks.stride(0) if masks is not None else 0, masks.stride(1) if masks is not None else 0, _ptr(state))
+                         log_decay.data_ptr(), gs[0] if len(gs) == 3 else 0, gs[-2] if token else 0, gs[-1], _ptr(masks), ml, mb, _ptr(state))
     return m, (q, k, v, log_decay, state, masks)
 
 
 def _launch_chunk(m, keep):
-    q, v = keep[0], keep[2]
-    dev = q.device
-    out = torch.empty(v.shape, dtype=v.dtype, device=dev)
-    state = torch.empty(m.B, m.H, m.dk, m.dv, dtype=torch.float32, device=dev)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        ws = torch.empty(lib.fmarl_memory_workspace(m, 0), dtype=torch.uint8, device=dev)
-        _lib.check(lib.fmarl_memory_chunk(m, _rows(out), state.data_ptr(), ws.data_ptr(), _stream(dev)), 'fmarl_memory_chunk')
+    v = keep[2]
+    out, state = v.new_empty(v.shape), v.new_empty((m.B, m.H, m.dk, m.dv), dtype=_F32)
+    ws = _workspace(v, _lib.load().fmarl_memory_workspace(m, 0))
+    _run('fmarl_memory_chunk', v.device, m, _rows(out), state.data_ptr(), ws.data_ptr())
     return out, state, ws
 
 
 def _launch_chunk_backward(m, keep, d_out, d_state, want_decay=True, forward_ws=None):
     q, k, v, g, state = keep[:5]
-    dev = q.device
     d_out = _last(d_out)
     if d_state is not None:
         d_state = d_state.contiguous()
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-    dg = torch.empty(g.shape, dtype=torch.float32, device=dev) if want_decay else None
-    ds = torch.empty(m.B, m.H, m.dk, m.dv, dtype=torch.float32, device=dev)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        ws = torch.empty(lib.fmarl_memory_workspace(m, 1), dtype=torch.uint8, device=dev)
-        _lib.check(lib.fmarl_memory_chunk_backward(m, _rows(d_out), _ptr(d_state), _rows(dq), _rows(dk), _rows(dv), _ptr(dg), ds.data_ptr(), _ptr(forward_ws),
-                                                   ws.data_ptr(),
-                                                   _stream(dev)), 'fmarl_memory_chunk_backward')
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dg = g.new_empty(g.shape) if want_decay else None
+    ds = g.new_empty((m.B, m.H, m.dk, m.dv))
+    ws = _workspace(v, _lib.load().fmarl_memory_workspace(m, 1))
+    _run('fmarl_memory_chunk_backward', v.device, m, _rows(d_out), _ptr(d_state), _rows(dq), _rows(dk), _rows(dv), _ptr(dg), ds.data_ptr(), _ptr(forward_ws),
+         ws.data_ptr())
     return dq, dk, dv, dg, ds
 
 
@@ -115,7 +142,7 @@ class _MemoryChunk(torch.autograd.Function):
         m, keep = _memory_args('memory_chunk', q, k, v, log_decay, state, masks, scale, 2)
         out, last, ws = _launch_chunk(m, keep)
         ctx.save_for_backward(*keep)
-        ctx.forward_ws = ws if any(ctx.needs_input_grad) else None   # long sequences: the states at their segments' starts
+        ctx.forward_ws = ws   # long sequences: the states at their segments' starts
         ctx.scale, ctx.state_shape = m.scale, None if state is None else state.shape
         ctx.set_materialize_grads(False)
         return out, last
@@ -142,11 +169,15 @@ def memory_chunk(q, k, v, log_decay, state=None, masks=None, scale=None):
     generator's ``masks`` (0: an episode starts at the token).  scale: dk ** -0.5 if None.  Rows ordered (L, chunk) as ``recurrent_generator``
     yields them are this layout: ``q.view(L, chunks, H, dk)``.  States, decays and all sums are float32 (the decays' prefix sums float64).
     Differentiable in q, k, v, log_decay and state, once."""
-    _need(q.dim() == 4 and v.dim() == 4, 'memory_chunk: q, k (L, B, H, dk) and v (L, B, H, dv), got %s, %s', tuple(q.shape), tuple(v.shape))
+    if q.dim() != 4 or v.dim() != 4:
+        _refuse('memory_chunk: q, k (L, B, H, dk) and v (L, B, H, dv), got %s, %s', tuple(q.shape), tuple(v.shape))
     if q.shape[0] == 0 or q.shape[1] == 0:
         _memory_args('memory_chunk', q, k, v, log_decay, state, masks, scale, 2)
         shape = (q.shape[1], q.shape[2], q.shape[3], v.shape[3])
         return v.clone(), torch.zeros(shape, dtype=torch.float32, device=q.device) if state is None else state.reshape(shape).clone()
+    if not _wants_grad(q, k, v, log_decay, state):
+        m, keep = _memory_args('memory_chunk', q, k, v, log_decay, state, masks, scale, 2)
+        return _launch_chunk(m, keep)[:2]
     return _MemoryChunk.apply(q, k, v, log_decay, state, masks, scale)
 
 
@@ -154,11 +185,13 @@ def memory_chunk_backward(q, k, v, log_decay, d_out, d_state=None, state=None, m
     """The gradients of ``memory_chunk`` as a plain call: (dq, dk, dv, d_log_decay, d_state0) from d_out (L, B, H, dv) and the gradient of the last
     state (None: zeros)."""
     m, keep = _memory_args('memory_chunk_backward', q, k, v, log_decay, state, masks, scale, 2)
-    _need(m.L > 0 and m.B > 0, 'memory_chunk_backward: no tokens')
+    if m.L == 0 or m.B == 0:
+        _refuse('memory_chunk_backward: no tokens')
     _same_device('memory_chunk_backward', q, d_out, d_state)
-    _need(d_out.shape == v.shape and d_out.dtype == v.dtype, 'memory_chunk_backward: d_out must be %s %s', tuple(v.shape), v.dtype)
-    if d_state is not None:
-        _need(d_state.dtype == torch.float32 and d_state.numel() == m.B * m.H * m.dk * m.dv, 'memory_chunk_backward: d_state must be float32 (B, H, dk, dv)')
+    if d_out.shape != v.shape or d_out.dtype != v.dtype:
+        _refuse('memory_chunk_backward: d_out must be %s %s, got %s %s', tuple(v.shape), v.dtype, tuple(d_out.shape), d_out.dtype)
+    if d_state is not None and (d_state.dtype != _F32 or d_state.numel() != m.B * m.H * m.dk * m.dv):
+        _refuse('memory_chunk_backward: d_state must be float32 (B, H, dk, dv), got %s %s', d_state.dtype, tuple(d_state.shape))
     return _launch_chunk_backward(m, keep, d_out, d_state)
 
 
@@ -166,22 +199,21 @@ def memory_step(q, k, v, log_decay, state, masks=None, scale=None, out_state=Non
     """``memory_chunk`` for one token per sequence, as an env step of the rollout takes it: ``(out, out_state)``.  q, k (B, H, dk), v (B, H, dv), log_decay
     (H,) or (B, H), masks B entries, state None or float32 with B H dk dv entries.  out_state: where the new state goes (float32, contiguous; the buffer's next slot, or ``state``
     itself), a new (B, H, dk, dv) tensor if None.  No gradient: refused where one would be recorded."""
-    _need(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, state))),
-          'memory_step records no gradient: call it under torch.no_grad(), or use memory_chunk')
+    if _wants_grad(q, k, v, log_decay, state):
+        _refuse('memory_step records no gradient: call it under torch.no_grad(), or use memory_chunk')
     m, keep = _memory_args('memory_step', q, k, v, log_decay, state, masks, scale, 1)
-    dev, n = q.device, m.B * m.H * m.dk * m.dv
+    n = m.B * m.H * m.dk * m.dv
     if out_state is None:
-        out_state = torch.empty(m.B, m.H, m.dk, m.dv, dtype=torch.float32, device=dev)
+        out_state = v.new_empty((m.B, m.H, m.dk, m.dv), dtype=_F32)
     else:
-        _need(out_state.device == dev and out_state.dtype == torch.float32 and out_state.numel() == n and out_state.is_contiguous(),
-              'memory_step: out_state must be contiguous float32 with %d entries on %s', n, dev)
+        if out_state.device != q.device or out_state.dtype != _F32 or out_state.numel() != n or not out_state.is_contiguous():
+            _refuse('memory_step: out_state must be contiguous float32 with %d entries on %s', n, q.device)
         if keep[4] is not None:
-            gap = abs(out_state.data_ptr() - keep[4].data_ptr())
-            _need(gap == 0 or gap >= 4 * n, 'memory_step: out_state overlaps state without being it')
-    out = torch.empty(v.shape, dtype=v.dtype, device=dev)
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.fmarl_memory_step(m, _rows(out), out_state.data_ptr(), _stream(dev)), 'fmarl_memory_step')
+            gap = abs(out_state.data_ptr() - m.state) if n else 0
+            if gap and gap < 4 * n:
+                _refuse('memory_step: out_state overlaps state without being it')
+    out = v.new_empty(v.shape)
+    _run('fmarl_memory_step', q.device, m, _rows(out), out_state.data_ptr())
     return out, out_state
 
 
@@ -189,43 +221,52 @@ def memory_step(q, k, v, log_decay, state, masks=None, scale=None, out_state=Non
 _WEIGHTS = ('scale', 'post_weight', 'post_bias', 'pre_weight', 'pre_bias')
 
 
-def _block_args(x, branch, gate, weights, groups, kind, gate_act, post_norm, pre_norm, eps):
-    """(FmarlBlock, 2-d views of x, branch and gate, the float32 weights); what has to live until the launch is in there."""
+def _block_args(x, branch, gate, weights, groups, layer, silu, post_norm, pre_norm, eps):
+    """(FmarlBlock, the tensors it points into, which have to live until the launch)."""
     _same_device('block_norm', x, branch, gate, *weights)
-    D = x.shape[-1] if x.dim() else 0
+    shape, D = x.shape, x.shape[-1]
     dtype = x.dtype if branch is None else branch.dtype
-    _need(dtype in _DTYPES and x.dtype in (dtype, torch.float32), 'block_norm: float32, bfloat16 or float16; x of the branch\'s type or float32, got %s, %s',
-          x.dtype, dtype)
-    for name, t in (('branch', branch), ('gate', gate)):
-        _need(t is None or (t.shape == x.shape and t.dtype == dtype), 'block_norm: %s must be %s %s', name, tuple(x.shape), dtype)
+    if dtype not in _DTYPES or (x.dtype != dtype and x.dtype != _F32):
+        _refuse('block_norm: float32, bfloat16 or float16; x of the branch\'s type or float32, got %s, %s', x.dtype, dtype)
+    x2 = _last(x.reshape(-1, D))
+    b2 = g2 = None
+    if branch is not None:
+        if branch.shape != shape:
+            _refuse('block_norm: branch must be %s, got %s', tuple(shape), tuple(branch.shape))
+        b2 = _last(branch.reshape(-1, D))
+    if gate is not None:
+        if gate.shape != shape or gate.dtype != dtype:
+            _refuse('block_norm: gate must be %s %s, got %s %s', tuple(shape), dtype, tuple(gate.shape), gate.dtype)
+        g2 = _last(gate.reshape(-1, D))
+    ws = []
     for name, w in zip(_WEIGHTS, weights):
-        _need(w is None or (tuple(w.shape) == (D,) and w.dtype == torch.float32), 'block_norm: %s must be float32 (%d,)', name, D)
-    _need(kind in ('rms', 'layer'), 'block_norm: kind must be rms or layer, got %r', kind)
-    _need(gate_act in ('sigmoid', 'silu'), 'block_norm: gate_act must be sigmoid or silu, got %r', gate_act)
-    rows = [None if t is None else _last(t.reshape(-1, D)) for t in (x, branch, gate)]
-    weights = [None if w is None else w.contiguous() for w in weights]
-    st = lambda t: 0 if t is None else t.stride(0)  # noqa: E731
-    b = _lib.FmarlBlock(rows[0].shape[0], D, int(groups), _DTYPES[dtype], _DTYPES[x.dtype], int(kind == 'layer'), int(gate_act == 'silu'), int(bool(post_norm)),
-                        int(bool(pre_norm)), float(eps), 0, _ptr(rows[0]), st(rows[0]), _ptr(rows[1]), st(rows[1]), _ptr(rows[2]), st(rows[2]),
-                        *[_ptr(w) for w in weights])
-    return b, rows, weights
+        if w is not None:
+            if w.dtype != _F32 or w.shape != (D,):
+                _refuse('block_norm: %s must be float32 (%d,), got %s %s', name, D, w.dtype, tuple(w.shape))
+            w = w.contiguous()
+        ws.append(w)
+    b = _lib.FmarlBlock(x2.shape[0], D, groups, _DTYPES[dtype], _DTYPES[x.dtype], layer, silu, post_norm, pre_norm, eps, 0, x2.data_ptr(), x2.stride(0), _ptr(b2),
+                        0 if b2 is None else b2.stride(0), _ptr(g2), 0 if g2 is None else g2.stride(0), *[None if w is None else w.data_ptr() for w in ws])
+    return b, (x2, b2, g2, ws)
+
+
+def _launch_block(x, branch, gate, weights, options):
+    b, keep = _block_args(x, branch, gate, weights, *options)
+    y = None if branch is None else x.new_empty(x.shape)
+    h = (x if branch is None else branch).new_empty(x.shape) if options[4] else None
+    _run('fmarl_block_norm', x.device, b, _ptr(y), _ptr(h))
+    return y, h
 
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias, options):
         weights = (scale, post_weight, post_bias, pre_weight, pre_bias)
-        b, rows, weights = _block_args(x, branch, gate, weights, *options)
-        dev = x.device
-        y = None if branch is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        h = torch.empty(x.shape, dtype=x.dtype if branch is None else branch.dtype, device=dev) if options[4] else None
-        lib = _lib.load()
-        with torch.cuda.device(dev):
-            _lib.check(lib.fmarl_block_norm(b, _ptr(y), _ptr(h), _stream(dev)), 'fmarl_block_norm')
+        out = _launch_block(x, branch, gate, weights, options)
         ctx.save_for_backward(x, branch, gate, *weights)
         ctx.options = options
         ctx.set_materialize_grads(False)
-        return y, h
+        return out
 
     @staticmethod
     @once_differentiable
@@ -234,18 +275,17 @@ class _BlockNorm(torch.autograd.Function):
         if dy is None and dh is None:
             return (None,) * 9
         need = ctx.needs_input_grad
-        b, rows, weights = _block_args(x, branch, gate, weights, *ctx.options)
-        dev, D = x.device, x.shape[-1]
-        dy, dh = (None if t is None else _last(t.reshape(-1, D)) for t in (dy, dh))
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dbranch, dgate = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (branch, gate))
-        dw = [torch.empty(D, dtype=torch.float32, device=dev) if w is not None and n else None for w, n in zip(weights, need[3:8])]
-        lib = _lib.load()
-        with torch.cuda.device(dev):
-            ws = torch.empty(lib.fmarl_block_norm_workspace(b), dtype=torch.uint8, device=dev)
-            _lib.check(lib.fmarl_block_norm_backward(b, _ptr(dy), 0 if dy is None else dy.stride(0), _ptr(dh), 0 if dh is None else dh.stride(0), dx.data_ptr(),
-                                                     _ptr(dbranch), _ptr(dgate), (C.c_void_p * 5)(*[_ptr(t) for t in dw]), ws.data_ptr(), _stream(dev)),
-                       'fmarl_block_norm_backward')
+        b, keep = _block_args(x, branch, gate, weights, *ctx.options)
+        D = b.dim
+        dy = None if dy is None else _last(dy.reshape(-1, D))
+        dh = None if dh is None else _last(dh.reshape(-1, D))
+        dx = x.new_empty(x.shape)
+        dbranch = None if branch is None else branch.new_empty(x.shape)
+        dgate = None if gate is None else gate.new_empty(x.shape)
+        dw = [w.new_empty(D) if w is not None and n else None for w, n in zip(weights, need[3:8])]
+        ws = _workspace(x, _lib.load().fmarl_block_norm_workspace(b))
+        _run('fmarl_block_norm_backward', x.device, b, _ptr(dy), 0 if dy is None else dy.stride(0), _ptr(dh), 0 if dh is None else dh.stride(0), dx.data_ptr(),
+             _ptr(dbranch), _ptr(dgate), (C.c_void_p * 5)(*[_ptr(t) for t in dw]), ws.data_ptr())
         return (dx, dbranch, dgate, *dw, None)
 
 
@@ -261,16 +301,30 @@ def block_norm(x, branch=None, gate=None, scale=None, post_weight=None, post_bia
     biases: float32 (D,).  Whatever is None is left out (factor 1, bias 0).  Without a branch y is x and h = n(x) pre_weight + pre_bias: the first
     block's start; ``post_norm=False`` takes the branch as it is, ``pre_norm=False`` returns h = None: the last block's end.  h is formed from y before its
     rounding.  Differentiable in all tensors, once; nothing but the inputs is kept for the backward pass."""
-    _need(x.dim() >= 1 and 1 <= x.shape[-1] <= 8192, 'block_norm: the last axis must hold 1..8192 elements, got %s', tuple(x.shape))
-    D = x.shape[-1]
-    _need(isinstance(groups, int) and 1 <= groups <= 256 and D % groups == 0, 'block_norm: groups must lie in 1..256 and divide %d, got %r', D, groups)
-    _need(branch is not None or (gate is None and scale is None and post_weight is None and post_bias is None),
-          'block_norm: gate, scale and post weights need a branch')
-    _need(post_norm or (post_weight is None and post_bias is None), 'block_norm: post weights need post_norm')
-    _need(pre_norm or (pre_weight is None and pre_bias is None), 'block_norm: pre weights need pre_norm')
-    _need(branch is not None or pre_norm, 'block_norm: without a branch and without pre_norm there is nothing to do')
-    _need(eps >= 0, 'block_norm: eps must not be negative')
-    y, h = _BlockNorm.apply(x, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias, (groups, kind, gate_act, bool(post_norm), bool(pre_norm), eps))
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
+        _refuse('block_norm: the last axis must hold 1..8192 elements, got %s', tuple(x.shape))
+    if not isinstance(groups, int) or not 1 <= groups <= 256 or x.shape[-1] % groups:
+        _refuse('block_norm: groups must lie in 1..256 and divide %d, got %r', x.shape[-1], groups)
+    if kind not in ('rms', 'layer'):
+        _refuse('block_norm: kind must be rms or layer, got %r', kind)
+    if gate_act not in ('sigmoid', 'silu'):
+        _refuse('block_norm: gate_act must be sigmoid or silu, got %r', gate_act)
+    if branch is None and not (gate is None and scale is None and post_weight is None and post_bias is None):
+        _refuse('block_norm: gate, scale and post weights need a branch')
+    if not post_norm and not (post_weight is None and post_bias is None):
+        _refuse('block_norm: post weights need post_norm')
+    if not pre_norm and not (pre_weight is None and pre_bias is None):
+        _refuse('block_norm: pre weights need pre_norm')
+    if branch is None and not pre_norm:
+        _refuse('block_norm: without a branch and without pre_norm there is nothing to do')
+    if not eps >= 0:
+        _refuse('block_norm: eps must not be negative, got %r', eps)
+    weights = (scale, post_weight, post_bias, pre_weight, pre_bias)
+    options = (groups, int(kind == 'layer'), int(gate_act == 'silu'), int(bool(post_norm)), int(bool(pre_norm)), eps)
+    if _wants_grad(x, branch, gate, *weights):
+        y, h = _BlockNorm.apply(x, branch, gate, *weights, options)
+    else:
+        y, h = _launch_block(x, branch, gate, weights, options)
     return (x if branch is None else y), h
 
 
@@ -281,35 +335,43 @@ _ACTION_TYPES = {torch.int64: 0, torch.int32: 1, torch.float32: 2}
 def _action_args(features, weight, bias, actions, available):
     """(FmarlActions, the laid out tensors, which have to live until the launch)."""
     _same_device('action_log_probs', features, weight, bias, actions, available)
-    K, V = weight.shape[1], weight.shape[0]
-    _need(features.dtype in _DTYPES and weight.dtype == features.dtype, 'action_log_probs: features and weight must be of one type out of float32, bfloat16, float16')
-    _need(bias is None or (tuple(bias.shape) == (V,) and bias.dtype == torch.float32), 'action_log_probs: bias must be (%d,)', V)
+    V, K = weight.shape
+    if features.dtype not in _DTYPES or weight.dtype != features.dtype:
+        _refuse('action_log_probs: features and weight must be of one type out of float32, bfloat16, float16, got %s, %s', features.dtype, weight.dtype)
+    if bias is not None:
+        if bias.shape != (V,):
+            _refuse('action_log_probs: bias must be (%d,), got %s', V, tuple(bias.shape))
+        bias = bias.contiguous()
     x, w = _last(features.reshape(-1, K)), _last(weight)
     M = x.shape[0]
-    _need(actions.dtype in _ACTION_TYPES and actions.numel() == M, 'action_log_probs: actions must be int64, int32 or float32 with %d entries, got %s %s', M,
-          actions.dtype, tuple(actions.shape))
-    actions = actions.reshape(M).contiguous()
+    if actions.dtype not in _ACTION_TYPES or actions.numel() != M:
+        _refuse('action_log_probs: actions must be int64, int32 or float32 with %d entries, got %s %s', M, actions.dtype, tuple(actions.shape))
+    actions = actions.contiguous()
+    kind = stride = 0
     if available is not None:
-        _need(available.dtype in (torch.float32, torch.bool, torch.uint8) and available.numel() == M * V and available.shape[-1] == V,
-              'action_log_probs: available_actions must be float32, bool or uint8 (..., %d) with %d entries, got %s %s', V, M * V, available.dtype, tuple(available.shape))
+        if available.dtype not in (_F32, torch.bool, torch.uint8) or available.numel() != M * V or available.shape[-1] != V:
+            _refuse('action_log_probs: available_actions must be float32, bool or uint8 (..., %d) with %d entries, got %s %s', V, M * V, available.dtype,
+                    tuple(available.shape))
         available = _last(available.reshape(M, V))
-    if bias is not None:
-        bias = bias.contiguous()
-    a = _lib.FmarlActions(M, K, V, _DTYPES[x.dtype], _ACTION_TYPES[actions.dtype], int(available is not None and available.dtype != torch.float32), 0, x.data_ptr(),
-                          x.stride(0), w.data_ptr(), w.stride(0), _ptr(bias), actions.data_ptr(), _ptr(available), 0 if available is None else available.stride(0))
+        kind, stride = int(available.dtype != _F32), available.stride(0)
+    a = _lib.FmarlActions(M, K, V, _DTYPES[x.dtype], _ACTION_TYPES[actions.dtype], kind, 0, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), _ptr(bias),
+                          actions.data_ptr(), _ptr(available), stride)
     return a, (x, w, bias, actions, available)
+
+
+def _launch_actions(features, weight, bias, actions, available):
+    a, keep = _action_args(features, weight, bias, actions, available)
+    shape = features.shape[:-1]
+    log_probs, entropy, lse = (features.new_empty(shape, dtype=_F32) for _ in range(3))
+    ws = _workspace(features, _lib.load().fmarl_action_log_probs_workspace(a, 0))
+    _run('fmarl_action_log_probs', features.device, a, log_probs.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ws.data_ptr())
+    return log_probs, entropy, lse
 
 
 class _ActionLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, features, weight, bias, actions, available):
-        a, keep = _action_args(features, weight, bias, actions, available)
-        dev, shape = features.device, features.shape[:-1]
-        log_probs, entropy, lse = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3))
-        lib = _lib.load()
-        with torch.cuda.device(dev):
-            ws = torch.empty(lib.fmarl_action_log_probs_workspace(a, 0), dtype=torch.uint8, device=dev)
-            _lib.check(lib.fmarl_action_log_probs(a, log_probs.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ws.data_ptr(), _stream(dev)), 'fmarl_action_log_probs')
+        log_probs, entropy, lse = _launch_actions(features, weight, bias, actions, available)
         ctx.save_for_backward(features, weight, bias, actions, available, entropy, lse)
         ctx.set_materialize_grads(False)
         return log_probs, entropy
@@ -321,17 +383,14 @@ class _ActionLogProbs(torch.autograd.Function):
         if d_log_probs is None and d_entropy is None:
             return (None,) * 5
         a, keep = _action_args(features, weight, bias, actions, available)
-        dev = features.device
-        dx, dw = torch.empty(features.shape, dtype=features.dtype, device=dev), torch.empty(weight.shape, dtype=weight.dtype, device=dev)
-        db = torch.empty(bias.shape, dtype=torch.float32, device=dev) if bias is not None and ctx.needs_input_grad[2] else None
+        dx, dw = features.new_empty(features.shape), weight.new_empty(weight.shape)
+        db = bias.new_empty(bias.shape) if bias is not None and ctx.needs_input_grad[2] else None
         if a.rows == 0:
             return dx, dw.zero_(), None if db is None else db.zero_(), None, None
         dl, de = (None if t is None else t.contiguous() for t in (d_log_probs, d_entropy))
-        lib = _lib.load()
-        with torch.cuda.device(dev):
-            ws = torch.empty(lib.fmarl_action_log_probs_workspace(a, 1), dtype=torch.uint8, device=dev)
-            _lib.check(lib.fmarl_action_log_probs_backward(a, entropy.data_ptr(), lse.data_ptr(), _ptr(dl), _ptr(de), dx.data_ptr(), dw.data_ptr(), _ptr(db), ws.data_ptr(),
-                                                           _stream(dev)), 'fmarl_action_log_probs_backward')
+        ws = _workspace(features, _lib.load().fmarl_action_log_probs_workspace(a, 1))
+        _run('fmarl_action_log_probs_backward', features.device, a, entropy.data_ptr(), lse.data_ptr(), _ptr(dl), _ptr(de), dx.data_ptr(), dw.data_ptr(), _ptr(db),
+             ws.data_ptr())
         return dx, dw, db, None, None
 
 
@@ -346,9 +405,12 @@ def action_log_probs(features, weight, bias, actions, available_actions=None):
     -inf, one that does not exist (>= V) NaN (and no gradient).  The logits are never stored: for many actions the softmax runs over pieces of them, and they
     are formed again for the gradient.  Differentiable in features, weight and bias, once.  Half precision operands: products are exact, sums float32; the
     gradient's dz is rounded to the operands' type before its two products."""
-    _need(weight.dim() == 2 and features.dim() >= 1 and features.shape[-1] == weight.shape[1] and 1 <= weight.shape[1] <= 16384 and 1 <= weight.shape[0] <= 1 << 20,
-          'action_log_probs: features (..., K) and weight (V, K) with K in 1..16384, V in 1..1048576, got %s, %s', tuple(features.shape), tuple(weight.shape))
-    if bias is not None and bias.dtype != torch.float32:
-        _need(bias.dtype == weight.dtype, 'action_log_probs: bias must be float32 or of the weight\'s type')
+    if weight.dim() != 2 or features.dim() < 1 or features.shape[-1] != weight.shape[1] or not 1 <= weight.shape[1] <= 16384 or not 1 <= weight.shape[0] <= 1 << 20:
+        _refuse('action_log_probs: features (..., K) and weight (V, K) with K in 1..16384, V in 1..1048576, got %s, %s', tuple(features.shape), tuple(weight.shape))
+    if bias is not None and bias.dtype != _F32:
+        if bias.dtype != weight.dtype:
+            _refuse('action_log_probs: bias must be float32 or of the weight\'s type, got %s', bias.dtype)
         bias = bias.float()
+    if not _wants_grad(features, weight, bias):
+        return _launch_actions(features, weight, bias, actions, available_actions)[:2]
     return _ActionLogProbs.apply(features, weight, bias, actions, available_actions)
