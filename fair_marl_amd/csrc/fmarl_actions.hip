@@ -4,8 +4,8 @@
 // Rows that take no part (a negative action: padding; nothing available) give 0, 0 and no gradient.  The logits are formed again for the
 // gradient.  Two ways to do it:
 //   * few actions (five per agent: the env's own): one pass over x per direction, W in LDS, bound by HBM -- actions_few_kernel;
-//   * many (the joint actions of several agents): matrix products of 128 x 128 tiles on the matrix units whose epilogues hold the softmax's running
-//     maximum and sums per tile (forwards) or write dz for a piece of the actions at a time (backwards) -- actions_gemm_kernel.
+//   * many (the joint actions of several agents): matrix products on the matrix units whose epilogues hold the softmax's running maximum and
+//     sums (forwards) or write dz for a piece of the actions at a time (backwards) -- actions_wide_kernel, and actions_gemm_kernel for float32.
 #include "fmarl_policy_dev.h"
 
 namespace fmarl {
@@ -238,10 +238,10 @@ __global__ __launch_bounds__(256) void actions_sums_kernel(const float *partial,
 }
 
 // ---- many actions -----------------------------------------------------------------------------------------------------------
-// dst (rows_pad, cols_pad) <- src (rows, cols; row stride), zeros around; or its transpose (cols_pad, rows_pad), with `lse` without the rows that take no
+// dst (rows_pad, cols_pad) <- src (rows, cols; row stride), zeros around, and trans <- its transpose where wanted; with `lse` without the rows that take no
 // part (what they hold, NaN too, does not reach dW).  64 x 64 tiles.
-template <typename T, bool TRANS>
-__global__ __launch_bounds__(256) void actions_pack_kernel(const T *src, int64_t stride, int64_t rows, int cols, T *dst, int64_t rows_pad, int cols_pad, const float *lse) {
+template <typename T>
+__global__ __launch_bounds__(256) void actions_pack_kernel(const T *src, int64_t stride, int64_t rows, int cols, T *dst, T *trans, int64_t rows_pad, int cols_pad, const float *lse) {
     __shared__ T tile[64][66];
     const int64_t r0 = (int64_t)blockIdx.x * 64;
     const int c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
@@ -249,14 +249,14 @@ __global__ __launch_bounds__(256) void actions_pack_kernel(const T *src, int64_t
     for (int i = 0; i < 16; ++i) {
         const int64_t r = r0 + ty + 4 * i;
         T v = r < rows && c0 + tx < cols ? src[r * stride + c0 + tx] : (T)0.f;
-        if (TRANS && lse && r < rows && lse[r] == __builtin_inff()) v = (T)0.f;
-        if (TRANS) tile[ty + 4 * i][tx] = v;
-        else dst[r * cols_pad + c0 + tx] = v;
+        if (lse && r < rows && lse[r] == __builtin_inff()) v = (T)0.f;
+        dst[r * cols_pad + c0 + tx] = v;
+        if (trans) tile[ty + 4 * i][tx] = v;
     }
-    if (TRANS) {
+    if (trans) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) dst[(int64_t)(c0 + ty + 4 * i) * rows_pad + r0 + tx] = tile[tx][ty + 4 * i];
+        for (int i = 0; i < 16; ++i) trans[(int64_t)(c0 + ty + 4 * i) * rows_pad + r0 + tx] = tile[tx][ty + 4 * i];
     }
 }
 
@@ -273,18 +273,9 @@ struct Gemm {
     float *za;                     // kStats: the taken action's logit, by row of the chunk
     char *dz, *dzt; int64_t ldz, ldzt;      // kDlogits: dz (rows, ldz) and its transpose
     float *db; int64_t ldb_part;   // kDlogits: (tiles of 64 rows, ldb_part) sums over the rows
-    const float *dz_scale;         // kDlogits: NULL or the power of two that dz is stored times
 };
 
 template <typename T> struct Frag;
-template <> struct Frag<__bf16> {
-    typedef bf16x8 type;
-    static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-};
-template <> struct Frag<_Float16> {
-    typedef f16x8 type;
-    static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-};
 template <> struct Frag<float> {   // four steps of four: the order of the contraction is free as long as both sides share it
     typedef f32x4 type;
     static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) {
@@ -368,7 +359,6 @@ __global__ __launch_bounds__(256) void actions_gemm_kernel(Gemm q) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) { const int v = vbase + 16 * i + r; bias[i][r] = a.bias && v < a.V ? a.bias[v] : 0.f; }
     if (EPI == kDlogits) __syncthreads();   // the operands' LDS is dead from here on
-    const float scale = EPI == kDlogits && q.dz_scale ? *q.dz_scale : 1.f;
     float dbs[4][4] = {};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -419,7 +409,7 @@ __global__ __launch_bounds__(256) void actions_gemm_kernel(Gemm q) {
                     d[r] = dlogit(acc[i][j][r], vbase + 16 * i + r == act, in, lse, ent, dl, de);
                     dbs[i][r] += d[r];
                 }
-                store4<T>(zrow + 16 * i, d * scale, 4, true);   // rounded to the operands' type: what the two products below read
+                store4<T>(zrow + 16 * i, d, 4, true);
             }
         }
     }
@@ -452,29 +442,279 @@ __global__ __launch_bounds__(256) void actions_gemm_kernel(Gemm q) {
     }
 }
 
-// the row's result from its slots of 64 actions
-__global__ __launch_bounds__(256) void actions_join_kernel(Actions a, const float *stats, int64_t stride, int slots, const float *za, int64_t row0, int64_t count) {
-    const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (m >= count) return;
+// ---- many actions, half precision -------------------------------------------------------------------------------------------
+// Tiles of 256 x 256 by eight waves of 128 x 64 (a wave's fragments are then read 0.75 times as fast as LDS can give them while its matrix instructions run), steps of
+// 64 along the contraction.  A step's operands go from memory straight to LDS (16 bytes a lane, 64 lanes side by side), the next step's -- of the next tile, too -- while
+// this one is multiplied.  The LDS image is linear -- the hardware writes lane after lane -- so its 16-byte pieces are permuted by the addresses that the lanes load
+// from, such that what a fragment read touches spreads over the banks.
+//   an operand whose contraction is contiguous: 256 rows of 128 bytes, piece p of row r in place p ^ (r & 7), a fragment is one 16-byte read;
+//   an operand whose rows are the contraction (T): 64 rows of 512 bytes, piece p of row r in place p ^ f(r), f(r) = 2 ((r & 3) + 4 ((r >> 3) & 3)); a fragment is two
+//   transposing reads (ds_read_b64_tr_b16: 16 lanes point at four rows of 16 and get a column each).  So dz, x and W serve both of their products as they lie.
+// Logits are formed in base 2: v_exp_f32 is a power of two, and z log2(e) - max one multiply-add.
+struct Wide {
+    const char *A, *B; int64_t lda, ldb;     // elements; whole tiles can be read
+    int ta, tb, steps, splits;               // tiles of A and of B, steps of the contraction; kStore: parts of the contraction, else parts of the outer tile's run
+    float *out; int64_t ldo, split_out;      // kStore: out[split][row of B][row of A]
+    Actions act; int64_t row0; int v0;       // kStats, kDlogits: A = W (actions from v0 on), B = x (rows from row0 on)
+    const float *bias2;                      // bias log2(e) of the padded actions, -inf beyond the last one
+    float *stats; int64_t stat_stride;       // kStats: (2 splits, 3, stat_stride)
+    float *za;                               // kStats: the taken action's logit in base 2, by row of the chunk
+    char *dz; int64_t ldz;                   // kDlogits: (rows, ldz)
+    float *db; int64_t ldb_part;             // kDlogits: (tiles of 64 rows, ldb_part) sums over the rows
+    const float *dz_scale;                   // kDlogits: NULL or the power of two that dz is stored times
+};
+
+template <typename T> struct Half;
+template <> struct Half<__bf16> {
+    typedef bf16x8 frag;
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Half<_Float16> {
+    typedef f16x8 frag;
+    static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kWideOperand = 32768, kWideLds = 4 * kWideOperand;   // bytes of an operand's step; two operands, two steps
+
+template <typename T, int EPI, bool TA, bool TB>
+__global__ __launch_bounds__(512) void actions_wide_kernel(Wide q) {
+    extern __shared__ __align__(128) char lds[];
+    typedef typename Half<T>::frag F;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4, g4 = g * 4;
+    // workgroups go round the eight XCDs in turn: each XCD takes a run of neighbouring work, whose operands its L2 then holds
+    const int n = gridDim.x, per = n / 8, extra = n % 8, xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
+    const int id = xcd * per + min(xcd, extra) + nth;
+    // kStore: one tile and a part of the contraction.  kStats: one tile of rows (B) and a run of the actions' tiles (A); kDlogits: one tile of actions and a run of the
+    // rows' tiles -- what is summed over the run stays in registers.
+    int ia, ib, split, first = 0, tiles = 1, s0 = 0, s1 = q.steps;
+    if (EPI == kStore) {
+        ia = id % q.ta; ib = id / q.ta % q.tb; split = id / (q.ta * q.tb);
+        s0 = (int)((int64_t)q.steps * split / q.splits); s1 = (int)((int64_t)q.steps * (split + 1) / q.splits);
+    } else if (EPI == kStats) {
+        ib = id % q.tb; split = id / q.tb;
+        first = ia = (int)((int64_t)q.ta * split / q.splits); tiles = (int)((int64_t)q.ta * (split + 1) / q.splits) - first;
+    } else {
+        ia = id % q.ta; split = id / q.ta;
+        first = ib = (int)((int64_t)q.tb * split / q.splits); tiles = (int)((int64_t)q.tb * (split + 1) / q.splits) - first;
+    }
+    const int steps = s1 - s0, total = steps * tiles;
+    // this lane's addresses of a step: four pieces of each operand per wave
+    int64_t fa[4], fb[4];   // bytes from the tile's start
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int rn = (wave * 4 + i) * 8 + (lane >> 3), pn = (lane & 7) ^ (lane >> 3);                      // contiguous contraction: row and piece
+        const int rt = (wave * 4 + i) * 2 + (lane >> 5), pt = (lane & 31) ^ (2 * ((rt & 3) + 4 * ((rt >> 3) & 3)));   // T
+        fa[i] = TA ? (int64_t)rt * q.lda * 2 + pt * 16 : (int64_t)rn * q.lda * 2 + pn * 16;
+        fb[i] = TB ? (int64_t)rt * q.ldb * 2 + pt * 16 : (int64_t)rn * q.ldb * 2 + pn * 16;
+    }
+    const int64_t step_a = TA ? 64 * q.lda * 2 : 128, step_b = TB ? 64 * q.ldb * 2 : 128, tile_a = TA ? 512 : 256 * q.lda * 2, tile_b = TB ? 512 : 256 * q.ldb * 2;
+    auto load = [&](int k) {   // step k of the run
+        const int tile = k / steps, s = s0 + k - tile * steps, buf = (k & 1) * 2 * kWideOperand;
+        const char *pa = q.A + (EPI == kStats ? ia + tile : ia) * tile_a + s * step_a, *pb = q.B + (EPI == kDlogits ? ib + tile : ib) * tile_b + s * step_b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(pa + fa[i]),
+                                             (__attribute__((address_space(3))) void *)(lds + buf + (wave * 4 + i) * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(pb + fb[i]),
+                                             (__attribute__((address_space(3))) void *)(lds + buf + kWideOperand + (wave * 4 + i) * 1024), 16, 0, 0);
+        }
+    };
+    const int ra = (wave & 1) * 128, rb = (wave >> 1) * 64;
+    auto fragment = [&](const char *at, bool t, int row, int kk) -> F {   // rows (T: columns) row .. row + 15, contraction 32 kk .. 32 kk + 31
+        if (!t) return *(const F *)(at + (row + c) * 128 + (((kk * 4 + g) ^ (c & 7)) * 16));
+        const int f = 2 * ((c >> 2) + 4 * g);
+        const char *p = at + (kk * 32 + 8 * g + (c >> 2)) * 512 + ((((row >> 3) ^ f) | ((c >> 1) & 1)) * 16) + (c & 1) * 8;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + 4 * 512));
+        return __builtin_bit_cast(F, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    const Actions &a = q.act;
+    // kStats: this lane's running maximum and sums of its four rows
+    float top[4], sum[4], tsum[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { top[j] = -__builtin_inff(); sum[j] = tsum[j] = 0.f; }
+    const float scale = EPI == kDlogits && q.dz_scale ? *q.dz_scale : 1.f;
+    f32x4 acc[8][4];
+    if (total > 0) load(0);
+    int k = 0;
+    for (int tile = 0; tile < tiles; ++tile) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < steps; ++s, ++k) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's share of the step is in LDS
+            __syncthreads();                                   // everybody's is, and nobody reads the other buffer any more
+            if (k + 1 < total) load(k + 1);
+            const char *la = lds + (k & 1) * 2 * kWideOperand, *lb = la + kWideOperand;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                F fb_[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) fb_[j] = fragment(lb, TB, rb + 16 * j, kk);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const F fa_ = fragment(la, TA, ra + 16 * i, kk);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = Half<T>::mma(fa_, fb_[j], acc[i][j]);
+                }
+            }
+        }
+        if (EPI == kStore) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float *o = q.out + split * q.split_out + ((int64_t)ib * 256 + rb + 16 * j + c) * q.ldo + (int64_t)ia * 256 + ra + g4;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) *(f32x4 *)(o + 16 * i) = acc[i][j];
+            }
+            continue;
+        }
+        const int va = (EPI == kStats ? ia + tile : ia) * 256 + ra + g4;   // this lane's actions of the chunk: va + 16 i + r
+        const int64_t m0 = (int64_t)(EPI == kDlogits ? ib + tile : ib) * 256 + rb + c;   // its rows of the chunk: m0 + 16 j
+        // z log2(e) + bias, -inf beyond the last action and where not available
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const f32x4 bv = *(const f32x4 *)(q.bias2 + q.v0 + va + 16 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = acc[i][j][r] * kLog2e + bv[r];
+                if (a.avail) {
+                    const uint32_t ok = available4(a, q.row0 + m0 + 16 * j, q.v0 + va + 16 * i);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] = (ok >> r) & 1 ? acc[i][j][r] : -__builtin_inff();
+                }
+            }
+        }
+        if (EPI == kStats) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t row = q.row0 + m0 + 16 * j;
+                const int want = row < a.rows ? action_of(a, row) - va : -1;   // the taken action among this lane's: want = 16 i + r
+                float most = top[j];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    most = fmaxf(fmaxf(most, fmaxf(acc[i][j][0], acc[i][j][1])), fmaxf(acc[i][j][2], acc[i][j][3]));
+                    if ((unsigned)(want - 16 * i) < 4u) {
+                        const int r = want - 16 * i;
+                        q.za[m0 + 16 * j] = r == 0 ? acc[i][j][0] : r == 1 ? acc[i][j][1] : r == 2 ? acc[i][j][2] : acc[i][j][3];
+                    }
+                }
+                const float ref = most == -__builtin_inff() ? 0.f : most;   // nothing yet: no infinity minus infinity
+                const float old = top[j] == -__builtin_inff() ? 0.f : exp2_fast(top[j] - ref);
+                float s = sum[j] * old, t = old == 0.f ? 0.f : old * (tsum[j] + (top[j] - ref) * sum[j]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float d = acc[i][j][r] - ref, e = exp2_fast(d);
+                        s += e;
+                        t += fmaxf(d, -1e4f) * e;   // (-inf times 0)
+                    }
+                top[j] = most; sum[j] = s; tsum[j] = t;
+            }
+        } else {
+            float lse2[4], A[4], B[4], dl[4];
+            int want[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t row = q.row0 + m0 + 16 * j;
+                lse2[j] = 3e38f; A[j] = B[j] = dl[j] = 0.f; want[j] = -1;
+                if (row < a.rows && a.lse[row] != __builtin_inff()) {
+                    // dz = p (de (-log p - H) - dl) + dl [v = a], times the power of two
+                    const float de = a.dent ? a.dent[row] * scale : 0.f;
+                    dl[j] = a.dlogp ? a.dlogp[row] * scale : 0.f;
+                    lse2[j] = a.lse[row] * kLog2e; A[j] = de * -0.693147181f; B[j] = -(dl[j] + de * a.ent[row]);
+                    if (lse2[j] != lse2[j]) B[j] = lse2[j];   // a row whose logits hold a NaN: its gradient is NaN
+                    want[j] = action_of(a, row) - q.v0 - va;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                f32x4 total4 = {0.f, 0.f, 0.f, 0.f};   // over this wave's 64 rows, unrounded
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f32x4 d;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float x = fmaxf(acc[i][j][r] - lse2[j], -1e4f);   // log2 p; -1e4: p is 0, and what it is multiplied with is finite
+                        d[r] = exp2_fast(x) * (x * A[j] + B[j]);
+                    }
+                    if ((unsigned)(want[j] - 16 * i) < 4u) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) d[r] += want[j] - 16 * i == r && acc[i][j][r] != -__builtin_inff() ? dl[j] : 0.f;
+                    }
+                    total4 += d;
+                    store4<T>((T *)q.dz + (m0 + 16 * j) * q.ldz + va + 16 * i, d, 4, true);   // rounded to the operands' type: what the two products read
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    total4[r] += row_turn<0x128>(total4[r]); total4[r] += row_turn<0x124>(total4[r]);
+                    total4[r] += row_turn<0x122>(total4[r]); total4[r] += row_turn<0x121>(total4[r]);
+                }
+                if (c == 0) *(f32x4 *)(q.db + (int64_t)((ib + tile) * 4 + (wave >> 1)) * q.ldb_part + va + 16 * i) = total4 * (1.f / scale);
+            }
+        }
+    }
+    if (EPI == kStats) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            // the four lanes of a row, then one slot per wave
+            float m = fmaxf(top[j], __shfl_xor(top[j], 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float ref = m == -__builtin_inff() ? 0.f : m, f = top[j] == -__builtin_inff() ? (sum[j] == 0.f ? 0.f : 1.f) : exp2_fast(top[j] - ref);
+            float s = sum[j] * f, t = f == 0.f ? 0.f : f * (tsum[j] + (top[j] == -__builtin_inff() ? 0.f : top[j] - ref) * sum[j]);
+            s += __shfl_xor(s, 16); s += __shfl_xor(s, 32);
+            t += __shfl_xor(t, 16); t += __shfl_xor(t, 32);
+            if (g == 0) {
+                float *o = q.stats + (int64_t)(split * 2 + (wave & 1)) * 3 * q.stat_stride + (int64_t)ib * 256 + rb + 16 * j + c;
+                o[0] = m; o[q.stat_stride] = s; o[2 * q.stat_stride] = t;
+            }
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void actions_bias2_kernel(const float *bias, int V, float *out, int n) {
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v < n) out[v] = v < V ? (bias ? bias[v] * kLog2e : 0.f) : -__builtin_inff();
+}
+
+// the row's result from its slots' maxima and sums: 16 rows a workgroup, 16 threads a row.  `two`: maxima, sums and the taken logit are in base 2
+__global__ __launch_bounds__(256) void actions_join_kernel(Actions a, const float *stats, int64_t stride, int slots, const float *za, int64_t row0, int64_t count, int two) {
+    __shared__ float red[3][16][17];
+    const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
+    const int64_t m = (int64_t)blockIdx.x * 16 + c;
     float top = -__builtin_inff(), s = 0.f, t = 0.f;
-    bool some = false;
-    for (int i = 0; i < slots; ++i) {
-        const float *p = stats + (int64_t)i * 3 * stride + m;
-        const float t1 = p[0], s1 = p[stride], d1 = p[2 * stride];
-        if (t1 == -__builtin_inff()) continue;
-        some = true;
-        if (t1 > top) {
-            const float f = top == -__builtin_inff() ? 0.f : exp_of(top - t1);
-            t = f == 0.f ? 0.f : f * (t + (top - t1) * s);
+    auto power = [&](float x) { return two ? exp2_fast(x) : exp_of(x); };
+    auto add = [&](float t1, float s1, float d1) {
+        if (s1 == 0.f) return;              // nothing there (a NaN is not 0)
+        if (!(t1 <= top)) {
+            const float f = top == -__builtin_inff() ? (s == 0.f ? 0.f : 1.f) : power(top - t1);
+            t = f == 0.f ? 0.f : f * (t + (top == -__builtin_inff() ? 0.f : top - t1) * s);
             s *= f; top = t1;
             s += s1; t += d1;
         } else {
-            const float f = exp_of(t1 - top);
-            s += f * s1; t += f == 0.f ? 0.f : f * (d1 + (t1 - top) * s1);
+            const float f = t1 == -__builtin_inff() ? 1.f : power(t1 - top);
+            s += f * s1; t += f == 0.f ? 0.f : f * (d1 + (t1 == -__builtin_inff() ? 0.f : t1 - top) * s1);
         }
+    };
+    if (m < count)
+        for (int i = k; i < slots; i += 16) {
+            const float *p = stats + (int64_t)i * 3 * stride + m;
+            add(p[0], p[stride], p[2 * stride]);
+        }
+    red[0][k][c] = top; red[1][k][c] = s; red[2][k][c] = t;
+    __syncthreads();
+    if (k == 0 && m < count) {
+        for (int i = 1; i < 16; ++i) add(red[0][i][c], red[1][i][c], red[2][i][c]);
+        const int act = action_of(a, row0 + m);
+        const float ln2 = 0.693147181f, z = act >= 0 && act < a.V ? za[m] : 0.f;
+        if (two) row_result(a, row0 + m, act, top == -__builtin_inff() ? 0.f : top * ln2, s, t * ln2, s != 0.f, z * ln2);
+        else row_result(a, row0 + m, act, top, s, t, s != 0.f, z);
     }
-    const int act = action_of(a, row0 + m);
-    row_result(a, row0 + m, act, top, s, t, some, act >= 0 && act < a.V ? za[m] : 0.f);
 }
 
 // out[row][col] = scale * sum of the parts (+ what `sum` holds); `sum` takes it while more is to come
@@ -585,40 +825,52 @@ int launch_few_t(int dtype, const Actions &s, int blocks, hipStream_t st) {
 
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
-// The sizes of the way for many actions.  Rows go in chunks and (backwards) actions in pieces, so that what is kept of a chunk -- three floats per row and 64 actions,
-// or dz and its transpose -- stays within 256 MB, the size of the last-level cache.
+// The sizes of the way for many actions.  Rows go in chunks and (backwards) actions in pieces, so that what is kept of a chunk -- dz (float32: and its transpose),
+// three floats per row and 64 actions -- stays within 256 MB, the size of the last-level cache.
 struct Plan {
+    int tile;                     // rows and columns of a tile: 128 (float32), 256
     int64_t Kp, Vp, Mc, P;        // padded features and actions, rows of a chunk, actions of a piece
     int split_x, split_w;         // parts of the contraction of dx and dW
-    size_t xp, wp, stats, za, xt, wt, dz, dzt, out, sumx, sumw, db, scale, total;
+    int split_z;                  // half precision: parts of a run of tiles (kStats: of the actions, kDlogits: of the rows)
+    size_t xp, wp, bias2, stats, za, xt, wt, dz, dzt, out, sumx, sumw, db, scale, total;
 };
+
+// parts of a contraction of `steps` for `tiles` tiles: enough that the chip is full (`fill` workgroups), none with fewer than four steps
+int parts_of(int64_t tiles, int64_t steps, int fill, int most) {
+    int64_t n = fill / tiles;
+    if (n > steps / 4) n = steps / 4;
+    return (int)(n < 1 ? 1 : n > most ? most : n);
+}
 
 Plan actions_plan(const FmarlActions *a, bool backward) {
     Plan p = {};
-    const int64_t e = elem_bytes(a->dtype), M = up(a->rows, 128), budget = 256ll << 20;
-    p.Kp = up(a->features, 128); p.Vp = up(a->actions, 128);
-    const int64_t keep = backward ? 2 * e * 128 : 12 * (p.Vp / 64);   // bytes per row that a chunk cannot do without
-    int64_t mc = budget / keep / 128 * 128;
+    const bool half = a->dtype != FMARL_T_F32;
+    const int64_t e = elem_bytes(a->dtype), budget = 256ll << 20;
+    p.tile = half ? 256 : 128;
+    const int64_t M = up(a->rows, p.tile), tile = p.tile, per = 128 / e;
+    p.Kp = up(a->features, tile); p.Vp = up(a->actions, tile);
+    int64_t keep = half ? 2 * p.Kp : backward ? 2 * e * 128 : 12 * (p.Vp / 64);   // bytes per row that a chunk cannot do without
+    int64_t mc = budget / keep / tile * tile;
     if (mc > 65536) mc = 65536;
     if (mc < 1024) mc = 1024;
     p.Mc = M < mc ? M : mc;
-    p.P = budget / (2 * e * p.Mc) / 128 * 128;
-    if (p.P < 128) p.P = 128;
+    p.P = budget / ((half ? 1 : 2) * e * p.Mc) / tile * tile;
+    if (p.P < tile) p.P = tile;
     if (p.P > p.Vp) p.P = p.Vp;
-    const int64_t tx = (p.Mc / 128) * (p.Kp / 128), tw = (p.P / 128) * (p.Kp / 128), per = 128 / e;
-    auto parts = [&](int64_t tiles, int64_t steps) {   // two workgroups per CU, none with fewer than eight steps
-        int64_t n = (512 + tiles - 1) / tiles;
-        if (n > steps / 8) n = steps / 8;
-        return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
-    };
-    p.split_x = parts(tx, p.P / per); p.split_w = parts(tw, p.Mc / per);
+    const int64_t tm = p.Mc / tile, tk = p.Kp / tile, tv = p.P / tile;
+    // half precision: one workgroup per CU (its LDS is 128 KB); float32: two
+    p.split_x = parts_of(tm * tk, p.P / per, half ? 256 : 512, half ? 16 : 64);
+    p.split_w = parts_of(tv * tk, p.Mc / per, half ? 256 : 512, half ? 16 : 64);
+    const int64_t run = backward ? tm : p.Vp / tile, rest = backward ? tv : tm;
+    p.split_z = (int)(256 / rest < 1 ? 1 : 256 / rest > run ? run : 256 / rest);
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += up256(bytes); return at; };
     p.xp = take(e * p.Mc * p.Kp); p.wp = take(e * p.Vp * p.Kp);
-    if (!backward) { p.stats = take(12 * (p.Vp / 64) * p.Mc); p.za = take(4 * p.Mc); }
+    if (half) p.bias2 = take(4 * p.Vp);
+    if (!backward) { p.stats = take(12 * (half ? 2 * p.split_z : p.Vp / 64) * p.Mc); p.za = take(4 * p.Mc); }
     else {
-        p.xt = take(e * p.Mc * p.Kp); p.wt = take(e * p.Vp * p.Kp);
-        p.dz = take(e * p.Mc * p.P); p.dzt = take(e * p.Mc * p.P);
+        if (!half) { p.xt = take(e * p.Mc * p.Kp); p.wt = take(e * p.Vp * p.Kp); p.dzt = take(e * p.Mc * p.P); }
+        p.dz = take(e * p.Mc * p.P);
         const int64_t ox = p.split_x * p.Mc * p.Kp, ow = p.split_w * p.P * p.Kp;
         p.out = take(4 * (ox > ow ? ox : ow));
         p.sumx = take(p.P < p.Vp ? 4 * p.Mc * p.Kp : 0);
@@ -630,30 +882,36 @@ Plan actions_plan(const FmarlActions *a, bool backward) {
     return p;
 }
 
-template <typename T, bool TRANS>
-void pack(const T *src, int64_t stride, int64_t rows, int cols, T *dst, int64_t rows_pad, int64_t cols_pad, const float *lse, hipStream_t st) {
-    hipLaunchKernelGGL((actions_pack_kernel<T, TRANS>), dim3((unsigned)(rows_pad / 64), (unsigned)(cols_pad / 64)), dim3(256), 0, st, src, stride, rows, cols, dst,
+// dst and (float32, backwards) its transpose
+template <typename T>
+void pack(const T *src, int64_t stride, int64_t rows, int cols, T *dst, T *trans, int64_t rows_pad, int64_t cols_pad, const float *lse, hipStream_t st) {
+    hipLaunchKernelGGL((actions_pack_kernel<T>), dim3((unsigned)(rows_pad / 64), (unsigned)(cols_pad / 64)), dim3(256), 0, st, src, stride, rows, cols, dst, trans,
                        rows_pad, (int)cols_pad, lse);
 }
 
-template <typename T, int EPI>
+template <int EPI>
 void gemm(const Gemm &q, hipStream_t st) {
-    hipLaunchKernelGGL((actions_gemm_kernel<T, EPI>), dim3((unsigned)(q.ta * q.tb * q.splits)), dim3(256), 0, st, q);
+    hipLaunchKernelGGL((actions_gemm_kernel<float, EPI>), dim3((unsigned)(q.ta * q.tb * q.splits)), dim3(256), 0, st, q);
 }
 
-template <typename T>
-int many_forward(const Actions &s, const Plan &p, char *base, hipStream_t st) {
-    const int64_t per = 128 / (int64_t)sizeof(T);
-    T *xp = (T *)(base + p.xp), *wp = (T *)(base + p.wp);
-    pack<T, false>((const T *)s.w, s.ws, s.V, s.K, wp, p.Vp, p.Kp, nullptr, st);
+template <typename T, int EPI, bool TA, bool TB>
+int wide(const Wide &q, int64_t blocks, hipStream_t st) {
+    HIP_OK(hipFuncSetAttribute((const void *)actions_wide_kernel<T, EPI, TA, TB>, hipFuncAttributeMaxDynamicSharedMemorySize, kWideLds));
+    hipLaunchKernelGGL((actions_wide_kernel<T, EPI, TA, TB>), dim3((unsigned)blocks), dim3(512), kWideLds, st, q);
+    return FMARL_OK;
+}
+
+int many_forward_f32(const Actions &s, const Plan &p, char *base, hipStream_t st) {
+    float *xp = (float *)(base + p.xp), *wp = (float *)(base + p.wp);
+    pack<float>((const float *)s.w, s.ws, s.V, s.K, wp, nullptr, p.Vp, p.Kp, nullptr, st);
     for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
         const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 128);
-        pack<T, false>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xp, mp, p.Kp, nullptr, st);
+        pack<float>((const float *)s.x + r0 * s.xs, s.xs, m, s.K, xp, nullptr, mp, p.Kp, nullptr, st);
         Gemm q = {};
-        q.A = (const char *)wp; q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(p.Vp / 128); q.tb = (int)(mp / 128); q.splits = 1; q.steps = (int)(p.Kp / per);
+        q.A = (const char *)wp; q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(p.Vp / 128); q.tb = (int)(mp / 128); q.splits = 1; q.steps = (int)(up(s.K, 32) / 32);
         q.act = s; q.row0 = r0; q.stats = (float *)(base + p.stats); q.stat_stride = p.Mc; q.za = (float *)(base + p.za);
-        gemm<T, kStats>(q, st);
-        hipLaunchKernelGGL(actions_join_kernel, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, st, s, (const float *)q.stats, p.Mc, (int)(p.Vp / 64), (const float *)q.za, r0, m);
+        gemm<kStats>(q, st);
+        hipLaunchKernelGGL(actions_join_kernel, dim3((unsigned)((m + 15) / 16)), dim3(256), 0, st, s, (const float *)q.stats, p.Mc, (int)(p.Vp / 64), (const float *)q.za, r0, m, 0);
         HIP_OK(hipGetLastError());
     }
     return FMARL_OK;
@@ -665,37 +923,84 @@ void reduce(const float *part, int64_t split_stride, int splits, int64_t ld, flo
                        cols, scale);
 }
 
-template <typename T>
-int many_backward(const Actions &s, const Plan &p, T *dx, T *dw, float *db, char *base, hipStream_t st) {
-    const int64_t per = 128 / (int64_t)sizeof(T);
-    T *xp = (T *)(base + p.xp), *wp = (T *)(base + p.wp), *xt = (T *)(base + p.xt), *wt = (T *)(base + p.wt), *dz = (T *)(base + p.dz), *dzt = (T *)(base + p.dzt);
+int many_backward_f32(const Actions &s, const Plan &p, float *dx, float *dw, float *db, char *base, hipStream_t st) {
+    float *xp = (float *)(base + p.xp), *wp = (float *)(base + p.wp), *xt = (float *)(base + p.xt), *wt = (float *)(base + p.wt), *dz = (float *)(base + p.dz), *dzt = (float *)(base + p.dzt);
     float *out = (float *)(base + p.out), *sumx = (float *)(base + p.sumx), *sumw = (float *)(base + p.sumw), *dbp = (float *)(base + p.db);
-    const float *scale = nullptr;
-    if (sizeof(T) == 2 && (float)(T)1e-30f == 0.f) {   // float16
-        scale = (const float *)(base + p.scale);
-        hipLaunchKernelGGL(actions_scale_kernel, dim3(1), dim3(1024), 0, st, s, (float *)(base + p.scale));
-    }
-    pack<T, false>((const T *)s.w, s.ws, s.V, s.K, wp, p.Vp, p.Kp, nullptr, st);
-    pack<T, true>((const T *)s.w, s.ws, s.V, s.K, wt, p.Vp, p.Kp, nullptr, st);
+    pack<float>((const float *)s.w, s.ws, s.V, s.K, wp, wt, p.Vp, p.Kp, nullptr, st);
     for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
         const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 128);
-        pack<T, false>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xp, mp, p.Kp, nullptr, st);
-        pack<T, true>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xt, mp, p.Kp, s.lse + r0, st);
+        pack<float>((const float *)s.x + r0 * s.xs, s.xs, m, s.K, xp, xt, mp, p.Kp, s.lse + r0, st);
         for (int64_t v0 = 0; v0 < p.Vp; v0 += p.P) {
             const int64_t n = p.Vp - v0 < p.P ? p.Vp - v0 : p.P, nv = s.V - v0 < n ? s.V - v0 : n;   // of this piece: padded and real actions
             Gemm q = {};
-            q.A = (const char *)(wp + v0 * p.Kp); q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(n / 128); q.tb = (int)(mp / 128); q.splits = 1; q.steps = (int)(p.Kp / per);
-            q.act = s; q.row0 = r0; q.v0 = (int)v0; q.dz = (char *)dz; q.dzt = (char *)dzt; q.ldz = p.P; q.ldzt = p.Mc; q.db = dbp; q.ldb_part = p.P; q.dz_scale = scale;
-            gemm<T, kDlogits>(q, st);
+            q.A = (const char *)(wp + v0 * p.Kp); q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(n / 128); q.tb = (int)(mp / 128); q.splits = 1; q.steps = (int)(up(s.K, 32) / 32);
+            q.act = s; q.row0 = r0; q.v0 = (int)v0; q.dz = (char *)dz; q.dzt = (char *)dzt; q.ldz = p.P; q.ldzt = p.Mc; q.db = dbp; q.ldb_part = p.P;
+            gemm<kDlogits>(q, st);
             if (db) hipLaunchKernelGGL(actions_bias_kernel, dim3((unsigned)((nv + 15) / 16)), dim3(256), 0, st, (const float *)dbp, p.P, (int)(mp / 64), db + v0, (int)nv, (int)(r0 > 0));
             q = Gemm{};   // dx += dz W: rows of W^T (features) against rows of dz
-            q.A = (const char *)(wt + v0); q.lda = p.Vp; q.B = (const char *)dz; q.ldb = p.P; q.ta = (int)(p.Kp / 128); q.tb = (int)(mp / 128); q.steps = (int)(n / per);
+            q.A = (const char *)(wt + v0); q.lda = p.Vp; q.B = (const char *)dz; q.ldb = p.P; q.ta = (int)(p.Kp / 128); q.tb = (int)(mp / 128); q.steps = (int)(n / 32);
             q.splits = p.split_x < q.steps ? p.split_x : q.steps; q.out = out; q.ldo = p.Kp; q.split_out = p.Mc * p.Kp;
-            gemm<T, kStore>(q, st);
-            reduce<T>(out, q.split_out, q.splits, p.Kp, sumx, v0 == 0, v0 + n >= p.Vp, dx + r0 * s.K, m, s.K, scale, st);
-            q.A = (const char *)xt; q.lda = mp; q.B = (const char *)dzt; q.ldb = p.Mc; q.tb = (int)(n / 128); q.steps = (int)(mp / per);   // dW: rows of x^T against rows of dz^T
+            gemm<kStore>(q, st);
+            reduce<float>(out, q.split_out, q.splits, p.Kp, sumx, v0 == 0, v0 + n >= p.Vp, dx + r0 * s.K, m, s.K, nullptr, st);
+            q.A = (const char *)xt; q.lda = mp; q.B = (const char *)dzt; q.ldb = p.Mc; q.tb = (int)(n / 128); q.steps = (int)(mp / 32);   // dW: rows of x^T against rows of dz^T
             q.splits = p.split_w < q.steps ? p.split_w : q.steps; q.split_out = p.P * p.Kp;
-            gemm<T, kStore>(q, st);
+            gemm<kStore>(q, st);
+            reduce<float>(out, q.split_out, q.splits, p.Kp, sumw + v0 * p.Kp, r0 == 0, r0 + m >= s.rows, dw + v0 * s.K, nv, s.K, nullptr, st);
+            HIP_OK(hipGetLastError());
+        }
+    }
+    return FMARL_OK;
+}
+
+template <typename T>
+int many_forward(const Actions &s, const Plan &p, char *base, hipStream_t st) {
+    T *xp = (T *)(base + p.xp), *wp = (T *)(base + p.wp);
+    float *bias2 = (float *)(base + p.bias2);
+    pack<T>((const T *)s.w, s.ws, s.V, s.K, wp, nullptr, p.Vp, p.Kp, nullptr, st);
+    hipLaunchKernelGGL(actions_bias2_kernel, dim3((unsigned)(p.Vp / 256)), dim3(256), 0, st, s.bias, s.V, bias2, (int)p.Vp);
+    for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
+        const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 256);
+        pack<T>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xp, nullptr, mp, p.Kp, nullptr, st);
+        Wide q = {};
+        q.A = (const char *)wp; q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(p.Vp / 256); q.tb = (int)(mp / 256); q.steps = (int)(up(s.K, 64) / 64); q.splits = p.split_z;
+        q.act = s; q.row0 = r0; q.bias2 = bias2; q.stats = (float *)(base + p.stats); q.stat_stride = p.Mc; q.za = (float *)(base + p.za);
+        if (int rc = wide<T, kStats, false, false>(q, (int64_t)q.tb * q.splits, st)) return rc;
+        hipLaunchKernelGGL(actions_join_kernel, dim3((unsigned)((m + 15) / 16)), dim3(256), 0, st, s, (const float *)q.stats, p.Mc, 2 * q.splits, (const float *)q.za, r0, m, 1);
+        HIP_OK(hipGetLastError());
+    }
+    return FMARL_OK;
+}
+
+template <typename T>
+int many_backward(const Actions &s, const Plan &p, T *dx, T *dw, float *db, char *base, hipStream_t st) {
+    T *xp = (T *)(base + p.xp), *wp = (T *)(base + p.wp), *dz = (T *)(base + p.dz);
+    float *bias2 = (float *)(base + p.bias2), *out = (float *)(base + p.out), *sumx = (float *)(base + p.sumx), *sumw = (float *)(base + p.sumw), *dbp = (float *)(base + p.db);
+    const float *scale = nullptr;
+    if ((float)(T)1e-30f == 0.f) {   // float16
+        scale = (const float *)(base + p.scale);
+        hipLaunchKernelGGL(actions_scale_kernel, dim3(1), dim3(1024), 0, st, s, (float *)(base + p.scale));
+    }
+    pack<T>((const T *)s.w, s.ws, s.V, s.K, wp, nullptr, p.Vp, p.Kp, nullptr, st);
+    hipLaunchKernelGGL(actions_bias2_kernel, dim3((unsigned)(p.Vp / 256)), dim3(256), 0, st, s.bias, s.V, bias2, (int)p.Vp);
+    for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
+        const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 256);
+        pack<T>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xp, nullptr, mp, p.Kp, s.lse + r0, st);
+        for (int64_t v0 = 0; v0 < p.Vp; v0 += p.P) {
+            const int64_t n = p.Vp - v0 < p.P ? p.Vp - v0 : p.P, nv = s.V - v0 < n ? s.V - v0 : n;   // of this piece: padded and real actions
+            Wide q = {};
+            q.A = (const char *)(wp + v0 * p.Kp); q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(n / 256); q.tb = (int)(mp / 256); q.steps = (int)(up(s.K, 64) / 64);
+            q.splits = p.split_z < q.tb ? p.split_z : q.tb;
+            q.act = s; q.row0 = r0; q.v0 = (int)v0; q.bias2 = bias2; q.dz = (char *)dz; q.ldz = p.P; q.db = dbp; q.ldb_part = p.P; q.dz_scale = scale;
+            if (int rc = wide<T, kDlogits, false, false>(q, (int64_t)q.ta * q.splits, st)) return rc;
+            if (db) hipLaunchKernelGGL(actions_bias_kernel, dim3((unsigned)((nv + 15) / 16)), dim3(256), 0, st, (const float *)dbp, p.P, (int)(mp / 64), db + v0, (int)nv, (int)(r0 > 0));
+            q = Wide{};   // dx += dz W: columns of W (features) against rows of dz
+            q.A = (const char *)(wp + v0 * p.Kp); q.lda = p.Kp; q.B = (const char *)dz; q.ldb = p.P; q.ta = (int)(p.Kp / 256); q.tb = (int)(mp / 256); q.steps = (int)(n / 64);
+            q.splits = p.split_x < q.steps ? p.split_x : q.steps; q.out = out; q.ldo = p.Kp; q.split_out = p.Mc * p.Kp;
+            if (int rc = wide<T, kStore, true, false>(q, (int64_t)q.ta * q.tb * q.splits, st)) return rc;
+            reduce<T>(out, q.split_out, q.splits, p.Kp, sumx, v0 == 0, v0 + n >= p.Vp, dx + r0 * s.K, m, s.K, scale, st);
+            q.A = (const char *)xp; q.B = (const char *)dz; q.tb = (int)(n / 256); q.steps = (int)(mp / 64);   // dW: columns of x against columns of dz
+            q.splits = p.split_w < q.steps ? p.split_w : q.steps; q.split_out = p.P * p.Kp;
+            if (int rc = wide<T, kStore, true, true>(q, (int64_t)q.ta * q.tb * q.splits, st)) return rc;
             reduce<T>(out, q.split_out, q.splits, p.Kp, sumw + v0 * p.Kp, r0 == 0, r0 + m >= s.rows, dw + v0 * s.K, nv, s.K, scale, st);
             HIP_OK(hipGetLastError());
         }
@@ -725,7 +1030,7 @@ int fmarl_action_log_probs(const FmarlActions *a, float *log_probs, float *entro
         return launch_few_t<false>(a->dtype, s, (int)(n < 2048 ? n : 2048), st);
     }
     const Plan p = actions_plan(a, false);
-    return a->dtype == FMARL_T_F32 ? many_forward<float>(s, p, (char *)workspace, st)
+    return a->dtype == FMARL_T_F32 ? many_forward_f32(s, p, (char *)workspace, st)
          : a->dtype == FMARL_T_BF16 ? many_forward<__bf16>(s, p, (char *)workspace, st) : many_forward<_Float16>(s, p, (char *)workspace, st);
 }
 
@@ -751,7 +1056,7 @@ int fmarl_action_log_probs_backward(const FmarlActions *a, const float *entropy,
     }
     const Plan p = actions_plan(a, true);
     char *ws = (char *)workspace;
-    return a->dtype == FMARL_T_F32 ? many_backward<float>(s, p, (float *)d_x, (float *)d_weight, d_bias, ws, st)
+    return a->dtype == FMARL_T_F32 ? many_backward_f32(s, p, (float *)d_x, (float *)d_weight, d_bias, ws, st)
          : a->dtype == FMARL_T_BF16 ? many_backward<__bf16>(s, p, (__bf16 *)d_x, (__bf16 *)d_weight, d_bias, ws, st)
                                     : many_backward<_Float16>(s, p, (_Float16 *)d_x, (_Float16 *)d_weight, d_bias, ws, st);
 }

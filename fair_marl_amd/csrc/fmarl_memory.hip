@@ -435,10 +435,6 @@ template <int M, int N, typename F> __device__ __forceinline__ void unroll(F f) 
     if constexpr (M < N) { f(std::integral_constant<int, M>()); unroll<M + 1, N>(f); }
 }
 
-template <int CTRL> __device__ __forceinline__ float row_turn(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
-}
-
 __device__ __forceinline__ float row_sum(float v) {   // over the 16 lanes of a row, in every lane: rotations by 8, 4, 2, 1
     v += row_turn<0x128>(v); v += row_turn<0x124>(v); v += row_turn<0x122>(v); v += row_turn<0x121>(v);
     return v;

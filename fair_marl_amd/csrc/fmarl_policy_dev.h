@@ -56,6 +56,11 @@ __device__ __forceinline__ void wave_sync() {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32: 1 ulp, 0 below 2^-126
 
+// v of another lane of the row of 16: a DPP control (0x120 + n: the row turned by n)
+template <int CTRL> __device__ __forceinline__ float row_turn(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
 }  // namespace policy
 
 int policy_fail(int code, const char *fmt, const char *a = "");   // libfmarl.hip: the text of fmarl_last_error()
