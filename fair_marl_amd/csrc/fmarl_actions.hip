@@ -444,19 +444,25 @@ __global__ __launch_bounds__(256) void actions_gemm_kernel(Gemm q) {
 
 // ---- many actions, half precision -------------------------------------------------------------------------------------------
 // Tiles of 256 x 256 by eight waves of 128 x 64 (a wave's fragments are then read 0.75 times as fast as LDS can give them while its matrix instructions run), steps of
-// 64 along the contraction.  A step's operands go from memory straight to LDS (16 bytes a lane, 64 lanes side by side), the next step's -- of the next tile, too -- while
-// this one is multiplied.  The LDS image is linear -- the hardware writes lane after lane -- so its 16-byte pieces are permuted by the addresses that the lanes load
-// from, such that what a fragment read touches spreads over the banks.
-//   an operand whose contraction is contiguous: 256 rows of 128 bytes, piece p of row r in place p ^ (r & 7), a fragment is one 16-byte read;
-//   an operand whose rows are the contraction (T): 64 rows of 512 bytes, piece p of row r in place p ^ f(r), f(r) = 2 ((r & 3) + 4 ((r >> 3) & 3)); a fragment is two
+// 32 along the contraction, 32 KB each; four of them have room in LDS, so three are on their way -- over the end of a tile into the next one's -- while one is multiplied.
+// They go from memory straight to LDS (16 bytes a lane, 64 lanes side by side).  The compiler waits for every such load before the next LDS read of any kind (it
+// took the loads of the next step for possible writers of this step's: 107 us for dx at 8 192 x 256 x 15 625 with two steps of 64), so they are issued in
+// assembly -- they have no result registers -- and waited for by count before the barrier: loads come back in order, and of those behind a step's at most eight are open.
+// The LDS image is linear -- the hardware writes lane after lane -- so its 16-byte pieces are permuted by the addresses that the lanes load from, such that what a
+// fragment read touches spreads over the banks.
+//   an operand whose contraction is contiguous: 256 rows of 64 bytes, piece p of row r in place p ^ ((r >> 2) & 3), a fragment is one 16-byte read;
+//   an operand whose rows are the contraction (T): 32 rows of 512 bytes, piece p of row r in place p ^ f(r), f(r) = 2 ((r & 3) + 4 (r >> 3)); a fragment is two
 //   transposing reads (ds_read_b64_tr_b16: 16 lanes point at four rows of 16 and get a column each).  So dz, x and W serve both of their products as they lie.
-// Logits are formed in base 2: v_exp_f32 is a power of two, and z log2(e) - max one multiply-add.
+// What an epilogue needs per action and per row comes the same way, with the first step of its tile: a load of its own would be waited for behind all steps on
+// their way.  Logits are formed in base 2: v_exp_f32 is a power of two, and z log2(e) - max one multiply-add.
 struct Wide {
     const char *A, *B; int64_t lda, ldb;     // elements; whole tiles can be read
     int ta, tb, steps, splits;               // tiles of A and of B, steps of the contraction; kStore: parts of the contraction, else parts of the outer tile's run
     float *out; int64_t ldo, split_out;      // kStore: out[split][row of B][row of A]
     Actions act; int64_t row0; int v0;       // kStats, kDlogits: A = W (actions from v0 on), B = x (rows from row0 on)
-    const float *bias2;                      // bias log2(e) of the padded actions, -inf beyond the last one
+    const float *bias2;                      // bias log2(e) of the padded actions from v0 on, -inf beyond the last one
+    const int *taken;                        // the rows' actions of the chunk, -1: takes no part; padded to whole tiles
+    const f32x4 *rows;                       // kDlogits: what the rows' gradients are made of (actions_rows_kernel), padded to whole tiles
     float *stats; int64_t stat_stride;       // kStats: (2 splits, 3, stat_stride)
     float *za;                               // kStats: the taken action's logit in base 2, by row of the chunk
     char *dz; int64_t ldz;                   // kDlogits: (rows, ldz)
@@ -477,56 +483,94 @@ template <> struct Half<_Float16> {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kWideOperand = 32768, kWideLds = 4 * kWideOperand;   // bytes of an operand's step; two operands, two steps
+constexpr int kWideOperand = 16384, kWideStep = 2 * kWideOperand, kWideExtra = 6144;   // bytes of an operand's step, of a step, of what a tile's epilogue needs: bias 1 KB, actions 1 KB, rows 4 KB
+constexpr int kWideLds = 4 * (kWideStep + kWideExtra);                                  // 152 KB of the CU's 160
 
-template <typename T, int EPI, bool TA, bool TB>
+// 16 bytes a lane from memory to LDS, lane after lane from byte `at` on (the same in every lane)
+__device__ __forceinline__ void load_lds(const char *p, uint32_t at) {
+    uint32_t m0;   // put back as it was: the compiler does not expect it to change
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0" : "=&s"(m0) : "s"(at), "v"(p) : "memory");
+}
+
+// What a row's gradient is made of: (lse log2(e), A, B, dlog_prob), dz = p (log2(p) A + B) + dlog_prob [v = a], A = -de ln 2, B = -(dlog_prob + de H), times the power of
+// two of `scale`; and its action.  Rows that take no part: 3e38, 0, 0, 0 and -1.
+__global__ __launch_bounds__(256) void actions_rows_kernel(Actions a, int64_t row0, int64_t padded, f32x4 *rows, int *taken, const float *scale) {
+    const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x, row = row0 + m;
+    if (m >= padded) return;
+    f32x4 v = {3e38f, 0.f, 0.f, 0.f};
+    int act = -1;
+    if (row < a.rows) {
+        act = action_of(a, row);
+        if (rows) {
+            const float lse = a.lse[row], s = scale ? *scale : 1.f;
+            if (lse != __builtin_inff()) {
+                const float de = a.dent ? a.dent[row] * s : 0.f, dl = a.dlogp ? a.dlogp[row] * s : 0.f;
+                v = f32x4{lse * kLog2e, de * -0.693147181f, lse != lse ? lse : -(dl + de * a.ent[row]), dl};   // logits that hold a NaN: a gradient of NaN
+            } else act = -1;
+        }
+    }
+    taken[m] = act;
+    if (rows) rows[m] = v;
+}
+
+template <typename T, int EPI, bool TA, bool TB, bool AVAIL>
 __global__ __launch_bounds__(512) void actions_wide_kernel(Wide q) {
     extern __shared__ __align__(128) char lds[];
     typedef typename Half<T>::frag F;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4, g4 = g * 4;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uint64_t)(__attribute__((address_space(3))) char *)lds);
     // workgroups go round the eight XCDs in turn: each XCD takes a run of neighbouring work, whose operands its L2 then holds
     const int n = gridDim.x, per = n / 8, extra = n % 8, xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
     const int id = xcd * per + min(xcd, extra) + nth;
     // kStore: one tile and a part of the contraction.  kStats: one tile of rows (B) and a run of the actions' tiles (A); kDlogits: one tile of actions and a run of the
     // rows' tiles -- what is summed over the run stays in registers.
-    int ia, ib, split, first = 0, tiles = 1, s0 = 0, s1 = q.steps;
+    int ia, ib, split, tiles = 1, s0 = 0, s1 = q.steps;
     if (EPI == kStore) {
         ia = id % q.ta; ib = id / q.ta % q.tb; split = id / (q.ta * q.tb);
         s0 = (int)((int64_t)q.steps * split / q.splits); s1 = (int)((int64_t)q.steps * (split + 1) / q.splits);
     } else if (EPI == kStats) {
         ib = id % q.tb; split = id / q.tb;
-        first = ia = (int)((int64_t)q.ta * split / q.splits); tiles = (int)((int64_t)q.ta * (split + 1) / q.splits) - first;
+        ia = (int)((int64_t)q.ta * split / q.splits); tiles = (int)((int64_t)q.ta * (split + 1) / q.splits) - ia;
     } else {
         ia = id % q.ta; split = id / q.ta;
-        first = ib = (int)((int64_t)q.tb * split / q.splits); tiles = (int)((int64_t)q.tb * (split + 1) / q.splits) - first;
+        ib = (int)((int64_t)q.tb * split / q.splits); tiles = (int)((int64_t)q.tb * (split + 1) / q.splits) - ib;
     }
     const int steps = s1 - s0, total = steps * tiles;
-    // this lane's addresses of a step: four pieces of each operand per wave
-    int64_t fa[4], fb[4];   // bytes from the tile's start
+    // this lane's addresses of a step, from the tile's start: two pieces of each operand per wave
+    int64_t fa[2], fb[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int rn = (wave * 4 + i) * 8 + (lane >> 3), pn = (lane & 7) ^ (lane >> 3);                      // contiguous contraction: row and piece
-        const int rt = (wave * 4 + i) * 2 + (lane >> 5), pt = (lane & 31) ^ (2 * ((rt & 3) + 4 * ((rt >> 3) & 3)));   // T
+    for (int i = 0; i < 2; ++i) {
+        const int rn = (wave * 2 + i) * 16 + (lane >> 2), pn = (lane & 3) ^ ((lane >> 4) & 3);                          // contiguous contraction: row and piece
+        const int rt = (wave * 2 + i) * 2 + (lane >> 5), pt = (lane & 31) ^ (2 * ((rt & 3) + 4 * (rt >> 3)));            // T
         fa[i] = TA ? (int64_t)rt * q.lda * 2 + pt * 16 : (int64_t)rn * q.lda * 2 + pn * 16;
         fb[i] = TB ? (int64_t)rt * q.ldb * 2 + pt * 16 : (int64_t)rn * q.ldb * 2 + pn * 16;
     }
-    const int64_t step_a = TA ? 64 * q.lda * 2 : 128, step_b = TB ? 64 * q.ldb * 2 : 128, tile_a = TA ? 512 : 256 * q.lda * 2, tile_b = TB ? 512 : 256 * q.ldb * 2;
-    auto load = [&](int k) {   // step k of the run
-        const int tile = k / steps, s = s0 + k - tile * steps, buf = (k & 1) * 2 * kWideOperand;
-        const char *pa = q.A + (EPI == kStats ? ia + tile : ia) * tile_a + s * step_a, *pb = q.B + (EPI == kDlogits ? ib + tile : ib) * tile_b + s * step_b;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(pa + fa[i]),
-                                             (__attribute__((address_space(3))) void *)(lds + buf + (wave * 4 + i) * 1024), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(pb + fb[i]),
-                                             (__attribute__((address_space(3))) void *)(lds + buf + kWideOperand + (wave * 4 + i) * 1024), 16, 0, 0);
+    const int64_t step_a = TA ? 32 * q.lda * 2 : 64, step_b = TB ? 32 * q.ldb * 2 : 64, tile_a = TA ? 512 : 256 * q.lda * 2, tile_b = TB ? 512 : 256 * q.ldb * 2;
+    const char *pa0 = q.A + ia * tile_a + s0 * step_a, *pb0 = q.B + ib * tile_b + s0 * step_b;
+    int lk = 0, ls = 0, lt = 0;   // the next step to load: of the run, of its tile, its tile of the run
+    auto load = [&]() {
+        const char *pa = pa0 + (EPI == kStats ? lt * tile_a : 0) + ls * step_a, *pb = pb0 + (EPI == kDlogits ? lt * tile_b : 0) + ls * step_b;
+        const uint32_t at = lds0 + (lk & 3) * kWideStep + wave * 2048;
+        if (EPI != kStore && ls == 0) {   // what the tile's epilogue needs: 256 biases (wave 0), 256 actions (wave 1), 256 rows (waves 2 .. 5)
+            const uint32_t to = lds0 + 4 * kWideStep + (lt & 3) * kWideExtra;
+            const int64_t v = (int64_t)(EPI == kStats ? ia + lt : ia) * 256, m = (int64_t)(EPI == kDlogits ? ib + lt : ib) * 256;
+            if (wave == 0) load_lds((const char *)(q.bias2 + v) + lane * 16, to);
+            else if (wave == 1) load_lds((const char *)(q.taken + m) + lane * 16, to + 1024);
+            else if (EPI == kDlogits && wave < 6) load_lds((const char *)(q.rows + m) + (wave - 2) * 1024 + lane * 16, to + wave * 1024);
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            load_lds(pa + fa[i], at + i * 1024);
+            load_lds(pb + fb[i], at + kWideOperand + i * 1024);
+        }
+        ++lk;
+        if (++ls == steps) { ls = 0; ++lt; }
     };
     const int ra = (wave & 1) * 128, rb = (wave >> 1) * 64;
-    auto fragment = [&](const char *at, bool t, int row, int kk) -> F {   // rows (T: columns) row .. row + 15, contraction 32 kk .. 32 kk + 31
-        if (!t) return *(const F *)(at + (row + c) * 128 + (((kk * 4 + g) ^ (c & 7)) * 16));
+    auto fragment = [&](const char *at, bool t, int row) -> F {   // rows (T: columns) row .. row + 15 of a step
+        if (!t) return *(const F *)(at + (row + c) * 64 + ((g ^ ((c >> 2) & 3)) * 16));
         const int f = 2 * ((c >> 2) + 4 * g);
-        const char *p = at + (kk * 32 + 8 * g + (c >> 2)) * 512 + ((((row >> 3) ^ f) | ((c >> 1) & 1)) * 16) + (c & 1) * 8;
+        const char *p = at + (8 * g + (c >> 2)) * 512 + ((((row >> 3) ^ f) | ((c >> 1) & 1)) * 16) + (c & 1) * 8;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + 4 * 512));
         return __builtin_bit_cast(F, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -536,9 +580,9 @@ __global__ __launch_bounds__(512) void actions_wide_kernel(Wide q) {
     float top[4], sum[4], tsum[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) { top[j] = -__builtin_inff(); sum[j] = tsum[j] = 0.f; }
-    const float scale = EPI == kDlogits && q.dz_scale ? *q.dz_scale : 1.f;
+    const float inv_scale = EPI == kDlogits && q.dz_scale ? 1.f / *q.dz_scale : 1.f;
     f32x4 acc[8][4];
-    if (total > 0) load(0);
+    for (int i = 0; i < 3 && lk < total; ++i) load();
     int k = 0;
     for (int tile = 0; tile < tiles; ++tile) {
 #pragma unroll
@@ -546,21 +590,23 @@ __global__ __launch_bounds__(512) void actions_wide_kernel(Wide q) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < steps; ++s, ++k) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's share of the step is in LDS
-            __syncthreads();                                   // everybody's is, and nobody reads the other buffer any more
-            if (k + 1 < total) load(k + 1);
-            const char *la = lds + (k & 1) * 2 * kWideOperand, *lb = la + kWideOperand;
+            // this wave's share of step k is in LDS once at most the four loads of each step behind it are open; behind the barrier everybody's is, and nobody reads step
+            // k - 1 any more, whose place the next load takes
+            if (k + 2 < total) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+            else if (k + 1 < total) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (lk < total) load();
+            const char *la = lds + (k & 3) * kWideStep, *lb = la + kWideOperand;
+            F fb_[4];
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                F fb_[4];
+            for (int j = 0; j < 4; ++j) fb_[j] = fragment(lb, TB, rb + 16 * j);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) fb_[j] = fragment(lb, TB, rb + 16 * j, kk);
+            for (int i = 0; i < 8; ++i) {
+                const F fa_ = fragment(la, TA, ra + 16 * i);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const F fa_ = fragment(la, TA, ra + 16 * i, kk);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = Half<T>::mma(fa_, fb_[j], acc[i][j]);
-                }
+                for (int j = 0; j < 4; ++j) acc[i][j] = Half<T>::mma(fa_, fb_[j], acc[i][j]);
             }
         }
         if (EPI == kStore) {
@@ -572,37 +618,46 @@ __global__ __launch_bounds__(512) void actions_wide_kernel(Wide q) {
             }
             continue;
         }
+        const char *more = lds + 4 * kWideStep + (tile & 3) * kWideExtra;
         const int va = (EPI == kStats ? ia + tile : ia) * 256 + ra + g4;   // this lane's actions of the chunk: va + 16 i + r
         const int64_t m0 = (int64_t)(EPI == kDlogits ? ib + tile : ib) * 256 + rb + c;   // its rows of the chunk: m0 + 16 j
-        // z log2(e) + bias, -inf beyond the last action and where not available
+        int want[4];   // the taken action among this lane's: want = 16 i + r
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const f32x4 bv = *(const f32x4 *)(q.bias2 + q.v0 + va + 16 * i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[i][j][r] = acc[i][j][r] * kLog2e + bv[r];
-                if (a.avail) {
-                    const uint32_t ok = available4(a, q.row0 + m0 + 16 * j, q.v0 + va + 16 * i);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[i][j][r] = (ok >> r) & 1 ? acc[i][j][r] : -__builtin_inff();
-                }
-            }
+        for (int j = 0; j < 4; ++j) {
+            const int t = ((const int *)(more + 1024))[rb + 16 * j + c];
+            want[j] = t < 0 ? -1 : t - q.v0 - va;
         }
+        // z log2(e) + bias, -inf beyond the last action and where not available
+        auto logits = [&](int i, int j, f32x4 bv) {
+            f32x4 z;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[r] = __builtin_fmaf(acc[i][j][r], kLog2e, bv[r]);
+            if (AVAIL) {
+                const uint32_t ok = available4(a, q.row0 + m0 + 16 * j, q.v0 + va + 16 * i);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[r] = (ok >> r) & 1 ? z[r] : -__builtin_inff();
+            }
+            return z;
+        };
+        auto bias = [&](int i) { return *(const f32x4 *)(more + (ra + 16 * i + g4) * 4); };
         if (EPI == kStats) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t row = q.row0 + m0 + 16 * j;
-                const int want = row < a.rows ? action_of(a, row) - va : -1;   // the taken action among this lane's: want = 16 i + r
-                float most = top[j];
+            for (int i = 0; i < 8; ++i) {
+                const f32x4 bv = bias(i);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    most = fmaxf(fmaxf(most, fmaxf(acc[i][j][0], acc[i][j][1])), fmaxf(acc[i][j][2], acc[i][j][3]));
-                    if ((unsigned)(want - 16 * i) < 4u) {
-                        const int r = want - 16 * i;
+                for (int j = 0; j < 4; ++j) {
+                    acc[i][j] = logits(i, j, bv);
+                    if ((unsigned)(want[j] - 16 * i) < 4u) {
+                        const int r = want[j] - 16 * i;
                         q.za[m0 + 16 * j] = r == 0 ? acc[i][j][0] : r == 1 ? acc[i][j][1] : r == 2 ? acc[i][j][2] : acc[i][j][3];
                     }
                 }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float most = top[j];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) most = fmaxf(fmaxf(most, fmaxf(acc[i][j][0], acc[i][j][1])), fmaxf(acc[i][j][2], acc[i][j][3]));
                 const float ref = most == -__builtin_inff() ? 0.f : most;   // nothing yet: no infinity minus infinity
                 const float old = top[j] == -__builtin_inff() ? 0.f : exp2_fast(top[j] - ref);
                 float s = sum[j] * old, t = old == 0.f ? 0.f : old * (tsum[j] + (top[j] - ref) * sum[j]);
@@ -617,45 +672,36 @@ __global__ __launch_bounds__(512) void actions_wide_kernel(Wide q) {
                 top[j] = most; sum[j] = s; tsum[j] = t;
             }
         } else {
-            float lse2[4], A[4], B[4], dl[4];
-            int want[4];
+            f32x4 rc[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t row = q.row0 + m0 + 16 * j;
-                lse2[j] = 3e38f; A[j] = B[j] = dl[j] = 0.f; want[j] = -1;
-                if (row < a.rows && a.lse[row] != __builtin_inff()) {
-                    // dz = p (de (-log p - H) - dl) + dl [v = a], times the power of two
-                    const float de = a.dent ? a.dent[row] * scale : 0.f;
-                    dl[j] = a.dlogp ? a.dlogp[row] * scale : 0.f;
-                    lse2[j] = a.lse[row] * kLog2e; A[j] = de * -0.693147181f; B[j] = -(dl[j] + de * a.ent[row]);
-                    if (lse2[j] != lse2[j]) B[j] = lse2[j];   // a row whose logits hold a NaN: its gradient is NaN
-                    want[j] = action_of(a, row) - q.v0 - va;
-                }
-            }
+            for (int j = 0; j < 4; ++j) rc[j] = ((const f32x4 *)(more + 2048))[rb + 16 * j + c];
+            T *zrow = (T *)q.dz + m0 * q.ldz + va;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                f32x4 total4 = {0.f, 0.f, 0.f, 0.f};   // over this wave's 64 rows, unrounded
+                const f32x4 bv = bias(i);
+                f32x4 all = {0.f, 0.f, 0.f, 0.f};   // over this wave's 64 rows, unrounded
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
+                    const f32x4 z = logits(i, j, bv);
                     f32x4 d;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float x = fmaxf(acc[i][j][r] - lse2[j], -1e4f);   // log2 p; -1e4: p is 0, and what it is multiplied with is finite
-                        d[r] = exp2_fast(x) * (x * A[j] + B[j]);
+                        const float x = fmaxf(z[r] - rc[j][0], -1e4f);   // log2 p; -1e4: p is 0, and what it is multiplied with is finite
+                        d[r] = exp2_fast(x) * __builtin_fmaf(x, rc[j][1], rc[j][2]);
                     }
                     if ((unsigned)(want[j] - 16 * i) < 4u) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) d[r] += want[j] - 16 * i == r && acc[i][j][r] != -__builtin_inff() ? dl[j] : 0.f;
+                        for (int r = 0; r < 4; ++r) d[r] += want[j] - 16 * i == r && z[r] != -__builtin_inff() ? rc[j][3] : 0.f;
                     }
-                    total4 += d;
-                    store4<T>((T *)q.dz + (m0 + 16 * j) * q.ldz + va + 16 * i, d, 4, true);   // rounded to the operands' type: what the two products read
+                    all += d;
+                    store4<T>(zrow + 16 * j * q.ldz + 16 * i, d, 4, true);   // rounded to the operands' type: what the two products read
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    total4[r] += row_turn<0x128>(total4[r]); total4[r] += row_turn<0x124>(total4[r]);
-                    total4[r] += row_turn<0x122>(total4[r]); total4[r] += row_turn<0x121>(total4[r]);
+                    all[r] += row_turn<0x128>(all[r]); all[r] += row_turn<0x124>(all[r]);
+                    all[r] += row_turn<0x122>(all[r]); all[r] += row_turn<0x121>(all[r]);
                 }
-                if (c == 0) *(f32x4 *)(q.db + (int64_t)((ib + tile) * 4 + (wave >> 1)) * q.ldb_part + va + 16 * i) = total4 * (1.f / scale);
+                if (c == 0) *(f32x4 *)(q.db + (int64_t)((ib + tile) * 4 + (wave >> 1)) * q.ldb_part + va + 16 * i) = all * inv_scale;
             }
         }
     }
@@ -832,7 +878,7 @@ struct Plan {
     int64_t Kp, Vp, Mc, P;        // padded features and actions, rows of a chunk, actions of a piece
     int split_x, split_w;         // parts of the contraction of dx and dW
     int split_z;                  // half precision: parts of a run of tiles (kStats: of the actions, kDlogits: of the rows)
-    size_t xp, wp, bias2, stats, za, xt, wt, dz, dzt, out, sumx, sumw, db, scale, total;
+    size_t xp, wp, bias2, taken, rows, stats, za, xt, wt, dz, dzt, out, sumx, sumw, db, scale, total;
 };
 
 // parts of a contraction of `steps` for `tiles` tiles: enough that the chip is full (`fill` workgroups), none with fewer than four steps
@@ -866,7 +912,7 @@ Plan actions_plan(const FmarlActions *a, bool backward) {
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += up256(bytes); return at; };
     p.xp = take(e * p.Mc * p.Kp); p.wp = take(e * p.Vp * p.Kp);
-    if (half) p.bias2 = take(4 * p.Vp);
+    if (half) { p.bias2 = take(4 * p.Vp); p.taken = take(4 * p.Mc); p.rows = take(backward ? 16 * p.Mc : 0); }
     if (!backward) { p.stats = take(12 * (half ? 2 * p.split_z : p.Vp / 64) * p.Mc); p.za = take(4 * p.Mc); }
     else {
         if (!half) { p.xt = take(e * p.Mc * p.Kp); p.wt = take(e * p.Vp * p.Kp); p.dzt = take(e * p.Mc * p.P); }
@@ -894,11 +940,18 @@ void gemm(const Gemm &q, hipStream_t st) {
     hipLaunchKernelGGL((actions_gemm_kernel<float, EPI>), dim3((unsigned)(q.ta * q.tb * q.splits)), dim3(256), 0, st, q);
 }
 
+template <typename T, int EPI, bool TA, bool TB, bool AVAIL>
+int wide_as(const Wide &q, int64_t blocks, hipStream_t st) {
+    HIP_OK(hipFuncSetAttribute((const void *)actions_wide_kernel<T, EPI, TA, TB, AVAIL>, hipFuncAttributeMaxDynamicSharedMemorySize, kWideLds));
+    hipLaunchKernelGGL((actions_wide_kernel<T, EPI, TA, TB, AVAIL>), dim3((unsigned)blocks), dim3(512), kWideLds, st, q);
+    return FMARL_OK;
+}
+
 template <typename T, int EPI, bool TA, bool TB>
 int wide(const Wide &q, int64_t blocks, hipStream_t st) {
-    HIP_OK(hipFuncSetAttribute((const void *)actions_wide_kernel<T, EPI, TA, TB>, hipFuncAttributeMaxDynamicSharedMemorySize, kWideLds));
-    hipLaunchKernelGGL((actions_wide_kernel<T, EPI, TA, TB>), dim3((unsigned)blocks), dim3(512), kWideLds, st, q);
-    return FMARL_OK;
+    if constexpr (EPI != kStore)
+        if (q.act.avail) return wide_as<T, EPI, TA, TB, true>(q, blocks, st);
+    return wide_as<T, EPI, TA, TB, false>(q, blocks, st);
 }
 
 int many_forward_f32(const Actions &s, const Plan &p, char *base, hipStream_t st) {
@@ -962,8 +1015,9 @@ int many_forward(const Actions &s, const Plan &p, char *base, hipStream_t st) {
         const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 256);
         pack<T>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xp, nullptr, mp, p.Kp, nullptr, st);
         Wide q = {};
-        q.A = (const char *)wp; q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(p.Vp / 256); q.tb = (int)(mp / 256); q.steps = (int)(up(s.K, 64) / 64); q.splits = p.split_z;
-        q.act = s; q.row0 = r0; q.bias2 = bias2; q.stats = (float *)(base + p.stats); q.stat_stride = p.Mc; q.za = (float *)(base + p.za);
+        q.A = (const char *)wp; q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(p.Vp / 256); q.tb = (int)(mp / 256); q.steps = (int)(up(s.K, 32) / 32); q.splits = p.split_z;
+        q.act = s; q.row0 = r0; q.bias2 = bias2; q.taken = (const int *)(base + p.taken); q.stats = (float *)(base + p.stats); q.stat_stride = p.Mc; q.za = (float *)(base + p.za);
+        hipLaunchKernelGGL(actions_rows_kernel, dim3((unsigned)(mp / 256)), dim3(256), 0, st, s, r0, mp, (f32x4 *)nullptr, (int *)(base + p.taken), (const float *)nullptr);
         if (int rc = wide<T, kStats, false, false>(q, (int64_t)q.tb * q.splits, st)) return rc;
         hipLaunchKernelGGL(actions_join_kernel, dim3((unsigned)((m + 15) / 16)), dim3(256), 0, st, s, (const float *)q.stats, p.Mc, 2 * q.splits, (const float *)q.za, r0, m, 1);
         HIP_OK(hipGetLastError());
@@ -985,20 +1039,22 @@ int many_backward(const Actions &s, const Plan &p, T *dx, T *dw, float *db, char
     for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
         const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 256);
         pack<T>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xp, nullptr, mp, p.Kp, s.lse + r0, st);
+        hipLaunchKernelGGL(actions_rows_kernel, dim3((unsigned)(mp / 256)), dim3(256), 0, st, s, r0, mp, (f32x4 *)(base + p.rows), (int *)(base + p.taken), scale);
         for (int64_t v0 = 0; v0 < p.Vp; v0 += p.P) {
             const int64_t n = p.Vp - v0 < p.P ? p.Vp - v0 : p.P, nv = s.V - v0 < n ? s.V - v0 : n;   // of this piece: padded and real actions
             Wide q = {};
-            q.A = (const char *)(wp + v0 * p.Kp); q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(n / 256); q.tb = (int)(mp / 256); q.steps = (int)(up(s.K, 64) / 64);
+            q.A = (const char *)(wp + v0 * p.Kp); q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(n / 256); q.tb = (int)(mp / 256); q.steps = (int)(up(s.K, 32) / 32);
             q.splits = p.split_z < q.tb ? p.split_z : q.tb;
-            q.act = s; q.row0 = r0; q.v0 = (int)v0; q.bias2 = bias2; q.dz = (char *)dz; q.ldz = p.P; q.db = dbp; q.ldb_part = p.P; q.dz_scale = scale;
+            q.act = s; q.row0 = r0; q.v0 = (int)v0; q.bias2 = bias2 + v0; q.taken = (const int *)(base + p.taken); q.rows = (const f32x4 *)(base + p.rows);
+            q.dz = (char *)dz; q.ldz = p.P; q.db = dbp; q.ldb_part = p.P; q.dz_scale = scale;
             if (int rc = wide<T, kDlogits, false, false>(q, (int64_t)q.ta * q.splits, st)) return rc;
             if (db) hipLaunchKernelGGL(actions_bias_kernel, dim3((unsigned)((nv + 15) / 16)), dim3(256), 0, st, (const float *)dbp, p.P, (int)(mp / 64), db + v0, (int)nv, (int)(r0 > 0));
             q = Wide{};   // dx += dz W: columns of W (features) against rows of dz
-            q.A = (const char *)(wp + v0 * p.Kp); q.lda = p.Kp; q.B = (const char *)dz; q.ldb = p.P; q.ta = (int)(p.Kp / 256); q.tb = (int)(mp / 256); q.steps = (int)(n / 64);
+            q.A = (const char *)(wp + v0 * p.Kp); q.lda = p.Kp; q.B = (const char *)dz; q.ldb = p.P; q.ta = (int)(p.Kp / 256); q.tb = (int)(mp / 256); q.steps = (int)(n / 32);
             q.splits = p.split_x < q.steps ? p.split_x : q.steps; q.out = out; q.ldo = p.Kp; q.split_out = p.Mc * p.Kp;
             if (int rc = wide<T, kStore, true, false>(q, (int64_t)q.ta * q.tb * q.splits, st)) return rc;
             reduce<T>(out, q.split_out, q.splits, p.Kp, sumx, v0 == 0, v0 + n >= p.Vp, dx + r0 * s.K, m, s.K, scale, st);
-            q.A = (const char *)xp; q.B = (const char *)dz; q.tb = (int)(n / 256); q.steps = (int)(mp / 64);   // dW: columns of x against columns of dz
+            q.A = (const char *)xp; q.B = (const char *)dz; q.tb = (int)(n / 256); q.steps = (int)(mp / 32);   // dW: columns of x against columns of dz
             q.splits = p.split_w < q.steps ? p.split_w : q.steps; q.split_out = p.P * p.Kp;
             if (int rc = wide<T, kStore, true, true>(q, (int64_t)q.ta * q.tb * q.splits, st)) return rc;
             reduce<T>(out, q.split_out, q.splits, p.Kp, sumw + v0 * p.Kp, r0 == 0, r0 + m >= s.rows, dw + v0 * s.K, nv, s.K, scale, st);
