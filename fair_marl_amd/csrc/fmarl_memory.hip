@@ -422,10 +422,10 @@ __global__ __launch_bounds__(512) void memory_tiles_kernel(Walk arg) {
 }
 
 // ---- small heads ------------------------------------------------------------------------------------------------------------
-// dy <= 32: the recurrence itself, token by token, on the vector units.  16 lanes (a DPP row) hold one head: lane c column c of its slice of the state, 16 NY
-// values of y each; y and x are broadcast from the lane that holds them by the multiply's own operand (row_newbcast), so a token costs three
+// dy <= 32, or few tokens: the recurrence itself, token by token, on the vector units.  16 lanes (a DPP row) hold one head, or R rows its y in shares of 32: lane c column c of
+// its slice of the state, 16 NY values of y each; y and x are broadcast from the lane that holds them by the multiply's own operand (row_newbcast), so a token costs three
 // instructions per 64 state entries and no LDS.  Four neighbouring heads share a wave: 256 bytes of a token's row side by side.  Against a walk on the
-// matrix units, where half of every 16-token tile is above the diagonal and chunks of ten tokens waste the rest: 239 -> 156 us for 30 720 x 4 heads of ten
+// matrix units, where half of every 16-token tile is above the diagonal and chunks of ten tokens waste the rest: 239 -> 133 us for 30 720 x 4 heads of ten
 // tokens (float32, 566 MB: 111 us at the copy rate of 5.1 TB/s).
 template <int M> __device__ __forceinline__ float row_lane(float v) {   // lane M of each row of 16, in every lane of the row
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + M, 0xf, 0xf, true));
@@ -500,20 +500,34 @@ template <int N> __device__ __forceinline__ void row_state(float (&S)[N], const 
     }
 }
 
-template <typename T, int NY, bool DOT>
+// the sum over the R neighbouring rows of 16 lanes that share a head, in all of them
+template <int R> __device__ __forceinline__ float rows_sum(float v) {
+    if constexpr (R >= 2) {
+        const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+        v = __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
+    }
+    if constexpr (R == 4) {
+        const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+        v = __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
+    }
+    return v;
+}
+
+template <typename T, int NY, int R, bool DOT>
 __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
     constexpr int TB = NY == 1 ? 8 : NY == 2 ? 4 : 2;   // tokens whose rows are in flight while as many are computed
     const int lane = threadIdx.x & 63, c = lane & 15;
-    const int64_t heads = a.B * a.H, groups = (heads + 3) / 4;
+    const int64_t heads = a.B * a.H, groups = (heads + 4 / R - 1) / (4 / R);
     const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (unit >= groups * a.nseg * a.slices) return;
-    const int64_t mine = unit % groups * 4 + (lane >> 4), rest = unit / groups;
+    const int64_t mine = unit % groups * (4 / R) + (lane >> 4) / R, rest = unit / groups;
     const bool have = mine < heads;
     const int64_t bh = have ? mine : heads - 1;
     const int slice = (int)(rest % a.slices), seg = (int)(rest / a.slices);
     const int64_t b = bh / a.H;
     const int h = (int)(bh - b * a.H);
-    const int z = slice * 16 + c, dy = a.dy;
+    const int part = (lane >> 4) % R, y0 = 16 * NY * part, dy = a.dy - y0;   // this row's share of y (none left: dy <= 0)
+    const int z = slice * 16 + c;
     const bool zin = z < a.dz;
     const int64_t t_begin = (int64_t)seg * a.seg_len, t_end = min(a.L, t_begin + a.seg_len), count = t_end - t_begin;
     // every load is made, from a place inside the row where the lane's own lies beyond it (a conditional load would have to arrive before its value's conversion, one after
@@ -526,8 +540,8 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
 
     float S[16 * NY];
     if (a.state) {
-        const float *ps = a.state + seg * a.seg_state_in + bh * (int64_t)a.dy * a.dz + (int64_t)z * a.s_z;
-        row_state(S, ps, a.s_y, dy, zin, a.s_y == 1 && (dy & 3) == 0 && ((uintptr_t)a.state & 15) == 0);
+        const float *ps = a.state + seg * a.seg_state_in + bh * (int64_t)a.dy * a.dz + (int64_t)z * a.s_z + y0 * a.s_y;
+        row_state(S, ps, a.s_y, dy, zin, a.s_y == 1 && (a.dy & 3) == 0 && ((uintptr_t)a.state & 15) == 0);
     } else {
 #pragma unroll
         for (int m = 0; m < 16 * NY; ++m) S[m] = 0.f;
@@ -542,7 +556,7 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
             const int64_t t = t_begin + min(i0 + i, count - 1);
 #pragma unroll
             for (int n = 0; n < NY; ++n) {
-                const int at = min(16 * n + c, dy - 1);
+                const int at = min(y0 + 16 * n + c, a.dy - 1);
                 if (!a.state_only) nx[i][n] = px[t * a.x.sl + at];
                 ny[i][n] = py[t * a.y.sl + at];
             }
@@ -579,16 +593,16 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
                 if (a.state_only) whole *= fresh ? 0.f : d;
                 else {
                     float nd = row_dot<NY>(x[i], S);       // from the tokens before
-                    nd = fresh ? 0.f : nd * d;
+                    nd = fresh ? 0.f : rows_sum<R>(nd) * d;
                     float xy = 0.f;
 #pragma unroll
                     for (int n = 0; n < NY; ++n) xy += x[i][n] * y[i][n];
-                    xy = row_sum(xy);
+                    xy = rows_sum<R>(row_sum(xy));
                     const int64_t t = t_begin + i0 + i;
-                    if (have && zin) po[t * a.out.sl] = (T)((nd + xy * zz[i]) * a.out_scale);
+                    if (have && zin && part == 0) po[t * a.out.sl] = (T)((nd + xy * zz[i]) * a.out_scale);
                     if (DOT) {
-                        const float dot = row_sum(nd * a.out_scale * ww[i]);
-                        if (have && c == 0) a.dot[slice * a.dot_slice + t * a.dot_sl + bh * a.dot_sh] = dot;
+                        const float dot = row_sum(zin ? nd * a.out_scale * ww[i] : 0.f);
+                        if (have && c == 0 && part == 0) a.dot[slice * a.dot_slice + t * a.dot_sl + bh * a.dot_sh] = dot;
                     }
                 }
                 row_update<NY>(S, d, fresh, y[i], zz[i]);
@@ -604,11 +618,11 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
         whole *= fresh ? 0.f : d;
     }
     if (a.state_out && have && zin) {
-        float *ps = a.state_out + seg * a.seg_state_out + bh * (int64_t)a.dy * a.dz + (int64_t)z * a.o_z;
+        float *ps = a.state_out + seg * a.seg_state_out + bh * (int64_t)a.dy * a.dz + (int64_t)z * a.o_z + y0 * a.o_y;
 #pragma unroll
         for (int m = 0; m < 16 * NY; ++m) if (m < dy) ps[m * a.o_y] = S[m];
     }
-    if (a.seg_decay && slice == 0 && c == 0 && have) a.seg_decay[seg * heads + bh] = whole;
+    if (a.seg_decay && slice == 0 && part == 0 && c == 0 && have) a.seg_decay[seg * heads + bh] = whole;
 }
 
 // All gradients of up to 16 tokens of heads up to 16 x 16 in one pass (the update's chunks): q, k, v and dout stay in registers -- 16 lanes a head, as above --, the state is walked
@@ -954,16 +968,23 @@ int memory_check(const FmarlMemory *m, const char *who) {
     return FMARL_OK;
 }
 
-// The recurrence on the vector units for y up to 32 wide, the matrix units beyond: at 16 x 16 the former takes two thirds of the latter's time, at 64 x 64
-// its three instructions per 64 state entries and token would cost twice the matrix units' time
-bool small_heads(int dy) { return dy <= 32; }
+// The recurrence on the vector units for y up to 32 wide and for few tokens, the matrix units beyond.  At 16 x 16 the former takes two thirds of the latter's time.  Wider,
+// its three instructions per 64 state entries and token cost more than a chunk of 32 tokens on the matrix units from about ten tokens on, or 32 where z has one
+// tile only (4 096 heads forwards, us, vector | matrix units: 64 x 64 bfloat16 1 token 37 | 53, 10 tokens 54 | 51, 16 tokens 64 | 51; 128 x 128 float32 1 token 160 | 265, 10
+// tokens 217 | 262, 32 tokens 440 | 286; 128 x 16 bfloat16 16 tokens 38 | 88, 32 tokens 62 | 89, 64 tokens 112 | 120).
+bool small_heads(int dy, int dz, int64_t L) { return dy <= 32 || L <= (dz <= 16 ? 32 : 10); }
+
+// heads that share a wave of memory_rows_kernel
+int heads_of_wave(int dy) { return dy <= 32 ? 4 : dy <= 64 ? 2 : 1; }
 
 // A batch with few heads has its tokens cut into segments that are walked side by side: up to 2 048 waves of four small heads or 768 workgroups of a large one (what
 // is resident at a time: 8 waves, 3 workgroups per CU -- one more would be a second round), at least 64 tokens each (a segment costs a second
 // read of k and v and a state in the workspace, which shorter ones would not repay).
 struct Segments { int nseg, len; };
 Segments memory_segments(const FmarlMemory *m) {
-    const int64_t heads = m->B * m->H, units = small_heads(m->dk) ? (heads + 3) / 4 : heads, want = small_heads(m->dk) ? 2048 : 768;
+    const int64_t heads = m->B * m->H, per = heads_of_wave(m->dk);
+    const bool small = small_heads(m->dk, m->dv, m->L);
+    const int64_t units = small ? (heads + per - 1) / per : heads, want = small ? 2048 : 768;
     int64_t n = want / units, most = m->L / 64;
     if (n > most) n = most;
     if (n < 2) return {1, (int)(m->L > 0x40000000 ? 0x40000000 : m->L)};
@@ -972,7 +993,7 @@ Segments memory_segments(const FmarlMemory *m) {
 }
 
 // columns of z that a wave of the small heads' kernel takes: 16; the large heads' workgroup takes them all
-int slices_of(int dy, int dz) { return small_heads(dy) ? (dz + 15) / 16 : 1; }
+int slices_of(int dy, int dz, int64_t L) { return small_heads(dy, dz, L) ? (dz + 15) / 16 : 1; }
 
 // up to 16 tokens of heads up to 16 x 16: every gradient in one kernel, whose registers hold all of it
 bool short_backward(const FmarlMemory *m) { return m->L <= 16 && m->dk <= 16 && m->dv <= 16; }
@@ -993,8 +1014,8 @@ Workspace memory_layout(const FmarlMemory *m, int backward) {
     }
     if (backward && short_backward(m)) w.partial = take(8 * heads);
     else if (backward) {
-        w.dot_q = take(4 * (size_t)slices_of(m->dv, m->dk) * m->L * heads);
-        w.dot_k = take(4 * (size_t)slices_of(m->dv, m->dk) * m->L * heads);
+        w.dot_q = take(4 * (size_t)slices_of(m->dv, m->dk, m->L) * m->L * heads);
+        w.dot_k = take(4 * (size_t)slices_of(m->dv, m->dk, m->L) * m->L * heads);
         w.partial = take(8 * heads);
         w.d_state = take(4 * heads * elems);
     }
@@ -1021,14 +1042,18 @@ int launch_tiles_as(const Walk &w, int64_t blocks, hipStream_t st) {
 template <typename T>
 int launch_walk_t(const Walk &w, hipStream_t st) {
     const int64_t heads = w.B * w.H;
-    if (small_heads(w.dy)) {
-        const int64_t blocks = ((heads + 3) / 4 * w.nseg * w.slices + 3) / 4;
+    if (small_heads(w.dy, w.dz, w.L)) {
+        const int per = heads_of_wave(w.dy);
+        const int64_t blocks = ((heads + per - 1) / per * w.nseg * w.slices + 3) / 4;
         if (blocks > 0xffffff) return policy_fail(FMARL_EINVAL, "memory: too many sequences");
         const dim3 grid((unsigned)blocks);
-        if (w.dy <= 16 && w.w.p) hipLaunchKernelGGL((memory_rows_kernel<T, 1, true>), grid, dim3(256), 0, st, w);
-        else if (w.dy <= 16) hipLaunchKernelGGL((memory_rows_kernel<T, 1, false>), grid, dim3(256), 0, st, w);
-        else if (w.w.p) hipLaunchKernelGGL((memory_rows_kernel<T, 2, true>), grid, dim3(256), 0, st, w);
-        else hipLaunchKernelGGL((memory_rows_kernel<T, 2, false>), grid, dim3(256), 0, st, w);
+#define FMARL_ROWS(NY, R) do { if (w.w.p) hipLaunchKernelGGL((memory_rows_kernel<T, NY, R, true>), grid, dim3(256), 0, st, w); \
+                               else hipLaunchKernelGGL((memory_rows_kernel<T, NY, R, false>), grid, dim3(256), 0, st, w); } while (0)
+        if (w.dy <= 16) FMARL_ROWS(1, 1);
+        else if (w.dy <= 32) FMARL_ROWS(2, 1);
+        else if (w.dy <= 64) FMARL_ROWS(2, 2);
+        else FMARL_ROWS(2, 4);
+#undef FMARL_ROWS
         return FMARL_OK;
     }
     const int64_t blocks = heads * w.nseg;
@@ -1037,7 +1062,7 @@ int launch_walk_t(const Walk &w, hipStream_t st) {
 }
 
 int launch_walk(Walk w, int dtype, hipStream_t st) {
-    w.slices = slices_of(w.dy, w.dz);
+    w.slices = slices_of(w.dy, w.dz, w.L);
     const int rc = dtype == FMARL_T_F32 ? launch_walk_t<float>(w, st) : dtype == FMARL_T_BF16 ? launch_walk_t<__bf16>(w, st) : launch_walk_t<_Float16>(w, st);
     if (rc) return rc;
     HIP_OK(hipGetLastError());
@@ -1211,7 +1236,7 @@ int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, co
         g.dot_q = (const float *)(base + ws.dot_q); g.dot_k = (const float *)(base + ws.dot_k);
         g.state = m->state; g.d_state = ds0; g.g = w0.g; g.gl = w0.gl; g.gb = w0.gb; g.gh = w0.gh; g.masks = w0.masks; g.ml = w0.ml; g.mb = w0.mb;
         g.dg = shared ? nullptr : d_log_decay; g.partial = shared ? (double *)(base + ws.partial) : nullptr;
-        g.L = m->L; g.B = m->B; g.H = m->H; g.elems = elems; g.slices = slices_of(m->dv, m->dk);
+        g.L = m->L; g.B = m->B; g.H = m->H; g.elems = elems; g.slices = slices_of(m->dv, m->dk, m->L);
         g.dot_sl = w0.dot_sl; g.dot_sh = w0.dot_sh;
         g.vec = (elems & 3) == 0 && (((uintptr_t)g.state | (uintptr_t)g.d_state) & 15) == 0;
         for (g.team = 1; g.state && g.team < 64 && g.team * 16 < elems;) g.team *= 2;   // 16 entries a lane at least
