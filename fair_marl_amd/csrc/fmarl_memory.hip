@@ -518,7 +518,7 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
     constexpr int TB = NY == 1 ? 8 : NY == 2 ? 4 : 2;   // tokens whose rows are in flight while as many are computed
     const int lane = threadIdx.x & 63, c = lane & 15;
     const int64_t heads = a.B * a.H, groups = (heads + 4 / R - 1) / (4 / R);
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // (the same in the wave: what follows from it is scalar)
     if (unit >= groups * a.nseg * a.slices) return;
     const int64_t mine = unit % groups * (4 / R) + (lane >> 4) / R, rest = unit / groups;
     const bool have = mine < heads;
@@ -735,10 +735,20 @@ __global__ __launch_bounds__(256) void memory_join_kernel(float *seg_states, con
     if (i >= total) return;
     const int64_t bh = i / elems;
     float S = init ? init[i] : 0.f;
-    for (int seg = 0; seg < nseg; ++seg) {
-        const float d = seg_decay[seg * heads + bh], u = seg_states[seg * total + i];
-        seg_states[seg * total + i] = S;
-        S = (d == 0.f ? 0.f : d * S) + u;
+    for (int seg0 = 0; seg0 < nseg; seg0 += 8) {   // eight loads in flight
+        float d[8], u[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int seg = min(seg0 + k, nseg - 1);
+            d[k] = seg_decay[seg * heads + bh];
+            u[k] = seg_states[seg * total + i];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (seg0 + k < nseg) {
+                seg_states[(seg0 + k) * total + i] = S;
+                S = (d[k] == 0.f ? 0.f : d[k] * S) + u[k];
+            }
     }
     if (last) last[i] = S;
 }
@@ -978,14 +988,14 @@ bool small_heads(int dy, int dz, int64_t L) { return dy <= 32 || L <= (dz <= 16 
 int heads_of_wave(int dy) { return dy <= 32 ? 4 : dy <= 64 ? 2 : 1; }
 
 // A batch with few heads has its tokens cut into segments that are walked side by side: up to 2 048 waves of four small heads or 768 workgroups of a large one (what
-// is resident at a time: 8 waves, 3 workgroups per CU -- one more would be a second round), at least 64 tokens each (a segment costs a second
-// read of k and v and a state in the workspace, which shorter ones would not repay).
+// is resident at a time: 8 waves, 3 workgroups per CU -- one more would be a second round), at least 32 or 64 tokens each (a segment costs a second
+// read of k and v and a state in the workspace, which shorter ones would not repay; 24 small heads of 16 x 16 and 500 tokens: 71 us with 64, 50 with 32).
 struct Segments { int nseg, len; };
 Segments memory_segments(const FmarlMemory *m) {
     const int64_t heads = m->B * m->H, per = heads_of_wave(m->dk);
     const bool small = small_heads(m->dk, m->dv, m->L);
     const int64_t units = small ? (heads + per - 1) / per : heads, want = small ? 2048 : 768;
-    int64_t n = want / units, most = m->L / 64;
+    int64_t n = want / units, most = m->L / (small ? 32 : 64);
     if (n > most) n = most;
     if (n < 2) return {1, (int)(m->L > 0x40000000 ? 0x40000000 : m->L)};
     const int64_t len = ((m->L + n - 1) / n + 31) / 32 * 32;
