@@ -112,7 +112,7 @@ template <typename T, bool DOT> __host__ __device__ constexpr int tiles_lds(int 
 enum { kOut = 0, kOutDot = 1, kState = 2 };   // what a walk leaves: out; out and its dots with w; the state alone
 
 template <typename T, int NK, int MODE, bool VEC>
-__global__ __launch_bounds__(512) void memory_tiles_kernel(Walk arg) {
+__global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory_tiles_kernel(Walk arg) {
     constexpr bool DOT = MODE == kOutDot, OUT = MODE != kState;
     typedef Pieces<T, DOT> PC;
     constexpr int NP = PC::in, PP = PC::p, XS = 32 * NK + 8;
@@ -755,7 +755,7 @@ __global__ __launch_bounds__(256) void memory_join_kernel(float *seg_states, con
 
 // dg_1 = <S_0, dS_0>, dg_{t+1} = dg_t - (q_t . dq_t - k_t . dk_t), 0 where an episode starts: the gradient of the log decays from the sums that the dq and
 // dk walks left, each without the token's own term (which is in both and cancels).  float64: the running difference outlives many tokens.
-// One workgroup of `blockDim` threads per (batch, head); every thread takes a run of tokens, the runs are joined by a scan.
+// One workgroup per (batch, head); every thread takes four tokens at a time, what they add is joined by a scan (64 heads of 4 096 tokens: 19 us).
 // Up to 64 tokens (decay_grad_short_kernel): `team` lanes per pair share its <S_0, dS_0>, one of them walks the tokens, eight of them loaded at a time.  (A
 // wave of 64 pairs after another: 1 650 us for 192 heads of 91 x 82.)
 struct DecayGrad {
@@ -769,13 +769,6 @@ struct DecayGrad {
     int64_t L, B;
     int H, elems, slices, team, vec;   // vec: both states on 16 bytes, elems a multiple of four
 };
-
-__device__ __forceinline__ double decay_step(const DecayGrad &a, int64_t t, int64_t bh) {
-    const int64_t n = a.L * a.B * a.H, i = t * a.dot_sl + bh * a.dot_sh;
-    double d = 0.0;
-    for (int s = 0; s < a.slices; ++s) d += (double)a.dot_q[s * n + i] - (double)a.dot_k[s * n + i];
-    return d;
-}
 
 __device__ __forceinline__ bool decay_fresh(const DecayGrad &a, int64_t t, int64_t b, int h) {
     return (a.masks && a.masks[t * a.ml + b * a.mb] == 0.f) || a.g[t * a.gl + b * a.gb + h * a.gh] == -__builtin_inff();
@@ -827,41 +820,65 @@ __global__ __launch_bounds__(256) void decay_grad_short_kernel(DecayGrad a) {
 }
 
 __global__ __launch_bounds__(1024) void decay_grad_long_kernel(DecayGrad a) {
-    __shared__ double part[1024], sums[16];
-    __shared__ int cut[1024];
-    const int64_t bh = blockIdx.x, heads = a.B * a.H, b = bh / a.H;
-    const int h = (int)(bh - b * a.H), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ double sums[16];
+    __shared__ int cuts[16];
+    const int64_t bh = blockIdx.x, heads = a.B * a.H, b = bh / a.H, n = a.L * heads;
+    const int h = (int)(bh - b * a.H), tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
     double first = 0.0;
     if (a.state)
-        for (int e = tid; e < a.elems; e += 1024) first += (double)a.state[bh * a.elems + e] * (double)a.d_state[bh * a.elems + e];
+#pragma unroll 4
+        for (int e = tid; e < a.elems; e += threads) first += (double)a.state[bh * a.elems + e] * (double)a.d_state[bh * a.elems + e];
     for (int off = 32; off; off >>= 1) first += __shfl_down(first, off);
     if (lane == 0) sums[wave] = first;
     __syncthreads();
-    first = 0.0;
-    for (int w = 0; w < 16; ++w) first += sums[w];
-    // this thread's run of tokens: what it adds behind its last start of an episode, and whether it holds one
-    const int64_t per = (a.L + 1023) / 1024, t0 = min(a.L, tid * per), t1 = min(a.L, t0 + per);
-    double add = 0.0;
-    int any = 0;
-    for (int64_t t = t0; t < t1; ++t) {
-        if (decay_fresh(a, t, b, h)) { add = 0.0; any = 1; }
-        add -= decay_step(a, t, bh);
-    }
-    part[tid] = add; cut[tid] = any;
-    __syncthreads();
-    for (int off = 1; off < 1024; off <<= 1) {   // inclusive scan of (add, cut): the later one wins where it holds a start
-        double p = part[tid]; int q = cut[tid];
-        if (tid >= off && !q) { p += part[tid - off]; q = cut[tid - off]; }
+    double carry = 0.0, sum = 0.0;   // carry: the gradient at the tokens' start
+    for (int w = 0; w < waves; ++w) carry += sums[w];
+    const float *pq = a.dot_q + bh * a.dot_sh, *pk = a.dot_k + bh * a.dot_sh;
+    for (int64_t tile = 0; tile < a.L; tile += 4 * threads) {
+        const int64_t t0 = tile + 4 * tid;
+        double step[4] = {0.0, 0.0, 0.0, 0.0};
+        bool fresh[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fresh[i] = decay_fresh(a, min(t0 + i, a.L - 1), b, h) && t0 + i < a.L;
+        for (int s = 0; s < a.slices; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t at = s * n + min(t0 + i, a.L - 1) * a.dot_sl;
+                step[i] += (double)pq[at] - (double)pk[at];
+            }
+        // what this thread's tokens add behind their last start of an episode, and whether they hold one; both scanned over the workgroup: the later one wins where
+        // it holds a start
+        double add = 0.0;
+        int cut = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (fresh[i]) { add = 0.0; cut = 1; }
+            add -= t0 + i < a.L ? step[i] : 0.0;
+        }
+        for (int off = 1; off < 64; off <<= 1) {
+            const double p = __shfl_up(add, off);
+            const int q = __shfl_up(cut, off);
+            if (lane >= off && !cut) { add += p; cut = q; }
+        }
+        __syncthreads();   // the sums before are read
+        if (lane == 63) { sums[wave] = add; cuts[wave] = cut; }
         __syncthreads();
-        part[tid] = p; cut[tid] = q;
-        __syncthreads();
-    }
-    double run = tid ? part[tid - 1] + (cut[tid - 1] ? 0.0 : first) : first, sum = 0.0;
-    for (int64_t t = t0; t < t1; ++t) {
-        if (decay_fresh(a, t, b, h)) run = 0.0;
-        if (a.dg) a.dg[t * heads + bh] = (float)run;
-        sum += run;
-        run -= decay_step(a, t, bh);
+        double run = carry;
+        for (int w = 0; w < waves; ++w) {
+            if (w == wave) run = carry;
+            carry = cuts[w] ? sums[w] : carry + sums[w];
+        }
+        const double p = __shfl_up(add, 1);
+        const int q = __shfl_up(cut, 1);
+        if (lane > 0) run = q ? p : run + p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (t0 + i < a.L) {
+                if (fresh[i]) run = 0.0;
+                if (a.dg) a.dg[(t0 + i) * heads + bh] = (float)run;
+                sum += run;
+                run -= step[i];
+            }
     }
     __syncthreads();
     for (int off = 32; off; off >>= 1) sum += __shfl_down(sum, off);
@@ -869,7 +886,7 @@ __global__ __launch_bounds__(1024) void decay_grad_long_kernel(DecayGrad a) {
     __syncthreads();
     if (tid == 0 && a.partial) {
         double s = 0.0;
-        for (int w = 0; w < 16; ++w) s += sums[w];
+        for (int w = 0; w < waves; ++w) s += sums[w];
         a.partial[bh] = s;
     }
 }
@@ -987,19 +1004,40 @@ bool small_heads(int dy, int dz, int64_t L) { return dy <= 32 || L <= (dz <= 16 
 // heads that share a wave of memory_rows_kernel
 int heads_of_wave(int dy) { return dy <= 32 ? 4 : dy <= 64 ? 2 : 1; }
 
-// A batch with few heads has its tokens cut into segments that are walked side by side: up to 2 048 waves of four small heads or 768 workgroups of a large one (what
-// is resident at a time: 8 waves, 3 workgroups per CU -- one more would be a second round), at least 32 or 64 tokens each (a segment costs a second
-// read of k and v and a state in the workspace, which shorter ones would not repay; 24 small heads of 16 x 16 and 500 tokens: 71 us with 64, 50 with 32).
+// workgroups of memory_tiles_kernel that a CU holds at a time: by registers (launch bounds) and LDS
+int tiles_resident(const FmarlMemory *m) {
+    const int nk = m->dk <= 64 ? 2 : 4, nz = (m->dv + 15) / 16, waves = nz < 4 ? 4 : nz;
+    const int regs = (nk == 4 ? 2 : m->dtype == FMARL_T_F32 ? 3 : 4) * 4 / waves;
+    const int lds = m->dtype == FMARL_T_F32 ? tiles_lds<float, false>(nk, nz) : m->dtype == FMARL_T_BF16 ? tiles_lds<__bf16, false>(nk, nz) : tiles_lds<_Float16, false>(nk, nz);
+    const int n = 160 * 1024 / lds < regs ? 160 * 1024 / lds : regs;
+    return n < 1 ? 1 : n;
+}
+
+// A batch with few heads has its tokens cut into segments that are walked side by side, at the price of a walk that leaves their states (a second read of k and v) and a
+// join.  Small heads: up to 2 048 waves (8 per CU), segments of 32 tokens at least (24 heads of 16 x 16 and 500 tokens: 71 us with 64, 50 with 32).  Large heads: as many
+// workgroups per CU as make the walk shortest; a chunk takes about 3 + 2 n units of time with n workgroups on its CU (64 x 64 bfloat16, 64 heads of 4 096 tokens,
+// training: n = 2 420 us, n = 3 372 us, n = 4 336 us; 40 x 72 float16, 72 heads of 1 023 tokens: n = 2 60 us, n = 3 70 us, whose segments are of 96 tokens and end unevenly).
 struct Segments { int nseg, len; };
 Segments memory_segments(const FmarlMemory *m) {
-    const int64_t heads = m->B * m->H, per = heads_of_wave(m->dk);
-    const bool small = small_heads(m->dk, m->dv, m->L);
-    const int64_t units = small ? (heads + per - 1) / per : heads, want = small ? 2048 : 768;
-    int64_t n = want / units, most = m->L / (small ? 32 : 64);
-    if (n > most) n = most;
-    if (n < 2) return {1, (int)(m->L > 0x40000000 ? 0x40000000 : m->L)};
-    const int64_t len = ((m->L + n - 1) / n + 31) / 32 * 32;
-    return {(int)((m->L + len - 1) / len), (int)len};
+    const int64_t heads = m->B * m->H;
+    Segments best = {1, (int)(m->L > 0x40000000 ? 0x40000000 : m->L)};
+    auto cut = [&](int64_t n, int least) {   // into n segments of `least` tokens at least
+        if (n > m->L / least) n = m->L / least;
+        if (n < 2) return Segments{1, best.len};
+        const int64_t len = ((m->L + n - 1) / n + 31) / 32 * 32;
+        return Segments{(int)((m->L + len - 1) / len), (int)len};
+    };
+    if (small_heads(m->dk, m->dv, m->L)) return cut(2048 / ((heads + heads_of_wave(m->dk) - 1) / heads_of_wave(m->dk)), 32);
+    const int resident = tiles_resident(m);
+    const auto cost = [&](const Segments &s) {
+        const int64_t blocks = heads * s.nseg, on_cu = (blocks + 255) / 256, rounds = (on_cu + resident - 1) / resident;
+        return (s.nseg > 1 ? 17 : 10) * ((s.len + 31ll) / 32) * rounds * (3 + 2 * (on_cu < resident ? on_cu : resident));
+    };
+    for (int k = 1; k <= resident; ++k) {
+        const Segments s = cut(256 * k / heads, 64);
+        if (cost(s) < cost(best)) best = s;
+    }
+    return best;
 }
 
 // columns of z that a wave of the small heads' kernel takes: 16; the large heads' workgroup takes them all
@@ -1251,7 +1289,10 @@ int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, co
         g.vec = (elems & 3) == 0 && (((uintptr_t)g.state | (uintptr_t)g.d_state) & 15) == 0;
         for (g.team = 1; g.state && g.team < 64 && g.team * 16 < elems;) g.team *= 2;   // 16 entries a lane at least
         if (few_tokens(m->L)) hipLaunchKernelGGL(decay_grad_short_kernel, dim3((unsigned)((heads * g.team + 255) / 256)), dim3(256), 0, st, g);
-        else hipLaunchKernelGGL(decay_grad_long_kernel, dim3((unsigned)heads), dim3(1024), 0, st, g);
+        else {
+            const int64_t most = m->L / 4 > elems / 16 ? m->L / 4 : elems / 16;   // four tokens and 16 state entries a thread, up to 1 024 threads
+            hipLaunchKernelGGL(decay_grad_long_kernel, dim3((unsigned)heads), dim3(most > 1024 ? 1024 : (int)(most + 63) / 64 * 64), 0, st, g);
+        }
         if (shared) hipLaunchKernelGGL(decay_sum_kernel, dim3((unsigned)m->H), dim3(256), 0, st, (const double *)(base + ws.partial), d_log_decay, m->B, m->H);
         HIP_OK(hipGetLastError());
     }
