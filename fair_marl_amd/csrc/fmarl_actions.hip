@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
             for (int j = 0; j < VT; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) { top = fmaxf(top, z[j][r]); some |= !(z[j][r] == -__builtin_inff()); }
-            top = fmaxf(top, __shfl_xor(top, 16)); top = fmaxf(top, __shfl_xor(top, 32));
+            top = lanes_max<16>(top, 64);
 #pragma unroll
             for (int j = 0; j < VT; ++j)
 #pragma unroll
@@ -152,10 +152,9 @@ __global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
                     s += e; t += d * e;
                     za = 16 * j + g4 + r == act ? z[j][r] : za;
                 }
-            int any = some;
-#pragma unroll
-            for (int off = 16; off < 64; off <<= 1) { s += __shfl_xor(s, off); t += __shfl_xor(t, off); za += __shfl_xor(za, off); any |= __shfl_xor(any, off); }
-            if (lane < 16 && real) row_result(a, row, act, top, s, t, any != 0, za);
+            s = lanes_sum<16>(s, 64); t = lanes_sum<16>(t, 64); za = lanes_sum<16>(za, 64);
+            const float any = lanes_max<16>(some ? 1.f : 0.f, 64);
+            if (lane < 16 && real) row_result(a, row, act, top, s, t, any != 0.f, za);
         } else {
             const bool in = real && lse != __builtin_inff();
 #pragma unroll
@@ -207,8 +206,7 @@ __global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float s = accb[j][r];
-#pragma unroll
-                        for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off);
+                        s = lanes_sum<1>(s, 16);
                         if (c == 0) lb[16 * j + g4 + r] = w ? lb[16 * j + g4 + r] + s : s;
                     }
                 }
@@ -381,7 +379,7 @@ __global__ __launch_bounds__(256) void actions_gemm_kernel(Gemm q) {
                     top = fmaxf(top, z != z ? __builtin_inff() : z);      // a NaN is not passed over: it makes the sums NaN
                     if (vbase + 16 * i + r == act) q.za[m] = z;
                 }
-            top = fmaxf(top, __shfl_xor(top, 16)); top = fmaxf(top, __shfl_xor(top, 32));
+            top = lanes_max<16>(top, 64);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -390,8 +388,7 @@ __global__ __launch_bounds__(256) void actions_gemm_kernel(Gemm q) {
                     const float d = none ? 0.f : acc[i][j][r] - top, e = none ? 0.f : exp_of(d);
                     s += e; t += d * e;
                 }
-            s += __shfl_xor(s, 16); s += __shfl_xor(s, 32);
-            t += __shfl_xor(t, 16); t += __shfl_xor(t, 32);
+            s = lanes_sum<16>(s, 64); t = lanes_sum<16>(t, 64);
             if (g == 0 && real) {
                 float *o = q.stats + (int64_t)(ia * 2 + (wave & 1)) * 3 * q.stat_stride + m;
                 o[0] = top; o[q.stat_stride] = s; o[2 * q.stat_stride] = t;
@@ -420,8 +417,7 @@ __global__ __launch_bounds__(256) void actions_gemm_kernel(Gemm q) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 float s = dbs[i][r];
-#pragma unroll
-                for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off);
+                s = lanes_sum<1>(s, 16);
                 if (c == 0) q.db[(int64_t)(ib * 2 + (wave >> 1)) * q.ldb_part + ia * 128 + ra + 16 * i + g4 + r] = s;
             }
         __syncthreads();
@@ -697,10 +693,7 @@ __global__ __launch_bounds__(512) void actions_wide_kernel(Wide q) {
                     store4<T>(zrow + 16 * j * q.ldz + 16 * i, d, 4, true);   // rounded to the operands' type: what the two products read
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    all[r] += row_turn<0x128>(all[r]); all[r] += row_turn<0x124>(all[r]);
-                    all[r] += row_turn<0x122>(all[r]); all[r] += row_turn<0x121>(all[r]);
-                }
+                for (int r = 0; r < 4; ++r) all[r] = lanes_sum<1>(all[r], 16);
                 if (c == 0) *(f32x4 *)(q.db + (int64_t)((ib + tile) * 4 + (wave >> 1)) * q.ldb_part + va + 16 * i) = all * inv_scale;
             }
         }
@@ -709,12 +702,10 @@ __global__ __launch_bounds__(512) void actions_wide_kernel(Wide q) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             // the four lanes of a row, then one slot per wave
-            float m = fmaxf(top[j], __shfl_xor(top[j], 16));
-            m = fmaxf(m, __shfl_xor(m, 32));
+            const float m = lanes_max<16>(top[j], 64);
             const float ref = m == -__builtin_inff() ? 0.f : m, f = top[j] == -__builtin_inff() ? (sum[j] == 0.f ? 0.f : 1.f) : exp2_fast(top[j] - ref);
             float s = sum[j] * f, t = f == 0.f ? 0.f : f * (tsum[j] + (top[j] == -__builtin_inff() ? 0.f : top[j] - ref) * sum[j]);
-            s += __shfl_xor(s, 16); s += __shfl_xor(s, 32);
-            t += __shfl_xor(t, 16); t += __shfl_xor(t, 32);
+            s = lanes_sum<16>(s, 64); t = lanes_sum<16>(t, 64);
             if (g == 0) {
                 float *o = q.stats + (int64_t)(split * 2 + (wave & 1)) * 3 * q.stat_stride + (int64_t)ib * 256 + rb + 16 * j + c;
                 o[0] = m; o[q.stat_stride] = s; o[2 * q.stat_stride] = t;
@@ -800,7 +791,7 @@ __global__ __launch_bounds__(1024) void actions_scale_kernel(Actions a, float *s
         const float v = (a.dlogp ? fabsf(a.dlogp[r]) : 0.f) + (a.dent ? fabsf(a.dent[r]) : 0.f) * lv;
         if (v < __builtin_inff()) m = fmaxf(m, v);
     }
-    for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    m = lanes_max<1>(m, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x == 0) {

@@ -37,8 +37,7 @@ struct Exchange { float *red, *row; int row_floats, flip; };
 
 template <int TL>
 __device__ __forceinline__ void team_sum2(float &v, float &w, Exchange &x) {
-#pragma unroll
-    for (int off = 1; off < (TL < 64 ? TL : 64); off <<= 1) { v += __shfl_xor(v, off); w += __shfl_xor(w, off); }
+    v = lanes_sum<1>(v, TL < 64 ? TL : 64); w = lanes_sum<1>(w, TL < 64 ? TL : 64);
     if (TL > 64) {
         float *red = x.red + x.flip * 32;
         x.flip ^= 1;
@@ -72,7 +71,7 @@ __device__ __forceinline__ void group_means(const Block &a, float (&v)[NV][4], i
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             float s = (v[n][0] + v[n][1]) + (v[n][2] + v[n][3]);
-            for (int off = 1; off < lanes; off <<= 1) s += __shfl_xor(s, off);
+            s = lanes_sum<1>(s, lanes);
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[n][r] = s * inv;
         }
@@ -95,7 +94,7 @@ __device__ __forceinline__ void group_means(const Block &a, float (&v)[NV][4], i
             const int g = g0 + l / per;
             float s = 0.f;
             if (g < a.groups) for (int e = l % per; e < size; e += per) s += row[g * size + e];
-            for (int off = 1; off < per; off <<= 1) s += __shfl_xor(s, off);
+            s = lanes_sum<1>(s, per);
             if (l % per == 0 && g < a.groups) sums[g] = s * inv;
         }
         team_sync<TL>();

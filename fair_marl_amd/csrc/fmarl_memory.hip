@@ -351,7 +351,7 @@ __global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory
                         if (DOT) {
                             const f32x4 wf = widen(wv), zf = widen(zv);
                             float dot = o[0] * wf[0] + o[1] * wf[1] + o[2] * wf[2] + o[3] * wf[3];
-                            dot += __shfl_xor(dot, 16); dot += __shfl_xor(dot, 32);
+                            dot = lanes_sum<16>(dot, 64);
                             if (g == 0) ldot[wave * 32 + t] = dot;
                             const float own = lown[t] * out_scale;
 #pragma unroll
@@ -435,10 +435,7 @@ template <int M, int N, typename F> __device__ __forceinline__ void unroll(F f) 
     if constexpr (M < N) { f(std::integral_constant<int, M>()); unroll<M + 1, N>(f); }
 }
 
-__device__ __forceinline__ float row_sum(float v) {   // over the 16 lanes of a row, in every lane: rotations by 8, 4, 2, 1
-    v += row_turn<0x128>(v); v += row_turn<0x124>(v); v += row_turn<0x122>(v); v += row_turn<0x121>(v);
-    return v;
-}
+__device__ __forceinline__ float row_sum(float v) { return lanes_sum<1>(v, 16); }
 
 // sum_m x_m S[m], x_m in lane m of the row; four partial sums, so that no add waits for the one before.  In assembly because the compiler does not put the lane
 // selection into a multiply-add (it emits a move for each: twice the instructions); s_nop 1: the two wait states between a vector write of x and its
@@ -498,19 +495,6 @@ template <int N> __device__ __forceinline__ void row_state(float (&S)[N], const 
 #pragma unroll
         for (int m = 0; m < N; ++m) S[m] = real && m < dy ? p[m * s_y] : 0.f;
     }
-}
-
-// the sum over the R neighbouring rows of 16 lanes that share a head, in all of them
-template <int R> __device__ __forceinline__ float rows_sum(float v) {
-    if constexpr (R >= 2) {
-        const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-        v = __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
-    }
-    if constexpr (R == 4) {
-        const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-        v = __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
-    }
-    return v;
 }
 
 template <typename T, int NY, int R, bool DOT>
@@ -593,15 +577,15 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
                 if (a.state_only) whole *= fresh ? 0.f : d;
                 else {
                     float nd = row_dot<NY>(x[i], S);       // from the tokens before
-                    nd = fresh ? 0.f : rows_sum<R>(nd) * d;
+                    nd = fresh ? 0.f : lanes_sum<16>(nd, 16 * R) * d;
                     float xy = 0.f;
 #pragma unroll
                     for (int n = 0; n < NY; ++n) xy += x[i][n] * y[i][n];
-                    xy = rows_sum<R>(row_sum(xy));
+                    xy = lanes_sum<1>(xy, 16 * R);
                     const int64_t t = t_begin + i0 + i;
                     if (have && zin && part == 0) po[t * a.out.sl] = (T)((nd + xy * zz[i]) * a.out_scale);
                     if (DOT) {
-                        const float dot = row_sum(zin ? nd * a.out_scale * ww[i] : 0.f);
+                        const float dot = lanes_sum<1>(zin ? nd * a.out_scale * ww[i] : 0.f, 16);
                         if (have && c == 0 && part == 0) a.dot[slice * a.dot_slice + t * a.dot_sl + bh * a.dot_sh] = dot;
                     }
                 }

@@ -61,6 +61,29 @@ template <int CTRL> __device__ __forceinline__ float row_turn(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
 
+// op over the lanes of a wave whose numbers differ in the bits from FROM (1, 16 or 32) up to below `to`, in all of them: within a row of 16 by DPP (a quad's neighbour, its other pair, a
+// half row mirrored -- whose quads hold one value each by then --, the row mirrored), beyond by the swaps of rows and halves.  No LDS pipe: a step is
+// a few cycles where ds_bpermute's is over fifty, and a row's norms are chains of such steps.
+template <int FROM, typename F> __device__ __forceinline__ float lanes_fold(float v, int to, F op) {
+    if (FROM <= 1) {
+        if (to > 1) v = op(v, row_turn<0xb1>(v));
+        if (to > 2) v = op(v, row_turn<0x4e>(v));
+        if (to > 4) v = op(v, row_turn<0x141>(v));
+        if (to > 8) v = op(v, row_turn<0x140>(v));
+    }
+    if (FROM <= 16 && to > 16) {
+        const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+        v = op(__builtin_bit_cast(float, (uint32_t)p[0]), __builtin_bit_cast(float, (uint32_t)p[1]));
+    }
+    if (to > 32) {
+        const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+        v = op(__builtin_bit_cast(float, (uint32_t)p[0]), __builtin_bit_cast(float, (uint32_t)p[1]));
+    }
+    return v;
+}
+template <int FROM> __device__ __forceinline__ float lanes_sum(float v, int to) { return lanes_fold<FROM>(v, to, [](float a, float b) { return a + b; }); }
+template <int FROM> __device__ __forceinline__ float lanes_max(float v, int to) { return lanes_fold<FROM>(v, to, [](float a, float b) { return fmaxf(a, b); }); }
+
 }  // namespace policy
 
 int policy_fail(int code, const char *fmt, const char *a = "");   // libfmarl.hip: the text of fmarl_last_error()
