@@ -105,8 +105,12 @@ __global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
     const int64_t tiles = (a.rows + 15) / 16, step = (int64_t)gridDim.x * 4;
     typedef typename Vec4<T>::type V4;
     V4 next[KT];
-    auto fetch = [&](int64_t tile) {
-        const int64_t row = tile * 16 + c;
+    int next_act = -1;
+    float next_lse = 0.f, next_ent = 0.f, next_dl = 0.f, next_de = 0.f;
+    auto fetch = [&](int64_t tile) {   // in flight while the tile before is computed
+        const int64_t row = tile * 16 + c, at = min(row, a.rows - 1);
+        next_act = action_of(a, at);
+        if (BACK) { next_lse = a.lse[at]; next_ent = a.ent[at]; if (a.dlogp) next_dl = a.dlogp[at]; if (a.dent) next_de = a.dent[at]; }
 #pragma unroll
         for (int k = 0; k < KT; ++k) next[k] = load4<T>((const T *)a.x + row * a.xs + 16 * k + g4, row < a.rows ? a.K - 16 * k - g4 : 0, a.xvec);
     };
@@ -118,9 +122,8 @@ __global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
         f32x4 x[KT], z[VT];
 #pragma unroll
         for (int k = 0; k < KT; ++k) x[k] = widen(next[k]);
-        const int act = real ? action_of(a, row) : -1;
-        float lse = 0.f, ent = 0.f, dl = 0.f, de = 0.f;
-        if (BACK && real) { lse = a.lse[row]; ent = a.ent[row]; dl = a.dlogp ? a.dlogp[row] : 0.f; de = a.dent ? a.dent[row] : 0.f; }
+        const int act = real ? next_act : -1;
+        const float lse = next_lse, ent = next_ent, dl = next_dl, de = next_de;
         if (tile + step < tiles) fetch(tile + step);
 #pragma unroll
         for (int j = 0; j < VT; ++j) {
@@ -225,7 +228,9 @@ __global__ __launch_bounds__(256) void actions_sums_kernel(const float *partial,
     const int c = threadIdx.x & 15, s = threadIdx.x >> 4;
     const int64_t i = (int64_t)blockIdx.x * 16 + c;
     double sum = 0.0;
-    if (i < n) for (int p = s; p < parts; p += 16) sum += (double)partial[p * n + i];
+    if (i < n)
+#pragma unroll 16
+        for (int p = s; p < parts; p += 16) sum += (double)partial[p * n + i];
     red[s][c] = sum;
     __syncthreads();
     if (s == 0 && i < n) {

@@ -382,11 +382,12 @@ bool row_aligned(const void *p, int64_t stride, int bytes) { return ((uintptr_t)
 
 int block_threads(int dim) { return dim <= 256 ? 256 : dim <= 512 ? 128 : dim <= 1024 ? 256 : dim <= 4096 ? 512 : 1024; }
 
-// Workgroups: what is resident at a time -- forwards five waves a SIMD, backwards three --, each looping over its share of the rows; backwards few beside the
+// Workgroups: each loops over its share of the rows.  Forwards five waves a SIMD, backwards three, one more of half precision rows and of long ones, whose bytes in flight or
+// barriers ask for it (us for training, three | four: 655 360 x 64 float32 443 | 473, bfloat16 276 | 265; 20 000 x 2 048 float32 476 | 436, bfloat16 324 | 275); backwards few beside the
 // rows, so that their partial sums of the weights' gradients (5 dim floats each) stay below a sixteenth of the bytes of the rows
 int block_workgroups(const FmarlBlock *b, bool backward) {
     const int threads = block_threads(b->dim), teams = b->dim <= 64 ? 16 : b->dim <= 128 ? 8 : b->dim <= 256 ? 4 : 1;
-    const int64_t want = backward ? (b->rows + 15) / 16 : (b->rows + teams - 1) / teams, most = (backward ? 3 : 5) * 65536 / threads;
+    const int64_t want = backward ? (b->rows + 15) / 16 : (b->rows + teams - 1) / teams, deep = b->dtype != FMARL_T_F32 || b->dim > 1024, most = ((backward ? 3 : 5) + deep) * 65536 / threads;
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
