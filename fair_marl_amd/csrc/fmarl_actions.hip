@@ -242,19 +242,33 @@ __global__ __launch_bounds__(256) void actions_sums_kernel(const float *partial,
 
 // ---- many actions -----------------------------------------------------------------------------------------------------------
 // dst (rows_pad, cols_pad) <- src (rows, cols; row stride), zeros around, and trans <- its transpose where wanted; with `lse` without the rows that take no
-// part (what they hold, NaN too, does not reach dW).  64 x 64 tiles.
+// part (what they hold, NaN too, does not reach dW).  64 x 64 tiles; up to two matrices of the same columns in a launch, the first one's `blocks` tiles of rows first.
+struct PackJob { const char *src; int64_t stride, rows, rows_pad; char *dst, *trans; const float *lse; };
+
 template <typename T>
-__global__ __launch_bounds__(256) void actions_pack_kernel(const T *src, int64_t stride, int64_t rows, int cols, T *dst, T *trans, int64_t rows_pad, int cols_pad, const float *lse) {
+__global__ __launch_bounds__(256) void actions_pack_kernel(PackJob j0, PackJob j1, int blocks, int cols, int cols_pad) {
     __shared__ T tile[64][66];
-    const int64_t r0 = (int64_t)blockIdx.x * 64;
-    const int c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const bool second = (int)blockIdx.x >= blocks;
+    const T *src = (const T *)(second ? j1.src : j0.src);
+    T *dst = (T *)(second ? j1.dst : j0.dst), *trans = (T *)(second ? j1.trans : j0.trans);
+    const float *lse = second ? j1.lse : j0.lse;
+    const int64_t stride = second ? j1.stride : j0.stride, rows = second ? j1.rows : j0.rows, rows_pad = second ? j1.rows_pad : j0.rows_pad;
+    const int64_t r0 = (int64_t)(second ? blockIdx.x - blocks : blockIdx.x) * 64;
+    const int c0 = blockIdx.y * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6, at = min(c0 + tx, cols - 1);
+    T v[16];
+    float l[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {   // every load is made, from a row and a column that are there, so that all are in flight
+        const int64_t r = min(r0 + ty + 4 * i, rows - 1);
+        v[i] = src[r * stride + at];
+        l[i] = lse ? lse[r] : 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int64_t r = r0 + ty + 4 * i;
-        T v = r < rows && c0 + tx < cols ? src[r * stride + c0 + tx] : (T)0.f;
-        if (lse && r < rows && lse[r] == __builtin_inff()) v = (T)0.f;
-        dst[r * cols_pad + c0 + tx] = v;
-        if (trans) tile[ty + 4 * i][tx] = v;
+        const T w = r < rows && c0 + tx < cols && l[i] != __builtin_inff() ? v[i] : (T)0.f;
+        dst[r * cols_pad + c0 + tx] = w;
+        if (trans) tile[ty + 4 * i][tx] = w;
     }
     if (trans) {
         __syncthreads();
@@ -767,6 +781,7 @@ __global__ __launch_bounds__(256) void actions_reduce_kernel(const float *part, 
     if (i >= rows * cols) return;
     const int64_t r = i / cols, at = r * ld + (i - r * cols);
     float s = first ? 0.f : sum[at];
+#pragma unroll 8
     for (int k = 0; k < splits; ++k) s += part[k * split_stride + at];
     if (last) out[i] = (T)(inv_scale ? s / *inv_scale : s);
     else sum[at] = s;
@@ -786,21 +801,28 @@ __global__ __launch_bounds__(256) void actions_bias_kernel(const float *part, in
 }
 
 // float16 operands: dz is stored times the power of two that brings the largest |dlog_prob| + |dentropy| (1 + log V) to 2^12, so that small upstream gradients
-// (a mean over a million rows) do not fall below float16's smallest numbers; the products are divided by it again.  One workgroup.
-__global__ __launch_bounds__(1024) void actions_scale_kernel(Actions a, float *scale) {
-    __shared__ float red[16];
+// (a mean over a million rows) do not fall below float16's smallest numbers; the products are divided by it again.  Maxima of up to 256 workgroups' rows first.
+const int kMaxima = 256;
+__global__ __launch_bounds__(256) void actions_maxima_kernel(Actions a, float *maxima) {
+    __shared__ float red[4];
     const float lv = 1.f + logf((float)a.V);
     float m = 0.f;
-    for (int64_t r = threadIdx.x; r < a.rows; r += 1024) {
-        if (a.lse[r] == __builtin_inff()) continue;
+#pragma unroll 4
+    for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * 256) {
         const float v = (a.dlogp ? fabsf(a.dlogp[r]) : 0.f) + (a.dent ? fabsf(a.dent[r]) : 0.f) * lv;
-        if (v < __builtin_inff()) m = fmaxf(m, v);
+        if (a.lse[r] != __builtin_inff() && v < __builtin_inff()) m = fmaxf(m, v);
     }
     m = lanes_max<1>(m, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
+    if (threadIdx.x == 0) maxima[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+__global__ __launch_bounds__(64) void actions_scale_kernel(const float *maxima, int parts, float *scale) {
+    float m = 0.f;
+    for (int i = threadIdx.x; i < parts; i += 64) m = fmaxf(m, maxima[i]);
+    m = lanes_max<1>(m, 64);
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) m = fmaxf(m, red[w]);
         int e = 0;
         if (m > 0.f) (void)frexpf(m, &e);
         *scale = ldexpf(1.f, min(120, max(-120, 12 - e)));
@@ -900,9 +922,9 @@ Plan actions_plan(const FmarlActions *a, bool backward) {
     if (p.P < tile) p.P = tile;
     if (p.P > p.Vp) p.P = p.Vp;
     const int64_t tm = p.Mc / tile, tk = p.Kp / tile, tv = p.P / tile;
-    // half precision: one workgroup per CU (its LDS is 128 KB); float32: two
-    p.split_x = parts_of(tm * tk, p.P / per, half ? 256 : 512, half ? 16 : 64);
-    p.split_w = parts_of(tv * tk, p.Mc / per, half ? 256 : 512, half ? 16 : 64);
+    // a workgroup per CU: half precision by its LDS (128 KB); float32 could hold two, whose shorter parts and longer sums cost more (12 345 x 625: 45 us a product, 32 us)
+    p.split_x = parts_of(tm * tk, p.P / per, 256, half ? 16 : 64);
+    p.split_w = parts_of(tv * tk, p.Mc / per, 256, half ? 16 : 64);
     const int64_t run = backward ? tm : p.Vp / tile, rest = backward ? tv : tm;
     p.split_z = (int)(256 / rest < 1 ? 1 : 256 / rest > run ? run : 256 / rest);
     size_t off = 0;
@@ -918,17 +940,19 @@ Plan actions_plan(const FmarlActions *a, bool backward) {
         p.sumx = take(p.P < p.Vp ? 4 * p.Mc * p.Kp : 0);
         p.sumw = take(p.Mc < M ? 4 * p.Vp * p.Kp : 0);
         p.db = take(4 * (p.Mc / 64) * p.P);
-        p.scale = take(4);
+        p.scale = take(4 * (1 + kMaxima));
     }
     p.total = off;
     return p;
 }
 
 // dst and (float32, backwards) its transpose
+// the rows from r0 on, and with the first of them the weights
 template <typename T>
-void pack(const T *src, int64_t stride, int64_t rows, int cols, T *dst, T *trans, int64_t rows_pad, int64_t cols_pad, const float *lse, hipStream_t st) {
-    hipLaunchKernelGGL((actions_pack_kernel<T>), dim3((unsigned)(rows_pad / 64), (unsigned)(cols_pad / 64)), dim3(256), 0, st, src, stride, rows, cols, dst, trans,
-                       rows_pad, (int)cols_pad, lse);
+void pack(const Actions &s, const Plan &p, int64_t r0, int64_t m, int64_t mp, T *xp, T *xt, T *wp, T *wt, const float *lse, hipStream_t st) {
+    const PackJob x = {(const char *)((const T *)s.x + r0 * s.xs), s.xs, m, mp, (char *)xp, (char *)xt, lse}, w = {(const char *)s.w, s.ws, s.V, p.Vp, (char *)wp, (char *)wt, nullptr};
+    const int64_t blocks = mp / 64 + (r0 == 0 ? p.Vp / 64 : 0);
+    hipLaunchKernelGGL((actions_pack_kernel<T>), dim3((unsigned)blocks, (unsigned)(p.Kp / 64)), dim3(256), 0, st, x, w, (int)(mp / 64), (int)s.K, (int)p.Kp);
 }
 
 template <int EPI>
@@ -952,10 +976,9 @@ int wide(const Wide &q, int64_t blocks, hipStream_t st) {
 
 int many_forward_f32(const Actions &s, const Plan &p, char *base, hipStream_t st) {
     float *xp = (float *)(base + p.xp), *wp = (float *)(base + p.wp);
-    pack<float>((const float *)s.w, s.ws, s.V, s.K, wp, nullptr, p.Vp, p.Kp, nullptr, st);
     for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
         const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 128);
-        pack<float>((const float *)s.x + r0 * s.xs, s.xs, m, s.K, xp, nullptr, mp, p.Kp, nullptr, st);
+        pack<float>(s, p, r0, m, mp, xp, nullptr, wp, nullptr, nullptr, st);
         Gemm q = {};
         q.A = (const char *)wp; q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(p.Vp / 128); q.tb = (int)(mp / 128); q.splits = 1; q.steps = (int)(up(s.K, 32) / 32);
         q.act = s; q.row0 = r0; q.stats = (float *)(base + p.stats); q.stat_stride = p.Mc; q.za = (float *)(base + p.za);
@@ -975,10 +998,9 @@ void reduce(const float *part, int64_t split_stride, int splits, int64_t ld, flo
 int many_backward_f32(const Actions &s, const Plan &p, float *dx, float *dw, float *db, char *base, hipStream_t st) {
     float *xp = (float *)(base + p.xp), *wp = (float *)(base + p.wp), *xt = (float *)(base + p.xt), *wt = (float *)(base + p.wt), *dz = (float *)(base + p.dz), *dzt = (float *)(base + p.dzt);
     float *out = (float *)(base + p.out), *sumx = (float *)(base + p.sumx), *sumw = (float *)(base + p.sumw), *dbp = (float *)(base + p.db);
-    pack<float>((const float *)s.w, s.ws, s.V, s.K, wp, wt, p.Vp, p.Kp, nullptr, st);
     for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
         const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 128);
-        pack<float>((const float *)s.x + r0 * s.xs, s.xs, m, s.K, xp, xt, mp, p.Kp, s.lse + r0, st);
+        pack<float>(s, p, r0, m, mp, xp, xt, wp, wt, s.lse + r0, st);
         for (int64_t v0 = 0; v0 < p.Vp; v0 += p.P) {
             const int64_t n = p.Vp - v0 < p.P ? p.Vp - v0 : p.P, nv = s.V - v0 < n ? s.V - v0 : n;   // of this piece: padded and real actions
             Gemm q = {};
@@ -1005,11 +1027,10 @@ template <typename T>
 int many_forward(const Actions &s, const Plan &p, char *base, hipStream_t st) {
     T *xp = (T *)(base + p.xp), *wp = (T *)(base + p.wp);
     float *bias2 = (float *)(base + p.bias2);
-    pack<T>((const T *)s.w, s.ws, s.V, s.K, wp, nullptr, p.Vp, p.Kp, nullptr, st);
     hipLaunchKernelGGL(actions_bias2_kernel, dim3((unsigned)(p.Vp / 256)), dim3(256), 0, st, s.bias, s.V, bias2, (int)p.Vp);
     for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
         const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 256);
-        pack<T>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xp, nullptr, mp, p.Kp, nullptr, st);
+        pack<T>(s, p, r0, m, mp, xp, nullptr, wp, nullptr, nullptr, st);
         Wide q = {};
         q.A = (const char *)wp; q.B = (const char *)xp; q.lda = q.ldb = p.Kp; q.ta = (int)(p.Vp / 256); q.tb = (int)(mp / 256); q.steps = (int)(up(s.K, 32) / 32); q.splits = p.split_z;
         q.act = s; q.row0 = r0; q.bias2 = bias2; q.taken = (const int *)(base + p.taken); q.stats = (float *)(base + p.stats); q.stat_stride = p.Mc; q.za = (float *)(base + p.za);
@@ -1028,13 +1049,14 @@ int many_backward(const Actions &s, const Plan &p, T *dx, T *dw, float *db, char
     const float *scale = nullptr;
     if ((float)(T)1e-30f == 0.f) {   // float16
         scale = (const float *)(base + p.scale);
-        hipLaunchKernelGGL(actions_scale_kernel, dim3(1), dim3(1024), 0, st, s, (float *)(base + p.scale));
+        const int parts = (int)(s.rows < 256 * kMaxima ? (s.rows + 255) / 256 : kMaxima);
+        hipLaunchKernelGGL(actions_maxima_kernel, dim3(parts), dim3(256), 0, st, s, (float *)(base + p.scale) + 1);
+        hipLaunchKernelGGL(actions_scale_kernel, dim3(1), dim3(64), 0, st, (const float *)(base + p.scale) + 1, parts, (float *)(base + p.scale));
     }
-    pack<T>((const T *)s.w, s.ws, s.V, s.K, wp, nullptr, p.Vp, p.Kp, nullptr, st);
     hipLaunchKernelGGL(actions_bias2_kernel, dim3((unsigned)(p.Vp / 256)), dim3(256), 0, st, s.bias, s.V, bias2, (int)p.Vp);
     for (int64_t r0 = 0; r0 < s.rows; r0 += p.Mc) {
         const int64_t m = s.rows - r0 < p.Mc ? s.rows - r0 : p.Mc, mp = up(m, 256);
-        pack<T>((const T *)s.x + r0 * s.xs, s.xs, m, s.K, xp, nullptr, mp, p.Kp, s.lse + r0, st);
+        pack<T>(s, p, r0, m, mp, xp, nullptr, wp, nullptr, s.lse + r0, st);
         hipLaunchKernelGGL(actions_rows_kernel, dim3((unsigned)(mp / 256)), dim3(256), 0, st, s, r0, mp, (f32x4 *)(base + p.rows), (int *)(base + p.taken), scale);
         for (int64_t v0 = 0; v0 < p.Vp; v0 += p.P) {
             const int64_t n = p.Vp - v0 < p.P ? p.Vp - v0 : p.P, nv = s.V - v0 < n ? s.V - v0 : n;   // of this piece: padded and real actions
