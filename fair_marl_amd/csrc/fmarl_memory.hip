@@ -1,5 +1,5 @@
 // The memory of a recurrent policy on gfx950: linear attention with a decay per head.  With r_t = 0 where an episode starts at t
-// (masks_t == 0; also where the decay is exactly zero) and 1 elsewhere,
+// (masks_t == 0; also where e^{g_t} is below float32's smallest number) and 1 elsewhere,
 //     S_t = r_t e^{g_t} S_{t-1} + k_t^T v_t          o_t = scale * q_t S_t
 // and backwards, with G_t the gradient of S_t,
 //     G_t = scale * q_t^T do_t + r_{t+1} e^{g_{t+1}} G_{t+1}      dq_t = scale * do_t S_t^T     dk_t = v_t G_t^T     dv_t = k_t G_t
@@ -38,6 +38,10 @@ struct Walk {
     int shift, state_only;
     float y_scale, out_scale;
 };
+
+// nothing from before reaches a token: an episode starts at it, or its decay's factor is below float32's smallest number (-inf, or a type's lowest value in its place, whose sum
+// with the other tokens' decays would lose theirs)
+__device__ __forceinline__ bool forgets(float g, float mask) { return mask == 0.f || g < -128.f; }
 
 // ---- large heads ------------------------------------------------------------------------------------------------------------
 // A workgroup walks one (batch, head, segment) in chunks of 32 tokens; wave w holds columns 16 w .. 16 w + 15 of the state (float32, in the accumulator layout of
@@ -245,12 +249,13 @@ __global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory
 #pragma unroll
                         for (int r = 0; r < 4; ++r) lzt[(i * 16 * nz + r) * 40 + zat[k]] = cz[i][r];
                 }
+            if (wave == 0) bad |= rm != 0.f && !(rg < 89.f);   // nor is a decay's factor in float32: its sums would reach the tokens behind a start
             if (subs == 1 && __ballot(bad) && lane == 0) lfr[flag] = 1;
             if (tid == 0) lfr[3 - flag] = 0;
             if (wave == 0) {
                 // prefix sums of the log decays (base 2), tokens that start afresh as bits; `head`: decay from before the chunk up to and with the token, `tail`: from behind it on
                 const bool live = only < 0 || tl == only;
-                const bool fresh = live && (rm == 0.f || rg == -__builtin_inff());
+                const bool fresh = live && forgets(rg, rm);
                 const uint32_t fr = (uint32_t)__ballot(fresh);
                 const double C = scan32(live && !fresh ? (double)rg * 1.4426950408889634074 : 0.0, lane);
                 const uint64_t u = __builtin_bit_cast(uint64_t, C);
@@ -385,7 +390,7 @@ __global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory
                     S[i] = mma_pieces<NP, 3, 2>(yt, uz, S[i]);
                 }
             }
-            whole *= all != -1.f ? all : 0.f;
+            whole = all != -1.f ? whole * all : 0.f;   // (selected: a factor that is not finite ends at a start too)
             if (DOT) {
                 __syncthreads();
                 if (wave == 0 && lane < 32 && lane < count && (only < 0 || lane == only)) {
@@ -405,7 +410,7 @@ __global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory
     if (shift) {
         const int64_t t = t_begin + length - 1;
         const float gt = e.g[t * e.gl + b * e.gb + h * e.gh], mt = e.masks ? e.masks[t * e.ml + b * e.mb] : 1.f;
-        behind = mt == 0.f || gt == -__builtin_inff() ? -1.f : exp2_fast((float)((double)gt * 1.4426950408889634074));
+        behind = forgets(gt, mt) ? -1.f : exp2_fast((float)((double)gt * 1.4426950408889634074));
     }
     if (e.state_out && holds) {
         float *ps = e.state_out + seg * e.seg_state_out + bh * (int64_t)(dy * dz) + (zc + c) * e.o_z;
@@ -566,7 +571,7 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
             ww[i] = DOT && zin ? (float)nw[i] : 0.f;
         }
         const bool real_decay = decayed(i0);
-        const float fresh_l = real_decay && (nm == 0.f || ng == -__builtin_inff()) ? 1.f : 0.f;
+        const float fresh_l = real_decay && forgets(ng, nm) ? 1.f : 0.f;
         const float decay_l = !real_decay ? 1.f : fresh_l != 0.f ? 0.f : exp2_fast((float)((double)ng * 1.4426950408889634074));
         if (i0 + TB < count) fetch(i0 + TB);
         unroll<0, TB>([&](auto ii) {
@@ -574,7 +579,7 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
             if (i0 + i < count) {
                 const float d = row_lane<i>(decay_l);
                 const bool fresh = row_lane<i>(fresh_l) != 0.f;
-                if (a.state_only) whole *= fresh ? 0.f : d;
+                if (a.state_only) whole = fresh ? 0.f : whole * d;
                 else {
                     float nd = row_dot<NY>(x[i], S);       // from the tokens before
                     nd = fresh ? 0.f : lanes_sum<16>(nd, 16 * R) * d;
@@ -595,11 +600,11 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
     }
     if (a.shift) {   // the last token's own decay lies behind it
         const float gt = pg[(t_end - 1) * a.gl], mt = pm ? pm[(t_end - 1) * a.ml] : 1.f;
-        const bool fresh = mt == 0.f || gt == -__builtin_inff();
+        const bool fresh = forgets(gt, mt);
         const float d = exp2_fast((float)((double)gt * 1.4426950408889634074));
 #pragma unroll
         for (int m = 0; m < 16 * NY; ++m) S[m] = fresh ? 0.f : S[m] * d;
-        whole *= fresh ? 0.f : d;
+        whole = fresh ? 0.f : whole * d;
     }
     if (a.state_out && have && zin) {
         float *ps = a.state_out + seg * a.seg_state_out + bh * (int64_t)a.dy * a.dz + (int64_t)z * a.o_z + y0 * a.o_y;
@@ -637,13 +642,22 @@ __global__ __launch_bounds__(256) void memory_short_backward_kernel(ShortGrad a)
     const int h = (int)(bh - b * a.H), K = a.dk_dim, V = a.dv_dim, L = a.L;
     const bool kin = c < K, vin = c < V;
     float q[16], k[16], v[16], o[16], xs[16];
+    {
+        T rq[16], rk[16], rv[16], ro[16];   // as in memory_rows_kernel: every load is made, from a token and a column that are there
+        const int ck = min(c, K - 1), cv = min(c, V - 1);
+        const T *pq = (const T *)a.q.p + b * a.q.sb + h * a.q.sh + ck, *pk = (const T *)a.k.p + b * a.k.sb + h * a.k.sh + ck;
+        const T *pv = (const T *)a.v.p + b * a.v.sb + h * a.v.sh + cv, *po = (const T *)a.o.p + b * a.o.sb + h * a.o.sh + cv;
 #pragma unroll
-    for (int t = 0; t < 16; ++t) {
-        const bool in = t < L;
-        q[t] = in && kin ? (float)((const T *)a.q.p)[t * a.q.sl + b * a.q.sb + h * a.q.sh + c] : 0.f;
-        k[t] = in && kin ? (float)((const T *)a.k.p)[t * a.k.sl + b * a.k.sb + h * a.k.sh + c] : 0.f;
-        v[t] = in && vin ? (float)((const T *)a.v.p)[t * a.v.sl + b * a.v.sb + h * a.v.sh + c] : 0.f;
-        o[t] = in && vin ? (float)((const T *)a.o.p)[t * a.o.sl + b * a.o.sb + h * a.o.sh + c] : 0.f;
+        for (int t = 0; t < 16; ++t)
+            if (t < L) { rq[t] = pq[t * a.q.sl]; rk[t] = pk[t * a.k.sl]; rv[t] = pv[t * a.v.sl]; ro[t] = po[t * a.o.sl]; }
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const bool in = t < L;
+            q[t] = in && kin ? (float)rq[t] : 0.f;
+            k[t] = in && kin ? (float)rk[t] : 0.f;
+            v[t] = in && vin ? (float)rv[t] : 0.f;
+            o[t] = in && vin ? (float)ro[t] : 0.f;
+        }
     }
     const float gl = c < L ? a.g[c * a.gl + b * a.gb + h * a.gh] : 0.f, ml = c < L && a.masks ? a.masks[c * a.ml + b * a.mb] : 1.f;
     const int64_t at = bh * (int64_t)K * V;
@@ -653,7 +667,7 @@ __global__ __launch_bounds__(256) void memory_short_backward_kernel(ShortGrad a)
 #pragma unroll
         for (int m = 0; m < 16; ++m) S[m] = 0.f;
     }
-    const float fresh_l = ml == 0.f || gl == -__builtin_inff() ? 1.f : 0.f;
+    const float fresh_l = forgets(gl, ml) ? 1.f : 0.f;
     const float decay_l = fresh_l != 0.f ? 0.f : exp2_fast((float)((double)gl * 1.4426950408889634074));
     unroll<0, 16>([&](auto tt) {
         constexpr int t = tt;
@@ -755,7 +769,7 @@ struct DecayGrad {
 };
 
 __device__ __forceinline__ bool decay_fresh(const DecayGrad &a, int64_t t, int64_t b, int h) {
-    return (a.masks && a.masks[t * a.ml + b * a.mb] == 0.f) || a.g[t * a.gl + b * a.gb + h * a.gh] == -__builtin_inff();
+    return forgets(a.g[t * a.gl + b * a.gb + h * a.gh], a.masks ? a.masks[t * a.ml + b * a.mb] : 1.f);
 }
 
 __global__ __launch_bounds__(256) void decay_grad_short_kernel(DecayGrad a) {
@@ -910,7 +924,7 @@ __global__ __launch_bounds__(256) void memory_step_kernel(Step a) {
     const float *S = a.state ? a.state + bh * (int64_t)a.dk * a.dv : nullptr;
     float *So = a.state_out + bh * (int64_t)a.dk * a.dv;
     const float g = a.g[b * a.gb + h * a.gh];
-    const bool carry = S && !(a.masks && a.masks[b * a.mb] == 0.f) && g != -__builtin_inff();
+    const bool carry = S && !forgets(g, a.masks ? a.masks[b * a.mb] : 1.f);
     const float decay = carry ? exp2_fast((float)((double)g * 1.4426950408889634074)) : 0.f;
     constexpr int W = VEC ? 4 : 1;
     // lanes along a row: the smallest power of two that covers it, so that few lanes idle and several rows share a wave
@@ -974,7 +988,7 @@ int memory_check(const FmarlMemory *m, const char *who) {
     if (m->shared_decay < 0 || m->shared_decay > 1 || (m->shared_decay && (m->decay_stride_l || m->decay_stride_b)))
         return policy_fail(FMARL_EINVAL, "%s: shared_decay must be 0, or 1 with strides of 0 over tokens and sequences", who);
     // a wave per head and slice: a launch holds fewer than 2^32 threads
-    if (m->B >= (1ll << 26) / m->H || m->L > (1ll << 40)) return policy_fail(FMARL_EINVAL, "%s: too many sequences (B H must stay below 2^26) or tokens", who);
+    if (m->B >= (1ll << 26) / m->H || m->L > (1ll << 30)) return policy_fail(FMARL_EINVAL, "%s: too many sequences (B H must stay below 2^26) or tokens (2^30)", who);
     if (m->L > 0 && m->B > 0 && (!m->q.data || !m->k.data || !m->v.data || !m->log_decay)) return policy_fail(FMARL_EINVAL, "%s: null argument", who);
     return FMARL_OK;
 }

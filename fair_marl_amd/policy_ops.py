@@ -164,7 +164,7 @@ def memory_chunk(q, k, v, log_decay, state=None, masks=None, scale=None):
         S_t = r_t exp(log_decay_t) S_{t-1} + k_t^T v_t,    out_t = scale q_t S_t,    r_t = 0 where masks_t == 0, else 1
 
     q, k (L, B, H, dk), v (L, B, H, dv) of one type (float32, bfloat16, float16), 1 <= dk, dv <= 128; out has v's type.  log_decay float32: (H,)
-    or one per token, (L, B, H); -inf forgets everything.  state: what the sequences bring, float32 with B H dk dv entries in any shape
+    or one per token, (L, B, H); below -128 (-inf, a type's lowest value) it forgets everything.  state: what the sequences bring, float32 with B H dk dv entries in any shape
     (the generator's ``rnn_states`` rows), None for zeros; the last state comes back as (B, H, dk, dv).  masks: L B entries as the
     generator's ``masks`` (0: an episode starts at the token).  scale: dk ** -0.5 if None.  Rows ordered (L, chunk) as ``recurrent_generator``
     yields them are this layout: ``q.view(L, chunks, H, dk)``.  States, decays and all sums are float32 (the decays' prefix sums float64).

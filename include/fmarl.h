@@ -520,8 +520,8 @@ typedef struct FmarlRows {
 /* Linear attention with a decay per head: the memory of a recurrent policy (what the reference keeps in the GRU behind rnn_states and masks,
  * onpolicy/algorithms/utils/rnn.py:26-84, here as a matrix per head).  Token t of sequence b, head h:
  *     S_t = r_t exp(g_t) S_{t-1} + k_t^T v_t,    out_t = scale q_t S_t,    r_t = 0 where masks_t == 0 (an episode starts), else 1.
- * q, k (L, B, H, dk), v (L, B, H, dv), 1 <= dk, dv <= 128, B H < 2^26; masks (L, B) or NULL; log_decay g (L, B, H) by its strides; -inf
- * forgets everything.  state (B, H, dk, dv) contiguous, NULL: zeros.  A state that is not carried on is not read
+ * q, k (L, B, H, dk), v (L, B, H, dv), 1 <= dk, dv <= 128, B H < 2^26, L <= 2^30; masks (L, B) or NULL; log_decay g (L, B, H) by its strides; below
+ * -128 (-inf, a type's lowest value) it forgets everything.  state (B, H, dk, dv) contiguous, NULL: zeros.  A state that is not carried on is not read
  * into the next one, whatever it holds. */
 typedef struct FmarlMemory {
     int64_t L, B;

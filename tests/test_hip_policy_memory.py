@@ -197,6 +197,48 @@ def test_decays_of_every_size():
     compare((out, last) + fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks), q, k, v, g, S, masks, 0.25, do, dS)
 
 
+@pytest.mark.parametrize('bad', [math.nan, math.inf])
+@pytest.mark.parametrize('shape', [(12, 2, 2, 16, 16), (40, 2, 1, 5, 7), (30, 2, 2, 100, 12), (90, 2, 2, 40, 24), (700, 1, 1, 16, 16), (700, 1, 1, 64, 64)], ids=str)
+def test_a_decay_that_is_no_number_ends_with_its_episode(shape, bad):
+    """a decay of NaN or infinity inside an episode: the episodes before and behind it are what they are with any other decay there"""
+    L, B, H, dk, dv = shape
+    q, k, v, g, S, masks, do, dS = make(*shape, F32, 'token', seed=31)
+    first, at, then = L // 4, L // 4 + 2, L // 2     # the bad episode's start, its bad decay, the next one's start
+    masks.fill_(1)
+    masks[(first, then), 0] = 0
+    clean = g.clone()
+    g[at, 0] = bad
+    run = lambda g: fm.memory_chunk(q, k, v, g, S, masks) + fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks)  # noqa: E731
+    got = run(g)
+    args = [x.double() for x in (q, k, v)]
+    want = recurrence(*args, clean.double(), S.double(), masks == 0, dk ** -0.5, do.double(), dS.double())
+    mag = recurrence(*[x.abs() for x in args], clean.double(), S.double().abs(), masks == 0, dk ** -0.5, do.double().abs(), dS.double().abs())
+    gamma = (2 * L + dk + dv + 200) * 2.0 ** -24
+    for i in (0, 2, 3, 4):
+        for rows in (slice(0, first), slice(then, L)):
+            close(got[i][rows, 0], want[i][rows, 0], gamma * mag[i][rows, 0] + step_of(got[i], want[i][rows, 0]))
+    for i in (1, 6):
+        close(got[i][0], want[i][0], gamma * mag[i][0] + step_of(got[i], want[i][0]))
+    assert bool(torch.isfinite(got[5][:first]).all()) and bool(torch.isfinite(got[5][then:]).all())
+    assert not bool(torch.isfinite(got[0][at, 0]).all())
+    if B > 1:   # the sequences beside it: not touched
+        for a, b in zip(got[:1] + got[2:6], run(clean)[:1] + run(clean)[2:6]):
+            assert torch.equal(a[:, 1], b[:, 1])
+
+
+@pytest.mark.parametrize('shape', [(12, 2, 2, 16, 16), (90, 2, 2, 40, 24), (700, 1, 1, 16, 16), (700, 1, 1, 64, 64)], ids=str)
+def test_decays_of_the_types_lowest_value(shape):
+    """a lowest value where -inf is meant: the small decays behind it keep their meaning"""
+    q, k, v, g, S, masks, do, dS = make(*shape, F32, 'token', seed=32)
+    masks.fill_(1)
+    g[torch.rand(g.shape, device=DEV) < 0.1] = torch.finfo(F32).min
+    out, last = fm.memory_chunk(q, k, v, g, S, masks)
+    compare((out, last) + fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks), q, k, v, g, S, masks, shape[3] ** -0.5, do, dS)
+    one = fm.memory_step(q[0], k[0], v[0], g[0], S, masks[0])
+    want = recurrence(q[:1].double(), k[:1].double(), v[:1].double(), g[:1].double(), S.double(), masks[:1] == 0, shape[3] ** -0.5)
+    assert float((one[1].double() - want[1]).abs().max()) < 1e-4
+
+
 def test_lengths_of_zero():
     z = lambda *s: torch.randn(*s, device=DEV)  # noqa: E731
     S = z(2, 3, 4, 5).requires_grad_()

@@ -12,6 +12,13 @@ if [ -n "$REV" ]; then
   (cd $R && git archive $REV fair_marl_amd/csrc include | tar -x -C $SRC)
 fi
 mkdir -p $R/fair_marl_amd/csrc/variants
-(cd $SRC/fair_marl_amd/csrc && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -mllvm -disable-machine-licm -Xclang -target-feature -Xclang -packed-fp32-ops \
-   -shared -fPIC "$@" -o $R/fair_marl_amd/csrc/variants/libfmarl_$NAME.so libfmarl.hip)
+cd $SRC/fair_marl_amd/csrc
+OBJS=
+for U in libfmarl fmarl_memory fmarl_block fmarl_actions; do   # (a revision from before the policy operators has the first only)
+  [ -f $U.hip ] || continue
+  FLAGS=; [ $U = libfmarl ] && FLAGS="-ffp-contract=off -mllvm -disable-machine-licm"
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops $FLAGS -fPIC "$@" -c -o /tmp/variant_${NAME}_$U.o $U.hip
+  OBJS="$OBJS /tmp/variant_${NAME}_$U.o"
+done
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $R/fair_marl_amd/csrc/variants/libfmarl_$NAME.so $OBJS
 echo "built fair_marl_amd/csrc/variants/libfmarl_$NAME.so from ${REV:-the working tree} $*"
