@@ -735,7 +735,9 @@ __global__ __launch_bounds__(512) void actions_wide_kernel(Wide q) {
 
 __global__ __launch_bounds__(256) void actions_bias2_kernel(const float *bias, int V, float *out, int n) {
     const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v < n) out[v] = v < V ? (bias ? bias[v] * kLog2e : 0.f) : -__builtin_inff();
+    if (v >= n) return;
+    const float b = v >= V ? -__builtin_inff() : bias ? bias[v] : 0.f;
+    out[v] = b == -__builtin_inff() ? b : fmaxf(b * kLog2e, -3.4028234e38f);   // a bias of the type's lowest value stays a number: its action is there
 }
 
 // the row's result from its slots' maxima and sums: 16 rows a workgroup, 16 threads a row.  `two`: maxima, sums and the taken logit are in base 2

@@ -179,6 +179,31 @@ def test_large_logits_and_small_upstream_gradients():
                 assert bool(((g.double() * s - w.double()).abs() <= step * w.double().abs() + s * tiny * 2.0 ** -10 + 1e-30 + step * float(w.abs().max())).all())
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('V', [5, 90])
+def test_bias_of_the_lowest_value(V, dtype):
+    """float32's lowest value in the bias where an action is not wanted: it is there all the same, with probability 0 and the gradient of a taken action; -inf takes it away"""
+    X, W, b, act, _, dl, _ = make(60, 32, V, dtype, seed=5, avail=False, pad=0.0)
+    b = b.float()
+    b[1], b[3] = torch.finfo(F32).min, -math.inf
+    act[:20], act[20:30] = 1, 3
+    act[30:] = torch.where((act[30:] == 1) | (act[30:] == 3), 0, act[30:])
+    leaves = [t.requires_grad_() for t in (X, W, b)]
+    lp, ent = fm.action_log_probs(X, W, b, act)
+    dX, dW, db = torch.autograd.grad((lp, ent), leaves, (dl, torch.ones_like(ent)))
+    assert bool((lp[:20] < -1e38).all()) and bool(torch.isfinite(lp[:20]).all()) and bool((lp[20:30] == -math.inf).all()) and bool(torch.isfinite(lp[30:]).all())
+    assert all(bool(torch.isfinite(t).all()) for t in (ent, dX, dW, db)) and float(db[3]) == 0
+    assert abs(float(db[1] - dl[:20].double().sum())) < 1e-5     # the taken action's 1 - p, p = 0: 20 additions of numbers up to 4, 20 x 4 x 2^-24 off at most
+    rest = [i for i in range(V) if i not in (1, 3)]
+    with torch.no_grad():   # the same rows without the two actions, in float64; the bounds as above
+        Xd, Wd = X[30:].double(), W[rest].double()
+        want, z, *_ = definition(Xd, Wd, b[rest].double(), torch.tensor([rest.index(int(a)) for a in act[30:]], device=DEV), None)
+        ez = ((32 + 4) * U * (Xd.abs() @ Wd.abs().t() + b[rest].double().abs())).amax(-1)
+        e_lp = 2 * ez + (V + 40) * U + 4 * U * (want[0].abs() + 2 * z.logsumexp(-1).abs())
+        e_H = (2 * want[1] + 2) * ez + 2 * (V + 64) * U * (want[1] + 2)
+        assert bool(((lp[30:] - want[0]).abs() <= e_lp).all()) and bool(((ent[30:] - want[1]).abs() <= e_H).all())
+
+
 @pytest.mark.parametrize('shape', [(30, 24, 5), (30, 24, 80)], ids=str)
 def test_gradient_against_differences(shape):
     X, W, b, act, av, dl, de = make(*shape, F32, seed=4)
