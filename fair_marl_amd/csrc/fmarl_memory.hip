@@ -55,6 +55,8 @@ __device__ __forceinline__ bool forgets(float g, float mask) { return mask == 0.
 // The decays' prefix sums are float64, so a weight e^{C_t - C_s} is right to float32 however fast the tokens before forgot.  A weight is selected, not multiplied to
 // zero: what an episode left behind (infinities too) does not reach the next one; a chunk that holds a value that is not finite is walked token by token, so
 // that it reaches later tokens only.
+// 64 heads of 4 096 tokens, 64 x 64, bfloat16 (segments of 256 tokens, four workgroups a CU): 33 us for the states alone, 48 us for out, 77 us for out with its sums against w, where the
+// bytes take 13 to 27 us and the matrix instructions 4 us: a chunk is three barriers and some 400 vector instructions a wave (pieces, weights, prefix sums), and those bound it.
 // pieces of an input (in), of P and the state as operands (p), highest order (sum of the pieces' numbers) kept in x y (in_order) and in out (out_order); u z has three pieces, kept to
 // order 2.  DOT: out is dotted with w before its rounding, for the decay's gradient, a difference of such sums: out to float32 there too.
 template <typename T, bool DOT> struct Pieces;
@@ -431,7 +433,8 @@ __global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory
 // its slice of the state, 16 NY values of y each; y and x are broadcast from the lane that holds them by the multiply's own operand (row_newbcast), so a token costs three
 // instructions per 64 state entries and no LDS.  Four neighbouring heads share a wave: 256 bytes of a token's row side by side.  Against a walk on the
 // matrix units, where half of every 16-token tile is above the diagonal and chunks of ten tokens waste the rest: 239 -> 133 us for 30 720 x 4 heads of ten
-// tokens (float32, 566 MB: 111 us at the copy rate of 5.1 TB/s).
+// tokens (float32, 566 MB: 111 us at the copy rate of 5.1 TB/s; 118 since the sums over lanes leave the LDS pipe).  Long sequences of small heads are bound by its
+// instructions: 2 000 heads of 16 x 16 and 3 193 tokens take 690 us, their bytes 330 us.
 template <int M> __device__ __forceinline__ float row_lane(float v) {   // lane M of each row of 16, in every lane of the row
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + M, 0xf, 0xf, true));
 }
@@ -617,7 +620,7 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
 // All gradients of up to 16 tokens of heads up to 16 x 16 in one pass (the update's chunks): q, k, v and dout stay in registers -- 16 lanes a head, as above --, the state is walked
 // forwards for dq, its gradient backwards for dk (lane = row) and dv (lane = column).  dg_t = <S_L, dS_L> + sum_{i >= t} (q_i . dq_i - k_i . dk_i), each
 // without the token's own term, 0 where an episode starts.  Reads and writes everything once: 928 MB for 30 720 x 4 heads of ten tokens, 182 us at the copy
-// rate; it takes 221 us, three walks and the decay's kernel took 872 us.
+// rate; it takes 222 us, three walks and the decay's kernel took 872 us.
 struct ShortGrad {
     WalkRows q, k, v, o, dq, dk, dv;
     const float *g; int64_t gl, gb, gh;
