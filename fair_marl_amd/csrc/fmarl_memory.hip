@@ -995,8 +995,13 @@ int memory_check(const FmarlMemory *m, const char *who) {
 // The recurrence on the vector units for y up to 32 wide and for few tokens, the matrix units beyond.  At 16 x 16 the former takes two thirds of the latter's time.  Wider,
 // its three instructions per 64 state entries and token cost more than a chunk of 32 tokens on the matrix units from about ten tokens on, or 32 where z has one
 // tile only (4 096 heads forwards, us, vector | matrix units: 64 x 64 bfloat16 1 token 37 | 53, 10 tokens 54 | 51, 16 tokens 64 | 51; 128 x 128 float32 1 token 160 | 265, 10
-// tokens 217 | 262, 32 tokens 440 | 286; 128 x 16 bfloat16 16 tokens 38 | 88, 32 tokens 62 | 89, 64 tokens 112 | 120).
-bool small_heads(int dy, int dz, int64_t L) { return dy <= 32 || L <= (dz <= 16 ? 32 : 10); }
+// tokens 217 | 262, 32 tokens 440 | 286; 128 x 16 bfloat16 16 tokens 38 | 88, 32 tokens 62 | 89, 64 tokens 112 | 120).  Beyond 64 with one tile of z a workgroup on the matrix
+// units has one wave that holds a state and three that only load, so many tokens are faster on the vector units too (106 x 7, 266 heads of 1 500 tokens: bfloat16 280 | 448, float32
+// 279 | 800; 72 heads of 412 tokens 81 | 57, 79 | 81).
+bool small_heads(int dy, int dz, int64_t L, int64_t heads) {
+    return dy <= 32 || L <= (dz <= 16 ? 32 : 10) || (dy > 64 && dz <= 16 && heads * L >= 65536);
+}
+bool small_heads(const FmarlMemory *m, int dy, int dz) { return small_heads(dy, dz, m->L, m->B * m->H); }
 
 // heads that share a wave of memory_rows_kernel
 int heads_of_wave(int dy) { return dy <= 32 ? 4 : dy <= 64 ? 2 : 1; }
@@ -1011,9 +1016,11 @@ int tiles_resident(const FmarlMemory *m) {
 }
 
 // A batch with few heads has its tokens cut into segments that are walked side by side, at the price of a walk that leaves their states (a second read of k and v) and a
-// join.  Small heads: up to 2 048 waves (8 per CU), segments of 32 tokens at least (24 heads of 16 x 16 and 500 tokens: 71 us with 64, 50 with 32).  Large heads: as many
-// workgroups per CU as make the walk shortest; a chunk takes about 3 + 2 n units of time with n workgroups on its CU (64 x 64 bfloat16, 64 heads of 4 096 tokens,
-// training: n = 2 420 us, n = 3 372 us, n = 4 336 us; 40 x 72 float16, 72 heads of 1 023 tokens: n = 2 60 us, n = 3 70 us, whose segments are of 96 tokens and end unevenly).
+// join, if that makes the walk shorter.  Small heads: with n waves on a SIMD, four at most, a token takes about 25 + 11 n units of time; segments of 32 tokens at least (24 heads of
+// 16 x 16 and 500 tokens: 71 us with 64, 50 with 32; 1 000 heads of 8 x 100 and 64 tokens: 67 us in two segments, 38 in one).  Large heads: with n workgroups on its CU a chunk
+// takes about 3 + 2 n units (64 x 64 bfloat16, 64 heads of 4 096 tokens, training: n = 2 420 us, n = 3 372 us, n = 4 336 us; 40 x 72 float16, 72 heads of 1 023 tokens: n = 2
+// 60 us, n = 3 70 us, whose segments are of 96 tokens and end unevenly); more segments where the gradient's walks are those of small heads and would
+// leave most of the chip idle (48 x 16 bfloat16, 266 heads of 412 tokens, backwards: 445 us in one segment, 167 in six).
 struct Segments { int nseg, len; };
 Segments memory_segments(const FmarlMemory *m) {
     const int64_t heads = m->B * m->H;
@@ -1024,7 +1031,19 @@ Segments memory_segments(const FmarlMemory *m) {
         const int64_t len = ((m->L + n - 1) / n + 31) / 32 * 32;
         return Segments{(int)((m->L + len - 1) / len), (int)len};
     };
-    if (small_heads(m->dk, m->dv, m->L)) return cut(2048 / ((heads + heads_of_wave(m->dk) - 1) / heads_of_wave(m->dk)), 32);
+    const auto waves = [&](int dy, int dz) { return (heads + heads_of_wave(dy) - 1) / heads_of_wave(dy) * ((dz + 15) / 16); };   // of an uncut walk of small heads
+    if (small_heads(m, m->dk, m->dv)) {
+        const int64_t uncut = waves(m->dk, m->dv);
+        const auto cost = [&](const Segments &s) {
+            const int64_t on_simd = (uncut * s.nseg + 1023) / 1024, rounds = (on_simd + 3) / 4;
+            return (s.nseg > 1 ? 16 : 10) * (int64_t)s.len * rounds * (25 + 11 * (on_simd < 4 ? on_simd : 4));
+        };
+        for (int k = 1; k <= 4; ++k) {
+            const Segments s = cut(1024 * k / uncut, 32);
+            if (cost(s) < cost(best)) best = s;
+        }
+        return best;
+    }
     const int resident = tiles_resident(m);
     const auto cost = [&](const Segments &s) {
         const int64_t blocks = heads * s.nseg, on_cu = (blocks + 255) / 256, rounds = (on_cu + resident - 1) / resident;
@@ -1034,11 +1053,15 @@ Segments memory_segments(const FmarlMemory *m) {
         const Segments s = cut(256 * k / heads, 64);
         if (cost(s) < cost(best)) best = s;
     }
+    if (small_heads(m, m->dv, m->dk) && waves(m->dv, m->dk) < 512) {   // the gradient's walks of dq and dk would leave most of the chip idle
+        const Segments s = cut(2048 / waves(m->dv, m->dk), 64);
+        if (s.nseg > best.nseg) best = s;
+    }
     return best;
 }
 
 // columns of z that a wave of the small heads' kernel takes: 16; the large heads' workgroup takes them all
-int slices_of(int dy, int dz, int64_t L) { return small_heads(dy, dz, L) ? (dz + 15) / 16 : 1; }
+int slices_of(const FmarlMemory *m, int dy, int dz) { return small_heads(m, dy, dz) ? (dz + 15) / 16 : 1; }
 
 // up to 16 tokens of heads up to 16 x 16: every gradient in one kernel, whose registers hold all of it
 bool short_backward(const FmarlMemory *m) { return m->L <= 16 && m->dk <= 16 && m->dv <= 16; }
@@ -1059,8 +1082,8 @@ Workspace memory_layout(const FmarlMemory *m, int backward) {
     }
     if (backward && short_backward(m)) w.partial = take(8 * heads);
     else if (backward) {
-        w.dot_q = take(4 * (size_t)slices_of(m->dv, m->dk, m->L) * m->L * heads);
-        w.dot_k = take(4 * (size_t)slices_of(m->dv, m->dk, m->L) * m->L * heads);
+        w.dot_q = take(4 * (size_t)slices_of(m, m->dv, m->dk) * m->L * heads);
+        w.dot_k = take(4 * (size_t)slices_of(m, m->dv, m->dk) * m->L * heads);
         w.partial = take(8 * heads);
         w.d_state = take(4 * heads * elems);
     }
@@ -1087,7 +1110,7 @@ int launch_tiles_as(const Walk &w, int64_t blocks, hipStream_t st) {
 template <typename T>
 int launch_walk_t(const Walk &w, hipStream_t st) {
     const int64_t heads = w.B * w.H;
-    if (small_heads(w.dy, w.dz, w.L)) {
+    if (small_heads(w.dy, w.dz, w.L, heads)) {
         const int per = heads_of_wave(w.dy);
         const int64_t blocks = ((heads + per - 1) / per * w.nseg * w.slices + 3) / 4;
         if (blocks > 0xffffff) return policy_fail(FMARL_EINVAL, "memory: too many sequences");
@@ -1107,7 +1130,7 @@ int launch_walk_t(const Walk &w, hipStream_t st) {
 }
 
 int launch_walk(Walk w, int dtype, hipStream_t st) {
-    w.slices = slices_of(w.dy, w.dz, w.L);
+    w.slices = small_heads(w.dy, w.dz, w.L, w.B * w.H) ? (w.dz + 15) / 16 : 1;
     const int rc = dtype == FMARL_T_F32 ? launch_walk_t<float>(w, st) : dtype == FMARL_T_BF16 ? launch_walk_t<__bf16>(w, st) : launch_walk_t<_Float16>(w, st);
     if (rc) return rc;
     HIP_OK(hipGetLastError());
@@ -1284,7 +1307,7 @@ int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, co
         g.dot_q = (const float *)(base + ws.dot_q); g.dot_k = (const float *)(base + ws.dot_k);
         g.state = m->state; g.d_state = ds0; g.g = w0.g; g.gl = w0.gl; g.gb = w0.gb; g.gh = w0.gh; g.masks = w0.masks; g.ml = w0.ml; g.mb = w0.mb;
         g.dg = shared ? nullptr : d_log_decay; g.partial = shared ? (double *)(base + ws.partial) : nullptr;
-        g.L = m->L; g.B = m->B; g.H = m->H; g.elems = elems; g.slices = slices_of(m->dv, m->dk, m->L);
+        g.L = m->L; g.B = m->B; g.H = m->H; g.elems = elems; g.slices = slices_of(m, m->dv, m->dk);
         g.dot_sl = w0.dot_sl; g.dot_sh = w0.dot_sh;
         g.vec = (elems & 3) == 0 && (((uintptr_t)g.state | (uintptr_t)g.d_state) & 15) == 0;
         for (g.team = 1; g.state && g.team < 64 && g.team * 16 < elems;) g.team *= 2;   // 16 entries a lane at least

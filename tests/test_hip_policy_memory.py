@@ -100,6 +100,15 @@ def test_chunk_and_gradients(shape, dtype, decay):
         compare((out, last) + grads, q, k, v, g, S, masks, shape[3] ** -0.5, do, dS)
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16], ids=str)
+@pytest.mark.parametrize('shape', [(700, 100, 1, 106, 7), (420, 45, 2, 48, 16), (300, 130, 2, 94, 21), (520, 130, 1, 7, 106), (64, 300, 3, 8, 100)], ids=str)
+def test_many_heads_that_are_wide_one_way(shape, dtype):
+    """walks whose two widths ask for different kernels and segments"""
+    q, k, v, g, S, masks, do, dS = make(*shape, dtype, 'token', seed=sum(shape), reset=0.02)
+    out, last = fm.memory_chunk(q, k, v, g, S, masks)
+    compare((out, last) + fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks), q, k, v, g, S, masks, shape[3] ** -0.5, do, dS)
+
+
 @pytest.mark.parametrize('shape', [(10, 9, 4, 16, 16), (200, 2, 2, 40, 24)], ids=str)
 def test_views_of_one_projection_in_any_order(shape):
     L, B, H, dk, dv = shape
