@@ -31,16 +31,26 @@ def _refuse(text, *args):
 def _same_device(op, first, *rest):
     if not first.is_cuda:
         _refuse('%s: tensors must be on a GPU, got one on %s', op, first.device)
-    dev = first.device
+    dev = first.get_device()
     for t in rest:
-        if t is not None and t.device != dev:
-            _refuse('%s: all tensors must be on %s, got one on %s', op, dev, t.device)
-    return dev
+        if t is not None and t.get_device() != dev:
+            _refuse('%s: all tensors must be on %s, got one on %s', op, first.device, t.device)
+
+
+def _once(backward):
+    """once_differentiable, without its context manager where no second gradient is asked for."""
+    guarded = once_differentiable(backward)
+    return staticmethod(lambda ctx, *grads: guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads))
 
 
 def _last(t):
     """t with a contiguous last axis."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _flat(t, n):
+    """t as rows of n, the last axis contiguous."""
+    return t if t.dim() == 2 and t.stride(1) == 1 else _last(t.reshape(-1, n))
 
 
 def _ptr(t):
@@ -56,13 +66,13 @@ def _wants_grad(*tensors):
 
 
 def _run(entry, dev, *args):
-    """One call of the C-ABI on dev's current stream."""
-    lib = _lib.load()
-    if torch.cuda.current_device() == dev.index:
-        rc = getattr(lib, entry)(*args, _raw_stream(dev.index) if _raw_stream else torch.cuda.current_stream(dev).cuda_stream)
+    """One call of the C-ABI on the current stream of the device with that number."""
+    call = getattr(_lib.load(), entry)
+    if torch.cuda.current_device() == dev:
+        rc = call(*args, _raw_stream(dev) if _raw_stream else torch.cuda.current_stream(dev).cuda_stream)
     else:
         with torch.cuda.device(dev):
-            rc = getattr(lib, entry)(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = call(*args, torch.cuda.current_stream(dev).cuda_stream)
     if rc:
         _lib.check(rc, entry)
 
@@ -88,37 +98,35 @@ def _memory_args(op, q, k, v, log_decay, state, masks, scale, lead):
         _refuse('%s: q and k (%sB, H, dk), v (%sB, H, dv), got %s, %s, %s', op, 'L, ' * (lead - 1), 'L, ' * (lead - 1), tuple(shape), tuple(k.shape), tuple(vshape))
     B, H, dk = shape[-3:]
     L, dv = shape[0] if lead == 2 else 1, vshape[-1]
-    gs = log_decay.stride()
-    token = len(gs) != 1
-    if log_decay.dtype != _F32 or log_decay.shape != (shape[:-1] if token else (H,)):
+    if log_decay.dtype != _F32 or log_decay.shape != (shape[:-1] if log_decay.dim() != 1 else (H,)):
         _refuse('%s: log_decay must be float32 (H,) or %s, got %s %s', op, tuple(shape[:-1]), log_decay.dtype, tuple(log_decay.shape))
-    ml = mb = 0
     if masks is not None:
         if masks.numel() != L * B:
             _refuse('%s: masks must hold %d entries, got %s', op, L * B, tuple(masks.shape))
         if masks.dtype != _F32:
             masks = masks.to(_F32)
-        if lead == 1:
-            masks = masks.reshape(B)
-            mb = masks.stride(0)
-        else:
-            masks = masks.reshape(L, B)
-            ml, mb = masks.stride()
+        masks = masks.reshape(B) if lead == 1 else masks.reshape(L, B)
     if state is not None:
         if state.dtype != _F32 or state.numel() != B * H * dk * dv:
             _refuse('%s: state must be float32 with B H dk dv = %d entries, got %s %s', op, B * H * dk * dv, state.dtype, tuple(state.shape))
         state = state.contiguous()
-    q, k, v = _last(q), _last(k), _last(v)
-    m = _lib.FmarlMemory(L, B, H, dk, dv, _DTYPES[q.dtype], dk ** -0.5 if scale is None else float(scale), 0 if token else 1, _rows(q), _rows(k), _rows(v),
-                         log_decay.data_ptr(), gs[0] if len(gs) == 3 else 0, gs[-2] if token else 0, gs[-1], _ptr(masks), ml, mb, _ptr(state))
-    return m, (q, k, v, log_decay, state, masks)
+    keep = (_last(q), _last(k), _last(v), log_decay, state, masks)
+    return _memory_struct(*keep, dk ** -0.5 if scale is None else float(scale)), keep
+
+
+def _memory_struct(q, k, v, g, state, masks, scale):
+    """FmarlMemory of checked, laid out tensors: masks (L, B) or (B)."""
+    shape, gs = q.shape, g.stride()
+    token, ms = len(gs) != 1, (0, 0) if masks is None else masks.stride()
+    return _lib.FmarlMemory(shape[0] if len(shape) == 4 else 1, shape[-3], shape[-2], shape[-1], v.shape[-1], _DTYPES[q.dtype], scale, 0 if token else 1, _rows(q), _rows(k), _rows(v),
+                            g.data_ptr(), gs[0] if len(gs) == 3 else 0, gs[-2] if token else 0, gs[-1], _ptr(masks), ms[0] if len(ms) == 2 else 0, ms[-1], _ptr(state))
 
 
 def _launch_chunk(m, keep):
     v = keep[2]
     out, state = v.new_empty(v.shape), v.new_empty((m.B, m.H, m.dk, m.dv), dtype=_F32)
     ws = _workspace(v, _lib.load().fmarl_memory_workspace(m, 0))
-    _run('fmarl_memory_chunk', v.device, m, _rows(out), state.data_ptr(), ws.data_ptr())
+    _run('fmarl_memory_chunk', v.get_device(), m, _rows(out), state.data_ptr(), ws.data_ptr())
     return out, state, ws
 
 
@@ -131,7 +139,7 @@ def _launch_chunk_backward(m, keep, d_out, d_state, want_decay=True, forward_ws=
     dg = g.new_empty(g.shape) if want_decay else None
     ds = g.new_empty((m.B, m.H, m.dk, m.dv))
     ws = _workspace(v, _lib.load().fmarl_memory_workspace(m, 1))
-    _run('fmarl_memory_chunk_backward', v.device, m, _rows(d_out), _ptr(d_state), _rows(dq), _rows(dk), _rows(dv), _ptr(dg), ds.data_ptr(), _ptr(forward_ws),
+    _run('fmarl_memory_chunk_backward', v.get_device(), m, _rows(d_out), _ptr(d_state), _rows(dq), _rows(dk), _rows(dv), _ptr(dg), ds.data_ptr(), _ptr(forward_ws),
          ws.data_ptr())
     return dq, dk, dv, dg, ds
 
@@ -147,11 +155,10 @@ class _MemoryChunk(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return out, last
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, d_out, d_state):
-        q, k, v, g, state, masks = ctx.saved_tensors
-        m, keep = _memory_args('memory_chunk', q, k, v, g, state, masks, ctx.scale, 2)
+        keep = q, k, v, g, state, masks = ctx.saved_tensors
+        m = _memory_struct(*keep, ctx.scale)
         if d_out is None:
             d_out = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
         dq, dk, dv, dg, ds = _launch_chunk_backward(m, keep, d_out, d_state, ctx.needs_input_grad[3], ctx.forward_ws)
@@ -213,7 +220,7 @@ def memory_step(q, k, v, log_decay, state, masks=None, scale=None, out_state=Non
             if gap and gap < 4 * n:
                 _refuse('memory_step: out_state overlaps state without being it')
     out = v.new_empty(v.shape)
-    _run('fmarl_memory_step', q.device, m, _rows(out), out_state.data_ptr())
+    _run('fmarl_memory_step', q.get_device(), m, _rows(out), out_state.data_ptr())
     return out, out_state
 
 
@@ -228,23 +235,21 @@ def _block_args(x, branch, gate, weights, groups, layer, silu, post_norm, pre_no
     dtype = x.dtype if branch is None else branch.dtype
     if dtype not in _DTYPES or (x.dtype != dtype and x.dtype != _F32):
         _refuse('block_norm: float32, bfloat16 or float16; x of the branch\'s type or float32, got %s, %s', x.dtype, dtype)
-    x2 = _last(x.reshape(-1, D))
-    b2 = g2 = None
-    if branch is not None:
-        if branch.shape != shape:
-            _refuse('block_norm: branch must be %s, got %s', tuple(shape), tuple(branch.shape))
-        b2 = _last(branch.reshape(-1, D))
-    if gate is not None:
-        if gate.shape != shape or gate.dtype != dtype:
-            _refuse('block_norm: gate must be %s %s, got %s %s', tuple(shape), dtype, tuple(gate.shape), gate.dtype)
-        g2 = _last(gate.reshape(-1, D))
-    ws = []
+    if branch is not None and branch.shape != shape:
+        _refuse('block_norm: branch must be %s, got %s', tuple(shape), tuple(branch.shape))
+    if gate is not None and (gate.shape != shape or gate.dtype != dtype):
+        _refuse('block_norm: gate must be %s %s, got %s %s', tuple(shape), dtype, tuple(gate.shape), gate.dtype)
     for name, w in zip(_WEIGHTS, weights):
-        if w is not None:
-            if w.dtype != _F32 or w.shape != (D,):
-                _refuse('block_norm: %s must be float32 (%d,), got %s %s', name, D, w.dtype, tuple(w.shape))
-            w = w.contiguous()
-        ws.append(w)
+        if w is not None and (w.dtype != _F32 or w.shape != (D,)):
+            _refuse('block_norm: %s must be float32 (%d,), got %s %s', name, D, w.dtype, tuple(w.shape))
+    return _block_struct(x, branch, gate, weights, groups, layer, silu, post_norm, pre_norm, eps)
+
+
+def _block_struct(x, branch, gate, weights, groups, layer, silu, post_norm, pre_norm, eps):
+    """The same of checked tensors."""
+    D, dtype = x.shape[-1], x.dtype if branch is None else branch.dtype
+    x2, b2, g2 = _flat(x, D), None if branch is None else _flat(branch, D), None if gate is None else _flat(gate, D)
+    ws = [None if w is None else w.contiguous() for w in weights]
     b = _lib.FmarlBlock(x2.shape[0], D, groups, _DTYPES[dtype], _DTYPES[x.dtype], layer, silu, post_norm, pre_norm, eps, 0, x2.data_ptr(), x2.stride(0), _ptr(b2),
                         0 if b2 is None else b2.stride(0), _ptr(g2), 0 if g2 is None else g2.stride(0), *[None if w is None else w.data_ptr() for w in ws])
     return b, (x2, b2, g2, ws)
@@ -254,7 +259,7 @@ def _launch_block(x, branch, gate, weights, options):
     b, keep = _block_args(x, branch, gate, weights, *options)
     y = None if branch is None else x.new_empty(x.shape)
     h = (x if branch is None else branch).new_empty(x.shape) if options[4] else None
-    _run('fmarl_block_norm', x.device, b, _ptr(y), _ptr(h))
+    _run('fmarl_block_norm', x.get_device(), b, _ptr(y), _ptr(h))
     return y, h
 
 
@@ -268,23 +273,21 @@ class _BlockNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dh):
         x, branch, gate, *weights = ctx.saved_tensors
         if dy is None and dh is None:
             return (None,) * 9
         need = ctx.needs_input_grad
-        b, keep = _block_args(x, branch, gate, weights, *ctx.options)
+        b, keep = _block_struct(x, branch, gate, weights, *ctx.options)
         D = b.dim
-        dy = None if dy is None else _last(dy.reshape(-1, D))
-        dh = None if dh is None else _last(dh.reshape(-1, D))
+        dy, dh = None if dy is None else _flat(dy, D), None if dh is None else _flat(dh, D)
         dx = x.new_empty(x.shape)
         dbranch = None if branch is None else branch.new_empty(x.shape)
         dgate = None if gate is None else gate.new_empty(x.shape)
         dw = [w.new_empty(D) if w is not None and n else None for w, n in zip(weights, need[3:8])]
         ws = _workspace(x, _lib.load().fmarl_block_norm_workspace(b))
-        _run('fmarl_block_norm_backward', x.device, b, _ptr(dy), 0 if dy is None else dy.stride(0), _ptr(dh), 0 if dh is None else dh.stride(0), dx.data_ptr(),
+        _run('fmarl_block_norm_backward', x.get_device(), b, _ptr(dy), 0 if dy is None else dy.stride(0), _ptr(dh), 0 if dh is None else dh.stride(0), dx.data_ptr(),
              _ptr(dbranch), _ptr(dgate), (C.c_void_p * 5)(*[_ptr(t) for t in dw]), ws.data_ptr())
         return (dx, dbranch, dgate, *dw, None)
 
@@ -338,20 +341,25 @@ def _action_args(features, weight, bias, actions, available):
     V, K = weight.shape
     if features.dtype not in _DTYPES or weight.dtype != features.dtype:
         _refuse('action_log_probs: features and weight must be of one type out of float32, bfloat16, float16, got %s, %s', features.dtype, weight.dtype)
-    if bias is not None:
-        if bias.shape != (V,):
-            _refuse('action_log_probs: bias must be (%d,), got %s', V, tuple(bias.shape))
-        bias = bias.contiguous()
-    x, w = _last(features.reshape(-1, K)), _last(weight)
-    M = x.shape[0]
+    if bias is not None and bias.shape != (V,):
+        _refuse('action_log_probs: bias must be (%d,), got %s', V, tuple(bias.shape))
+    M = features.numel() // K
     if actions.dtype not in _ACTION_TYPES or actions.numel() != M:
         _refuse('action_log_probs: actions must be int64, int32 or float32 with %d entries, got %s %s', M, actions.dtype, tuple(actions.shape))
-    actions = actions.contiguous()
+    if available is not None and (available.dtype not in (_F32, torch.bool, torch.uint8) or available.numel() != M * V or available.shape[-1] != V):
+        _refuse('action_log_probs: available_actions must be float32, bool or uint8 (..., %d) with %d entries, got %s %s', V, M * V, available.dtype, tuple(available.shape))
+    return _action_struct(features, weight, bias, actions, available)
+
+
+def _action_struct(features, weight, bias, actions, available):
+    """The same of checked tensors."""
+    V, K = weight.shape
+    x, w, actions = _flat(features, K), _last(weight), actions.contiguous()
+    M = x.shape[0]
+    if bias is not None:
+        bias = bias.contiguous()
     kind = stride = 0
     if available is not None:
-        if available.dtype not in (_F32, torch.bool, torch.uint8) or available.numel() != M * V or available.shape[-1] != V:
-            _refuse('action_log_probs: available_actions must be float32, bool or uint8 (..., %d) with %d entries, got %s %s', V, M * V, available.dtype,
-                    tuple(available.shape))
         available = _last(available.reshape(M, V))
         kind, stride = int(available.dtype != _F32), available.stride(0)
     a = _lib.FmarlActions(M, K, V, _DTYPES[x.dtype], _ACTION_TYPES[actions.dtype], kind, 0, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), _ptr(bias),
@@ -364,7 +372,7 @@ def _launch_actions(features, weight, bias, actions, available):
     shape = features.shape[:-1]
     log_probs, entropy, lse = (features.new_empty(shape, dtype=_F32) for _ in range(3))
     ws = _workspace(features, _lib.load().fmarl_action_log_probs_workspace(a, 0))
-    _run('fmarl_action_log_probs', features.device, a, log_probs.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ws.data_ptr())
+    _run('fmarl_action_log_probs', features.get_device(), a, log_probs.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ws.data_ptr())
     return log_probs, entropy, lse
 
 
@@ -376,20 +384,19 @@ class _ActionLogProbs(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return log_probs, entropy
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, d_log_probs, d_entropy):
         features, weight, bias, actions, available, entropy, lse = ctx.saved_tensors
         if d_log_probs is None and d_entropy is None:
             return (None,) * 5
-        a, keep = _action_args(features, weight, bias, actions, available)
+        a, keep = _action_struct(features, weight, bias, actions, available)
         dx, dw = features.new_empty(features.shape), weight.new_empty(weight.shape)
         db = bias.new_empty(bias.shape) if bias is not None and ctx.needs_input_grad[2] else None
         if a.rows == 0:
             return dx, dw.zero_(), None if db is None else db.zero_(), None, None
         dl, de = (None if t is None else t.contiguous() for t in (d_log_probs, d_entropy))
         ws = _workspace(features, _lib.load().fmarl_action_log_probs_workspace(a, 1))
-        _run('fmarl_action_log_probs_backward', features.device, a, entropy.data_ptr(), lse.data_ptr(), _ptr(dl), _ptr(de), dx.data_ptr(), dw.data_ptr(), _ptr(db),
+        _run('fmarl_action_log_probs_backward', features.get_device(), a, entropy.data_ptr(), lse.data_ptr(), _ptr(dl), _ptr(de), dx.data_ptr(), dw.data_ptr(), _ptr(db),
              ws.data_ptr())
         return dx, dw, db, None, None
 
