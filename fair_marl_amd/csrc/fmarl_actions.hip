@@ -796,7 +796,9 @@ __global__ __launch_bounds__(256) void actions_bias_kernel(const float *part, in
     __shared__ double red[16][17];
     const int c = threadIdx.x & 15, s = threadIdx.x >> 4, v = blockIdx.x * 16 + c;
     double sum = 0.0;
-    if (v < n) for (int p = s; p < parts; p += 16) sum += (double)part[p * ld + v];
+    if (v < n)
+#pragma unroll 16
+        for (int p = s; p < parts; p += 16) sum += (double)part[p * ld + v];
     red[s][c] = sum;
     __syncthreads();
     if (s == 0 && v < n) {
