@@ -19,16 +19,21 @@ template <> struct Vec4<float> { typedef f32x4 type; };
 template <> struct Vec4<__bf16> { typedef bf16x4 type; };
 template <> struct Vec4<_Float16> { typedef f16x4 type; };
 
-// four consecutive elements at p: one load where `vec` (p is a multiple of four elements of the type), else element by element, zero beyond `left`
+// four elements that start anywhere: the memory takes one access of any alignment for them
+template <typename T> struct Loose4 { typedef typename Vec4<T>::type type __attribute__((aligned(sizeof(T)))); };
+
+// four consecutive elements at p, zero beyond `left`: one load; where `vec`, p is a multiple of four elements and left one of four, else the row's last ones come one by one
 template <typename T>
 __device__ __forceinline__ typename Vec4<T>::type load4(const T *p, int left, bool vec) {
     typedef typename Vec4<T>::type V;
     V v = {(T)0.f, (T)0.f, (T)0.f, (T)0.f};
     if (vec) {
-        if (left > 0) v = *(const V *)p;   // (left is a multiple of four here)
+        if (left > 0) v = *(const V *)p;
+    } else if (left >= 4) {
+        v = *(const typename Loose4<T>::type *)p;
     } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) if (r < left) v[r] = p[r];
+        for (int r = 0; r < 3; ++r) if (r < left) v[r] = p[r];
     }
     return v;
 }
@@ -39,9 +44,11 @@ __device__ __forceinline__ void store4(T *p, f32x4 a, int left, bool vec) {
     const V v = {(T)a[0], (T)a[1], (T)a[2], (T)a[3]};   // round to nearest even, once, at the end
     if (vec) {
         if (left > 0) *(V *)p = v;
+    } else if (left >= 4) {
+        *(typename Loose4<T>::type *)p = v;
     } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) if (r < left) p[r] = v[r];
+        for (int r = 0; r < 3; ++r) if (r < left) p[r] = v[r];
     }
 }
 
