@@ -81,7 +81,7 @@ __device__ __forceinline__ float dlogit(float z, bool hot, bool in, float lse, f
 // x), so a row's softmax is over a lane's registers and two lane exchanges, and dx^T = W^T dz^T takes dz^T as it lies.  VT * 16 >= V, KT * 16 >= K.  x is loaded
 // once, in float4s; float32 products for every type.  The gradient of W is summed over a wave's tiles in registers, over the workgroup in LDS and
 // over the workgroups by actions_sums_kernel, always in the same order.  2 097 152 rows of 64 float32, five actions: 131 us forwards (4.4 TB/s), 225 + 5 us backwards (5.0 TB/s).
-template <typename T, int VT, int KT, bool BACK>
+template <typename T, int VT, int KT, bool BACK, bool VEC>
 __global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
     constexpr int PK = 16 * KT + 4;
     __shared__ __align__(16) float lw[16 * VT * PK], lb[16 * VT];
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
         next_act = action_of(a, at);
         if (BACK) { next_lse = a.lse[at]; next_ent = a.ent[at]; if (a.dlogp) next_dl = a.dlogp[at]; if (a.dent) next_de = a.dent[at]; }
 #pragma unroll
-        for (int k = 0; k < KT; ++k) next[k] = load4<T>((const T *)a.x + row * a.xs + 16 * k + g4, row < a.rows ? a.K - 16 * k - g4 : 0, a.xvec);
+        for (int k = 0; k < KT; ++k) next[k] = load4<T>((const T *)a.x + row * a.xs + 16 * k + g4, row < a.rows ? a.K - 16 * k - g4 : 0, VEC);
     };
     int64_t tile = (int64_t)blockIdx.x * 4 + wave;
     if (tile < tiles) fetch(tile);
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
                 for (int j = 0; j < VT; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o = __builtin_amdgcn_mfma_f32_16x16x4f32(lw[(16 * j + g4 + r) * PK + 16 * k + c], z[j][r], o, 0, 0, 0);
-                if (real) store4<T>((T *)a.dx + row * a.K + 16 * k + g4, o, a.K - 16 * k - g4, a.dxvec);
+                if (real) store4<T>((T *)a.dx + row * a.K + 16 * k + g4, o, a.K - 16 * k - g4, VEC);
             }
 #pragma unroll
             for (int j = 0; j < VT; ++j) {
@@ -880,7 +880,9 @@ int few_workgroups(const FmarlActions *a) {   // four waves of 16 rows each; 1 0
 template <typename T, bool BACK>
 int launch_few(const Actions &s, int blocks, hipStream_t st) {
     const int vt = (s.V + 15) / 16, kt = (s.K + 15) / 16;
-#define FMARL_FEW(VT, KT) hipLaunchKernelGGL((actions_few_kernel<T, VT, KT, BACK>), dim3(blocks), dim3(256), 0, st, s)
+    const bool vec = s.xvec && (!BACK || s.dxvec);   // known at compile time: as an argument it costs the loads in flight (2 097 152 x 64 x 5 training: 438 us, 368)
+#define FMARL_FEW(VT, KT) do { if (vec) hipLaunchKernelGGL((actions_few_kernel<T, VT, KT, BACK, true>), dim3(blocks), dim3(256), 0, st, s); \
+                               else hipLaunchKernelGGL((actions_few_kernel<T, VT, KT, BACK, false>), dim3(blocks), dim3(256), 0, st, s); } while (0)
     if (vt <= 1) { if (kt <= 2) FMARL_FEW(1, 2); else if (kt <= 4) FMARL_FEW(1, 4); else if (kt <= 8) FMARL_FEW(1, 8); else FMARL_FEW(1, 16); }
     else if (vt <= 2) { if (kt <= 2) FMARL_FEW(2, 2); else if (kt <= 4) FMARL_FEW(2, 4); else FMARL_FEW(2, 8); }
     else { if (kt <= 2) FMARL_FEW(4, 2); else FMARL_FEW(4, 4); }
