@@ -5,8 +5,8 @@
 //     dy' = dy + N^T(dh pre_weight) = dx      dr = dy' scale      du = dr act(gate)      dgate = dr u act'(gate)
 //     dbranch = N_groups^T(du post_weight)    and the weights' gradients are sums over the rows of dy' r, du n, du, dh n, dh.
 // Nothing is kept from the forward pass: the backward one reads x, branch and gate again and forms y unrounded.  All of it is bytes: forward five
-// rows, backward eight; the arithmetic is float32.  655 360 rows of 64 float32: 168 us forwards (5.0 TB/s), 274 + 5 us backwards (4.9 TB/s); 16 383 rows of 1 000 bfloat16 in groups of
-// 125: 45 us (3.7 TB/s) and 95 + 9 us (2.8 TB/s): there the sums between the waves of a row bound it, two for each group norm through LDS.
+// rows, backward eight; the arithmetic is float32.  655 360 rows of 64 float32: 165 us forwards (5.1 TB/s), 270 + 5 us backwards (5.0 TB/s); 16 383 rows of 1 000 bfloat16 in groups of
+// 125: 44 us (3.7 TB/s) and 94 + 9 us (2.8 TB/s): there the sums between the waves of a row bound it, two for each group norm through LDS.
 #include "fmarl_policy_dev.h"
 
 namespace fmarl {
