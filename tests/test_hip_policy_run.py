@@ -2,6 +2,7 @@
 log-probabilities from its features, then the update's recurrent minibatches over the same buffer -- against the same policy in plain float64 torch."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import fair_marl_amd as fm
 from fair_marl_amd.rollout_buffer import DeviceRolloutBuffer
@@ -150,3 +151,31 @@ def test_buffer_entry_points_refuse():
         buf.insert_actions(4, z(5, 3, 7), z(5, 7), None, z(5, 3))
     lp, en = buf.insert_actions(0, z(5, 3, 7), z(5, 7), None, z(5, 3))
     assert float((en - 5 ** 0 * torch.log(torch.tensor(5.0))).abs().max().cpu()) < 1e-6
+
+
+def test_saved_tensors_elsewhere_and_second_gradients():
+    """what the backward pass needs may be formed again (checkpointing) or come back from the host at another address: the same gradients; a gradient of a gradient is refused"""
+    gen = torch.Generator().manual_seed(3)
+    rn = lambda *s: torch.randn(*s, generator=gen).to(DEV).requires_grad_()  # noqa: E731
+    big = rn(12, 6, 2, 21)                      # rows with odd strides inside
+    x, branch, w, head, bias = rn(72, 20), rn(72, 20), rn(20), rn(V, 20), rn(V)
+    q, k, v, g, S = big[..., :8], big[..., 8:16], big[..., 16:], rn(12, 6, 2), rn(6, 2, 8, 5)
+    act = torch.randint(0, V, (72,), generator=gen).to(DEV)
+    leaves = (big, g, S, x, branch, w, head, bias)
+
+    def loss():
+        o, last = fm.memory_chunk(q, k, v, torch.nn.functional.logsigmoid(g), S)
+        y, h = fm.block_norm(x, branch, None, w, None, None, w, groups=2, kind='layer')
+        lp, ent = fm.action_log_probs(h, head, bias, act)
+        return o.square().sum() + last.sum() + y.sum() + (lp * ent).sum()
+
+    want = torch.autograd.grad(loss(), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        offloaded = loss()
+    again = torch.utils.checkpoint.checkpoint(loss, use_reentrant=False)
+    for got in (torch.autograd.grad(offloaded, leaves), torch.autograd.grad(again, leaves)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for leaf in (S, x, head):
+        first, = torch.autograd.grad(loss(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            first.sum().backward()
