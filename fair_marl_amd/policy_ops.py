@@ -205,12 +205,13 @@ def memory_chunk_backward(q, k, v, log_decay, d_out, d_state=None, state=None, m
 def memory_step(q, k, v, log_decay, state, masks=None, scale=None, out_state=None):
     """``memory_chunk`` for one token per sequence, as an env step of the rollout takes it: ``(out, out_state)``.  q, k (B, H, dk), v (B, H, dv), log_decay
     (H,) or (B, H), masks B entries, state None or float32 with B H dk dv entries.  out_state: where the new state goes (float32, contiguous; the buffer's next slot, or ``state``
-    itself), a new (B, H, dk, dv) tensor if None.  No gradient: refused where one would be recorded."""
+    itself), a new (B, H, dk, dv) tensor if None; to autograd it is written in place.  No gradient: refused where one would be recorded."""
     if _wants_grad(q, k, v, log_decay, state):
         _refuse('memory_step records no gradient: call it under torch.no_grad(), or use memory_chunk')
     m, keep = _memory_args('memory_step', q, k, v, log_decay, state, masks, scale, 1)
     n = m.B * m.H * m.dk * m.dv
-    if out_state is None:
+    given = out_state is not None
+    if not given:
         out_state = v.new_empty((m.B, m.H, m.dk, m.dv), dtype=_F32)
     else:
         if out_state.device != q.device or out_state.dtype != _F32 or out_state.numel() != n or not out_state.is_contiguous():
@@ -221,6 +222,8 @@ def memory_step(q, k, v, log_decay, state, masks=None, scale=None, out_state=Non
                 _refuse('memory_step: out_state overlaps state without being it')
     out = v.new_empty(v.shape)
     _run('fmarl_memory_step', q.get_device(), m, _rows(out), out_state.data_ptr())
+    if given:
+        torch.autograd.graph.increment_version(out_state)   # written behind autograd's back: a graph that keeps what it held has to see that
     return out, out_state
 
 
