@@ -9,11 +9,13 @@
 
 All run on the current stream of their tensors' device, take any strides as long as the last axis is contiguous (a tensor whose last axis is
 not is copied), read nothing back and are capturable in a graph.  Gradients come through torch.autograd; ``memory_chunk_backward`` is the
-same gradient as a plain call, for a step that is captured without an autograd graph.  There is no CPU form: tensors off the GPU are refused.
+same gradient as a plain call, for a step that is captured without an autograd graph.  There is no CPU form: tensors off the GPU are refused.  So are
+forward-mode tangents, and calls under a tracer (torch.jit.trace, make_fx), which would keep nothing of them.
 """
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -26,6 +28,19 @@ _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)   # (2 us les
 # A call's host time is most of a small call's: arguments are checked by plain conditions, messages are formed only when one fails.
 def _refuse(text, *args):
     raise ValueError(text % args if args else text)
+
+
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def _seen_by_torch(op, *tensors):
+    """Refuses a call whose kernels torch would have to know of: one that it records, one that it forms a tangent of (it sees new, unwritten tensors only)."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _refuse('%s: no forward-mode derivative', op)
+    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
+        _refuse('%s: cannot be traced', op)
 
 
 def _same_device(op, first, *rest):
@@ -176,6 +191,7 @@ def memory_chunk(q, k, v, log_decay, state=None, masks=None, scale=None):
     generator's ``masks`` (0: an episode starts at the token).  scale: dk ** -0.5 if None.  Rows ordered (L, chunk) as ``recurrent_generator``
     yields them are this layout: ``q.view(L, chunks, H, dk)``.  States, decays and all sums are float32 (the decays' prefix sums float64).
     Differentiable in q, k, v, log_decay and state, once."""
+    _seen_by_torch('memory_chunk', q, k, v, log_decay, state)
     if q.dim() != 4 or v.dim() != 4:
         _refuse('memory_chunk: q, k (L, B, H, dk) and v (L, B, H, dv), got %s, %s', tuple(q.shape), tuple(v.shape))
     if q.shape[0] == 0 or q.shape[1] == 0:
@@ -191,6 +207,7 @@ def memory_chunk(q, k, v, log_decay, state=None, masks=None, scale=None):
 def memory_chunk_backward(q, k, v, log_decay, d_out, d_state=None, state=None, masks=None, scale=None):
     """The gradients of ``memory_chunk`` as a plain call: (dq, dk, dv, d_log_decay, d_state0) from d_out (L, B, H, dv) and the gradient of the last
     state (None: zeros)."""
+    _seen_by_torch('memory_chunk_backward', q, k, v, log_decay, d_out, d_state, state)
     m, keep = _memory_args('memory_chunk_backward', q, k, v, log_decay, state, masks, scale, 2)
     if m.L == 0 or m.B == 0:
         _refuse('memory_chunk_backward: no tokens')
@@ -206,6 +223,7 @@ def memory_step(q, k, v, log_decay, state, masks=None, scale=None, out_state=Non
     """``memory_chunk`` for one token per sequence, as an env step of the rollout takes it: ``(out, out_state)``.  q, k (B, H, dk), v (B, H, dv), log_decay
     (H,) or (B, H), masks B entries, state None or float32 with B H dk dv entries.  out_state: where the new state goes (float32, contiguous; the buffer's next slot, or ``state``
     itself), a new (B, H, dk, dv) tensor if None; to autograd it is written in place.  No gradient: refused where one would be recorded."""
+    _seen_by_torch('memory_step', q, k, v, log_decay, state)
     if _wants_grad(q, k, v, log_decay, state):
         _refuse('memory_step records no gradient: call it under torch.no_grad(), or use memory_chunk')
     m, keep = _memory_args('memory_step', q, k, v, log_decay, state, masks, scale, 1)
@@ -307,6 +325,8 @@ def block_norm(x, branch=None, gate=None, scale=None, post_weight=None, post_bia
     biases: float32 (D,).  Whatever is None is left out (factor 1, bias 0).  Without a branch y is x and h = n(x) pre_weight + pre_bias: the first
     block's start; ``post_norm=False`` takes the branch as it is, ``pre_norm=False`` returns h = None: the last block's end.  h is formed from y before its
     rounding.  Differentiable in all tensors, once; nothing but the inputs is kept for the backward pass."""
+    weights = (scale, post_weight, post_bias, pre_weight, pre_bias)
+    _seen_by_torch('block_norm', x, branch, gate, *weights)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
         _refuse('block_norm: the last axis must hold 1..8192 elements, got %s', tuple(x.shape))
     if not isinstance(groups, int) or not 1 <= groups <= 256 or x.shape[-1] % groups:
@@ -325,7 +345,6 @@ def block_norm(x, branch=None, gate=None, scale=None, post_weight=None, post_bia
         _refuse('block_norm: without a branch and without pre_norm there is nothing to do')
     if not eps >= 0:
         _refuse('block_norm: eps must not be negative, got %r', eps)
-    weights = (scale, post_weight, post_bias, pre_weight, pre_bias)
     options = (groups, int(kind == 'layer'), int(gate_act == 'silu'), int(bool(post_norm)), int(bool(pre_norm)), eps)
     if _wants_grad(x, branch, gate, *weights):
         y, h = _BlockNorm.apply(x, branch, gate, *weights, options)
@@ -415,6 +434,7 @@ def action_log_probs(features, weight, bias, actions, available_actions=None):
     -inf, one that does not exist (>= V) NaN (and no gradient).  The logits are never stored: for many actions the softmax runs over pieces of them, and they
     are formed again for the gradient.  Differentiable in features, weight and bias, once.  Half precision operands: products are exact, sums float32; the
     gradient's dz is rounded to the operands' type before its two products."""
+    _seen_by_torch('action_log_probs', features, weight, bias)
     if weight.dim() != 2 or features.dim() < 1 or features.shape[-1] != weight.shape[1] or not 1 <= weight.shape[1] <= 16384 or not 1 <= weight.shape[0] <= 1 << 20:
         _refuse('action_log_probs: features (..., K) and weight (V, K) with K in 1..16384, V in 1..1048576, got %s, %s', tuple(features.shape), tuple(weight.shape))
     if bias is not None and bias.dtype != _F32:
