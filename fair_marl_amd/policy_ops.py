@@ -10,9 +10,10 @@
 All run on the current stream of their tensors' device, take any strides as long as the last axis is contiguous (a tensor whose last axis is
 not is copied), read nothing back and are capturable in a graph.  Gradients come through torch.autograd; ``memory_chunk_backward`` is the
 same gradient as a plain call, for a step that is captured without an autograd graph.  There is no CPU form: tensors off the GPU are refused.  So are
-forward-mode tangents, and calls under a tracer (torch.jit.trace, make_fx), which would keep nothing of them.
+forward-mode tangents, and calls under a tracer (torch.jit.trace, make_fx), which would keep nothing of them; torch.compile runs them between its graphs.
 """
 import ctypes as C
+import functools
 
 import torch
 from torch.autograd import forward_ad
@@ -30,7 +31,7 @@ def _refuse(text, *args):
     raise ValueError(text % args if args else text)
 
 
-_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_tracing, _dispatch_mode, _PROXY, _compiling = torch._C._get_tracing_state, torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY, torch.compiler.is_compiling
 
 
 def _seen_by_torch(op, *tensors):
@@ -39,8 +40,16 @@ def _seen_by_torch(op, *tensors):
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 _refuse('%s: no forward-mode derivative', op)
-    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
+    if _tracing() is not None or _dispatch_mode(_PROXY) is not None:
         _refuse('%s: cannot be traced', op)
+
+
+def _uncompiled(op):
+    """op as torch.compile has to call it: as it is, between two graphs (what it does with the C-ABI's structures is not what a compiler takes it for)."""
+    @functools.wraps(op)
+    def call(*args, **kwargs):
+        return (torch.compiler.disable(op) if _compiling() else op)(*args, **kwargs)
+    return call
 
 
 def _same_device(op, first, *rest):
@@ -180,6 +189,7 @@ class _MemoryChunk(torch.autograd.Function):
         return dq, dk, dv, dg, None if state is None else ds.view(ctx.state_shape), None, None
 
 
+@_uncompiled
 def memory_chunk(q, k, v, log_decay, state=None, masks=None, scale=None):
     """Linear attention with a decay per head over L tokens of B sequences: ``(out, last_state)``.
 
@@ -204,6 +214,7 @@ def memory_chunk(q, k, v, log_decay, state=None, masks=None, scale=None):
     return _MemoryChunk.apply(q, k, v, log_decay, state, masks, scale)
 
 
+@_uncompiled
 def memory_chunk_backward(q, k, v, log_decay, d_out, d_state=None, state=None, masks=None, scale=None):
     """The gradients of ``memory_chunk`` as a plain call: (dq, dk, dv, d_log_decay, d_state0) from d_out (L, B, H, dv) and the gradient of the last
     state (None: zeros)."""
@@ -219,6 +230,7 @@ def memory_chunk_backward(q, k, v, log_decay, d_out, d_state=None, state=None, m
     return _launch_chunk_backward(m, keep, d_out, d_state)
 
 
+@_uncompiled
 def memory_step(q, k, v, log_decay, state, masks=None, scale=None, out_state=None):
     """``memory_chunk`` for one token per sequence, as an env step of the rollout takes it: ``(out, out_state)``.  q, k (B, H, dk), v (B, H, dv), log_decay
     (H,) or (B, H), masks B entries, state None or float32 with B H dk dv entries.  out_state: where the new state goes (float32, contiguous; the buffer's next slot, or ``state``
@@ -313,6 +325,7 @@ class _BlockNorm(torch.autograd.Function):
         return (dx, dbranch, dgate, *dw, None)
 
 
+@_uncompiled
 def block_norm(x, branch=None, gate=None, scale=None, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, groups=1, kind='rms',
                gate_act='sigmoid', post_norm=True, pre_norm=True, eps=1e-5):
     """The end of a residual block and the start of the next one in one pass: ``(y, h)``.
@@ -423,6 +436,7 @@ class _ActionLogProbs(torch.autograd.Function):
         return dx, dw, db, None, None
 
 
+@_uncompiled
 def action_log_probs(features, weight, bias, actions, available_actions=None):
     """Log-probability and entropy of discrete actions: ``(log_probs, entropy)``, float32, of the features' leading shape.
 
