@@ -123,7 +123,7 @@ __device__ __forceinline__ void row_means(const Block &a, float (&v)[NV][4], flo
 
 // n (in place) and 1 / sqrt(..) of the groups of o; two passes over the registers where the mean is taken off first
 template <int TL, int NV>
-__device__ __forceinline__ void norm_groups(const Block &a, float (&o)[NV][4], float (&inv)[NV][4], int l, Exchange &x) {
+__device__ __forceinline__ void norm_groups(const Block &a, float eps, float (&o)[NV][4], float (&inv)[NV][4], int l, Exchange &x) {
     if (a.layer) {
         FMARL_EACH(inv[n][r] = o[n][r])
         group_means<TL, NV>(a, inv, l, x);
@@ -131,11 +131,11 @@ __device__ __forceinline__ void norm_groups(const Block &a, float (&o)[NV][4], f
     }
     FMARL_EACH(inv[n][r] = o[n][r] * o[n][r])
     group_means<TL, NV>(a, inv, l, x);
-    FMARL_EACH(inv[n][r] = rsqrtf(inv[n][r] + a.eps); o[n][r] *= inv[n][r])
+    FMARL_EACH(inv[n][r] = rsqrtf(inv[n][r] + eps); o[n][r] *= inv[n][r])
 }
 
 template <int TL, int NV>
-__device__ __forceinline__ float norm_row(const Block &a, float (&y)[NV][4], int l, Exchange &x) {
+__device__ __forceinline__ float norm_row(const Block &a, float eps, float (&y)[NV][4], int l, Exchange &x) {
     float mean;
     if (a.layer) {
         row_means<TL, NV>(a, y, mean, x);
@@ -143,7 +143,7 @@ __device__ __forceinline__ float norm_row(const Block &a, float (&y)[NV][4], int
     }
     float s = 0.f;
     FMARL_EACH(s += y[n][r] * y[n][r])
-    const float inv = rsqrtf(team_sum<TL>(s, x) * (1.f / a.dim) + a.eps);
+    const float inv = rsqrtf(team_sum<TL>(s, x) * (1.f / a.dim) + eps);
     FMARL_EACH(y[n][r] *= inv)
     return inv;
 }
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(Block a) {
         if (a.branch) {
             if (a.post_norm) {
                 float inv[NV][4];
-                norm_groups<TL, NV>(a, o, inv, l, ex);
+                norm_groups<TL, NV>(a, a.eps, o, inv, l, ex);
                 FMARL_EACH(o[n][r] = o[n][r] * pw[n][r] + pb[n][r])
             }
             if (a.gate) FMARL_EACH(const float s = sigmoid(g[n][r]); o[n][r] *= a.silu ? g[n][r] * s : s)
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(Block a) {
             store_row<TX, TL, NV, VEC>(a, y, a.y, row, l);
         }
         if (a.h) {
-            norm_row<TL, NV>(a, y, l, ex);
+            norm_row<TL, NV>(a, a.eps, y, l, ex);
             FMARL_EACH(y[n][r] = y[n][r] * rw[n][r] + rb[n][r])
             store_row<TB, TL, NV, VEC>(a, y, a.h, row, l);
         }
@@ -269,18 +269,19 @@ __global__ __launch_bounds__(THREADS, NV == 1 && sizeof(TX) == 2 ? 4 : 1) void b
     fetch((int64_t)blockIdx.x * kTeams + team);
     for (int64_t row0 = (int64_t)blockIdx.x * kTeams; row0 < a.rows; row0 += step) {
         const int64_t row = row0 + team;
+        const float eps = row < a.rows ? a.eps : 1.f;   // a row of zeros beyond the last one adds nothing to the sums, nor where eps is 0 (1 / sqrt(0) times 0 would be NaN)
         float y[NV][4], u[NV][4], g[NV][4], inv[NV][4], d[NV][4], dh[NV][4];
         widen_row<TL, VEC>(a, y, nx, l); widen_row<TL, VEC>(a, u, no, l); widen_row<TL, VEC>(a, g, ng, l); widen_row<TL, VEC>(a, d, nd, l); widen_row<TL, VEC>(a, dh, nh, l);
         fetch(row + step);
         // forward again: u = n(branch) from here on, y unrounded
         if (a.branch) {
-            if (a.post_norm) norm_groups<TL, NV>(a, u, inv, l, ex);
+            if (a.post_norm) norm_groups<TL, NV>(a, eps, u, inv, l, ex);
             FMARL_EACH(const float s = a.gate ? sigmoid(g[n][r]) : 1.f;
                        const float f = a.gate && a.silu ? g[n][r] * s : s;
                        y[n][r] = in ? y[n][r] + sc[n][r] * (u[n][r] * pw[n][r] + pb[n][r]) * f : 0.f)
         }
         if (a.pre_norm && a.dh) {
-            const float yi = norm_row<TL, NV>(a, y, l, ex);   // y: its norm from here on
+            const float yi = norm_row<TL, NV>(a, eps, y, l, ex);   // y: its norm from here on
             float m1 = 0.f, m2 = 0.f;
             FMARL_EACH(acc[3][n][r] += dh[n][r] * y[n][r]; acc[4][n][r] += dh[n][r]; dh[n][r] *= rw[n][r];
                        m1 += dh[n][r]; m2 += dh[n][r] * y[n][r])
