@@ -627,7 +627,7 @@ struct ShortGrad {
     const float *masks; int64_t ml, mb;
     const float *state, *d_state;
     float *d_state0, *dg;            // NULL: not wanted
-    double *partial;                 // (B, H) sums of dg, or NULL
+    double *partial;                 // (B, H) sums of dg; NULL: dg is not wanted
     int64_t B;
     int L, H, dk_dim, dv_dim, wide;  // wide: states are read and written in float4s
     float scale;
@@ -766,7 +766,7 @@ struct DecayGrad {
     const float *g; int64_t gl, gb, gh;
     const float *masks; int64_t ml, mb;
     float *dg;                       // (L, B, H) or NULL
-    double *partial;                 // (B, H): sums over the tokens, or NULL
+    double *partial;                 // (B, H): sums over the tokens
     int64_t L, B;
     int H, elems, slices, team, vec;   // vec: both states on 16 bytes, elems a multiple of four
 };
@@ -817,7 +817,7 @@ __global__ __launch_bounds__(256) void decay_grad_short_kernel(DecayGrad a) {
                 run -= step[i];
             }
     }
-    if (a.partial) a.partial[bh] = sum;
+    a.partial[bh] = sum;
 }
 
 __global__ __launch_bounds__(1024) void decay_grad_long_kernel(DecayGrad a) {
@@ -885,10 +885,161 @@ __global__ __launch_bounds__(1024) void decay_grad_long_kernel(DecayGrad a) {
     for (int off = 32; off; off >>= 1) sum += __shfl_down(sum, off);
     if (lane == 0) sums[wave] = sum;
     __syncthreads();
-    if (tid == 0 && a.partial) {
+    if (tid == 0) {
         double s = 0.0;
         for (int w = 0; w < waves; ++w) s += sums[w];
         a.partial[bh] = s;
+    }
+}
+
+// The running difference does not come back from an infinity or a NaN: one in q or d_out reaches the gradients behind it, one in k or v (in the short kernel, which runs backwards)
+// those before it, where the definition has numbers.  A head whose sum is not finite is formed again from the definition, an episode at a time: backwards the gradient of the
+// state, G, down to the token whose G_t is not finite (all before it are not either); at the token behind that one -- or at the episode's start --
+// dg_t = r_t e^{g_t} <S_{t-1}, G_t> itself, with the state walked there forwards, and the running difference on from it up to the first S_t that is not finite.  The tokens outside have
+// no finite gradient.  A workgroup takes its share of the heads and passes over those with finite sums: 5 us of a backward pass where all are (chunks of ten tokens 320 -> 326 us, 4 096
+// tokens 332 -> 337).  States in LDS: in registers they spilled, and the launch alone cost 17 to 36 us.
+struct DecayAgain {
+    WalkRows q, k, v, o;
+    const float *g; int64_t gl, gb, gh;
+    const float *masks; int64_t ml, mb;
+    const float *state, *d_state;           // NULL: zeros
+    float *dg;                              // (L, B, H) or NULL
+    double *partial;                        // (B, H)
+    float *behind; int64_t b_sl, b_sh;      // room for L floats of each (b, h); NULL: up to 16 tokens
+    int64_t L, B;
+    int H, dk, dv;
+    float scale;
+};
+
+__device__ __forceinline__ bool not_finite(float v) { return !(v - v == 0.f); }
+
+template <typename T>
+__global__ __launch_bounds__(1024) void decay_again_kernel(DecayAgain a) {
+    extern __shared__ __align__(16) char smem[];
+    __shared__ double sums[2][16];
+    __shared__ float few[16];
+    __shared__ int flags[1024], start;
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, elems = a.dk * a.dv;
+    float *G = (float *)smem, *S = G + elems;   // (a thread reads and writes its own entries only)
+    const int64_t heads = a.B * a.H, first = heads * blockIdx.x / gridDim.x, end = heads * (blockIdx.x + 1) / gridDim.x;
+    int flip = 0;
+    auto total = [&](double v) {                // over the workgroup; two places in turn: one barrier
+        for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
+        flip ^= 1;
+        if (lane == 0) sums[flip][wave] = v;
+        __syncthreads();
+        v = 0.0;
+        for (int w = 0; w < threads >> 6; ++w) v += sums[flip][w];
+        return v;
+    };
+    for (int64_t base = first; base < end; base += threads) {
+        const int count = (int)min((int64_t)threads, end - base);
+        const double s = tid < count ? a.partial[base + tid] : 0.0;
+        flags[tid] = !(s - s == 0.0);
+        if (!__syncthreads_or(flags[tid])) continue;
+        for (int j = 0; j < count; ++j) {
+            if (!flags[j]) continue;
+            const int64_t bh = base + j, b = bh / a.H;
+            const int h = (int)(bh - b * a.H);
+            const float *pg = a.g + b * a.gb + h * a.gh, *pm = a.masks ? a.masks + b * a.mb : nullptr;
+            const T *pq = (const T *)a.q.p + b * a.q.sb + h * a.q.sh, *pk = (const T *)a.k.p + b * a.k.sb + h * a.k.sh;
+            const T *pv = (const T *)a.v.p + b * a.v.sb + h * a.v.sh, *po = (const T *)a.o.p + b * a.o.sb + h * a.o.sh;
+            float *behind = a.behind ? a.behind + bh * a.b_sh : few;
+            const int64_t b_sl = a.behind ? a.b_sl : 1;
+            auto fresh = [&](int64_t t) { return forgets(pg[t * a.gl], pm ? pm[t * a.ml] : 1.f); };
+            auto decay = [&](int64_t t) { return exp2_fast((float)((double)pg[t * a.gl] * 1.4426950408889634074)); };
+            double sum = 0.0;                   // (thread 0)
+            for (int64_t e1 = a.L, e0; e1 > 0; e1 = e0) {
+                int bad = 0;
+                for (int e = tid; e < elems; e += threads) {
+                    G[e] = e1 == a.L && a.d_state ? a.d_state[bh * elems + e] : 0.f;
+                    bad |= not_finite(G[e]);
+                }
+                int64_t from = e1;              // the first token whose G_t is finite, as far as they are walked
+                e0 = e1 - 1;
+                bool dead = __syncthreads_or(bad);
+                for (; !dead; --e0) {
+                    const T *q = pq + e0 * a.q.sl, *k = pk + e0 * a.k.sl, *v = pv + e0 * a.v.sl, *o = po + e0 * a.o.sl;
+                    double x = 0.0;
+                    bad = 0;
+                    for (int e = tid; e < elems; e += threads) {
+                        const int y = e / a.dv, z = e - y * a.dv;
+                        x += (double)((float)k[y] * (float)v[z]) * G[e];
+                        bad |= not_finite(G[e] + a.scale * (float)q[y] * (float)o[z]);
+                    }
+                    x = total(x);
+                    if (tid == 0) behind[e0 * b_sl] = (float)x;
+                    dead = __syncthreads_or(bad);
+                    if (dead) break;            // G: what the token behind passes on
+                    from = e0;
+                    const bool starts = fresh(e0);
+                    const float d = starts ? 0.f : decay(e0);
+                    for (int e = tid; e < elems; e += threads) {
+                        const int y = e / a.dv, z = e - y * a.dv;
+                        G[e] = starts ? 0.f : (G[e] + a.scale * (float)q[y] * (float)o[z]) * d;
+                    }
+                    if (starts || e0 == 0) break;
+                }
+                if (dead) {                     // the episode's start, as many tokens at a time as there are threads
+                    for (;; e0 -= threads) {
+                        if (tid == 0) start = -1;
+                        __syncthreads();
+                        const int64_t t = e0 - tid;
+                        if (t >= 0 && (t == 0 || fresh(t))) atomicMax(&start, threads - 1 - tid);
+                        __syncthreads();
+                        const int found = start;
+                        __syncthreads();
+                        if (found >= 0) { e0 -= threads - 1 - found; break; }
+                    }
+                }
+                const bool starts = fresh(e0);
+                if (from == e1) {               // no finite gradient in it but a start's
+                    const float nan = __builtin_nanf("");
+                    if (a.dg) for (int64_t t = e0 + tid; t < e1; t += threads) a.dg[t * heads + bh] = t == e0 && starts ? 0.f : nan;
+                    if (!starts || e1 - e0 > 1) sum += nan;
+                    continue;
+                }
+                bad = 0;
+                for (int e = tid; e < elems; e += threads) {
+                    S[e] = !starts && a.state ? a.state[bh * elems + e] : 0.f;
+                    bad |= not_finite(S[e]);
+                }
+                bool lost = __syncthreads_or(bad);
+                double run = 0.0;
+                for (int64_t t = e0; t < e1; ++t) {
+                    const bool afresh = starts && t == e0, there = t >= from && !lost;
+                    if (there && t == from && !afresh) {
+                        double x = 0.0;
+                        for (int e = tid; e < elems; e += threads) x += (double)S[e] * G[e];
+                        run = total(x);
+                    }
+                    const double dg = afresh ? 0.0 : there ? run : (double)__builtin_nanf("");
+                    if (tid == 0) {
+                        if (a.dg) a.dg[t * heads + bh] = (float)dg;
+                        sum += dg;
+                    }
+                    if (lost) continue;
+                    const T *q = pq + t * a.q.sl, *k = pk + t * a.k.sl, *v = pv + t * a.v.sl, *o = po + t * a.o.sl;
+                    const float d = afresh ? 0.f : decay(t);
+                    double x = 0.0;
+                    bad = 0;
+                    for (int e = tid; e < elems; e += threads) {
+                        const int y = e / a.dv, z = e - y * a.dv;
+                        const float c = S[e] * d;
+                        if (there && !afresh) x += (double)(a.scale * (float)q[y] * (float)o[z]) * c;
+                        S[e] = c + (float)k[y] * (float)v[z];
+                        bad |= not_finite(S[e]);
+                    }
+                    if (there) {
+                        x = total(x);
+                        if (tid == 0) run -= x - (double)behind[t * b_sl];
+                    }
+                    lost = __syncthreads_or(bad);
+                }
+            }
+            if (tid == 0) a.partial[bh] = sum;
+        }
+        __syncthreads();
     }
 }
 
@@ -1058,6 +1209,30 @@ Segments memory_segments(const FmarlMemory *m) {
         if (s.nseg > best.nseg) best = s;
     }
     return best;
+}
+
+template <typename T>
+int launch_again(const DecayAgain &a, hipStream_t st) {
+    const int64_t heads = a.B * a.H;
+    const int elems = a.dk * a.dv, threads = elems > 960 ? 1024 : (elems + 63) / 64 * 64, lds = 8 * elems;   // a state entry a thread, up to 1 024
+    if (lds > 48 * 1024) HIP_OK(hipFuncSetAttribute((const void *)decay_again_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL(decay_again_kernel<T>, dim3((unsigned)(heads < 512 ? heads : 512)), dim3(threads), lds, st, a);
+    return FMARL_OK;
+}
+
+// the decay's gradient again for heads that hold what is not finite, and its sums over the batch
+int finish_decay(const FmarlMemory *m, const FmarlRows &d_out, const float *d_state, float *d_log_decay, double *partial, float *behind, int64_t b_sl, int64_t b_sh, hipStream_t st) {
+    DecayAgain a = {};
+    const int dt = m->dtype;
+    a.q = walk_rows(m->q, m->dk, dt); a.k = walk_rows(m->k, m->dk, dt); a.v = walk_rows(m->v, m->dv, dt); a.o = walk_rows(d_out, m->dv, dt);
+    a.g = m->log_decay; a.gl = m->decay_stride_l; a.gb = m->decay_stride_b; a.gh = m->decay_stride_h; a.masks = m->masks; a.ml = m->mask_stride_l; a.mb = m->mask_stride_b;
+    a.state = m->state; a.d_state = d_state; a.dg = m->shared_decay ? nullptr : d_log_decay; a.partial = partial; a.behind = behind; a.b_sl = b_sl; a.b_sh = b_sh;
+    a.L = m->L; a.B = m->B; a.H = m->H; a.dk = m->dk; a.dv = m->dv; a.scale = m->scale;
+    const int rc = dt == FMARL_T_F32 ? launch_again<float>(a, st) : dt == FMARL_T_BF16 ? launch_again<__bf16>(a, st) : launch_again<_Float16>(a, st);
+    if (rc) return rc;
+    if (m->shared_decay) hipLaunchKernelGGL(decay_sum_kernel, dim3((unsigned)m->H), dim3(256), 0, st, (const double *)partial, d_log_decay, m->B, m->H);
+    HIP_OK(hipGetLastError());
+    return FMARL_OK;
 }
 
 // columns of z that a wave of the small heads' kernel takes: 16; the large heads' workgroup takes them all
@@ -1261,16 +1436,15 @@ int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, co
         g.dq = walk_rows(*d_q, m->dk, dt); g.dk = walk_rows(*d_k, m->dk, dt); g.dv = walk_rows(*d_v, m->dv, dt);
         g.g = w0.g; g.gl = w0.gl; g.gb = w0.gb; g.gh = w0.gh; g.masks = w0.masks; g.ml = w0.ml; g.mb = w0.mb;
         g.state = m->state; g.d_state = d_state; g.d_state0 = d_state0; g.dg = m->shared_decay ? nullptr : d_log_decay;
-        g.partial = m->shared_decay && d_log_decay ? (double *)(base + ws.partial) : nullptr;
+        g.partial = d_log_decay ? (double *)(base + ws.partial) : nullptr;
         g.B = m->B; g.L = (int)m->L; g.H = m->H; g.dk_dim = m->dk; g.dv_dim = m->dv; g.scale = m->scale;
         g.wide = (m->dv & 3) == 0 && (((uintptr_t)m->state | (uintptr_t)d_state | (uintptr_t)d_state0) & 15) == 0;
         const dim3 grid((unsigned)((heads + 15) / 16));
         if (dt == FMARL_T_F32) hipLaunchKernelGGL(memory_short_backward_kernel<float>, grid, dim3(256), 0, st, g);
         else if (dt == FMARL_T_BF16) hipLaunchKernelGGL(memory_short_backward_kernel<__bf16>, grid, dim3(256), 0, st, g);
         else hipLaunchKernelGGL(memory_short_backward_kernel<_Float16>, grid, dim3(256), 0, st, g);
-        if (g.partial) hipLaunchKernelGGL(decay_sum_kernel, dim3((unsigned)m->H), dim3(256), 0, st, (const double *)g.partial, d_log_decay, m->B, m->H);
         HIP_OK(hipGetLastError());
-        return FMARL_OK;
+        return d_log_decay ? finish_decay(m, *d_out, d_state, d_log_decay, g.partial, nullptr, 0, 0, st) : FMARL_OK;
     }
     const int elems = m->dk * m->dv;
     float *seg_s = (float *)(base + ws.seg_s), *seg_g = (float *)(base + ws.seg_g), *decay = (float *)(base + ws.decay);
@@ -1303,10 +1477,9 @@ int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, co
     if (int rc = launch_walk(w, dt, st)) return rc;
     if (d_log_decay) {
         DecayGrad g = {};
-        const bool shared = m->shared_decay != 0;
         g.dot_q = (const float *)(base + ws.dot_q); g.dot_k = (const float *)(base + ws.dot_k);
         g.state = m->state; g.d_state = ds0; g.g = w0.g; g.gl = w0.gl; g.gb = w0.gb; g.gh = w0.gh; g.masks = w0.masks; g.ml = w0.ml; g.mb = w0.mb;
-        g.dg = shared ? nullptr : d_log_decay; g.partial = shared ? (double *)(base + ws.partial) : nullptr;
+        g.dg = m->shared_decay ? nullptr : d_log_decay; g.partial = (double *)(base + ws.partial);
         g.L = m->L; g.B = m->B; g.H = m->H; g.elems = elems; g.slices = slices_of(m, m->dv, m->dk);
         g.dot_sl = w0.dot_sl; g.dot_sh = w0.dot_sh;
         g.vec = (elems & 3) == 0 && (((uintptr_t)g.state | (uintptr_t)g.d_state) & 15) == 0;
@@ -1316,8 +1489,8 @@ int fmarl_memory_chunk_backward(const FmarlMemory *m, const FmarlRows *d_out, co
             const int64_t most = m->L / 4 > elems / 16 ? m->L / 4 : elems / 16;   // four tokens and 16 state entries a thread, up to 1 024 threads
             hipLaunchKernelGGL(decay_grad_long_kernel, dim3((unsigned)heads), dim3(most > 1024 ? 1024 : (int)(most + 63) / 64 * 64), 0, st, g);
         }
-        if (shared) hipLaunchKernelGGL(decay_sum_kernel, dim3((unsigned)m->H), dim3(256), 0, st, (const double *)(base + ws.partial), d_log_decay, m->B, m->H);
         HIP_OK(hipGetLastError());
+        return finish_decay(m, *d_out, d_state, d_log_decay, g.partial, (float *)(base + ws.dot_k), w0.dot_sl, w0.dot_sh, st);   // (the sums of dk are read by then)
     }
     return FMARL_OK;
 }

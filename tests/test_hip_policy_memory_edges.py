@@ -1,0 +1,60 @@
+"""-m gpu: the policy's memory where one form of its kernels ends and the next begins, with values that cancel, overflow or are no numbers.  The recurrence in float64 and the
+bounds are those of test_hip_policy_memory.py."""
+import math
+
+import pytest
+import torch
+
+import fair_marl_amd as fm
+from test_hip_policy_memory import BF16, DEV, F16, F32, close, compare, make, recurrence, step_of
+
+pytestmark = pytest.mark.gpu
+
+
+SHAPES = [(12, 2, 2, 16, 16), (16, 5, 1, 5, 7), (40, 2, 1, 5, 7), (30, 2, 2, 100, 12), (90, 2, 2, 40, 24), (700, 1, 1, 16, 16), (700, 1, 2, 64, 64), (300, 1, 1, 128, 100)]
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('bad', [math.nan, math.inf])
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+def test_the_decays_gradient_next_to_what_is_no_number(shape, bad, dtype):
+    """dg_t = r_t e^{g_t} <S_{t-1}, G_t>: what is not finite in k or v reaches the tokens behind it, in q or d_out those before it, and none of another episode; between the two,
+    and beside a start, the gradient is finite"""
+    L, B, H, dk, dv = shape
+    for at, what in enumerate(('d_out', 'k', 'd_out, then v', 'q at a start', 'k, then d_out', 'states')):
+        q, k, v, g, S, masks, do, dS = make(*shape, dtype, 'token', seed=50 + at)
+        clean = [t.clone() for t in (q, k, v, g, S, masks, do, dS)]
+        e0, s1, s2, e1 = L // 6, L // 3, L // 3 + max(2, L // 4), L - L // 6    # an episode and two of its tokens
+        masks.fill_(1)
+        masks[e0, 0] = masks[e1, 0] = 0
+        if what.startswith('d_out'):
+            do[s1, 0, :, dv // 2] = bad
+        if what == 'k':
+            k[s2, 0, 0] = bad
+        if what == 'd_out, then v':
+            v[s2, 0, :, 0] = bad
+        if what == 'q at a start':
+            q[e0, 0, :, dk - 1] = bad
+        if what == 'k, then d_out':
+            k[s1, 0, :, 0], do[s2, 0, :, 0] = bad, bad
+        if what == 'states':
+            S[0, 0], dS[0, H - 1, 0, 0] = bad, bad
+        got = fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks)
+        shared = fm.memory_chunk_backward(q, k, v, g[0, 0].contiguous(), do, dS, S, masks)[3]
+        wide = [t.double() for t in (q, k, v)]
+        want = recurrence(*wide, g.double(), S.double(), masks == 0, dk ** -0.5, do.double(), dS.double())[5]
+        cq, ck, cv, _, cS, _, cdo, cdS = [t.double().abs() for t in clean]
+        mag = recurrence(cq, ck, cv, g.double(), cS, masks == 0, dk ** -0.5, cdo, cdS)
+        gamma = (2 * L + dk + dv + 200) * 2.0 ** -24
+        add = (cq * mag[2]).sum(-1) + (ck * mag[3]).sum(-1)
+        bound = gamma * ((cS * mag[6]).sum((-1, -2)) + torch.cumsum(add, 0))
+        fine = torch.isfinite(want)
+        assert bool((~fine).any()) or what == 'q at a start'
+        assert torch.equal(torch.isfinite(got[3]), fine), what
+        close(torch.where(fine, got[3], 0.0), torch.where(fine, want, 0.0), torch.where(fine, bound + want.abs() * 2.0 ** -24, 0.0), what)
+        head = recurrence(*wide, g[0, 0].double().expand(L, B, H), S.double(), masks == 0, dk ** -0.5, do.double(), dS.double())[5].sum((0, 1))
+        assert torch.equal(torch.isfinite(shared), torch.isfinite(head)), what
+        if what == 'q at a start':
+            mag = recurrence(cq, ck, cv, g[0, 0].double().expand(L, B, H), cS, masks == 0, dk ** -0.5, cdo, cdS)
+            run = (cS * mag[6]).sum((-1, -2)) + torch.cumsum((cq * mag[2]).sum(-1) + (ck * mag[3]).sum(-1), 0)
+            close(shared, head, gamma * run.sum((0, 1)) + head.abs() * 2.0 ** -24, what)
