@@ -64,13 +64,17 @@ template <bool DOT> struct Pieces<__bf16, DOT> { static constexpr int in = 1, p 
 template <bool DOT> struct Pieces<_Float16, DOT> { static constexpr int in = 2, p = DOT ? 3 : 2, in_order = 2, out_order = DOT ? 2 : 1; };
 template <bool DOT> struct Pieces<float, DOT> { static constexpr int in = 3, p = 3, in_order = 2, out_order = 2; };
 
-// the pieces of four inputs, piece by piece; a bfloat16 value is its own
+// the pieces of four inputs, piece by piece; a bfloat16 value is its own.  What float32 holds beyond bfloat16's largest number (3.39e38) leaves a remainder, not an infinity: a type's
+// lowest value may stand where nothing is read
 template <typename T, int N> __device__ __forceinline__ void cut4(typename Vec4<T>::type v, bf16x4 (&p)[N]) {
     f32x4 f = widen(v);
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) { p[i][r] = (__bf16)f[r]; f[r] -= (float)p[i][r]; }
+        for (int r = 0; r < 4; ++r) {
+            p[i][r] = (__bf16)(N == 3 && i == 0 ? __builtin_amdgcn_fmed3f(f[r], -0x1.fep127f, 0x1.fep127f) : f[r]);
+            f[r] -= (float)p[i][r];
+        }
 }
 template <> __device__ __forceinline__ void cut4<__bf16, 1>(bf16x4 v, bf16x4 (&p)[1]) { p[0] = v; }
 
@@ -372,9 +376,9 @@ __global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory
                 const f32x4 u0 = *(const f32x4 *)(lwout + g4), u1 = *(const f32x4 *)(lwout + 16 + g4);
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
-                    float v = (float)zt[0][r];
+                    float v = (float)zt[NP - 1][r];   // (the small ones first: exact, and no infinity on the way)
 #pragma unroll
-                    for (int i = 1; i < NP; ++i) v += (float)zt[i][r];
+                    for (int i = NP - 2; i >= 0; --i) v += (float)zt[i][r];
                     v *= r < 4 ? u0[r & 3] : u1[r & 3];
 #pragma unroll
                     for (int i = 0; i < 3; ++i) { uz[i][r] = (__bf16)v; v -= (float)uz[i][r]; }

@@ -58,3 +58,36 @@ def test_the_decays_gradient_next_to_what_is_no_number(shape, bad, dtype):
             mag = recurrence(cq, ck, cv, g[0, 0].double().expand(L, B, H), cS, masks == 0, dk ** -0.5, cdo, cdS)
             run = (cS * mag[6]).sum((-1, -2)) + torch.cumsum((cq * mag[2]).sum(-1) + (ck * mag[3]).sum(-1), 0)
             close(shared, head, gamma * run.sum((0, 1)) + head.abs() * 2.0 ** -24, what)
+
+
+@pytest.mark.parametrize('value', [torch.finfo(F32).min, torch.finfo(F32).max])
+@pytest.mark.parametrize('shape', [(10, 3, 2, 16, 16), (40, 2, 1, 64, 64), (40, 2, 1, 16, 100), (300, 1, 2, 100, 40)], ids=str)
+def test_the_types_lowest_value_in_another_episode(shape, value):
+    """padding of float32's lowest or largest value before an episode's start, in q, k, v and d_out: nothing of it behind the start, nor before it backwards"""
+    L, B, H, dk, dv = shape
+    q, k, v, g, S, masks, do, dS = make(*shape, F32, 'token', seed=62)
+    masks.fill_(1)
+    then = L // 2
+    masks[then] = 0
+    clean = [t.clone() for t in (q, k, v, do)]
+    for t in (q, k, v, do):
+        t[then - 2] = value
+    out, last = fm.memory_chunk(q, k, v, g, S, masks)
+    grads = fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks)
+    cq, ck, cv, cdo = [t.double() for t in clean]
+    args = g.double(), S.double(), masks == 0, dk ** -0.5
+    want = recurrence(cq, ck, cv, *args, cdo, dS.double())
+    mag = recurrence(cq.abs(), ck.abs(), cv.abs(), g.double(), S.double().abs(), masks == 0, dk ** -0.5, cdo.abs(), dS.double().abs())
+    gamma = (2 * L + dk + dv + 200) * 2.0 ** -24
+    for name, a, i in (('out', out, 0), ('dq', grads[0], 2), ('dk', grads[1], 3), ('dv', grads[2], 4)):
+        close(a[then:], want[i][then:], gamma * mag[i][then:] + step_of(a, want[i][then:]), name)
+    close(last, want[1], gamma * mag[1] + step_of(last, want[1]), 'state')
+    # the other way round: in the later episode, nothing of it before the start
+    q, k, v, do = (t.float() for t in clean)
+    for t in (q, k, v, do):
+        t[then + 1] = value
+    out, _ = fm.memory_chunk(q, k, v, g, S, masks)
+    grads = fm.memory_chunk_backward(q, k, v, g, do, dS, S, masks)
+    for name, a, i in (('out', out, 0), ('dq', grads[0], 2), ('dk', grads[1], 3), ('dv', grads[2], 4)):
+        close(a[:then], want[i][:then], gamma * mag[i][:then] + step_of(a, want[i][:then]), name)
+    close(grads[4], want[6], gamma * mag[6] + step_of(grads[4], want[6]), 'dS0')
