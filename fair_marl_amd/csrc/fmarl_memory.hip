@@ -48,8 +48,8 @@ __device__ __forceinline__ bool forgets(float g, float mask) { return mask == 0.
 // mfma_f32_16x16x32_bf16: row 4 * (lane / 16) + r, column lane % 16), so a chunk is read once for all of it:
 //     P^T = y x^T, weighted (three 16 x 16 tiles, shared out over the waves);  out^T = z^T P^T + S^T x^T;  S = e^C S + y^T (u z).
 // All products are bfloat16 ones of exact pieces: a bfloat16 value is one piece, a float16 value two, a float32 value three (8 + 8 + 8 bits), and what is
-// formed in float32 (P, S, u z) is cut into two or three; products whose place is below 2^-24 of the result (2^-16 where the output has 8 or 11 bits) are left out.  Per
-// product of 16 x 16 x 32 that is 1 to 6 instructions of 16 cycles against eight of 32 cycles of mfma_f32_16x16x4f32.
+// formed in float32 (P, S, u z) is cut into three, whatever the output's type: terms that cancel leave what their last bits hold.  Products whose place is below 2^-24 of the result
+// are left out.  Per product of 16 x 16 x 32 that is 1 to 6 instructions of 16 cycles against eight of 32 cycles of mfma_f32_16x16x4f32.
 // The accumulator layout serves as either operand's layout if the contraction runs in the order 8 * (lane / 16) + 4 * tile + r for the index 16 * tile + 4 * (lane / 16) + r
 // (two tiles to a contraction of 32): rows in LDS are stored in that order, so every operand is one 16-byte read.
 // The decays' prefix sums are float64, so a weight e^{C_t - C_s} is right to float32 however fast the tokens before forgot.  A weight is selected, not multiplied to
@@ -57,12 +57,11 @@ __device__ __forceinline__ bool forgets(float g, float mask) { return mask == 0.
 // that it reaches later tokens only.
 // 64 heads of 4 096 tokens, 64 x 64, bfloat16 (segments of 256 tokens, four workgroups a CU): 33 us for the states alone, 48 us for out, 77 us for out with its sums against w, where the
 // bytes take 13 to 27 us and the matrix instructions 4 us: a chunk is three barriers and some 400 vector instructions a wave (pieces, weights, prefix sums), and those bound it.
-// pieces of an input (in), of P and the state as operands (p), highest order (sum of the pieces' numbers) kept in x y (in_order) and in out (out_order); u z has three pieces, kept to
-// order 2.  DOT: out is dotted with w before its rounding, for the decay's gradient, a difference of such sums: out to float32 there too.
-template <typename T, bool DOT> struct Pieces;
-template <bool DOT> struct Pieces<__bf16, DOT> { static constexpr int in = 1, p = DOT ? 3 : 2, in_order = 0, out_order = DOT ? 2 : 1; };
-template <bool DOT> struct Pieces<_Float16, DOT> { static constexpr int in = 2, p = DOT ? 3 : 2, in_order = 2, out_order = DOT ? 2 : 1; };
-template <bool DOT> struct Pieces<float, DOT> { static constexpr int in = 3, p = 3, in_order = 2, out_order = 2; };
+// pieces of an input, and the highest order (sum of the pieces' numbers) kept in x y; P, the state as an operand and u z have three pieces, kept to order 2
+template <typename T> struct Pieces;
+template <> struct Pieces<__bf16> { static constexpr int in = 1, in_order = 0; };
+template <> struct Pieces<_Float16> { static constexpr int in = 2, in_order = 2; };
+template <> struct Pieces<float> { static constexpr int in = 3, in_order = 2; };
 
 // the pieces of four inputs, piece by piece; a bfloat16 value is its own.  What float32 holds beyond bfloat16's largest number (3.39e38) leaves a remainder, not an infinity: a type's
 // lowest value may stand where nothing is read
@@ -115,8 +114,8 @@ __device__ __forceinline__ double scan32(double v, int lane) {
 }
 
 // LDS of a workgroup, in bytes: x, y (32 tokens), y^T, z^T (rows of 32 tokens), P^T, per-token floats
-template <typename T, bool DOT> __host__ __device__ constexpr int tiles_lds(int nk, int nz) {
-    return Pieces<T, DOT>::in * 2 * (2 * 32 * (32 * nk + 8) + (32 * nk + 16 * nz) * 40) + Pieces<T, DOT>::p * 2 * 32 * 40 + 32 * 8 + 4 * 32 * 4 + 8 * 32 * 4;
+template <typename T> __host__ __device__ constexpr int tiles_lds(int nk, int nz) {
+    return Pieces<T>::in * 2 * (2 * 32 * (32 * nk + 8) + (32 * nk + 16 * nz) * 40) + 3 * 2 * 32 * 40 + 32 * 8 + 4 * 32 * 4 + 8 * 32 * 4;
 }
 
 enum { kOut = 0, kOutDot = 1, kState = 2 };   // what a walk leaves: out; out and its dots with w; the state alone
@@ -124,8 +123,7 @@ enum { kOut = 0, kOutDot = 1, kState = 2 };   // what a walk leaves: out; out an
 template <typename T, int NK, int MODE, bool VEC>
 __global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory_tiles_kernel(Walk arg) {
     constexpr bool DOT = MODE == kOutDot, OUT = MODE != kState;
-    typedef Pieces<T, DOT> PC;
-    constexpr int NP = PC::in, PP = PC::p, XS = 32 * NK + 8;
+    constexpr int NP = Pieces<T>::in, PP = 3, XS = 32 * NK + 8;
     typedef typename Vec4<T>::type V;
     extern __shared__ __align__(16) char smem[];
     // the arguments are read where they are used, through a pointer the compiler cannot see through: all at once they do not fit the scalar registers (a hundred
@@ -298,7 +296,7 @@ __global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory
                             fy[i] = *(const bf16x8 *)(ly + (i * 32 + 16 * ts + c) * XS + 32 * kk + 8 * g);
                             fx[i] = *(const bf16x8 *)(lx + (i * 32 + 16 * tt + c) * XS + 32 * kk + 8 * g);
                         }
-                        P = mma_pieces<NP, NP, PC::in_order>(fy, fx, P);
+                        P = mma_pieces<NP, NP, Pieces<T>::in_order>(fy, fx, P);
                     }
                     const int t = 16 * tt + c;
                     const double Ct = lc[t];
@@ -339,7 +337,7 @@ __global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory
                             bf16x8 fx[NP];
 #pragma unroll
                             for (int i = 0; i < NP; ++i) fx[i] = *(const bf16x8 *)(lx + (i * 32 + 16 * tt + c) * XS + 32 * kk + 8 * g);
-                            in[tt] = mma_pieces<PP, NP, PC::out_order>(st, fx, in[tt]);
+                            in[tt] = mma_pieces<PP, NP, 2>(st, fx, in[tt]);
                         }
                     }
 #pragma unroll
@@ -355,7 +353,7 @@ __global__ __launch_bounds__(512, NK == 2 && sizeof(T) == 2 ? 4 : 2) void memory
                         bf16x8 fp[PP];
 #pragma unroll
                         for (int i = 0; i < PP; ++i) fp[i] = *(const bf16x8 *)(lp + (i * 32 + t) * 40 + 8 * g);
-                        o = mma_pieces<NP, PP, PC::out_order>(zt, fp, o);
+                        o = mma_pieces<NP, PP, 2>(zt, fp, o);
                         const float win = lwin[t];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) o[r] = (win != -1.f ? o[r] + win * in[tt][r] : o[r]) * out_scale;
@@ -1165,7 +1163,7 @@ int heads_of_wave(int dy) { return dy <= 32 ? 4 : dy <= 64 ? 2 : 1; }
 int tiles_resident(const FmarlMemory *m) {
     const int nk = m->dk <= 64 ? 2 : 4, nz = (m->dv + 15) / 16, waves = nz < 4 ? 4 : nz;
     const int regs = (nk == 4 ? 2 : m->dtype == FMARL_T_F32 ? 3 : 4) * 4 / waves;
-    const int lds = m->dtype == FMARL_T_F32 ? tiles_lds<float, false>(nk, nz) : m->dtype == FMARL_T_BF16 ? tiles_lds<__bf16, false>(nk, nz) : tiles_lds<_Float16, false>(nk, nz);
+    const int lds = m->dtype == FMARL_T_F32 ? tiles_lds<float>(nk, nz) : m->dtype == FMARL_T_BF16 ? tiles_lds<__bf16>(nk, nz) : tiles_lds<_Float16>(nk, nz);
     const int n = 160 * 1024 / lds < regs ? 160 * 1024 / lds : regs;
     return n < 1 ? 1 : n;
 }
@@ -1272,7 +1270,7 @@ Workspace memory_layout(const FmarlMemory *m, int backward) {
 
 template <typename T, int NK, int MODE, bool VEC>
 int launch_tiles(const Walk &w, int64_t blocks, hipStream_t st) {
-    const int nz = (w.dz + 15) / 16, lds = tiles_lds<T, MODE == kOutDot>(NK, nz);
+    const int nz = (w.dz + 15) / 16, lds = tiles_lds<T>(NK, nz);
     if (lds > 64 * 1024) HIP_OK(hipFuncSetAttribute((const void *)memory_tiles_kernel<T, NK, MODE, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     hipLaunchKernelGGL((memory_tiles_kernel<T, NK, MODE, VEC>), dim3((unsigned)blocks), dim3(64 * (nz < 4 ? 4 : nz)), lds, st, w);
     return FMARL_OK;

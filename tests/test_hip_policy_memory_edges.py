@@ -60,6 +60,47 @@ def test_the_decays_gradient_next_to_what_is_no_number(shape, bad, dtype):
             close(shared, head, gamma * run.sum((0, 1)) + head.abs() * 2.0 ** -24, what)
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('shape', [(40, 2, 1, 64, 64), (300, 1, 2, 100, 40)], ids=str)
+def test_states_that_cancel(shape, dtype):
+    """q (k, backwards) takes the difference of two rows of a state of about a thousand; nothing decays and nothing is added.  The products are exact, so out is within two float32
+    additions of the terms, and its own rounding, of the difference: the state is float32 in whatever form the matrix units take it."""
+    L, B, H, dk, dv = shape
+    gen = torch.Generator().manual_seed(60)
+    S = (1000 + torch.randn(B, H, dk, dv, generator=gen)).to(DEV)
+    pick = torch.zeros(L, B, H, dk, dtype=dtype, device=DEV)
+    for t in range(L):
+        pick[t, :, :, t % dk], pick[t, :, :, (7 * t + 1) % dk] = 1, -1
+    zero, none = torch.zeros_like(pick), torch.zeros(L, B, H, dv, dtype=dtype, device=DEV)
+    g = torch.zeros(H, device=DEV)
+    want = (pick.double().unsqueeze(-1) * S.double()).sum(-2)
+    bound = 2 * 2.0 ** -24 * (pick.double().abs().unsqueeze(-1) * S.double()).sum(-2)
+    out, last = fm.memory_chunk(pick, zero, none, g, S, scale=1.0)
+    close(out, want, bound + step_of(out, want), 'out')
+    assert torch.equal(last, S)
+    dv_ = fm.memory_chunk_backward(zero, pick, none, g, none, S, None, scale=1.0)[2]
+    close(dv_, want, bound + step_of(dv_, want), 'dv')
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+def test_products_that_cancel(dtype):
+    """two keys whose products with q are near 1025.6 and -1025.6, their values equal: out is the small difference, to the float32 additions of the two terms and its own rounding"""
+    L, dk, dv = 48, 64, 64
+    gen = torch.Generator().manual_seed(61)
+    q = torch.zeros(L, 1, 1, dk, dtype=dtype)
+    k, v = torch.zeros_like(q), torch.zeros(L, 1, 1, dv, dtype=dtype)
+    q[8:, 0, 0, 0], q[8:, 0, 0, 1], q[8:, 0, 0, 2] = 16, 2.0 ** -4, 1
+    k[2, 0, 0, 0], k[5, 0, 0, 0], k[2, 0, 0, 2], k[5, 0, 0, 2] = 64, -64, 1.5, -1.5
+    k[2, 0, 0, 1], k[5, 0, 0, 1] = torch.rand(2, generator=gen).to(dtype) + 1
+    v[2], v[5] = 1, 1
+    q, k, v = q.to(DEV), k.to(DEV), v.to(DEV)
+    out, _ = fm.memory_chunk(q, k, v, torch.zeros(1, device=DEV), None, scale=1.0)
+    want = recurrence(q.double(), k.double(), v.double(), torch.zeros(L, 1, 1, device=DEV).double(), torch.zeros(1, 1, dk, dv, device=DEV).double(), torch.zeros(L, 1, device=DEV) != 0, 1.0)[0]
+    mag = recurrence(q.double().abs(), k.double().abs(), v.double(), torch.zeros(L, 1, 1, device=DEV).double(), torch.zeros(1, 1, dk, dv, device=DEV).double(),
+                     torch.zeros(L, 1, device=DEV) != 0, 1.0)[0]
+    close(out, want, 2 * 2.0 ** -24 * mag + step_of(out, want), 'out')     # near 1024 a rounding is off by 2^-14 at most: one in each product q k, two where the terms are added
+
+
 @pytest.mark.parametrize('value', [torch.finfo(F32).min, torch.finfo(F32).max])
 @pytest.mark.parametrize('shape', [(10, 3, 2, 16, 16), (40, 2, 1, 64, 64), (40, 2, 1, 16, 100), (300, 1, 2, 100, 40)], ids=str)
 def test_the_types_lowest_value_in_another_episode(shape, value):
