@@ -173,19 +173,19 @@ class _MemoryChunk(torch.autograd.Function):
     def forward(ctx, q, k, v, log_decay, state, masks, scale):
         m, keep = _memory_args('memory_chunk', q, k, v, log_decay, state, masks, scale, 2)
         out, last, ws = _launch_chunk(m, keep)
-        ctx.save_for_backward(*keep)
-        ctx.forward_ws = ws   # long sequences: the states at their segments' starts
+        ctx.save_for_backward(*keep, ws if ws.numel() > 256 else None)   # long sequences: the states at their segments' starts
         ctx.scale, ctx.state_shape = m.scale, None if state is None else state.shape
         ctx.set_materialize_grads(False)
         return out, last
 
     @_once
     def backward(ctx, d_out, d_state):
-        keep = q, k, v, g, state, masks = ctx.saved_tensors
+        *keep, ws = ctx.saved_tensors
+        v, state = keep[2], keep[4]
         m = _memory_struct(*keep, ctx.scale)
         if d_out is None:
             d_out = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
-        dq, dk, dv, dg, ds = _launch_chunk_backward(m, keep, d_out, d_state, ctx.needs_input_grad[3], ctx.forward_ws)
+        dq, dk, dv, dg, ds = _launch_chunk_backward(m, keep, d_out, d_state, ctx.needs_input_grad[3], ws)
         return dq, dk, dv, dg, None if state is None else ds.view(ctx.state_shape), None, None
 
 

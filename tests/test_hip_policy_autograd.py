@@ -1,6 +1,7 @@
 """-m gpu: the policy's operators and autograd's bookkeeping -- tensors written in place, tensors kept for the backward pass."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import fair_marl_amd as fm
 from fair_marl_amd.rollout_buffer import DeviceRolloutBuffer
@@ -45,3 +46,36 @@ def test_a_buffer_slot_stepped_in_place_is_seen():
         buf.memory_step(0, q.view(5, 3, 2, 4), k.view(5, 3, 2, 4), v.view(5, 3, 2, 8), g.view(5, 3, 2))
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         out.sum().backward()
+
+
+@pytest.mark.parametrize('shape', [(2048, 1, 2, 64, 64), (2048, 2, 4, 16, 16)], ids=str)
+def test_segment_states_go_with_the_saved_tensors(shape):
+    """long sequences: the states at their segments' starts (here as many bytes as the rows, or more) are moved, dropped and freed as every saved tensor is"""
+    q, k, v, g, S = inputs(*shape, seed=1)
+    leaves = [t.requires_grad_() for t in (q, k, v, g, S)]
+    run = lambda: fm.memory_chunk(*leaves)  # noqa: E731
+    with torch.no_grad():
+        d = [torch.randn_like(t) for t in run()]
+    want = torch.autograd.grad(run(), leaves, d)
+    own = sum(t.numel() * 4 for t in d)
+    asked = lambda: torch.cuda.memory_stats()['requested_bytes.all.current']  # noqa: E731
+
+    def left(f):
+        before = asked()
+        out = f()
+        return out, asked() - before
+
+    with torch.autograd.graph.save_on_cpu():
+        offloaded, kept = left(run)
+    assert kept <= own, (kept, own)
+    again, kept = left(lambda: torch.utils.checkpoint.checkpoint(run, use_reentrant=False))
+    assert kept <= own, (kept, own)
+    for out in (offloaded, again):
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, d), want))
+    out, kept = left(run)
+    assert kept > own                                      # an ordinary pass keeps them,
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, d, retain_graph=True), want))
+    got, freed = left(lambda: torch.autograd.grad(out, leaves, d))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    grads = sum(t.numel() * 4 for t in leaves)
+    assert freed <= grads - (kept - own), (freed, grads, kept, own)   # and gives them back with the graph, while its outputs live
