@@ -782,14 +782,14 @@ __global__ __launch_bounds__(256) void actions_join_kernel(Actions a, const floa
 template <typename T>
 __global__ __launch_bounds__(256) void actions_reduce_kernel(const float *part, int64_t split_stride, int splits, int64_t ld, float *sum, int first, int last, T *out,
                                                              int64_t rows, int cols, const float *inv_scale) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * cols) return;
-    const int64_t r = i / cols, at = r * ld + (i - r * cols);
-    float s = first ? 0.f : sum[at];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / cols, at = r * ld + (i - r * cols);
+        float s = first ? 0.f : sum[at];
 #pragma unroll 8
-    for (int k = 0; k < splits; ++k) s += part[k * split_stride + at];
-    if (last) out[i] = (T)(inv_scale ? s / *inv_scale : s);
-    else sum[at] = s;
+        for (int k = 0; k < splits; ++k) s += part[k * split_stride + at];
+        if (last) out[i] = (T)(inv_scale ? s / *inv_scale : s);
+        else sum[at] = s;
+    }
 }
 
 __global__ __launch_bounds__(256) void actions_bias_kernel(const float *part, int64_t ld, int parts, float *db, int n, int add) {
@@ -1000,7 +1000,8 @@ int many_forward_f32(const Actions &s, const Plan &p, char *base, hipStream_t st
 
 template <typename T>
 void reduce(const float *part, int64_t split_stride, int splits, int64_t ld, float *sum, bool first, bool last, T *out, int64_t rows, int cols, const float *scale, hipStream_t st) {
-    hipLaunchKernelGGL((actions_reduce_kernel<T>), dim3((unsigned)((rows * cols + 255) / 256)), dim3(256), 0, st, part, split_stride, splits, ld, sum, (int)first, (int)last, out, rows,
+    const int64_t blocks = (rows * cols + 255) / 256, most = 1 << 22;   // a launch holds fewer than 2^32 threads, the weights may be 2^34
+    hipLaunchKernelGGL((actions_reduce_kernel<T>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, part, split_stride, splits, ld, sum, (int)first, (int)last, out, rows,
                        cols, scale);
 }
 

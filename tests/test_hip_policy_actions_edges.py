@@ -1,0 +1,38 @@
+"""-m gpu: action_log_probs where its tiles, pieces and chunks end and begin, and at the ends of its types.  Definition and bounds are those of test_hip_policy_actions.py."""
+import pytest
+import torch
+
+import fair_marl_amd as fm
+from test_hip_policy_actions import BF16, DEV, U
+
+pytestmark = pytest.mark.gpu
+
+
+def test_more_weights_than_threads_of_a_launch():
+    """2^32 weights (524 288 actions of 8 192 features): every row of their gradient is formed"""
+    M, K, V = 3, 8192, 1 << 19
+    gen = torch.Generator(device=DEV).manual_seed(72)
+    X = torch.randn(M, K, device=DEV, generator=gen).to(BF16)
+    W = torch.empty(V, K, dtype=BF16, device=DEV)
+    for a in range(0, V, 1 << 16):      # (rows of a table: 4 billion normal numbers take longer than the rest)
+        W[a:a + (1 << 16)] = torch.randn(1 << 10, K, device=DEV, generator=gen).to(BF16).repeat(64, 1) * K ** -0.5
+    act = torch.tensor([0, V // 2 + 1, V - 1], device=DEV)
+    dl = torch.tensor([1.0, -2.0, 0.5], device=DEV)
+    leaves = X.requires_grad_(), W.requires_grad_()
+    lp, ent = fm.action_log_probs(*leaves, None, act)
+    dX, dW = torch.autograd.grad(lp, leaves, dl)
+    with torch.no_grad():
+        z = torch.cat([(X.float() @ W[a:a + (1 << 16)].float().t()).double() for a in range(0, V, 1 << 16)], 1)
+        p = torch.softmax(z, -1)
+        want = torch.log_softmax(z, -1)[torch.arange(M, device=DEV), act]
+        # a logit is off by K u sum |x w| (here: K 0.64 K^-0.5 = 58 on average, within 12 of it), the sums over V terms by V u at most
+        ez = (K + 4) * U * 70.0
+        assert float((lp.double() - want).abs().max()) <= 2 * ez + (V + 40) * U + 4 * U * 40
+        for rows in (slice(0, 600), slice(V // 2 - 300, V // 2 + 300), slice(V - 600, V)):
+            hot = (torch.arange(V, device=DEV)[rows][None] == act[:, None]).double()
+            dz = dl.double()[:, None] * (hot - p[:, rows])
+            exact, size = dz.t() @ X.double(), dz.abs().t() @ X.double().abs()
+            # dz: p's relative error, half a step of its type; the product's three terms, half a step of its own type
+            bound = (2 * ez + (V + 40) * U + 8 * U * 40 + 2.0 ** -8) * size + 8 * U * size + 2.0 ** -8 * exact.abs()
+            assert bool(((dW[rows].double() - exact).abs() <= bound).all())
+        assert not bool((dW.view(-1, 1 << 16).abs().amax(1) == 0).any())     # no stretch is left out
