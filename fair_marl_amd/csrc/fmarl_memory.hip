@@ -1074,7 +1074,7 @@ template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void memory_step_kernel(Step a) {
     constexpr int W = VEC ? 4 : 1;
     const int lz = 1 << a.lz, team = 1 << a.team, rows = team >> a.lz, j = threadIdx.x & (team - 1), row = j >> a.lz, cl = j & (lz - 1);
-    const uint32_t bh = (blockIdx.x * 256 + threadIdx.x) >> a.team;   // (B H < 2^26: fewer than 2^32 threads)
+    const uint32_t bh = (blockIdx.x * 256 + threadIdx.x) >> a.team;   // (fewer than 2^32 threads)
     if (bh >= a.B * a.H) return;
     const uint32_t b = bh / (uint32_t)a.H, h = bh - b * (uint32_t)a.H;
     const T *q = (const T *)a.q.p + b * a.q.sb + h * a.q.sh, *k = (const T *)a.k.p + b * a.k.sb + h * a.k.sh, *v = (const T *)a.v.p + b * a.v.sb + h * a.v.sh;
@@ -1380,6 +1380,7 @@ int fmarl_memory_step(const FmarlMemory *m, const FmarlRows *out, float *state_o
     while (s.lz < 6 && (vec ? 4 : 1) << s.lz < m->dv) ++s.lz;
     for (s.team = s.lz; s.team < 6 && 1 << s.team < m->dk << s.lz;) ++s.team;
     const int64_t blocks = ((m->B * m->H << s.team) + 255) / 256;
+    if (blocks > 0xffffff) return policy_fail(FMARL_EINVAL, "fmarl_memory_step: too many sequences for heads of this size (a launch holds fewer than 2^32 threads)");
     hipStream_t st = (hipStream_t)stream;
 #define FMARL_STEP(T) do { if (vec) hipLaunchKernelGGL((memory_step_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, s); \
                            else hipLaunchKernelGGL((memory_step_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, st, s); } while (0)
