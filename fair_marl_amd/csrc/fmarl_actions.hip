@@ -59,12 +59,12 @@ __device__ __forceinline__ uint32_t available4(const Actions &a, int64_t row, in
 
 __device__ __forceinline__ float exp_of(float x) { return exp2_fast(x * kLog2e); }
 
-// what the tiles' (max, sum e^{z - max}, sum (z - max) e^{z - max}) say of a row; top == -inf and !some: nothing available
-__device__ __forceinline__ void row_result(const Actions &a, int64_t row, int act, float top, float s, float t, bool some, float za) {
+// what the tiles' (max, sum e^{z - max}, sum (z - max) e^{z - max}) say of a row, logits in units of `unit`; top == -inf and !some: nothing available
+__device__ __forceinline__ void row_result(const Actions &a, int64_t row, int act, float top, float s, float t, bool some, float za, float unit) {
     float lp = 0.f, en = 0.f, ls = __builtin_inff();
     if (act >= 0 && some) {
         const float l = logf(s);
-        lp = (za - top) - l; en = l - t / s; ls = top + l;
+        lp = (za - top) * unit - l; en = l - t * unit / s; ls = top * unit + l;   // (the difference first: 0 where the action is the largest, however far out)
         if (act >= a.V) { lp = en = __builtin_nanf(""); ls = __builtin_inff(); }   // no such action: seen in the result, without a gradient
     }
     a.logp[row] = lp; a.ent[row] = en; a.lse[row] = ls;
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
                 }
             s = lanes_sum<16>(s, 64); t = lanes_sum<16>(t, 64); za = lanes_sum<16>(za, 64);
             const float any = lanes_max<16>(some ? 1.f : 0.f, 64);
-            if (lane < 16 && real) row_result(a, row, act, top, s, t, any != 0.f, za);
+            if (lane < 16 && real) row_result(a, row, act, top, s, t, any != 0.f, za, 1.f);
         } else {
             const bool in = real && lse != __builtin_inff();
 #pragma unroll
@@ -523,7 +523,9 @@ __global__ __launch_bounds__(256) void actions_rows_kernel(Actions a, int64_t ro
             const float lse = a.lse[row], s = scale ? *scale : 1.f;
             if (lse != __builtin_inff()) {
                 const float de = a.dent ? a.dent[row] * s : 0.f, dl = a.dlogp ? a.dlogp[row] * s : 0.f;
-                v = f32x4{lse * kLog2e, de * -0.693147181f, lse != lse ? lse : -(dl + de * a.ent[row]), dl};   // logits that hold a NaN: a gradient of NaN
+                // a row of lowest biases only: exactly where actions_bias2_kernel leaves its logits, so that their difference is 0
+                const float lse2 = lse <= -2.3e38f ? -3.4028234e38f : lse * kLog2e;
+                v = f32x4{lse2, de * -0.693147181f, lse != lse ? lse : -(dl + de * a.ent[row]), dl};   // logits that hold a NaN: a gradient of NaN
             } else act = -1;
         }
     }
@@ -772,9 +774,8 @@ __global__ __launch_bounds__(256) void actions_join_kernel(Actions a, const floa
     if (k == 0 && m < count) {
         for (int i = 1; i < 16; ++i) add(red[0][i][c], red[1][i][c], red[2][i][c]);
         const int act = action_of(a, row0 + m);
-        const float ln2 = 0.693147181f, z = act >= 0 && act < a.V ? za[m] : 0.f;
-        if (two) row_result(a, row0 + m, act, top == -__builtin_inff() ? 0.f : top * ln2, s, t * ln2, s != 0.f, z * ln2);
-        else row_result(a, row0 + m, act, top, s, t, s != 0.f, z);
+        const float z = act >= 0 && act < a.V ? za[m] : 0.f;
+        row_result(a, row0 + m, act, two && top == -__builtin_inff() ? 0.f : top, s, t, s != 0.f, z, two ? 0.693147181f : 1.f);
     }
 }
 

@@ -3,9 +3,28 @@ import pytest
 import torch
 
 import fair_marl_amd as fm
-from test_hip_policy_actions import BF16, DEV, U
+from test_hip_policy_actions import BF16, DEV, F16, F32, U, make, run
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('V', [5, 90])
+def test_a_single_action_whose_bias_is_the_lowest_value(V, dtype):
+    """rows whose one available action has float32's lowest value for a bias: it is taken with certainty, and no gradient comes of it"""
+    X, W, b, act, _, dl, de = make(60, 32, V, dtype, seed=71, avail=False, pad=0.0)
+    b = b.float()
+    b[1] = torch.finfo(F32).min
+    act[:30] = 1
+    act[30:] = torch.where(act[30:] == 1, 0, act[30:])
+    av = torch.ones(60, V, dtype=torch.bool, device=DEV)
+    av[:30] = False
+    av[:30, 1] = True
+    lp, ent, dX, dW, db = run(X, W, b, act, av, dl, de)
+    assert bool((lp[:30] == 0).all()) and bool((ent[:30] == 0).all()) and bool((dX[:30] == 0).all())
+    assert float(db[1]) == 0 and bool((dW[1] == 0).all())        # the rows that have others: probability 0
+    rest = run(X[30:], W, b, act[30:], None, dl[30:], de[30:])
+    assert torch.equal(lp[30:], rest[0]) and torch.equal(ent[30:], rest[1])
 
 
 def test_more_weights_than_threads_of_a_launch():
