@@ -1,11 +1,68 @@
 """-m gpu: action_log_probs where its tiles, pieces and chunks end and begin, and at the ends of its types.  Definition and bounds are those of test_hip_policy_actions.py."""
+import math
+
 import pytest
 import torch
 
 import fair_marl_amd as fm
-from test_hip_policy_actions import BF16, DEV, F16, F32, U, make, run
+from fair_marl_amd import _lib
+from test_hip_policy_actions import BF16, DEV, F16, F32, U, check, make, run
 
 pytestmark = pytest.mark.gpu
+
+
+def up(n, m):
+    return (n + m - 1) // m * m
+
+
+def half_plan(M, K, V, backward):
+    """The sizes of the half precision way for many actions: (tiles in a workgroup's run, pieces of the actions, chunks of the rows), after a look that the library still works by
+    them: its workspace is the sum of what they ask for."""
+    Mp, Kp, Vp = up(M, 256), up(K, 256), up(V, 256)
+    Mc = min(Mp, max(1024, min(65536, (256 << 20) // (2 * Kp) // 256 * 256)))
+    P = min(Vp, max(256, (256 << 20) // (2 * Mc) // 256 * 256))
+    tm, tk, tv = Mc // 256, Kp // 256, P // 256
+    parts = lambda tiles, steps: max(1, min(256 // tiles, steps // 4, 16))  # noqa: E731
+    sx, sw = parts(tm * tk, P // 64), parts(tv * tk, Mc // 64)
+    turns, rest = (tm, tv) if backward else (Vp // 256, tm)
+    sz = max(1, min(256 // rest, turns))
+    sizes = [2 * Mc * Kp, 2 * Vp * Kp, 4 * Vp, 4 * Mc, 16 * Mc if backward else 0]
+    if backward:
+        sizes += [2 * Mc * P, 4 * max(sx * Mc * Kp, sw * P * Kp), 4 * Mc * Kp if P < Vp else 0, 4 * Vp * Kp if Mc < Mp else 0, 4 * (Mc // 64) * P, 4 * 257]
+    else:
+        sizes += [12 * 2 * sz * Mc, 4 * Mc]
+    a = _lib.FmarlActions(M, K, V, _lib.T_BF16, 0, 0, 0, 4096, K, 4096, K, None, 4096, None, 0)
+    assert _lib.load().fmarl_action_log_probs_workspace(a, int(backward)) == sum(up(n, 256) for n in sizes), 'the plan is another one: choose sizes that have several tiles and pieces'
+    return -(-turns // sz), -(-Vp // P), -(-Mp // Mc)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16], ids=str)
+@pytest.mark.parametrize('shape,kind', [((16384, 24, 4096), 'maxima that rise'), ((16384, 96, 4096), 'maxima that fall'), ((16300, 40, 4000), 'tiles without an action'),
+                                        ((16300, 300, 4000), 'without a mask')], ids=str)
+def test_runs_of_several_tiles(shape, kind, dtype):
+    """a workgroup walks four tiles one after the other, forwards and backwards: the running maximum and sums, the loads over a tile's end (one step a tile: three tiles on their way)"""
+    assert half_plan(*shape, False)[0] >= 3 and half_plan(*shape, True)[0] >= 3
+    t = make(*shape, dtype, seed=sum(shape), avail=kind == 'tiles without an action')
+    V, b, act, av = shape[2], t[2], t[3], t[4]
+    tile = torch.arange(V, device=DEV) // 256
+    if kind == 'maxima that rise':
+        b.add_(2.0 * tile.to(dtype))
+    if kind == 'maxima that fall':
+        b.sub_(2.0 * tile.to(dtype))
+    if av is not None:      # first, middle and last tiles of a run without an available action, and all but one of them
+        rows = torch.arange(shape[0], device=DEV)[:, None] % 5
+        av &= ~(((rows == 0) & (tile % 4 == 0)) | ((rows == 1) & (tile % 4 == 2)) | ((rows == 2) & (tile % 4 == 3)) | ((rows == 3) & (tile != 6)))
+        av[torch.arange(shape[0], device=DEV), act.clamp(min=0)] |= act >= 0
+    check(*t, run(*t))
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16], ids=str)
+def test_pieces_of_the_actions_in_half_precision(dtype):
+    """two pieces of the actions, the last one narrower, for each of two chunks of the rows"""
+    shape = (66000, 16, 2200)
+    assert half_plan(*shape, True)[1:] == (2, 2)
+    t = make(*shape, dtype, seed=70, avail=False)
+    check(*t, run(*t))
 
 
 @pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)

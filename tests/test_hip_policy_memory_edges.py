@@ -11,6 +11,19 @@ from test_hip_policy_memory import BF16, DEV, F16, F32, close, compare, make, re
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize('decay', ['token', 'head'])
+@pytest.mark.parametrize('dtype', [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize('shape', [(1, 3, 2, 64, 64), (10, 37, 2, 64, 64), (10, 5, 3, 33, 100), (7, 3, 1, 128, 128), (32, 3, 2, 48, 16), (9, 5, 1, 65, 39), (10, 3, 3, 97, 5)], ids=str)
+def test_few_tokens_of_wide_heads(shape, dtype, decay):
+    """rows of lanes that share a head: two up to 64 wide, four beyond, the last with a part of its share or none; heads that do not fill the last wave"""
+    q, k, v, g, S, masks, do, dS = make(*shape, dtype, decay, seed=sum(shape) + 1)
+    leaves = [t.requires_grad_() for t in (q, k, v, g, S)]
+    out, last = fm.memory_chunk(q, k, v, g, S, masks)
+    grads = torch.autograd.grad((out, last), leaves, (do, dS))
+    with torch.no_grad():
+        compare((out, last) + grads, q, k, v, g, S, masks, shape[3] ** -0.5, do, dS)
+
+
 SHAPES = [(12, 2, 2, 16, 16), (16, 5, 1, 5, 7), (40, 2, 1, 5, 7), (30, 2, 2, 100, 12), (90, 2, 2, 40, 24), (700, 1, 1, 16, 16), (700, 1, 2, 64, 64), (300, 1, 1, 128, 100)]
 
 
