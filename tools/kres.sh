@@ -1,6 +1,9 @@
 #!/bin/bash
 # measurement aid: registers / scratch / occupancy of every kernel of a translation unit (compiler remarks, no GPU needed): tools/kres.sh [libfmarl | fmarl_memory | fmarl_block | fmarl_actions]
-cd "$(dirname "$0")/../fair_marl_amd/csrc" && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -mllvm -disable-machine-licm -Xclang -target-feature -Xclang -packed-fp32-ops -c -fPIC -Rpass-analysis=kernel-resource-usage -o /tmp/kres_lib.o "${1:-libfmarl}.hip" 2>&1 | python3 -c "
+# compiled as __graft_entry__.build() does
+U=${1:-libfmarl}
+cd "$(dirname "$0")/.." && FLAGS=$(python3 -c "import sys, __graft_entry__ as g; print(*g.flags(sys.argv[1]))" $U) || exit 1
+cd fair_marl_amd/csrc && ${HIPCC:-/opt/rocm/bin/hipcc} $FLAGS -Rpass-analysis=kernel-resource-usage -o /tmp/kres_lib.o $U.hip 2>&1 | python3 -c "
 import sys,re
 cur=None
 for l in sys.stdin:
