@@ -168,11 +168,18 @@ def _launch_chunk_backward(m, keep, d_out, d_state, want_decay=True, forward_ws=
     return dq, dk, dv, dg, ds
 
 
+def _no_tokens(v, state, shape):
+    return v.new_empty(v.shape), v.new_zeros(shape, dtype=_F32) if state is None else state.reshape(shape).clone()
+
+
 class _MemoryChunk(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, masks, scale):
         m, keep = _memory_args('memory_chunk', q, k, v, log_decay, state, masks, scale, 2)
-        out, last, ws = _launch_chunk(m, keep)
+        if m.L == 0 or m.B == 0:
+            out, last, ws = _no_tokens(v, state, (m.B, m.H, m.dk, m.dv)) + (v.new_empty(0),)
+        else:
+            out, last, ws = _launch_chunk(m, keep)
         ctx.save_for_backward(*keep, ws if ws.numel() > 256 else None)   # long sequences: the states at their segments' starts
         ctx.scale, ctx.state_shape = m.scale, None if state is None else state.shape
         ctx.set_materialize_grads(False)
@@ -183,6 +190,9 @@ class _MemoryChunk(torch.autograd.Function):
         *keep, ws = ctx.saved_tensors
         v, state = keep[2], keep[4]
         m = _memory_struct(*keep, ctx.scale)
+        if m.L == 0 or m.B == 0:
+            ds = None if state is None else torch.zeros_like(state) if d_state is None else d_state.clone()
+            return (*(torch.zeros_like(t) for t in keep[:4]), None if ds is None else ds.reshape(ctx.state_shape), None, None)
         if d_out is None:
             d_out = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
         dq, dk, dv, dg, ds = _launch_chunk_backward(m, keep, d_out, d_state, ctx.needs_input_grad[3], ws)
@@ -204,12 +214,10 @@ def memory_chunk(q, k, v, log_decay, state=None, masks=None, scale=None):
     _seen_by_torch('memory_chunk', q, k, v, log_decay, state)
     if q.dim() != 4 or v.dim() != 4:
         _refuse('memory_chunk: q, k (L, B, H, dk) and v (L, B, H, dv), got %s, %s', tuple(q.shape), tuple(v.shape))
-    if q.shape[0] == 0 or q.shape[1] == 0:
-        _memory_args('memory_chunk', q, k, v, log_decay, state, masks, scale, 2)
-        shape = (q.shape[1], q.shape[2], q.shape[3], v.shape[3])
-        return v.clone(), torch.zeros(shape, dtype=torch.float32, device=q.device) if state is None else state.reshape(shape).clone()
     if not _wants_grad(q, k, v, log_decay, state):
         m, keep = _memory_args('memory_chunk', q, k, v, log_decay, state, masks, scale, 2)
+        if m.L == 0 or m.B == 0:
+            return _no_tokens(v, state, (m.B, m.H, m.dk, m.dv))
         return _launch_chunk(m, keep)[:2]
     return _MemoryChunk.apply(q, k, v, log_decay, state, masks, scale)
 

@@ -1,0 +1,31 @@
+"""-m gpu: the policy's operators on nothing: every input still has a gradient, of zeros."""
+import pytest
+import torch
+
+import fair_marl_amd as fm
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+
+
+def z(*shape, dtype=torch.float32):
+    return torch.randn(*shape, device=DEV).to(dtype).requires_grad_()
+
+
+@pytest.mark.parametrize('decay', ['token', 'head'])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('L,B', [(0, 2), (5, 0), (0, 0)])
+def test_no_tokens(L, B, dtype, decay):
+    q, k, v, S = z(L, B, 3, 4, dtype=dtype), z(L, B, 3, 4, dtype=dtype), z(L, B, 3, 5, dtype=dtype), z(B, 60)
+    g = z(*((L, B, 3) if decay == 'token' else (3,)))
+    with torch.no_grad():
+        g[..., 0] = -float('inf')
+    for state in (S, None):
+        out, last = fm.memory_chunk(q, k, v, g, state, torch.ones(L, B, device=DEV))
+        assert out.shape == v.shape and out.dtype == dtype and last.shape == (B, 3, 4, 5) and last.dtype == torch.float32
+        assert torch.equal(last, torch.zeros_like(last) if state is None else S.view_as(last))
+        leaves = [q, k, v, g] + ([] if state is None else [S])
+        d = torch.randn_like(last)
+        got = torch.autograd.grad((out, last), leaves, (torch.ones_like(out), d))
+        assert all(a.shape == t.shape and a.dtype == t.dtype for a, t in zip(got, leaves)) and bool((got[3] == 0).all())
+        assert state is None or torch.equal(got[4], d.view_as(S))
