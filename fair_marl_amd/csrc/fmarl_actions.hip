@@ -1099,6 +1099,7 @@ extern "C" {
 
 size_t fmarl_action_log_probs_workspace(const FmarlActions *a, int backward) {
     if (actions_check(a, "fmarl_action_log_probs_workspace")) return 0;
+    if (a->rows == 0) return 256;   // (nothing runs; a plan divides by the rows)
     if (actions_few(a)) return backward ? up256((size_t)few_workgroups(a) * ((size_t)a->actions * a->features + a->actions) * 4) : 256;
     return actions_plan(a, backward != 0).total;
 }

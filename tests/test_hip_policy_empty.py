@@ -29,3 +29,16 @@ def test_no_tokens(L, B, dtype, decay):
         got = torch.autograd.grad((out, last), leaves, (torch.ones_like(out), d))
         assert all(a.shape == t.shape and a.dtype == t.dtype for a, t in zip(got, leaves)) and bool((got[3] == 0).all())
         assert state is None or torch.equal(got[4], d.view_as(S))
+
+
+def test_no_rows():
+    x, branch, gate, w = z(0, 3, 16), z(0, 3, 16), z(0, 3, 16), [z(16) for _ in range(5)]
+    y, h = fm.block_norm(x, branch, gate, *w, groups=2, kind='layer')
+    assert y.shape == h.shape == x.shape
+    got = torch.autograd.grad((y, h), [x, branch, gate] + w, (torch.ones_like(y), torch.ones_like(h)))
+    assert all(a.shape == t.shape and bool((a == 0).all()) for a, t in zip(got, [x, branch, gate] + w))
+    for V in (5, 90):
+        X, W, b = z(0, 7), z(V, 7), z(V)
+        out = fm.action_log_probs(X, W, b, torch.zeros(0, dtype=torch.int64, device=DEV))
+        got = torch.autograd.grad(out, (X, W, b), [torch.ones_like(t) for t in out])
+        assert all(a.shape == t.shape and bool((a == 0).all()) for a, t in zip(got, (X, W, b)))
