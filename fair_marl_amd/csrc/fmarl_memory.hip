@@ -686,13 +686,14 @@ __global__ __launch_bounds__(256) void memory_short_backward_kernel(ShortGrad a)
             q[t] *= a.scale;           // from here on only in G's and dk's, dv's own terms
         }
     });
-    float run = 0.f;
+    double run = 0.0;   // (its terms are float32, their sum on the way may need more)
     if (a.d_state) {
         row_state(G, a.d_state + at + c * V, 1, V, kin, a.wide);
         row_state(C, a.d_state + at + c, V, K, vin, false);
+        float last = 0.f;
 #pragma unroll
-        for (int m = 0; m < 16; ++m) run += S[m] * G[m];
-        run = row_sum(run);
+        for (int m = 0; m < 16; ++m) last += S[m] * G[m];
+        run = row_sum(last);
     } else {
 #pragma unroll
         for (int m = 0; m < 16; ++m) G[m] = C[m] = 0.f;
@@ -705,12 +706,12 @@ __global__ __launch_bounds__(256) void memory_short_backward_kernel(ShortGrad a)
             const float nk = row_dot<1>(v1, G), nv = row_dot<1>(k1, C), vo = row_sum(v[t] * o[t]), qk = row_sum(q[t] * k[t]);
             if (have && kin) ((T *)a.dk.p)[t * a.dk.sl + b * a.dk.sb + h * a.dk.sh + c] = (T)(nk + q[t] * vo);
             if (have && vin) ((T *)a.dv.p)[t * a.dv.sl + b * a.dv.sb + h * a.dv.sh + c] = (T)(nv + o[t] * qk);
-            run += xs[t] - row_sum(k[t] * nk);
+            run += (double)xs[t] - row_sum(k[t] * nk);
             const bool fresh = row_lane<t>(fresh_l) != 0.f;
-            const float dg = fresh ? 0.f : run, d = row_lane<t>(decay_l);
-            if (fresh) run = 0.f;
-            sum += dg;
-            if (a.dg && have && c == 0) a.dg[t * heads + bh] = dg;
+            if (fresh) run = 0.0;
+            const float d = row_lane<t>(decay_l);
+            sum += run;
+            if (a.dg && have && c == 0) a.dg[t * heads + bh] = (float)run;
             row_update<1>(G, d, false, o1, q[t] * d);
             row_update<1>(C, d, false, q1, o[t] * d);
             if (__ballot(fresh))

@@ -145,3 +145,17 @@ def test_the_types_lowest_value_in_another_episode(shape, value):
     for name, a, i in (('out', out, 0), ('dq', grads[0], 2), ('dk', grads[1], 3), ('dv', grads[2], 4)):
         close(a[:then], want[i][:then], gamma * mag[i][:then] + step_of(a, want[i][:then]), name)
     close(grads[4], want[6], gamma * mag[6] + step_of(grads[4], want[6]), 'dS0')
+
+
+@pytest.mark.parametrize('L', [6, 16])
+def test_the_running_difference_of_few_tokens_keeps_small_terms(L):
+    """one row, one column, nothing decays: dg_t = S G_t with G_t the sum of q_j d_out_j behind, 2^24, 2^24 + 1 and 1.  Every term is exact in float32, their sum is not on its way"""
+    z = lambda *s: torch.zeros(*s, device=DEV)  # noqa: E731
+    q, k, do = z(L, 1, 1, 1), z(L, 1, 1, 1), z(L, 1, 1, 1)
+    q[-1], do[-1], q[-2], do[-2], q[-4], do[-4] = 4096, 4096, 1, 1, -4096, 4096
+    want = torch.ones(L, dtype=torch.float64)
+    want[-1], want[-2], want[-3] = 2.0 ** 24, 2.0 ** 24 + 1, 2.0 ** 24 + 1
+    for g in (z(L, 1, 1), z(1)):
+        dg = fm.memory_chunk_backward(q, k, k.clone(), g, do, None, torch.ones(1, 1, 1, 1, device=DEV), None, scale=1.0)[3]
+        exact = want.view(L, 1, 1) if g.dim() == 3 else want.sum().view(1)
+        assert torch.equal(dg.cpu(), exact.float())
