@@ -80,7 +80,7 @@ __device__ __forceinline__ float dlogit(float z, bool hot, bool in, float lse, f
 // 16 rows a wave at a time, logits as z^T = W x^T in the accumulator layout of mfma_f32_16x16x4f32 (row 4 * (lane / 16) + r: action, column lane % 16: row of
 // x), so a row's softmax is over a lane's registers and two lane exchanges, and dx^T = W^T dz^T takes dz^T as it lies.  VT * 16 >= V, KT * 16 >= K.  x is loaded
 // once, in float4s; float32 products for every type.  The gradient of W is summed over a wave's tiles in registers, over the workgroup in LDS and
-// over the workgroups by actions_sums_kernel, always in the same order.  2 097 152 rows of 64 float32, five actions: 131 us forwards (4.4 TB/s), 227 + 5 us backwards (4.9 TB/s).
+// over the workgroups by actions_sums_kernel, always in the same order.  2 097 152 rows of 64 float32, five actions: 131 us forwards back to back (4.4 TB/s; 152 between other passes), 227 + 5 us backwards (4.9 TB/s).
 template <typename T, int VT, int KT, bool BACK, bool VEC>
 __global__ __launch_bounds__(256) void actions_few_kernel(Actions a) {
     constexpr int PK = 16 * KT + 4;
@@ -471,8 +471,8 @@ __global__ __launch_bounds__(256) void actions_gemm_kernel(Gemm q) {
 //   transposing reads (ds_read_b64_tr_b16: 16 lanes point at four rows of 16 and get a column each).  So dz, x and W serve both of their products as they lie.
 // What an epilogue needs per action and per row comes the same way, with the first step of its tile: a load of its own would be waited for behind all steps on
 // their way.  Logits are formed in base 2: v_exp_f32 is a power of two, and z log2(e) - max one multiply-add.
-// 8 192 x 256 x 15 625 bfloat16, 65.5 GFLOP a product: dx 88 us, dW 74 us (745, 885 TFLOP/s; a large product by the library 1 085), with the softmax's sums 112 us, with dz
-// written 149 us: their epilogues (an exponential per logit; 256 MB of dz) are not hidden behind the matrix instructions.
+// 8 192 x 256 x 15 625 bfloat16, 65.5 GFLOP a product: dx 87 us, dW 75 us (753, 873 TFLOP/s; a large product by the library 1 085), with the softmax's sums 113 us, with dz
+// written 152 us: their epilogues (an exponential per logit; 256 MB of dz) are not hidden behind the matrix instructions.
 struct Wide {
     const char *A, *B; int64_t lda, ldb;     // elements; whole tiles can be read
     int ta, tb, steps, splits;               // tiles of A and of B, steps of the contraction; kStore: parts of the contraction, else parts of the outer tile's run
@@ -714,7 +714,9 @@ __global__ __launch_bounds__(512) void actions_wide_kernel(Wide q) {
                         for (int r = 0; r < 4; ++r) d[r] += want[j] - 16 * i == r && z[r] != -__builtin_inff() ? rc[j][3] : 0.f;
                     }
                     all += d;
-                    store4<T>(zrow + 16 * j * q.ldz + 16 * i, d, 4, true);   // rounded to the operands' type: what the two products read
+                    // rounded to the operands' type: what the two products read.  The gradients' error is then 1.4 times that of their own rounding (8 192 x 256 x 15 625 bfloat16: 0.0023
+                    // of their norm, 0.0017 with dz in float32, as here with dz in two pieces, whose second writing and products made the training pass 781 us instead of 475)
+                    store4<T>(zrow + 16 * j * q.ldz + 16 * i, d, 4, true);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) all[r] = lanes_sum<1>(all[r], 16);

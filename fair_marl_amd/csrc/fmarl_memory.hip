@@ -55,7 +55,7 @@ __device__ __forceinline__ bool forgets(float g, float mask) { return mask == 0.
 // The decays' prefix sums are float64, so a weight e^{C_t - C_s} is right to float32 however fast the tokens before forgot.  A weight is selected, not multiplied to
 // zero: what an episode left behind (infinities too) does not reach the next one; a chunk that holds a value that is not finite is walked token by token, so
 // that it reaches later tokens only.
-// 64 heads of 4 096 tokens, 64 x 64, bfloat16 (segments of 256 tokens, four workgroups a CU): 33 us for the states alone, 48 us for out, 77 us for out with its sums against w, where the
+// 64 heads of 4 096 tokens, 64 x 64, bfloat16 (segments of 256 tokens, four workgroups a CU): 33 us for the states alone, 53 us for out, 77 us for out with its sums against w, where the
 // bytes take 13 to 27 us and the matrix instructions 4 us: a chunk is three barriers and some 400 vector instructions a wave (pieces, weights, prefix sums), and those bound it.
 // pieces of an input, and the highest order (sum of the pieces' numbers) kept in x y; P, the state as an operand and u z have three pieces, kept to order 2
 template <typename T> struct Pieces;
@@ -622,7 +622,7 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
 // All gradients of up to 16 tokens of heads up to 16 x 16 in one pass (the update's chunks): q, k, v and dout stay in registers -- 16 lanes a head, as above --, the state is walked
 // forwards for dq, its gradient backwards for dk (lane = row) and dv (lane = column).  dg_t = <S_L, dS_L> + sum_{i >= t} (q_i . dq_i - k_i . dk_i), each
 // without the token's own term, 0 where an episode starts.  Reads and writes everything once: 928 MB for 30 720 x 4 heads of ten tokens, 182 us at the copy
-// rate; it takes 222 us, three walks and the decay's kernel took 872 us.
+// rate; it takes 229 us, three walks and the decay's kernel took 872 us.
 struct ShortGrad {
     WalkRows q, k, v, o, dq, dk, dv;
     const float *g; int64_t gl, gb, gh;
@@ -1059,7 +1059,7 @@ __global__ __launch_bounds__(256) void decay_sum_kernel(const double *partial, f
 
 // One token per sequence (a rollout's env step): S' = r e^g S + k^T v, o = scale q S'.  The state is read and written once, 8 dk dv bytes per head, and
 // nothing else weighs: HBM.  A head has a team of lanes that covers its state in float4s, up to a wave, lane = (row group, four columns); o is summed over the row groups.  Float4s
-// go past the caches, which no byte of them finds again.  16 x 16 float32, 2 621 440 heads (6.0 GB): 1 315 us, 4.6 TB/s; 64 x 64, 160 000 heads: 930 us, 5.8 TB/s; 4 x 4, 4 million heads: 130 us
+// go past the caches, which no byte of them finds again.  16 x 16 float32, 2 621 440 heads (6.0 GB): 1 286 us, 4.7 TB/s; 64 x 64, 160 000 heads: 930 us, 5.8 TB/s; 4 x 4, 4 million heads: 130 us
 // (a wave each 1 480 us).  A loop over the heads in as many workgroups as are resident is slower (1 377 us at best): too few loads are in flight.
 struct Step {
     WalkRows q, k, v, out;

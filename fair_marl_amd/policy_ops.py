@@ -454,8 +454,9 @@ def action_log_probs(features, weight, bias, actions, available_actions=None):
     one per row, int64, int32 or float32 (the buffer's ``actions``; a trailing 1 is fine); available_actions: (..., V) float32, bool or uint8, or None.  A row with a
     negative action (padding) or nothing available takes no part: 0, 0 and no gradient.  An unavailable action has log-probability
     -inf, one that does not exist (>= V) NaN (and no gradient).  The logits are never stored: for many actions the softmax runs over pieces of them, and they
-    are formed again for the gradient.  Differentiable in features, weight and bias, once.  Half precision operands: products are exact, sums float32; the
-    gradient's dz is rounded to the operands' type before its two products."""
+    are formed again for the gradient, with the row's log-sum in float32: logits in the thousands cost the gradient's probabilities their last digits (2^-24 of the logit).
+    Differentiable in features, weight and bias, once.  Half precision operands: products are exact, sums float32; with many actions the gradient's dz is rounded to the operands'
+    type before its two products (the gradients' error is 1.4 times that of their own rounding)."""
     _seen_by_torch('action_log_probs', features, weight, bias)
     if weight.dim() != 2 or features.dim() < 1 or features.shape[-1] != weight.shape[1] or not 1 <= weight.shape[1] <= 16384 or not 1 <= weight.shape[0] <= 1 << 20:
         _refuse('action_log_probs: features (..., K) and weight (V, K) with K in 1..16384, V in 1..1048576, got %s, %s', tuple(features.shape), tuple(weight.shape))
