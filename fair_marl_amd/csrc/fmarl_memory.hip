@@ -621,7 +621,7 @@ __global__ __launch_bounds__(256) void memory_rows_kernel(Walk a) {
 
 // All gradients of up to 16 tokens of heads up to 16 x 16 in one pass (the update's chunks): q, k, v and dout stay in registers -- 16 lanes a head, as above --, the state is walked
 // forwards for dq, its gradient backwards for dk (lane = row) and dv (lane = column).  dg_t = <S_L, dS_L> + sum_{i >= t} (q_i . dq_i - k_i . dk_i), each
-// without the token's own term, 0 where an episode starts.  Reads and writes everything once: 928 MB for 30 720 x 4 heads of ten tokens, 182 us at the copy
+// without the token's own term, 0 where an episode starts: its error is 2^-24 of the terms from the token to the end.  Reads and writes everything once: 928 MB for 30 720 x 4 heads of ten tokens, 182 us at the copy
 // rate; it takes 229 us, three walks and the decay's kernel took 872 us.
 struct ShortGrad {
     WalkRows q, k, v, o, dq, dk, dv;
